@@ -1,0 +1,534 @@
+"""The operators that a server of many requests adds to this library's decode path, as cases to measure.
+
+Kinds:
+
+  shared    one decode step's attention for a batch whose sequences share a
+            long prefix (smol_attn_decode_shared): one image or system prompt
+            and many questions, many hypotheses of one recording
+  scored    one decode step's attention that also adds up how much weight
+            each cached row receives (smol_attn_decode_scored)
+  evict     the rows of a cache that received the least weight make room
+            (smol_kv_cache_evict)
+  adapters  a shared bf16 projection with a low-rank adapter of its own for
+            every request of the batch (smol_linear_adapters_dev)
+
+`run` computes an operator with elementary torch operations in 32 bits where
+`own` is false, and through the library (smol_attn.py) where it is true.
+Cached rows, queries and new rows are N(0, 1) with norm weights near 1.5
+(scores of a standard deviation near 1.5), accumulated weights are
+lognormal, projection weights N(0, 1 / in).
+"""
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+DEV = "cuda"
+EPS = 1e-6
+
+# head layouts: (query heads, kv heads, head_dim, rope pairing, theta, per-head Q/K norm)
+HEADS = {
+    "qwen": (16, 8, 128, "neox", 1e6, True),           # Qwen3-ASR decoders
+    "plain": (16, 8, 128, "neox", 1e6, False),         # the same without the per-head norm
+    "mqa": (8, 1, 256, "interleaved", 1e4, False),     # Gemma-2B-style MQA
+    "gemma": (8, 4, 256, "interleaved", 1e6, True),    # Gemma 3 style
+    "small": (8, 4, 64, "neox", 1e6, True),
+    "odd": (15, 5, 80, "neox", 1e4, False),            # 3 query heads a kv head, head_dim off the powers of two
+}
+
+
+def listed():
+    return [
+        # four hypotheses of a short recording: latency
+        dict(name="shared_4_on_500", op="shared", heads="qwen", n_seq=4, prefix=500, len_lo=1, len_hi=24, bf16=False,
+             window=0, cap=0.0),
+        # sixteen questions on one long document, answers of different lengths
+        dict(name="shared_16_on_4096", op="shared", heads="qwen", n_seq=16, prefix=4096, len_lo=0, len_hi=400,
+             bf16=False, window=0, cap=0.0),
+        # one kv head for all, capped scores, an odd prefix, bf16 projections
+        dict(name="shared_mqa_24_on_8191", op="shared", heads="mqa", n_seq=24, prefix=8191, len_lo=16, len_hi=512,
+             bf16=True, window=0, cap=50.0),
+        # a full batch on a very long prefix: the largest
+        dict(name="shared_64_on_16384", op="shared", heads="plain", n_seq=64, prefix=16384, len_lo=0, len_hi=1023,
+             bf16=False, window=0, cap=0.0),
+        # a stream whose cache is held to a budget: latency
+        dict(name="scored_1_of_1024", op="scored", heads="qwen", n_seq=1, len_lo=1024, len_hi=1024, bf16=False,
+             decay=1.0, cap=0.0),
+        # a served batch of such streams
+        dict(name="scored_16_of_4096", op="scored", heads="qwen", n_seq=16, len_lo=3000, len_hi=4160, bf16=False,
+             decay=1.0, cap=0.0),
+        # a small decoder's stream drops its least used rows
+        dict(name="evict_1_300_to_256", op="evict", heads="small", n_seq=1, rows_lo=300, rows_hi=300, keep=256,
+             first=4, recent=32),
+        # the regular trimming of a batch: 64 steps' rows make room for the next 64
+        dict(name="evict_16_4160_to_4096", op="evict", heads="qwen", n_seq=16, rows_lo=4160, rows_hi=4160, keep=4096,
+             first=4, recent=512),
+        # long prompts are cut down once: most kept rows move
+        dict(name="evict_32_8192_to_1024", op="evict", heads="qwen", n_seq=32, rows_lo=8100, rows_hi=8192, keep=1024,
+             first=4, recent=128),
+        # three requests' steps through a query projection, an adapter each
+        dict(name="adapters_3_rank_8", op="adapters", seq=3, in_dim=1024, out_dim=2048, n_adapters=3, rank=8,
+             bf16=False, segments=False, bare=0.0),
+        # a served batch through a fused projection, some rows without an adapter
+        dict(name="adapters_32_rank_16", op="adapters", seq=32, in_dim=1024, out_dim=4096, n_adapters=16, rank=16,
+             bf16=False, segments=False, bare=0.1),
+        # prompts of several requests, one after the other
+        dict(name="adapters_1536_rank_32", op="adapters", seq=1536, in_dim=1024, out_dim=2048, n_adapters=6, rank=32,
+             bf16=True, segments=True, bare=0.0),
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 0.4)))))))
+
+
+def _bounded(c):
+    """fewer sequences where a case would cost more than the largest listed one of its kind"""
+    for unit in ("bytes", "flops"):
+        most = max(work(k)[unit] for k in listed() if k["op"] == c["op"])
+        while work(c)[unit] > most:
+            c["n_seq"] = (c["n_seq"] + 1) // 2
+    return c
+
+
+def draw(rng):
+    op = rng.choice(["shared", "shared", "scored", "evict", "adapters", "adapters"])
+    heads = rng.choice(sorted(HEADS))
+    if op == "shared":
+        hi = _log(rng, 1, 1023)
+        c = dict(op=op, heads=heads, n_seq=_log(rng, 1, 64), prefix=_log(rng, 16, 16384), len_lo=rng.randint(0, hi),
+                 len_hi=hi, bf16=rng.random() < 0.5, window=rng.choice([0, 0, 0, _log(rng, 32, 8192)]),
+                 cap=rng.choice([0.0, 0.0, 30.0, 50.0]))
+        return _bounded(c)
+    if op == "scored":
+        hi = _log(rng, 1, 4160)
+        c = dict(op=op, heads=heads, n_seq=_log(rng, 1, 32), len_lo=rng.randint(0, hi), len_hi=hi,
+                 bf16=rng.random() < 0.5, decay=rng.choice([1.0, 1.0, 0.99, 0.0]), cap=rng.choice([0.0, 0.0, 50.0]))
+        return _bounded(c)
+    if op == "evict":
+        hi = _log(rng, 20, 8192)
+        keep = rng.randint(hi // 8 + 1, hi)
+        first = rng.randint(0, min(8, keep // 2))
+        return dict(op=op, heads=heads, n_seq=_log(rng, 1, 32), rows_lo=rng.randint(hi // 2, hi), rows_hi=hi, keep=keep,
+                    first=first, recent=rng.randint(0, keep - first))
+    return dict(op=op, seq=_log(rng, 1, 1536), in_dim=_log(rng, 64, 2048), out_dim=_log(rng, 64, 2048),
+                n_adapters=_log(rng, 1, 32), rank=rng.choice([4, 8, 16, 24, 32, 64]), bf16=rng.random() < 0.5,
+                segments=rng.random() < 0.5, bare=rng.choice([0.0, 0.2]))
+
+
+def work(c):
+    """each cached row, weight and input read once, each output written once"""
+    if c["op"] == "adapters":
+        m, k, n, r = c["seq"], c["in_dim"], c["out_dim"], c["rank"]
+        used = min(c["n_adapters"], m)
+        el = 2 if c["bf16"] else 4
+        return {"bytes": 2 * n * k + 2 * used * r * (k + n) + el * m * (k + n),
+                "flops": 2 * m * n * k + 2 * m * (1 - c["bare"]) * r * (k + n)}
+    hq, hkv, hd = HEADS[c["heads"]][:3]
+    n = c["n_seq"]
+    if c["op"] == "evict":
+        rows, keep = (c["rows_lo"] + c["rows_hi"]) / 2, c["keep"]
+        if rows <= keep:
+            return {"bytes": n * hkv * rows * 16, "flops": 0}
+        # each free choice falls on a row below `keep` or on one above it as their numbers are
+        moved = min(rows - keep, keep) * max(0.0, 1 - max(c["recent"], rows - keep) / rows)
+        return {"bytes": n * hkv * (8 * rows + 8 * keep + moved * hd * 8), "flops": 0}
+    mean = (c["len_lo"] + c["len_hi"]) / 2
+    io = n * (hq * hd * ((2 if c["bf16"] else 4) + 4) + 2 * hkv * hd * ((2 if c["bf16"] else 4) + 2))
+    if c["op"] == "scored":
+        return {"bytes": n * mean * hkv * (4 * hd + 8) + io, "flops": 4 * n * hq * hd * (mean + 1)}
+    seen, own_rows = c["prefix"], mean + 1
+    if c["window"]:
+        own_rows = min(own_rows, c["window"])
+        seen = max(0, min(seen, c["window"] - own_rows))
+    return {"bytes": (seen + n * mean) * hkv * hd * 4 + io, "flops": 4 * n * hq * hd * (seen + own_rows)}
+
+
+# ------------------------------------------------------------------ inputs
+
+_tables = {}
+
+
+def _table(hd, theta, n):
+    """The decoders' cos and sin rows [n][hd / 2] (fp32): 1 / theta^(2 d / hd) and its products with the positions
+    are rounded to fp32, as the models' tables are; their cosines and sines are taken in 64 bits."""
+    size = 1024
+    while size < n:
+        size *= 2
+    if (hd, theta, size) not in _tables:
+        e = np.arange(0, hd, 2, dtype=np.float32) / np.float32(hd)
+        inv = np.float32(1) / (np.float64(theta) ** e.astype(np.float64)).astype(np.float32)
+        ang = (np.arange(size, dtype=np.float32)[:, None] * inv[None, :]).astype(np.float64)
+        _tables[hd, theta, size] = tuple(torch.from_numpy(f(ang).astype(np.float32)).to(DEV) for f in (np.cos, np.sin))
+    return _tables[hd, theta, size]
+
+
+def _round64(n):
+    return max(64, (n + 63) // 64 * 64)
+
+
+def _lengths(c, seed, lo, hi):
+    """one length a sequence, the longest of the case among them, and the cache slots they live in"""
+    r = random.Random(seed * 7919 + 17)
+    n = c["n_seq"]
+    lens = [r.randint(lo, hi) for _ in range(n)]
+    lens[r.randrange(n)] = hi
+    slots = list(range(n + 1))
+    r.shuffle(slots)
+    return lens, slots[:n]
+
+
+def _inputs(c, seed):
+    """the tensors of one case, alike for every side"""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed * 1000003 + 11)
+
+    def normal(*shape, dtype=torch.float32, std=1.0):
+        x = torch.empty(shape, dtype=dtype, device=DEV)
+        x.normal_(0.0, std, generator=g)
+        return x
+
+    if c["op"] == "adapters":
+        m, k, n, na, r = c["seq"], c["in_dim"], c["out_dim"], c["n_adapters"], c["rank"]
+        py = random.Random(seed * 104729 + 5)
+        if c["segments"]:
+            cuts = sorted(py.randint(0, m) for _ in range(na - 1))
+            ids = [sum(s >= cut for cut in cuts) for s in range(m)]
+        else:
+            ids = [py.randrange(na) for _ in range(m)]
+        ids = [-1 if py.random() < c["bare"] else a for a in ids]
+        return dict(x=normal(m, k, dtype=torch.bfloat16 if c["bf16"] else torch.float32),
+                    w=normal(n, k, dtype=torch.bfloat16, std=k ** -0.5), bias=normal(n, std=0.1),
+                    a=normal(na, r, k, dtype=torch.bfloat16, std=k ** -0.5),
+                    b=normal(na, n, r, dtype=torch.bfloat16, std=r ** -0.5),
+                    scale=[0.5 + 0.25 * (i % 5) for i in range(na)], ids=ids)
+    hq, hkv, hd, pairing, theta, norm = HEADS[c["heads"]]
+    if c["op"] == "evict":
+        rows, slots = _lengths(c, seed, c["rows_lo"], c["rows_hi"])
+        cap, ns = _round64(c["rows_hi"]), c["n_seq"] + 1
+        mass = torch.exp(normal(ns, hkv, cap, std=1.5))
+        # rows of a cache that was trimmed before: their positions have gaps and are not in order
+        order = torch.rand((ns, hkv, cap), generator=g, device=DEV)
+        pos = torch.full((ns, hkv, cap), -1, dtype=torch.int32, device=DEV)
+        ends = []
+        for n, s in zip(rows, slots):
+            end = n + 1000
+            ends.append(end)
+            p = torch.arange(n, device=DEV, dtype=torch.int32) + 1000
+            p[: min(c["first"], n)] -= 1000
+            early = n - min(n, c["recent"] // 2)
+            by = torch.cat([torch.argsort(order[s, :, :early], dim=-1),
+                            torch.arange(early, n, device=DEV).expand(hkv, n - early)], 1)
+            pos[s, :, :n] = p[by]
+        return dict(k=normal(ns, hkv, cap, hd, dtype=torch.bfloat16), v=normal(ns, hkv, cap, hd, dtype=torch.bfloat16),
+                    mass=mass, pos=pos, rows=rows, slots=slots, ends=ends)
+    lens, slots = _lengths(c, seed, c["len_lo"], c["len_hi"])
+    n = c["n_seq"]
+    dt = torch.bfloat16 if c["bf16"] else torch.float32
+    cap = _round64(c["len_hi"] + 1)
+    d = dict(q=normal(n, hq * hd, dtype=dt), k_new=normal(n, hkv * hd, dtype=dt), v_new=normal(n, hkv * hd, dtype=dt),
+             q_norm=1.5 + normal(hd, std=0.1) if norm else None, k_norm=1.0 + normal(hd, std=0.1) if norm else None,
+             lens=lens, slots=slots, scale=hd ** -0.5, inter=pairing == "interleaved")
+    if not norm:
+        d["scale"] *= 1.5
+    live = torch.zeros((n + 1, 1, cap, 1), dtype=torch.bfloat16, device=DEV)  # rows that no sequence has written are zero
+    for l, s in zip(lens, slots):
+        live[s, :, :l] = 1
+    d["k"] = normal(n + 1, hkv, cap, hd, dtype=torch.bfloat16).mul_(live)
+    d["v"] = normal(n + 1, hkv, cap, hd, dtype=torch.bfloat16).mul_(live)
+    if c["op"] == "shared":
+        pc = _round64(c["prefix"])
+        d["pk"] = normal(1, hkv, pc, hd, dtype=torch.bfloat16)
+        d["pv"] = normal(1, hkv, pc, hd, dtype=torch.bfloat16)
+        d["pos"] = [c["prefix"] + l for l in lens]
+    else:
+        d["pos"] = [3 * l + 5 for l in lens]  # two rows of three were evicted before
+        d["mass"] = torch.exp(normal(n + 1, hkv, cap))
+        d["row_pos"] = torch.randint(0, 3 * cap, (n + 1, hkv, cap), generator=g, device=DEV, dtype=torch.int32)
+    table = _table(hd, theta, max(d["pos"]) + 1)
+    at = torch.tensor(d["pos"], device=DEV)
+    d["cos"], d["sin"] = table[0][at], table[1][at]
+    return d
+
+
+_kept = {}  # the context and the position tables that a program makes once
+
+
+def _sa():
+    import importlib
+    sa = importlib.import_module("smol-genius_amd.smol_attn")
+    if "ctx" not in _kept:
+        _kept["ctx"] = sa.Context(0)
+    return sa, _kept["ctx"]
+
+
+def _cache(sa, ctx, k, v):
+    """a cache of the library that holds these rows"""
+    ns, hkv, cap, hd = k.shape
+    kv = sa.KVCache(ctx, 1, ns, hkv, hd, cap)
+    kt, vt = kv.views(0)
+    kt.copy_(k)
+    vt.copy_(v.view(ns, hkv, cap // 32, 32, hd).transpose(-1, -2))
+    return kv, kt, vt.transpose(-1, -2)
+
+
+def prepare(case, seed):
+    c = case
+    d = _inputs(c, seed)
+    d["case"] = c
+    if c["op"] == "adapters":
+        d["mine"] = torch.tensor(d["ids"], device=DEV)
+        d["scales"] = torch.tensor(d["scale"], device=DEV)
+    else:
+        d["at"] = torch.tensor(d["slots"], device=DEV)
+        if c["op"] == "evict":
+            d["mass_out"], d["pos_out"] = torch.zeros_like(d["mass"]), torch.zeros_like(d["pos"])
+            d["n_rows"], d["n_ends"] = torch.tensor(d["rows"], device=DEV), torch.tensor(d["ends"], device=DEV)
+        else:
+            d["n_rows"], d["at_pos"] = torch.tensor(d["lens"], device=DEV), torch.tensor(d["pos"], device=DEV)
+    if own:
+        sa, ctx = _sa()
+        if c["op"] == "adapters":
+            d["set"] = sa.Adapters(ctx, list(zip(d["a"], d["b"], d["scale"])))
+            return d
+        d["kv"], d["k"], d["v"] = _cache(sa, ctx, d["k"], d["v"])
+        if c["op"] == "shared":
+            d["prefix_kv"], d["pk"], d["pv"] = _cache(sa, ctx, d["pk"], d["pv"])
+        if c["op"] != "evict":
+            hq, hkv, hd, pairing, theta, _ = HEADS[c["heads"]]
+            key = (hd, theta, pairing)
+            if key not in _kept:
+                _kept[key] = sa.RopeTable(ctx, hd, theta, sa.ROPE_INTERLEAVED if d["inter"] else sa.ROPE_NEOX)
+            _kept[key].ensure(max(d["pos"]) + 1)
+            d["rope"] = _kept[key]
+    return d
+
+
+# -------------------------------------------------------------- plain forms
+
+def _normed(x, w):
+    if w is None:
+        return x
+    return x * w / torch.sqrt((x * x).mean(-1, keepdim=True) + EPS)
+
+
+def _rotated(x, cos, sin, inter):
+    """x [n][heads][hd] by the table rows cos, sin [n][hd / 2]"""
+    cos, sin = cos[:, None], sin[:, None]
+    a, b = (x[..., 0::2], x[..., 1::2]) if inter else x.chunk(2, -1)
+    y = (a * cos - b * sin, b * cos + a * sin)
+    return torch.stack(y, -1).flatten(-2) if inter else torch.cat(y, -1)
+
+
+def _step(s, c):
+    """Q and the new key, normalised and rotated, and the new value (32 bits); the rows' bf16 copies go to the cache"""
+    hq, hkv, hd = HEADS[c["heads"]][:3]
+    n = c["n_seq"]
+    q = _rotated(_normed(s["q"].float().view(n, hq, hd), s["q_norm"]), s["cos"], s["sin"], s["inter"])
+    k = _rotated(_normed(s["k_new"].float().view(n, hkv, hd), s["k_norm"]), s["cos"], s["sin"], s["inter"])
+    v = s["v_new"].float().view(n, hkv, hd)
+    s["k"][s["at"], :, s["n_rows"]] = k.to(torch.bfloat16)
+    s["v"][s["at"], :, s["n_rows"]] = v.to(torch.bfloat16)
+    return q.view(n, hkv, hq // hkv, hd), k, v
+
+
+def _capped(x, cap):
+    return torch.tanh(x / cap) * cap if cap > 0 else x
+
+
+def _own_rows(s, c, q, k, v):
+    """scores [n][kv][G][m] and values [n][kv][m][hd] of each sequence's own rows, the new one at its full precision"""
+    n = c["n_seq"]
+    m = max(s["lens"]) + 1
+    each = torch.arange(n, device=DEV)
+    ks, vs = s["k"][s["at"], :, :m].float(), s["v"][s["at"], :, :m].float()
+    ks[each, :, s["n_rows"]], vs[each, :, s["n_rows"]] = k, v
+    return _capped(q @ ks.transpose(-1, -2) * s["scale"], c["cap"]), vs
+
+
+def _run_shared(s, c):
+    hq, hkv, hd = HEADS[c["heads"]][:3]
+    n, p, grp = c["n_seq"], c["prefix"], hq // hkv
+    q, k, v = _step(s, c)
+    mine, vs = _own_rows(s, c, q, k, v)
+    pk, pv = s["pk"][0, :, :p].float(), s["pv"][0, :, :p].float()
+    rows = q.transpose(0, 1).reshape(hkv, n * grp, hd)
+    both = _capped(rows @ pk.transpose(-1, -2) * s["scale"], c["cap"]).view(hkv, n, grp, p).transpose(0, 1)
+    row, at = torch.arange(mine.shape[-1], device=DEV), s["n_rows"][:, None]
+    seen, seen_p = row <= at, torch.ones((n, p), dtype=torch.bool, device=DEV)
+    if c["window"]:
+        low = s["at_pos"][:, None] - c["window"]
+        seen, seen_p = seen & (row + p > low), torch.arange(p, device=DEV) > low
+    inf = float("-inf")
+    mine = mine.masked_fill(~seen[:, None, None], inf)
+    both = both.masked_fill(~seen_p[:, None, None], inf)
+    top = torch.maximum(mine.amax(-1, keepdim=True), both.amax(-1, keepdim=True))
+    mine, both = torch.exp(mine - top), torch.exp(both - top)
+    total = mine.sum(-1, keepdim=True) + both.sum(-1, keepdim=True)
+    o = (both.transpose(0, 1).reshape(hkv, n * grp, p) @ pv).view(hkv, n, grp, hd).transpose(0, 1)
+    return {"out": ((o + mine @ vs) / total).reshape(n, hq * hd), "k": s["k"], "v": _slabs(s["v"])}
+
+
+def _slabs(v):
+    return v.view(v.shape[0], v.shape[1], -1, 32, v.shape[3])
+
+
+def _run_scored(s, c):
+    hq, hkv, hd = HEADS[c["heads"]][:3]
+    q, k, v = _step(s, c)
+    x, vs = _own_rows(s, c, q, k, v)
+    row, at = torch.arange(x.shape[-1], device=DEV), s["n_rows"][:, None]
+    x = x.masked_fill(~(row <= at)[:, None, None], float("-inf"))
+    x = torch.exp(x - x.amax(-1, keepdim=True))
+    x = x / x.sum(-1, keepdim=True)
+    m = x.shape[-1]
+    got, had = x.sum(2), s["mass"][s["at"], :, :m]
+    new, old = (row == at)[:, None], (row < at)[:, None]
+    s["mass"][s["at"], :, :m] = torch.where(new, got, torch.where(old, had * c["decay"] + got, had))
+    s["row_pos"][s["at"], :, s["n_rows"]] = s["at_pos"][:, None].to(torch.int32)
+    return {"out": (x @ vs).reshape(c["n_seq"], hq * hd), "mass": s["mass"], "row_pos": s["row_pos"], "k": s["k"],
+            "v": _slabs(s["v"])}
+
+
+def _run_evict(s, c):
+    at, keep = s["at"], c["keep"]
+    mass, pos = s["mass"][at], s["pos"][at]
+    n, hkv, cap = mass.shape
+    row = torch.arange(cap, device=DEV)
+    rows, ends = s["n_rows"][:, None, None], s["n_ends"][:, None, None]
+    rank = (mass + 0.0).view(torch.int32).long()  # positive numbers keep their order as whole ones
+    rank = torch.where((pos < c["first"]) | (pos >= ends - c["recent"]), 1 << 40, rank)
+    rank = torch.where(row < rows, rank, -1)
+    order = torch.sort(rank, dim=-1, descending=True, stable=True).indices
+    kept = torch.zeros_like(rank, dtype=torch.bool).scatter_(-1, order[..., :keep], True) & (row < rows)
+    left = torch.clamp(rows, max=keep)
+    hole, mover = ~kept & (row < left), kept & (row >= left)
+    movers = torch.sort((~mover).to(torch.uint8), dim=-1, stable=True).indices
+    src = torch.where(hole, movers.gather(-1, (hole.cumsum(-1) - 1).clamp(min=0)), row.expand_as(movers))
+    for name in ("k", "v"):
+        x = s[name][at]
+        s[name][at] = x.gather(2, src[..., None].expand_as(x))
+    live = row < left
+    s["mass_out"][at] = torch.where(live, mass.gather(-1, src), s["mass_out"][at])
+    s["pos_out"][at] = torch.where(live, pos.gather(-1, src), s["pos_out"][at])
+    return {"k": s["k"], "v": _slabs(s["v"]), "mass": s["mass_out"], "row_pos": s["pos_out"]}
+
+
+def _run_adapters(s, c):
+    na, r, k = s["a"].shape
+    x = s["x"].float()
+    y = x @ s["w"].float().t() + s["bias"]
+    mine = (s["mine"][:, None] == torch.arange(na, device=DEV)) * s["scales"]
+    t = (x @ s["a"].float().view(na * r, k).t()).view(-1, na, r) * mine[..., None]
+    y = y + t.view(-1, na * r) @ s["b"].float().transpose(1, 2).reshape(na * r, -1)
+    # the bf16 decoder's projections cut the low bits off
+    return {"y": (y.view(torch.int32) & -65536).view(torch.float32).to(torch.bfloat16) if c["bf16"] else y}
+
+
+def run(state):
+    s, c = state, state["case"]
+    if not own:
+        return {"shared": _run_shared, "scored": _run_scored, "evict": _run_evict, "adapters": _run_adapters}[c["op"]](s, c)
+    sa, ctx = _sa()
+    if c["op"] == "adapters":
+        y = sa.linear_adapters(ctx, s["x"], s["w"], s["set"], s["ids"], bias=s["bias"], out_bf16=c["bf16"])
+        return {"y": y.view(torch.bfloat16) if c["bf16"] else y}
+    if c["op"] == "evict":
+        sa.kv_evict(s["kv"], 0, s["slots"], s["rows"], s["ends"], s["mass"], s["pos"], c["keep"], first=c["first"],
+                    recent=c["recent"], mass_out=s["mass_out"], pos_out=s["pos_out"])
+        return {"k": s["k"], "v": s["v"], "mass": s["mass_out"], "row_pos": s["pos_out"]}
+    hq = HEADS[c["heads"]][0]
+    if c["op"] == "shared":
+        out = sa.decode_shared(ctx, s["prefix_kv"], 0, c["prefix"], s["kv"], 0, s["rope"], s["slots"], s["lens"], s["q"],
+                               s["k_new"], s["v_new"], hq, s["scale"], window=c["window"], cap=c["cap"],
+                               q_norm=s["q_norm"], k_norm=s["k_norm"], eps=EPS)
+        return {"out": out, "k": s["k"], "v": s["v"]}
+    out = sa.decode_scored(ctx, s["kv"], 0, s["rope"], s["slots"], s["lens"], s["pos"], s["q"], s["k_new"], s["v_new"], hq,
+                           s["scale"], s["mass"], s["row_pos"], decay=c["decay"], cap=c["cap"], q_norm=s["q_norm"],
+                           k_norm=s["k_norm"], eps=EPS)
+    return {"out": out, "mass": s["mass"], "row_pos": s["row_pos"], "k": s["k"], "v": s["v"]}
+
+
+# ------------------------------------------------------------------ 64 bits
+
+def _exact_row(x, w, cos, sin, inter):
+    """heads [h][hd] of one token in 64 bits: x w / sqrt(mean x^2 + eps), then the pairs as complex numbers times
+    cos + i sin"""
+    x = x.double()
+    if w is not None:
+        x = x * (x.pow(2).mean(-1, keepdim=True) + EPS).rsqrt() * w.double()
+    turn = torch.complex(cos.double(), sin.double())
+    if inter:
+        return torch.view_as_real(torch.complex(x[:, 0::2].contiguous(), x[:, 1::2].contiguous()) * turn).flatten(1)
+    half = x.shape[1] // 2
+    z = torch.complex(x[:, :half].contiguous(), x[:, half:].contiguous()) * turn
+    return torch.cat([z.real, z.imag], 1)
+
+
+def _exact_decode(c, d):
+    hq, hkv, hd = HEADS[c["heads"]][:3]
+    grp = hq // hkv
+    ck, cv = d["k"].double(), d["v"].double()
+    out = torch.zeros((c["n_seq"], hq * hd), dtype=torch.float64, device=DEV)
+    mass = d["mass"].double() if c["op"] == "scored" else None
+    for i, (l, s, p) in enumerate(zip(d["lens"], d["slots"], d["pos"])):
+        q = _exact_row(d["q"][i].view(hq, hd), d["q_norm"], d["cos"][i], d["sin"][i], d["inter"])
+        ck[s, :, l] = _exact_row(d["k_new"][i].view(hkv, hd), d["k_norm"], d["cos"][i], d["sin"][i], d["inter"])
+        cv[s, :, l] = d["v_new"][i].double().view(hkv, hd)
+        keys, vals = ck[s, :, : l + 1], cv[s, :, : l + 1]
+        if c["op"] == "shared":
+            keys = torch.cat([d["pk"][0, :, : c["prefix"]].double(), keys], 1)
+            vals = torch.cat([d["pv"][0, :, : c["prefix"]].double(), vals], 1)
+            if c["window"]:
+                keys, vals = keys[:, max(0, p - c["window"] + 1):], vals[:, max(0, p - c["window"] + 1):]
+        z = torch.bmm(q.view(hkv, grp, hd), keys.transpose(1, 2).contiguous()) * d["scale"]
+        if c["cap"] > 0:
+            z = c["cap"] * (z / c["cap"]).tanh()
+        w = z.softmax(-1)
+        out[i] = torch.bmm(w, vals.contiguous()).reshape(-1)
+        if mass is not None:
+            mass[s, :, :l] = c["decay"] * mass[s, :, :l] + w.sum(1)[:, :l]
+            mass[s, :, l] = w.sum(1)[:, l]
+    ans = {"out": out, "k": ck, "v": _slabs(cv)}
+    if mass is not None:
+        ans.update(mass=mass, row_pos=None)
+    return ans
+
+
+def _exact_evict(c, d):
+    mass, pos = d["mass"].cpu().numpy(), d["pos"].cpu().numpy()
+    k, v = d["k"].double(), d["v"].double()
+    left = torch.zeros(mass.shape, dtype=torch.float64)
+    for n, s, end in zip(d["rows"], d["slots"], d["ends"]):
+        m = min(n, c["keep"])
+        for g in range(mass.shape[1]):
+            safe = (pos[s, g, :n] < c["first"]) | (pos[s, g, :n] >= end - c["recent"])
+            # by (protected, weight, lower row): the last key of lexsort counts first
+            best = np.lexsort((np.arange(n), -mass[s, g, :n].astype(np.float64), ~safe))[:m]
+            kept = np.zeros(n, bool)
+            kept[best] = True
+            dst, src = np.flatnonzero(~kept[:m]), m + np.flatnonzero(kept[m:])
+            row = np.arange(m)
+            row[dst] = src
+            left[s, g, :m] = torch.from_numpy(mass[s, g][row].astype(np.float64))
+            for x in (k, v):
+                x[s, g, torch.from_numpy(dst).to(DEV)] = x[s, g, torch.from_numpy(src).to(DEV)]
+    return {"k": k, "v": _slabs(v), "mass": left, "row_pos": None}
+
+
+def exact(case, seed):
+    c, d = case, _inputs(case, seed)
+    if c["op"] == "evict":
+        return _exact_evict(c, d)
+    if c["op"] != "adapters":
+        return _exact_decode(c, d)
+    x = d["x"].double()
+    y = x @ d["w"].double().t() + d["bias"].double()
+    ids = torch.tensor(d["ids"], device=DEV)
+    for i, sc in enumerate(d["scale"]):
+        at = torch.nonzero(ids == i).flatten()
+        y[at] += sc * ((x[at] @ d["a"][i].double().t()) @ d["b"][i].double().t())
+    return {"y": y}
