@@ -192,6 +192,13 @@ SMOL_ATTN_API int smol_kv_cache_write(smol_kv_cache *kv, int layer, int slot, in
 SMOL_ATTN_API int smol_kv_cache_read(smol_kv_cache *kv, int layer, int slot, int pos0, int n,
                                      uint16_t *k_out, uint16_t *v_out);
 
+/* device addresses of one layer's rows, for callers that read or fill a cache
+ * with kernels of their own: *k bf16 [n_slots][n_kv_heads][capacity][head_dim],
+ * *vt bf16 [n_slots][n_kv_heads][capacity / 32][head_dim][32] (V transposed
+ * within 32-row slabs). Valid until the cache grows or is destroyed; work on
+ * them is ordered by the caller with the context's stream. */
+SMOL_ATTN_API int smol_kv_cache_pointers(const smol_kv_cache *kv, int layer, void **k, void **vt);
+
 /* ---- attention on device pointers -----------------------------------------
  * window > 0: sliding window (keys with pos - window < key <= pos,
  * attention.c:176-273); cap > 0: score = cap * tanh(score / cap)
@@ -264,6 +271,76 @@ SMOL_ATTN_API int smol_attn_decode_noalloc(smol_attn_ctx *ctx, smol_kv_cache *kv
                                            const void *v_new, int dtype, int n_heads, float scale,
                                            int window, float cap, const float *q_norm,
                                            const float *k_norm, float eps, float *out);
+
+/* ---- a batch on a shared prefix; a cache held to a budget --------------------
+ * No counterparts in the reference, which decodes one sequence at a time.
+ *
+ * Common to the two decode steps below. The new token of sequence i is used
+ * in fp32 by the call that appends it and stored as bf16 (nearest even). The
+ * scores of a row are a 24-bit split of Q against the cache's bf16 bits, the
+ * probabilities carry 16 bits into P.V, everything else is fp32; there is no
+ * range limit. A cached row that holds NaN or infinity makes the outputs of the
+ * sequences that see it NaN, and of no other; rows at or past a sequence's length are never used. A
+ * sequence's result does not depend on what the cache holds elsewhere, but the
+ * order of its sums follows the batch's shape. Slots are host arrays, each
+ * slot at most once. Calls grow the cache, the table and the context's
+ * workspace as needed. Under stream capture they may not grow anything and
+ * take at most 128 sequences (SMOL_ATTN_ERR_UNSUPPORTED otherwise: run the
+ * call once before the capture); the captured call keeps the slots, lengths
+ * and positions that it was made with, and it uses the context's workspace, so
+ * its replays are ordered with the context's other calls by the caller. */
+
+/* One decode step of n_seq sequences that all continue the same prefix:
+ * positions [0, prefix_len) are the rows of (layer, prefix_slot) of the cache
+ * `prefix`, written once, and sequence i's own rows, len[i] of them, are
+ * positions prefix_len + 0 .. len[i] - 1 in rows 0 .. len[i] - 1 of
+ * (layer, slots[i]) of `kv`. The new token gets position prefix_len + len[i]
+ * and row len[i]; out[i] is the attention of q[i] over the prefix, the own
+ * rows and the new token. `prefix` and `kv` have the same heads; they may be
+ * one cache (then prefix_slot is none of slots). The prefix is read once for
+ * the whole batch. Norm, RoPE, window, cap and layouts as for
+ * smol_attn_decode_qknorm (NULL norm weights skip a norm). */
+SMOL_ATTN_API int smol_attn_decode_shared(smol_attn_ctx *ctx, const smol_kv_cache *prefix, int prefix_slot,
+                                          int prefix_len, smol_kv_cache *kv, int layer, const smol_rope_table *rope,
+                                          int n_seq, const int *slots, const int *len, const void *q,
+                                          const void *k_new, const void *v_new, int dtype, int n_heads, float scale,
+                                          int window, float cap, const float *q_norm, const float *k_norm, float eps,
+                                          float *out);
+
+/* One decode step on caches whose rows need not be consecutive positions
+ * (some were evicted), which also adds up each row's weight. Sequence i has
+ * rows[i] rows in (layer, slots[i]); the new token becomes row rows[i] and is
+ * rotated to position pos[i]; all rows are visible. Afterwards, with p the
+ * softmax weights and the sum over the query heads of a kv head,
+ *   mass[slots[i]][g][j] = decay * mass[slots[i]][g][j] + sum_h p_h[j]   j < rows[i]
+ *   mass[slots[i]][g][rows[i]] = sum_h p_h[rows[i]]
+ *   row_pos[slots[i]][g][rows[i]] = pos[i]
+ * decay 1 accumulates, below 1 forgets, 0 keeps the last step's weights
+ * (mass is then not read). mass (fp32) and row_pos (int) are device arrays
+ * [n_slots][n_kv_heads][stride] of this layer, stride > rows[i]; no other
+ * element of theirs is written. */
+SMOL_ATTN_API int smol_attn_decode_scored(smol_attn_ctx *ctx, smol_kv_cache *kv, int layer,
+                                          const smol_rope_table *rope, int n_seq, const int *slots, const int *rows,
+                                          const int *pos, const void *q, const void *k_new, const void *v_new,
+                                          int dtype, int n_heads, float scale, float cap, const float *q_norm,
+                                          const float *k_norm, float eps, float *mass, int *row_pos, int stride,
+                                          float decay, float *out);
+
+/* Takes the least used rows out of (layer, slots[i]): of rows[i] rows, `keep`
+ * stay for every kv head (all of them where rows[i] <= keep). Rows with a
+ * position below `first`, or at or past ends[i] - recent (ends[i]: one past
+ * the newest position), come before all others; then the larger mass, NaN
+ * above infinity; ties go to the lower row; first + recent <= keep. The kept
+ * rows below `keep` stay where they are; the kept rows at or past it move to
+ * the freed rows, both in ascending order, with their mass and position. The
+ * sequence then has min(rows[i], keep) rows; the rows behind them are left as
+ * they were. mass_out and pos_out may be mass and row_pos themselves (both),
+ * or arrays apart from them, of which rows [0, min(rows[i], keep)) are
+ * written. Layouts as for smol_attn_decode_scored. Enqueued on the cache's
+ * context's stream. */
+SMOL_ATTN_API int smol_kv_cache_evict(smol_kv_cache *kv, int layer, int n_seq, const int *slots, const int *rows,
+                                      const int *ends, const float *mass, const int *row_pos, float *mass_out,
+                                      int *pos_out, int stride, int keep, int first, int recent);
 
 /* Causal attention on flat device arrays, no cache and no RoPE: the device
  * form of smol_causal_attention (attention.c:153-170). K, V: [seq_k][n_kv*hd]. */

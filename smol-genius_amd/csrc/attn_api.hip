@@ -16,6 +16,7 @@
 #include <limits.h>
 #include <math.h>
 #include <stdarg.h>
+#include <stddef.h>
 #include <stdint.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -46,6 +47,10 @@ extern "C" int smol_launch_fb(const SkParams *sp, int hd, int n_items, int nt, h
 extern "C" int smol_launch_win(const WinParams *wp, int hd, int n_tiles, int max_len, hipStream_t st, hipEvent_t e0,
                                hipEvent_t e1);
 extern "C" int smol_win_max_keys(int hd, int in_dtype, int precise);
+extern "C" int smol_shared_tile_rows(int hd, int rows);
+extern "C" int smol_launch_shared(const ShParams *p, int hd, int tile_rows, int max_len, hipStream_t st, hipEvent_t e0,
+                                  hipEvent_t e1);
+extern "C" int smol_launch_evict(const EvictParams *p, int max_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
 extern "C" int smol_launch_to_bf16_trunc(const float *x, uint16_t *y, long long n, hipStream_t st);
 extern "C" int smol_launch_bf16_norm_rope(uint16_t *x, const float *w, uint16_t *x2, const float *w2, int H2,
                                           float eps, const float *cos_t, const float *sin_t, int pos0, int seq, int H,
@@ -1843,6 +1848,303 @@ extern "C" int smol_attn_decode_noalloc(smol_attn_ctx *ctx, smol_kv_cache *kv, i
     CallShape cs{true, q, k_new, v_new, dtype, n_heads, Hkv, hd, (long long)n_heads * hd,
                  (long long)Hkv * hd, scale, cap, window, rope, 1, 1, kv, layer, out, q_norm, k_norm, eps, true};
     return run_decode(ctx, cs, dc);
+}
+
+/* ------------------------------- a batch on a shared prefix; a cache held to a budget */
+
+/* A call that needs more device memory than there is, or a table's upload,
+ * cannot be captured: an allocation ends the capture, and a replayed upload
+ * would read a host buffer that later calls have written. */
+static int check_capture(smol_attn_ctx *ctx, const char *what, bool grows) {
+    if (!grows) return 0;
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(ctx->stream, &cs));
+    if (cs == hipStreamCaptureStatusNone) return 0;
+    return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%s under stream capture (run the call once before, with at most %d sequences)",
+                what, SH_ARG_SEQS);
+}
+
+/* cache growth and the table's, refused under capture */
+static int reserve_step(smol_attn_ctx *ctx, smol_kv_cache *kv, int rows, const smol_rope_table *rope, int hd, int positions) {
+    int rc;
+    if ((rc = check_capture(ctx, "cache growth", rows > kv->cap))) return rc;
+    if ((rc = check_capture(ctx, "RoPE table growth", rope && positions > rope->cap))) return rc;
+    if ((rc = smol_kv_cache_reserve(kv, rows))) return rc;
+    return check_rope(ctx, rope, hd, positions);
+}
+
+/* one head's rows of a slot are addressed with 31 bits */
+static int check_region(const smol_kv_cache *kv) {
+    return (long long)kv->cap * kv->hd * 2 <= 0x7FFF0000LL
+               ? 0 : fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d rows of head_dim %d a slot", kv->cap, kv->hd);
+}
+
+/* slots in range, each once; lengths >= 0 */
+static int check_slots(const smol_kv_cache *kv, int n_seq, const int *slots, const int *len, int *max_len) {
+    std::vector<char> seen(kv->n_slots, 0);
+    *max_len = 0;
+    for (int i = 0; i < n_seq; i++) {
+        if (slots[i] < 0 || slots[i] >= kv->n_slots) return fail(SMOL_ATTN_ERR_ARG, "slot %d out of range", slots[i]);
+        if (seen[slots[i]]) return fail(SMOL_ATTN_ERR_ARG, "slot %d appears twice", slots[i]);
+        seen[slots[i]] = 1;
+        if (len[i] < 0 || len[i] > INT_MAX - 64) return fail(SMOL_ATTN_ERR_ARG, "%d rows", len[i]);
+        *max_len = std::max(*max_len, len[i]);
+    }
+    return 0;
+}
+
+/* Plans and launches k_sh and k_sh_merge. sp: the sequences, the prefix
+ * (pk, pvt, pcap, p_len) and what the call's options set are filled in. */
+static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int layer, const std::vector<ShSeq> &seqs,
+                      int max_len) {
+    const int hd = kv->hd, Hkv = kv->n_kv, n = (int)seqs.size(), G = sp.Hq / Hkv, rows = n * G;
+    sp.kc = kv->k + (size_t)layer * kv_layer_elems(kv);
+    sp.vtc = kv->vt + (size_t)layer * kv_layer_elems(kv);
+    sp.c_slot_stride = (long long)kv_slot_elems(kv);
+    sp.cap = kv->cap;
+    sp.Hkv = Hkv;
+    sp.G = G;
+    sp.n_seq = n;
+    /* what the window leaves */
+    int p_first = 0, max_own = 0;
+    long long own_slabs = 0;
+    for (const ShSeq &q : seqs) {
+        const int first = sp.window > 0 ? std::max(0, q.pos - sp.window + 1 - sp.p_len) & ~(SMOL_SLAB - 1) : 0;
+        max_own = std::max(max_own, q.len - first);
+        own_slabs += (q.len - first + SMOL_SLAB - 1) / SMOL_SLAB;
+    }
+    if (sp.window > 0 && sp.p_len > 0) {
+        int lo = INT_MAX;
+        for (const ShSeq &q : seqs) lo = std::min(lo, std::max(0, q.pos - sp.window + 1));
+        p_first = std::min(lo, sp.p_len) & ~(SMOL_SLAB - 1);
+    }
+    sp.p_first = p_first;
+    const int tile = smol_shared_tile_rows(hd, rows);
+    const int p_slabs = (sp.p_len - p_first + SMOL_SLAB - 1) / SMOL_SLAB, own_max = (max_own + SMOL_SLAB - 1) / SMOL_SLAB;
+    sp.n_rb = (rows + tile - 1) / tile;
+    sp.s_rb = (G + 15) / 16;
+    /* equally long chunks of at least a slab a wave, as many as fill the device */
+    const long long units = (long long)Hkv * sp.n_rb * p_slabs + Hkv * (long long)sp.s_rb * own_slabs;
+    long long c = (units + 2LL * ctx->cu_count - 1) / (2LL * ctx->cu_count);
+    c = std::max(c, ((long long)std::max(p_slabs, own_max) + SH_MAX_SPLIT - 1) / SH_MAX_SPLIT);
+    c = std::max(4LL, (c + 3) & ~3LL);
+    if (c > (INT_MAX >> 6)) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d rows", max_len);
+    sp.p_chunk = sp.s_chunk = (int)c * SMOL_SLAB;
+    sp.n_ps = (int)((p_slabs + c - 1) / c);
+    sp.n_ss = std::max(1, (int)((own_max + c - 1) / c));
+    const long long pblocks = ((long long)Hkv * sp.n_ps + 7) / 8 * 8 * sp.n_rb;
+    const long long sblocks = (long long)sp.n_ss * n * Hkv * sp.s_rb;
+    if (pblocks + sblocks > INT_MAX / 2 || (long long)n * sp.Hq + (long long)n * Hkv * (max_len / 1024 + 1) > INT_MAX / 2)
+        return fail(SMOL_ATTN_ERR_UNSUPPORTED, "decode call too large (%d sequences)", n);
+    sp.n_pblocks = (int)pblocks;
+
+    WorkPlan wk;
+    const size_t p_rows = (size_t)sp.n_ps * Hkv * rows, s_rows = (size_t)n * Hkv * sp.n_ss * G;
+    const size_t o_po = wk.take(p_rows * hd * 4), o_pml = wk.take(p_rows * 8);
+    const size_t o_so = wk.take(s_rows * hd * 4), o_sml = wk.take(s_rows * 8);
+    sp.l_stride = (max_len + SMOL_SLAB - 1) & ~(SMOL_SLAB - 1);
+    const size_t o_lg = wk.take(sp.mass ? (size_t)n * sp.Hq * sp.l_stride * 4 : 0), o_ln = wk.take(sp.mass ? (size_t)n * sp.Hq * 4 : 0);
+    int rc;
+    if ((rc = check_capture(ctx, "workspace growth", wk.bytes > ctx->work.cap))) return rc;
+    if ((rc = dev_reserve(ctx->work, wk.bytes, ctx->stream))) return rc;
+    unsigned char *w = (unsigned char *)ctx->work.p;
+    sp.p_o = (float *)(w + o_po);
+    sp.p_ml = (float *)(w + o_pml);
+    sp.s_o = (float *)(w + o_so);
+    sp.s_ml = (float *)(w + o_sml);
+    sp.logits = (float *)(w + o_lg);
+    sp.logit_new = (float *)(w + o_ln);
+    sp.seqs_dev = nullptr;
+    if (n <= SH_ARG_SEQS) {
+        memcpy(sp.seqs, seqs.data(), n * sizeof(ShSeq));
+    } else {
+        if ((rc = check_capture(ctx, "a batch's table", true))) return rc;
+        if ((rc = upload_desc(ctx, seqs.data(), n * sizeof(ShSeq)))) return rc;
+        sp.seqs_dev = (const ShSeq *)ctx->desc.p;
+    }
+    const int mk = timing_begin(ctx, 1);
+    rc = smol_launch_shared(&sp, hd, tile, max_len, ctx->stream, mark_a(ctx, mk), mark_b(ctx, mk));
+    if (rc)
+        return fail(rc == -1 ? SMOL_ATTN_ERR_UNSUPPORTED : SMOL_ATTN_ERR_DEVICE, "k_sh launch (hd %d): %s", hd,
+                    rc == -1 ? "unsupported configuration" : hipGetErrorString(hipGetLastError()));
+    return SMOL_ATTN_OK;
+}
+
+/* the arguments that both decode steps share, checked, and their part of the kernel's */
+static int shared_args(smol_attn_ctx *ctx, smol_kv_cache *kv, int layer, const smol_rope_table *rope, int n_seq,
+                       const int *slots, const int *len, const void *q, const void *k_new, const void *v_new, int dtype,
+                       int n_heads, float scale, int window, float cap, const float *q_norm, const float *k_norm, float eps,
+                       float *out, ShParams &sp, int *max_len) {
+    if (!kv) return fail(SMOL_ATTN_ERR_ARG, "cache is NULL");
+    int rc = check_common(ctx, dtype, n_heads, kv->n_kv, kv->hd, q, out);
+    if (rc) return rc;
+    if ((rc = check_norm(q_norm, k_norm, eps, 1))) return rc;
+    if (kv->ctx != ctx) return fail(SMOL_ATTN_ERR_ARG, "cache belongs to another context");
+    if (layer < 0 || layer >= kv->n_layers) return fail(SMOL_ATTN_ERR_ARG, "layer %d out of range", layer);
+    if (n_seq <= 0 || !slots || !len || !k_new || !v_new) return fail(SMOL_ATTN_ERR_ARG, "bad decode batch");
+    if (rope && rope->ctx != ctx) return fail(SMOL_ATTN_ERR_ARG, "rope table belongs to another context");
+    if (rope && rope->hd != kv->hd) return fail(SMOL_ATTN_ERR_ARG, "rope table head_dim %d != %d", rope->hd, kv->hd);
+    if ((rc = check_aligned(k_new, v_new))) return rc;
+    if ((rc = check_slots(kv, n_seq, slots, len, max_len))) return rc;
+    memset(&sp, 0, offsetof(ShParams, seqs));
+    sp.q_in = q; sp.k_in = k_new; sp.v_in = v_new; sp.in_dtype = dtype;
+    sp.q_norm = q_norm; sp.k_norm = k_norm; sp.norm_eps = eps;
+    sp.qscale = (float)(scale * LOG2E_D);
+    sp.out = out; sp.Hq = n_heads;
+    sp.window = window;
+    sp.cap2 = cap > 0.0f ? (float)(cap * LOG2E_D) : 0.0f;
+    return 0;
+}
+
+/* after the table has its final size */
+static void shared_rope(const smol_rope_table *rope, ShParams &sp) {
+    sp.rope_kind = SMOL_ROPE_OFF;
+    if (!rope) return;
+    sp.rope_cos = rope->cos_d;
+    sp.rope_sin = rope->sin_d;
+    sp.rope_kind = rope->type == SMOL_ROPE_INTERLEAVED ? SMOL_ROPE_INTERLEAVED_K : SMOL_ROPE_NEOX_K;
+}
+
+extern "C" int smol_attn_decode_shared(smol_attn_ctx *ctx, const smol_kv_cache *prefix, int prefix_slot, int prefix_len,
+                                       smol_kv_cache *kv, int layer, const smol_rope_table *rope, int n_seq,
+                                       const int *slots, const int *len, const void *q, const void *k_new,
+                                       const void *v_new, int dtype, int n_heads, float scale, int window, float cap,
+                                       const float *q_norm, const float *k_norm, float eps, float *out) {
+    ShParams sp;
+    int max_len = 0;
+    int rc = shared_args(ctx, kv, layer, rope, n_seq, slots, len, q, k_new, v_new, dtype, n_heads, scale, window, cap, q_norm,
+                         k_norm, eps, out, sp, &max_len);
+    if (rc) return rc;
+    if (!prefix) return fail(SMOL_ATTN_ERR_ARG, "prefix cache is NULL");
+    if (prefix->ctx != ctx) return fail(SMOL_ATTN_ERR_ARG, "prefix cache belongs to another context");
+    if (prefix->hd != kv->hd || prefix->n_kv != kv->n_kv)
+        return fail(SMOL_ATTN_ERR_ARG, "prefix cache of %d heads of %d, the sequences' has %d of %d", prefix->n_kv, prefix->hd,
+                    kv->n_kv, kv->hd);
+    if (layer >= prefix->n_layers || prefix_slot < 0 || prefix_slot >= prefix->n_slots)
+        return fail(SMOL_ATTN_ERR_ARG, "prefix layer %d / slot %d out of range", layer, prefix_slot);
+    if (prefix_len < 0 || prefix_len > prefix->cap)
+        return fail(SMOL_ATTN_ERR_ARG, "prefix of %d rows in a cache of %d", prefix_len, prefix->cap);
+    if (max_len > INT_MAX - 64 - prefix_len) return fail(SMOL_ATTN_ERR_ARG, "position %d + %d", prefix_len, max_len);
+    if (prefix == kv)
+        for (int i = 0; i < n_seq; i++)
+            if (slots[i] == prefix_slot) return fail(SMOL_ATTN_ERR_ARG, "slot %d is the prefix's", prefix_slot);
+    if ((rc = reserve_step(ctx, kv, max_len + 1, rope, kv->hd, prefix_len + max_len + 1))) return rc;
+    if ((rc = check_region(kv)) || (rc = check_region(prefix))) return rc;
+    shared_rope(rope, sp);
+    const size_t at = (size_t)layer * kv_layer_elems(prefix) + (size_t)prefix_slot * kv_slot_elems(prefix);
+    sp.pk = prefix->k + at;
+    sp.pvt = prefix->vt + at;
+    sp.pcap = prefix->cap;
+    sp.p_len = prefix_len;
+    std::vector<ShSeq> seqs;
+    seqs.reserve(n_seq);
+    for (int i = 0; i < n_seq; i++) seqs.push_back({slots[i], len[i], prefix_len + len[i], 0});
+    return run_shared(ctx, sp, kv, layer, seqs, max_len);
+}
+
+extern "C" int smol_attn_decode_scored(smol_attn_ctx *ctx, smol_kv_cache *kv, int layer, const smol_rope_table *rope,
+                                       int n_seq, const int *slots, const int *rows, const int *pos, const void *q,
+                                       const void *k_new, const void *v_new, int dtype, int n_heads, float scale, float cap,
+                                       const float *q_norm, const float *k_norm, float eps, float *mass, int *row_pos,
+                                       int stride, float decay, float *out) {
+    ShParams sp;
+    int max_len = 0, max_pos = 0;
+    int rc = shared_args(ctx, kv, layer, rope, n_seq, slots, rows, q, k_new, v_new, dtype, n_heads, scale, 0, cap, q_norm,
+                         k_norm, eps, out, sp, &max_len);
+    if (rc) return rc;
+    if (!pos || !mass || !row_pos) return fail(SMOL_ATTN_ERR_ARG, "NULL tensor");
+    if (((uintptr_t)mass | (uintptr_t)row_pos) & 3) return fail(SMOL_ATTN_ERR_ARG, "mass/row_pos must be 4-byte aligned");
+    if (!(decay >= 0.0f) || decay > FLT_MAX) return fail(SMOL_ATTN_ERR_ARG, "decay %g", (double)decay);
+    if (max_len >= stride) return fail(SMOL_ATTN_ERR_ARG, "row %d in mass rows of %d", max_len, stride);
+    for (int i = 0; i < n_seq; i++) {
+        if (pos[i] < 0 || pos[i] > INT_MAX - 64) return fail(SMOL_ATTN_ERR_ARG, "pos %d", pos[i]);
+        max_pos = std::max(max_pos, pos[i]);
+    }
+    if ((rc = reserve_step(ctx, kv, max_len + 1, rope, kv->hd, max_pos + 1))) return rc;
+    if ((rc = check_region(kv))) return rc;
+    shared_rope(rope, sp);
+    sp.mass = mass;
+    sp.row_pos = row_pos;
+    sp.m_stride = stride;
+    sp.decay = decay;
+    std::vector<ShSeq> seqs;
+    seqs.reserve(n_seq);
+    for (int i = 0; i < n_seq; i++) seqs.push_back({slots[i], rows[i], pos[i], 0});
+    return run_shared(ctx, sp, kv, layer, seqs, max_len);
+}
+
+extern "C" int smol_kv_cache_evict(smol_kv_cache *kv, int layer, int n_seq, const int *slots, const int *rows,
+                                   const int *ends, const float *mass, const int *row_pos, float *mass_out, int *pos_out,
+                                   int stride, int keep, int first, int recent) {
+    if (!kv) return fail(SMOL_ATTN_ERR_ARG, "cache is NULL");
+    smol_attn_ctx *ctx = kv->ctx;
+    if (layer < 0 || layer >= kv->n_layers) return fail(SMOL_ATTN_ERR_ARG, "layer %d out of range", layer);
+    if (n_seq <= 0 || !slots || !rows || !ends) return fail(SMOL_ATTN_ERR_ARG, "bad batch");
+    if (!mass || !row_pos || !mass_out || !pos_out) return fail(SMOL_ATTN_ERR_ARG, "NULL tensor");
+    if (((uintptr_t)mass | (uintptr_t)row_pos | (uintptr_t)mass_out | (uintptr_t)pos_out) & 3)
+        return fail(SMOL_ATTN_ERR_ARG, "mass/row_pos must be 4-byte aligned");
+    if (keep <= 0 || first < 0 || recent < 0 || first > keep - recent)
+        return fail(SMOL_ATTN_ERR_ARG, "keep %d of them the first %d and the last %d", keep, first, recent);
+    int max_rows = 0;
+    int rc = check_slots(kv, n_seq, slots, rows, &max_rows);
+    if (rc) return rc;
+    if (max_rows > kv->cap || max_rows > stride)
+        return fail(SMOL_ATTN_ERR_ARG, "%d rows in a cache of %d, mass rows of %d", max_rows, kv->cap, stride);
+    for (int i = 0; i < n_seq; i++)
+        if (ends[i] < 0) return fail(SMOL_ATTN_ERR_ARG, "end %d", ends[i]);
+    /* in place, or apart: a partial overlap, or one array apart and the other not, is refused */
+    const size_t bytes = (size_t)kv->n_slots * kv->n_kv * stride * 4;
+    auto overlap = [bytes](const void *a, const void *b) {
+        return (const char *)a < (const char *)b + bytes && (const char *)b < (const char *)a + bytes;
+    };
+    const bool in_place = mass_out == mass && pos_out == row_pos;
+    if (overlap(mass, row_pos) || overlap(mass_out, pos_out) || overlap(mass, pos_out) || overlap(row_pos, mass_out) ||
+        (!in_place && (overlap(mass, mass_out) || overlap(row_pos, pos_out))))
+        return fail(SMOL_ATTN_ERR_ARG, "overlapping arrays (mass_out and pos_out may both be the inputs)");
+    const long long pairs = (long long)n_seq * kv->n_kv;
+    const int max_moves = max_rows > keep ? std::min(keep, max_rows - keep) : 0;
+    if (pairs * ((max_moves + 31) / 32 + 1) > INT_MAX / 2) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "batch too large");
+    if ((rc = set_device(ctx))) return rc;
+    EvictParams ep;
+    memset(&ep, 0, offsetof(EvictParams, seqs));
+    ep.kc = kv->k + (size_t)layer * kv_layer_elems(kv);
+    ep.vtc = kv->vt + (size_t)layer * kv_layer_elems(kv);
+    ep.c_slot_stride = (long long)kv_slot_elems(kv);
+    ep.cap = kv->cap;
+    ep.hd = kv->hd;
+    ep.Hkv = kv->n_kv;
+    ep.mass = mass; ep.row_pos = row_pos; ep.mass_out = mass_out; ep.pos_out = pos_out; ep.m_stride = stride;
+    ep.keep = keep; ep.first = first; ep.recent = recent;
+    ep.max_moves = max_moves;
+    ep.n_seq = n_seq;
+    WorkPlan wk;
+    const size_t o_mv = wk.take((size_t)pairs * 2 * max_moves * 4), o_n = wk.take((size_t)pairs * 4);
+    if ((rc = check_capture(ctx, "workspace growth", wk.bytes > ctx->work.cap))) return rc;
+    if ((rc = dev_reserve(ctx->work, wk.bytes, ctx->stream))) return rc;
+    ep.moves = (int *)((unsigned char *)ctx->work.p + o_mv);
+    ep.n_moves = (int *)((unsigned char *)ctx->work.p + o_n);
+    std::vector<ShSeq> seqs;
+    seqs.reserve(n_seq);
+    for (int i = 0; i < n_seq; i++) seqs.push_back({slots[i], rows[i], ends[i], 0});
+    if (n_seq <= SH_ARG_SEQS) {
+        memcpy(ep.seqs, seqs.data(), n_seq * sizeof(ShSeq));
+    } else {
+        if ((rc = check_capture(ctx, "a batch's table", true))) return rc;
+        if ((rc = upload_desc(ctx, seqs.data(), n_seq * sizeof(ShSeq)))) return rc;
+        ep.seqs_dev = (const ShSeq *)ctx->desc.p;
+    }
+    const int mk = timing_begin(ctx, 2);
+    rc = smol_launch_evict(&ep, max_rows, ctx->stream, mark_a(ctx, mk), mark_b(ctx, mk));
+    if (rc) return fail(SMOL_ATTN_ERR_DEVICE, "cache eviction: %s", hipGetErrorString(hipGetLastError()));
+    return SMOL_ATTN_OK;
+}
+
+extern "C" int smol_kv_cache_pointers(const smol_kv_cache *kv, int layer, void **k, void **vt) {
+    if (!kv || !k || !vt) return fail(SMOL_ATTN_ERR_ARG, "NULL argument");
+    if (layer < 0 || layer >= kv->n_layers) return fail(SMOL_ATTN_ERR_ARG, "layer %d out of range", layer);
+    *k = kv->k + (size_t)layer * kv_layer_elems(kv);
+    *vt = kv->vt + (size_t)layer * kv_layer_elems(kv);
+    return SMOL_ATTN_OK;
 }
 
 extern "C" int smol_attn_causal(smol_attn_ctx *ctx, const void *q, const void *k, const void *v,

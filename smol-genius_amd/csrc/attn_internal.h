@@ -275,6 +275,53 @@ typedef struct {
     DecItem items[DEC_ARG_ITEMS];
 } DecParams;
 
+/* ---- k_sh, k_sh_merge (attn_shared.hip): a decode step on a shared prefix, or with the rows' weights ---- */
+#define SH_ARG_SEQS 128   /* sequences passed in the kernel arguments */
+#define SH_MAX_SPLIT 64   /* chunks of the prefix, and of one sequence's own rows, at most */
+typedef struct {
+    int slot;      /* cache slot of the sequence's own rows */
+    int len;       /* own rows in the cache: the new token becomes row len */
+    int pos;       /* position of the new token (RoPE row, window) */
+    int pad;
+} ShSeq;
+
+typedef struct {
+    const uint16_t *pk; const uint16_t *pvt; int pcap; int p_len; /* the prefix slot's layer: K, V^T [kv][pcap rows] */
+    uint16_t *kc; uint16_t *vtc; long long c_slot_stride; int cap; /* the layer's own rows, at slot 0 */
+    const void *q_in; const void *k_in; const void *v_in; int in_dtype;
+    const float *rope_cos; const float *rope_sin; int rope_kind;
+    const float *q_norm; const float *k_norm; float norm_eps;
+    float qscale;              /* scale * log2 e */
+    float *out; int Hq, Hkv, G;
+    int window; float cap2;    /* window > 0: positions > pos - window; cap2 > 0: softcap in log2 units */
+    /* the items: n_pblocks workgroups of (prefix chunk, row block, kv head), then (chunk, sequence, kv head, 16 heads) */
+    int n_pblocks, n_rb, n_ps, p_chunk, n_ss, s_chunk, s_rb;
+    int p_first;               /* the prefix chunks' first key (a window leaves out what lies before), a slab's start */
+    float *p_o; float *p_ml;   /* [prefix chunk][kv][n_seq G] outputs [hd] and (m, l) */
+    float *s_o; float *s_ml;   /* [sequence][kv][own chunk][G] */
+    /* mass non-null: the capped scores (log2 units) [sequence][Hq][l_stride], the new token's [sequence][Hq], and what
+     * they are added to: [slot][kv][m_stride] */
+    float *logits; float *logit_new; long long l_stride;
+    float *mass; int *row_pos; int m_stride; float decay;
+    int n_seq;
+    const ShSeq *seqs_dev;     /* the sequences when n_seq > SH_ARG_SEQS */
+    ShSeq seqs[SH_ARG_SEQS];
+} ShParams;
+
+/* ---- k_evict_select, k_evict_move (attn_evict.hip) ---- */
+typedef struct {
+    uint16_t *kc; uint16_t *vtc; long long c_slot_stride; int cap; /* the layer, at slot 0 */
+    int hd, Hkv;
+    const float *mass; const int *row_pos; float *mass_out; int *pos_out; int m_stride; /* [slot][kv][m_stride] */
+    int keep, first, recent;
+    int *moves;                /* [pair][2 max_moves]: holes, then the rows that fill them */
+    int *n_moves;              /* [pair] */
+    int max_moves;
+    int n_seq;
+    const ShSeq *seqs_dev;     /* (slot, rows, end) of each sequence when n_seq > SH_ARG_SEQS */
+    ShSeq seqs[SH_ARG_SEQS];
+} EvictParams;
+
 /* ---- k_gemm (gemm.hip), k_gemm_rs (gemm_rs.hip) and k_gemm_sw (gemm_sw.hip): the projections on bf16 MFMA ---- */
 #define GEMM_CFGS 8 /* their tile configurations (smol_gemm_tile) */
 struct GemmParams {

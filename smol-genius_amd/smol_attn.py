@@ -71,6 +71,14 @@ SIGNATURES = [
                                  _c_float, _c_int, _c_float, _vp, _vp, _c_float, _vp], _c_int),
     ("smol_attn_decode_noalloc", [_vp, _vp, _c_int, _vp, _c_int, _IP, _IP, _vp, _vp, _vp, _c_int, _c_int,
                                   _c_float, _c_int, _c_float, _vp, _vp, _c_float, _vp], _c_int),
+    # a batch on a shared prefix; a cache held to a budget
+    ("smol_attn_decode_shared", [_vp, _vp, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _IP, _IP, _vp, _vp, _vp, _c_int,
+                                 _c_int, _c_float, _c_int, _c_float, _vp, _vp, _c_float, _vp], _c_int),
+    ("smol_attn_decode_scored", [_vp, _vp, _c_int, _vp, _c_int, _IP, _IP, _IP, _vp, _vp, _vp, _c_int, _c_int, _c_float,
+                                 _c_float, _vp, _vp, _c_float, _vp, _vp, _c_int, _c_float, _vp], _c_int),
+    ("smol_kv_cache_evict", [_vp, _c_int, _c_int, _IP, _IP, _IP, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int],
+     _c_int),
+    ("smol_kv_cache_pointers", [_vp, _c_int, ctypes.POINTER(_vp), ctypes.POINTER(_vp)], _c_int),
     ("smol_attn_apply_rope", [_vp, _vp, _vp, _IP, _c_int, _c_int], _c_int),
     ("smol_attn_norm_rope", [_vp, _vp, _vp, _vp, _c_float, _IP, _c_int, _c_int, _c_int], _c_int),
     ("smol_attn_norm_rope_bf16", [_vp, _vp, _vp, _vp, _c_float, _c_int, _c_int, _c_int, _c_int], _c_int),
@@ -291,6 +299,14 @@ def rope_fill_host(pos0, n_pos, head_dim, theta, rope_type=ROPE_NEOX):
     return c, s
 
 
+class _DeviceMemory:
+    """16-bit device memory of a handle, in the form that torch.as_tensor takes"""
+
+    def __init__(self, owner, ptr, shape):
+        self.owner = owner
+        self.__cuda_array_interface__ = dict(shape=shape, typestr="<i2", data=(ptr, False), version=2)
+
+
 class KVCache:
     """Device bf16 KV cache: layers x slots x kv_heads x capacity x head_dim."""
 
@@ -331,6 +347,20 @@ class KVCache:
         _check(load().smol_kv_cache_read(self.h, layer, slot, pos0, n, k.ctypes.data_as(_U16P),
                                          v.ctypes.data_as(_U16P)), "smol_kv_cache_read")
         return k, v
+
+    def views(self, layer):
+        """One layer's rows as torch views of the cache's own memory (bf16): K [slots, kv_heads, capacity, head_dim] and
+        V^T [slots, kv_heads, capacity / 32, head_dim, 32]. Valid until the cache grows or closes; work on them
+        is ordered with the context's stream by the caller."""
+        import torch
+        k, vt = _vp(), _vp()
+        _check(load().smol_kv_cache_pointers(self.h, layer, ctypes.byref(k), ctypes.byref(vt)), "smol_kv_cache_pointers")
+        ns, nk, cap, hd = self.n_slots, self.n_kv_heads, self.capacity, self.head_dim
+
+        def view(p, shape):
+            mem = _DeviceMemory(self, p.value, shape)
+            return torch.as_tensor(mem, device="cuda:%d" % self.ctx.device).view(torch.bfloat16)
+        return view(k, (ns, nk, cap, hd)), view(vt, (ns, nk, cap // 32, hd, 32))
 
     def close(self):
         if self.h:
@@ -423,6 +453,95 @@ def decode(ctx, kv, layer, rope, slots, pos, q, k_new, v_new, n_heads, scale, wi
     (device float32 [head_dim]) select smol_attn_decode_qknorm."""
     return decode_call(ctx, kv, layer, rope, slots, pos, q, k_new, v_new, n_heads, scale, window, cap, out,
                        q_norm, k_norm, eps)()
+
+
+def _on(ctx, t, dtypes, shape, what):
+    """the address of a contiguous tensor of these dtypes and this shape on the context's device"""
+    if not t.is_cuda or t.device.index != ctx.device or not t.is_contiguous():
+        raise SmolAttnError("%s must be a contiguous tensor on device %d" % (what, ctx.device))
+    if t.dtype not in dtypes:
+        raise SmolAttnError("%s is %s" % (what, t.dtype))
+    if tuple(t.shape) != tuple(shape):
+        raise SmolAttnError("%s has shape %s, not %s" % (what, tuple(t.shape), tuple(shape)))
+    return t.data_ptr()
+
+
+def _host_ints(a, n, what):
+    a = np.ascontiguousarray(a, np.int32)
+    if a.shape != (n,):
+        raise SmolAttnError("%s: %d numbers are wanted, got shape %s" % (what, n, a.shape))
+    return a, a.ctypes.data_as(_IP)
+
+
+def _step_args(ctx, kv, q, k_new, v_new, n_heads, q_norm, k_norm, out):
+    """what the two decode steps below share: addresses of q, k, v, the norms and out, and the dtype code"""
+    import torch
+    n, hd, kvd = q.shape[0], kv.head_dim, kv.n_kv_heads * kv.head_dim
+    dt = _dtype_code(q)
+    ptrs = [_on(ctx, q, (q.dtype,), (n, n_heads * hd), "q")]
+    ptrs += [_on(ctx, t, (q.dtype,), (n, kvd), nm) for t, nm in ((k_new, "k_new"), (v_new, "v_new"))]
+    norms = [None if w is None else _on(ctx, w, (torch.float32,), (hd,), nm)
+             for w, nm in ((q_norm, "q_norm"), (k_norm, "k_norm"))]
+    if out is None:
+        out = torch.empty((n, n_heads * hd), dtype=torch.float32, device=q.device)
+    return n, ptrs, dt, norms, out, _on(ctx, out, (torch.float32,), (n, n_heads * hd), "out")
+
+
+def decode_shared(ctx, prefix, prefix_slot, prefix_len, kv, layer, rope, slots, lens, q, k_new, v_new, n_heads, scale,
+                  window=0, cap=0.0, out=None, q_norm=None, k_norm=None, eps=1e-6):
+    """One decode step of sequences that share the first prefix_len positions, rows of `prefix` at prefix_slot; see
+    smol_attn_decode_shared. lens: each sequence's own rows in `kv` before the step. Returns out [n, n_heads*hd]."""
+    n, ptrs, dt, norms, out, optr = _step_args(ctx, kv, q, k_new, v_new, n_heads, q_norm, k_norm, out)
+    sl, slp = _host_ints(slots, n, "slots")
+    le, lep = _host_ints(lens, n, "lens")
+    _check(load().smol_attn_decode_shared(ctx.h, prefix.h, prefix_slot, prefix_len, kv.h, layer, rope.h if rope else None, n,
+                                          slp, lep, *ptrs, dt, n_heads, scale, window, cap, *norms, eps, optr),
+           "smol_attn_decode_shared")
+    return out
+
+
+def _score_arrays(ctx, kv, mass, row_pos):
+    import torch
+    if mass.dim() != 3:
+        raise SmolAttnError("mass must be [slots, kv_heads, stride]")
+    shape = (kv.n_slots, kv.n_kv_heads, mass.shape[2])
+    return _on(ctx, mass, (torch.float32,), shape, "mass"), _on(ctx, row_pos, (torch.int32,), shape, "row_pos"), shape[2]
+
+
+def decode_scored(ctx, kv, layer, rope, slots, rows, pos, q, k_new, v_new, n_heads, scale, mass, row_pos, decay=1.0,
+                  cap=0.0, out=None, q_norm=None, k_norm=None, eps=1e-6):
+    """One decode step that also adds each row's weight to mass [slots, kv_heads, stride] (float32) and notes the new
+    row's position in row_pos (int32, same shape); see smol_attn_decode_scored. rows: rows in use, pos: the new
+    tokens' positions. Returns out [n, n_heads*hd]."""
+    n, ptrs, dt, norms, out, optr = _step_args(ctx, kv, q, k_new, v_new, n_heads, q_norm, k_norm, out)
+    sl, slp = _host_ints(slots, n, "slots")
+    ro, rop = _host_ints(rows, n, "rows")
+    po, pop = _host_ints(pos, n, "pos")
+    mp, rp, stride = _score_arrays(ctx, kv, mass, row_pos)
+    _check(load().smol_attn_decode_scored(ctx.h, kv.h, layer, rope.h if rope else None, n, slp, rop, pop, *ptrs, dt, n_heads,
+                                          scale, cap, *norms, eps, mp, rp, stride, decay, optr), "smol_attn_decode_scored")
+    return out
+
+
+def kv_evict(kv, layer, slots, rows, ends, mass, row_pos, keep, first=0, recent=0, mass_out=None, pos_out=None):
+    """Keeps `keep` of the rows of each slot, by position and mass; see smol_kv_cache_evict. mass and row_pos are
+    updated in place unless mass_out and pos_out (both) are given. Returns them."""
+    ctx = kv.ctx
+    if (mass_out is None) != (pos_out is None):
+        raise SmolAttnError("mass_out and pos_out are given together")
+    if mass_out is None:
+        mass_out, pos_out = mass, row_pos
+    n = len(slots)
+    sl, slp = _host_ints(slots, n, "slots")
+    ro, rop = _host_ints(rows, n, "rows")
+    en, enp = _host_ints(ends, n, "ends")
+    mp, rp, stride = _score_arrays(ctx, kv, mass, row_pos)
+    mo, po, stride_out = _score_arrays(ctx, kv, mass_out, pos_out)
+    if stride != stride_out:
+        raise SmolAttnError("mass_out has another stride than mass")
+    _check(load().smol_kv_cache_evict(kv.h, layer, n, slp, rop, enp, mp, rp, mo, po, stride, keep, first, recent),
+           "smol_kv_cache_evict")
+    return mass_out, pos_out
 
 
 def causal(ctx, q, k, v, seq_q, seq_k, n_heads, n_kv_heads, head_dim, scale, q_offset, window=0, cap=0.0,
