@@ -57,6 +57,35 @@ SMOL_ATTN_API int smol_linear_qkv_dev(smol_attn_ctx *ctx, void *q, void *k, void
                                       int x_dtype, const uint16_t *wq, const uint16_t *wk, const uint16_t *wv,
                                       int seq, int in_dim, int q_dim, int kv_dim);
 
+/* ---- a low-rank adapter for every row ------------------------------------
+ *
+ * No counterpart in the reference, which serves one model to one caller. A
+ * set holds n adapters of one projection in_dim -> out_dim: adapter i is
+ * scale[i] * B_i A_i with a[i] [rank[i]][in_dim] and b[i] [out_dim][rank[i]]
+ * (device bf16, row-major; 1 <= rank <= 128). Creation copies the weights
+ * into the set's own layout and waits for the copy: later changes to a[i] or
+ * b[i] do not reach it. */
+typedef struct smol_adapters smol_adapters;
+SMOL_ATTN_API int smol_adapters_create(smol_attn_ctx *ctx, int n, int in_dim, int out_dim, const uint16_t *const *a,
+                                       const uint16_t *const *b, const int *rank, const float *scale,
+                                       smol_adapters **out);
+/* waits for the context's stream, then frees the set (before its context) */
+SMOL_ATTN_API int smol_adapters_destroy(smol_adapters *set);
+
+/* y[s] = W x[s] (+ bias) + scale_a B_a (A_a x[s]) with a = ids[s], or without
+ * the last term where ids[s] is -1: smol_linear_dev with an adapter a row.
+ * ids: host array [seq]; rows of one adapter need not follow each other. The
+ * shared product has smol_linear_dev's precision; A_a x and B_a (A_a x) are
+ * fp32 sums of fp32 inputs (24 bits) and the exact bf16 weights, and a bf16 y is
+ * truncated once, from the whole sum. y (16-byte aligned) overlaps neither x
+ * nor W. Uses the context's workspace. Under stream capture the call must
+ * have been made once before, with at most 40 groups of 16 rows that share an
+ * adapter (SMOL_ATTN_ERR_UNSUPPORTED otherwise); the captured call keeps its
+ * ids. */
+SMOL_ATTN_API int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype, const void *x, int x_dtype,
+                                           const uint16_t *w, const float *bias, int seq, int in_dim, int out_dim,
+                                           const smol_adapters *set, const int *ids);
+
 /* ---- a decoder layer's operations around its projections ----------------
  *
  * The decoders wrap their projections in an RMSNorm of the input, a gated

@@ -1,0 +1,423 @@
+/*
+ * adapters.hip - a shared bf16 projection with a low-rank adapter of its own
+ * for every row (smol_linear_adapters_dev): for row s with adapter a,
+ *     y_s = W x_s + bias + scale_a B_a (A_a x_s),   A_a [rank][in], B_a [out][rank].
+ *
+ * The shared product is the library's own (linear.hip). The low-rank part is
+ * two thin products over tiles of 16 rows that share an adapter (the host
+ * sorts the rows; the rows of a tile need not follow each other):
+ *   k_adapt_in   t^T = A x^T, the in_dim cut into chunks so that few tiles still
+ *                fill the device; each chunk writes its own partial t, so the
+ *                sum's order is fixed;
+ *   k_adapt_out  adds scale B t to y: the chunks' t are summed as they are read.
+ * Both run on v_mfma_f32_16x16x32_bf16 with the weights as the A operand, so a
+ * lane holds four consecutive ranks (outputs) of one row and stores them
+ * together. An fp32 x and t are split into three bf16 parts (24 bits), so the
+ * low-rank part is as exact as an fp32 product of the bf16 weights.
+ *
+ * The weights of a set are packed once, at its creation: ranks padded with
+ * zeros to the matrix instruction's sizes, so no load needs a bound.
+ */
+#include "attn_device.h"
+
+#include <limits.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "../../include/smol_linear.h"
+
+extern "C" int smol_internal_fail(int code, const char *msg);
+extern "C" int smol_internal_ctx_device(smol_attn_ctx *ctx);
+extern "C" int smol_internal_ctx_cus(smol_attn_ctx *ctx);
+extern "C" void smol_internal_timing_events(smol_attn_ctx *ctx, int kind, hipEvent_t *a, hipEvent_t *b);
+extern "C" int smol_internal_work(smol_attn_ctx *ctx, size_t bytes, void **p);
+extern "C" int smol_internal_upload(smol_attn_ctx *ctx, const void *host, size_t bytes, const void **dev);
+
+namespace {
+
+constexpr int AD_MAX_RANK = 128;
+constexpr int AD_TPB = 256, AD_NW = AD_TPB / 64;
+constexpr int AD_ARG_TILES = 40;
+constexpr int AD_TIMING_KIND = 2;
+
+struct AdTile {
+    int adapter, n;
+    int row[16]; /* rows past n repeat the first */
+};
+
+struct AdParams {
+    const void *x; int x_bf16; int vec;
+    int in_dim, out_dim, seq;
+    const uint16_t *a; int ra, kp;   /* [adapter][ra][kp] */
+    const uint16_t *b; int np, rp;   /* [adapter][np][rp] */
+    const float *scale; const int *rank; /* [adapter] */
+    float *t; int n_tiles, n_chunks, chunk; /* [chunk][tile][16][ra]; chunk: 32-wide steps of in_dim */
+    const float *base;               /* fp32 [seq][out] that the low-rank part is added to */
+    void *y; int y_bf16;             /* fp32 y is base itself */
+    const AdTile *tiles_dev;
+    AdTile tiles[AD_ARG_TILES];
+};
+
+__device__ __forceinline__ void ad_split3(const float *x, b8 &p0, b8 &p1, b8 &p2) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const __bf16 a = (__bf16)x[i];
+        const float r = x[i] - (float)a;
+        const __bf16 b = (__bf16)r;
+        p0[i] = a;
+        p1[i] = b;
+        p2[i] = (__bf16)(r - (float)b);
+    }
+}
+
+/* NT: rank tiles of 16 that the accumulators hold */
+template <int NT, bool XBF>
+__global__ __launch_bounds__(AD_TPB) void k_adapt_in(const AdParams p) {
+    __shared__ __attribute__((aligned(16))) float s_t[AD_NW * 16 * NT * 16];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tile = blockIdx.x % p.n_tiles, chunk = blockIdx.x / p.n_tiles;
+    const AdTile *tl = (p.tiles_dev ? p.tiles_dev : p.tiles) + tile;
+    const int ad = tl->adapter, nt = (p.rank[ad] + 15) / 16;
+    const long long row = tl->row[c];
+    const uint16_t *a = p.a + ((long long)ad * p.ra + c) * p.kp + 8 * j;
+    f4 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
+    const int s1 = min((chunk + 1) * p.chunk, p.kp / 32);
+    for (int s = chunk * p.chunk + wave; s < s1; s += AD_NW) {
+        const int k0 = 32 * s + 8 * j;
+        b8 xp[XBF ? 1 : 3];
+        if constexpr (XBF) {
+            const uint16_t *x = (const uint16_t *)p.x + row * p.in_dim + k0;
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (p.vec) {
+                if (k0 < p.in_dim) w = *reinterpret_cast<const uint4 *>(x);
+            } else {
+                uint32_t v[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = k0 + i < p.in_dim ? x[i] : 0u;
+                w = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+            }
+            xp[0] = as_b8(w);
+        } else {
+            const float *x = (const float *)p.x + row * p.in_dim + k0;
+            float v[8];
+            if (p.vec) {
+                /* in_dim is a multiple of 8 */
+                const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 u = k0 < p.in_dim ? *reinterpret_cast<const float4 *>(x) : z;
+                const float4 w = k0 < p.in_dim ? *reinterpret_cast<const float4 *>(x + 4) : z;
+                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w; v[4] = w.x; v[5] = w.y; v[6] = w.z; v[7] = w.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = k0 + i < p.in_dim ? x[i] : 0.0f;
+            }
+            ad_split3(v, xp[0], xp[1], xp[2]);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (t >= nt) break;
+            const b8 w = as_b8(*reinterpret_cast<const uint4 *>(a + (long long)t * 16 * p.kp + 32 * s));
+#pragma unroll
+            for (int q = XBF ? 0 : 2; q >= 0; q--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xp[q], acc[t], 0, 0, 0);
+        }
+    }
+    /* lane (c, j): ranks 16 t + 4 j .. + 3 of row c */
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+        *reinterpret_cast<f4 *>(s_t + ((wave * 16 + c) * NT + t) * 16 + 4 * j) = acc[t];
+    __syncthreads();
+    float *out = p.t + ((long long)chunk * p.n_tiles + tile) * 16 * p.ra;
+    for (int e = tid; e < 16 * nt * 4; e += AD_TPB) {
+        const int r = e / (nt * 4), q = e - r * nt * 4;
+        f4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < AD_NW; w++) sum += *reinterpret_cast<f4 *>(s_t + ((w * 16 + r) * NT) * 16 + 4 * q);
+        *reinterpret_cast<f4 *>(out + r * p.ra + 4 * q) = sum;
+    }
+}
+
+constexpr int AD_OUT = 64; /* outputs of a k_adapt_out wave */
+
+/* KS: 32-wide steps over the rank */
+template <int KS>
+__global__ __launch_bounds__(AD_TPB) void k_adapt_out(const AdParams p) {
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tile = blockIdx.x % p.n_tiles, o0 = (blockIdx.x / p.n_tiles * AD_NW + wave) * AD_OUT;
+    if (o0 >= p.out_dim) return;
+    const AdTile *tl = (p.tiles_dev ? p.tiles_dev : p.tiles) + tile;
+    const int ad = tl->adapter, rank = p.rank[ad];
+    const float scale = p.scale[ad];
+    const long long row = tl->row[c];
+    const bool live = c < tl->n;
+    b8 tp[KS][3];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+        const int r = 32 * ks + 8 * j;
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        /* k_adapt_in writes whole tiles of 16 ranks */
+        if (r < ((rank + 15) & ~15)) {
+            const float *t = p.t + (long long)tile * 16 * p.ra + c * p.ra + r;
+            for (int q = 0; q < p.n_chunks; q++, t += (long long)p.n_tiles * 16 * p.ra) {
+                const float4 x = *reinterpret_cast<const float4 *>(t), z = *reinterpret_cast<const float4 *>(t + 4);
+                v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += z.x; v[5] += z.y; v[6] += z.z; v[7] += z.w;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= scale;
+        ad_split3(v, tp[ks][0], tp[ks][1], tp[ks][2]);
+    }
+    const uint16_t *b = p.b + ((long long)ad * p.np + o0 + c) * p.rp + 8 * j;
+#pragma unroll
+    for (int u = 0; u < AD_OUT / 16; u++) {
+        const int o = o0 + 16 * u + 4 * j;
+        if (o0 + 16 * u >= p.out_dim) break;
+        f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            if (32 * ks >= rank) break;
+            const b8 w = as_b8(*reinterpret_cast<const uint4 *>(b + (long long)16 * u * p.rp + 32 * ks));
+#pragma unroll
+            for (int q = 2; q >= 0; q--) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, tp[ks][q], acc, 0, 0, 0);
+        }
+        if (!live) continue;
+        const long long at = row * p.out_dim + o;
+        if (!p.y_bf16 && (p.out_dim & 3) == 0 && o < p.out_dim) {
+            f4 *y = reinterpret_cast<f4 *>((float *)p.y + at);
+            *y = *reinterpret_cast<const f4 *>(p.base + at) + acc;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (o + i < p.out_dim) {
+                    const float v = p.base[at + i] + acc[i];
+                    if (p.y_bf16) ((uint16_t *)p.y)[at + i] = (uint16_t)(__float_as_uint(v) >> 16);
+                    else ((float *)p.y)[at + i] = v;
+                }
+        }
+    }
+}
+
+/* rows without an adapter, bf16 y: the shared product alone, truncated */
+__global__ __launch_bounds__(256) void k_adapt_bare(uint16_t *y, const float *base, long long n) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) y[i] = (uint16_t)(__float_as_uint(base[i]) >> 16);
+}
+
+/* dst [rows][stride] = src [rows][cols], zeros behind; rows past src_rows are zeros */
+__global__ __launch_bounds__(256) void k_adapt_pack(uint16_t *dst, const uint16_t *src, int rows, int stride, int src_rows,
+                                                    int cols) {
+    const long long n = (long long)rows * stride;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const int r = (int)(i / stride), q = (int)(i - (long long)r * stride);
+        dst[i] = r < src_rows && q < cols ? src[(long long)r * cols + q] : (uint16_t)0;
+    }
+}
+
+int afail(int code, const char *msg) { return smol_internal_fail(code, msg); }
+
+#define AHIP(expr)                                                                          \
+    do {                                                                                    \
+        hipError_t e_ = (expr);                                                             \
+        if (e_ != hipSuccess) return afail(SMOL_ATTN_ERR_DEVICE, hipGetErrorString(e_));    \
+    } while (0)
+
+} // namespace
+
+struct smol_adapters {
+    smol_attn_ctx *ctx;
+    int device;
+    hipStream_t stream;
+    int n, in_dim, out_dim, max_rank, ra, rp, kp, np;
+    void *mem = nullptr;
+    uint16_t *a, *b;
+    float *scale;
+    int *rank;
+};
+
+extern "C" int smol_adapters_destroy(smol_adapters *s) {
+    if (!s) return SMOL_ATTN_OK;
+    hipSetDevice(s->device);
+    hipStreamSynchronize(s->stream);
+    if (s->mem) hipFree(s->mem);
+    delete s;
+    return SMOL_ATTN_OK;
+}
+
+extern "C" int smol_adapters_create(smol_attn_ctx *ctx, int n, int in_dim, int out_dim, const uint16_t *const *a,
+                                    const uint16_t *const *b, const int *rank, const float *scale, smol_adapters **out) {
+    if (!ctx || !out) return afail(SMOL_ATTN_ERR_ARG, "smol_adapters_create: null context or result");
+    *out = nullptr;
+    if (n <= 0 || in_dim <= 0 || out_dim <= 0 || !a || !b || !rank || !scale)
+        return afail(SMOL_ATTN_ERR_ARG, "smol_adapters_create: sizes or null arrays");
+    int max_rank = 0;
+    for (int i = 0; i < n; i++) {
+        if (rank[i] < 1 || rank[i] > AD_MAX_RANK) return afail(SMOL_ATTN_ERR_UNSUPPORTED, "smol_adapters_create: a rank outside 1 .. 128");
+        if (!a[i] || !b[i]) return afail(SMOL_ATTN_ERR_ARG, "smol_adapters_create: null weights");
+        max_rank = std::max(max_rank, rank[i]);
+    }
+    AHIP(hipSetDevice(smol_internal_ctx_device(ctx)));
+    smol_adapters *s = new smol_adapters();
+    s->ctx = ctx;
+    s->device = smol_internal_ctx_device(ctx);
+    s->stream = static_cast<hipStream_t>(smol_attn_ctx_stream(ctx));
+    s->n = n;
+    s->in_dim = in_dim;
+    s->out_dim = out_dim;
+    s->max_rank = max_rank;
+    s->ra = (max_rank + 15) & ~15;
+    s->rp = (max_rank + 31) & ~31;
+    s->kp = (int)(((long long)in_dim + 31) & ~31LL);
+    s->np = (int)(((long long)out_dim + AD_OUT - 1) / AD_OUT * AD_OUT);
+    const size_t ab = ((size_t)n * s->ra * s->kp * 2 + 255) & ~(size_t)255, bb = ((size_t)n * s->np * s->rp * 2 + 255) & ~(size_t)255;
+    const size_t sb = ((size_t)n * 4 + 255) & ~(size_t)255;
+    hipError_t e = hipMalloc(&s->mem, ab + bb + 2 * sb);
+    if (e != hipSuccess) {
+        delete s;
+        hipGetLastError();
+        return afail(e == hipErrorOutOfMemory ? SMOL_ATTN_ERR_NOMEM : SMOL_ATTN_ERR_DEVICE, "smol_adapters_create: device memory");
+    }
+    s->a = static_cast<uint16_t *>(s->mem);
+    s->b = reinterpret_cast<uint16_t *>(static_cast<char *>(s->mem) + ab);
+    s->scale = reinterpret_cast<float *>(static_cast<char *>(s->mem) + ab + bb);
+    s->rank = reinterpret_cast<int *>(static_cast<char *>(s->mem) + ab + bb + sb);
+    for (int i = 0; i < n && e == hipSuccess; i++) {
+        auto pack = [&](uint16_t *dst, const uint16_t *src, int rows, int stride, int src_rows, int cols) {
+            const long long blocks = std::min<long long>(((long long)rows * stride + 255) / 256, 4096);
+            hipLaunchKernelGGL(k_adapt_pack, dim3((unsigned)blocks), dim3(256), 0, s->stream, dst, src, rows, stride, src_rows, cols);
+        };
+        pack(s->a + (size_t)i * s->ra * s->kp, a[i], s->ra, s->kp, rank[i], in_dim);
+        pack(s->b + (size_t)i * s->np * s->rp, b[i], s->np, s->rp, out_dim, rank[i]);
+        e = hipGetLastError();
+    }
+    /* pageable host memory: the copies return when they have been made */
+    if (e == hipSuccess) e = hipMemcpyAsync(s->scale, scale, (size_t)n * 4, hipMemcpyHostToDevice, s->stream);
+    if (e == hipSuccess) e = hipMemcpyAsync(s->rank, rank, (size_t)n * 4, hipMemcpyHostToDevice, s->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(s->stream);
+    if (e != hipSuccess) {
+        smol_adapters_destroy(s);
+        return afail(SMOL_ATTN_ERR_DEVICE, hipGetErrorString(e));
+    }
+    *out = s;
+    return SMOL_ATTN_OK;
+}
+
+template <int NT>
+static void launch_in(const AdParams &p, unsigned blocks, hipStream_t st) {
+    if (p.x_bf16) hipLaunchKernelGGL((k_adapt_in<NT, true>), dim3(blocks), dim3(AD_TPB), 0, st, p);
+    else hipLaunchKernelGGL((k_adapt_in<NT, false>), dim3(blocks), dim3(AD_TPB), 0, st, p);
+}
+
+extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype, const void *x, int x_dtype, const uint16_t *w,
+                                        const float *bias, int seq, int in_dim, int out_dim, const smol_adapters *set,
+                                        const int *ids) {
+    if (!ctx) return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: null context");
+    if ((x_dtype != SMOL_ATTN_F32 && x_dtype != SMOL_ATTN_BF16) || (y_dtype != SMOL_ATTN_F32 && y_dtype != SMOL_ATTN_BF16))
+        return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: dtype");
+    if (!set || !ids) return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: null adapters or ids");
+    if (set->ctx != ctx) return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: adapters of another context");
+    if (seq < 0 || in_dim != set->in_dim || out_dim != set->out_dim)
+        return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: sizes differ from the adapters'");
+    if (seq == 0) return SMOL_ATTN_OK;
+    if (!y || !x || !w) return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: null pointer");
+    const int xs = x_dtype == SMOL_ATTN_BF16 ? 2 : 4, ys = y_dtype == SMOL_ATTN_BF16 ? 2 : 4;
+    if (((uintptr_t)x & (xs - 1)) || ((uintptr_t)y & 15)) return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: alignment");
+    if ((long long)seq * in_dim > INT_MAX / 4 || (long long)seq * out_dim > INT_MAX / 4)
+        return afail(SMOL_ATTN_ERR_UNSUPPORTED, "smol_linear_adapters_dev: sizes beyond the supported range");
+    if ((const char *)x < (const char *)y + (size_t)seq * out_dim * ys && (const char *)y < (const char *)x + (size_t)seq * in_dim * xs)
+        return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: y overlaps x");
+    /* the rows by adapter, tiles of at most 16 */
+    std::vector<int> count(set->n, 0);
+    int bare = 0;
+    for (int s = 0; s < seq; s++) {
+        if (ids[s] < -1 || ids[s] >= set->n) return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: an id outside the set");
+        if (ids[s] < 0) bare++;
+        else count[ids[s]]++;
+    }
+    if (bare == seq) return smol_linear_dev(ctx, y, y_dtype, x, x_dtype, w, bias, seq, in_dim, out_dim);
+    std::vector<int> first(set->n, 0);
+    int n_tiles = 0;
+    for (int i = 0; i < set->n; i++) {
+        first[i] = n_tiles;
+        n_tiles += (count[i] + 15) / 16;
+        count[i] = 0;
+    }
+    std::vector<AdTile> tiles(n_tiles);
+    for (int s = 0; s < seq; s++) {
+        const int id = ids[s];
+        if (id < 0) continue;
+        AdTile &t = tiles[first[id] + count[id] / 16];
+        const int k = count[id]++ % 16;
+        if (k == 0) {
+            t.adapter = id;
+            for (int i = 0; i < 16; i++) t.row[i] = s;
+        }
+        t.row[k] = s;
+        t.n = k + 1;
+    }
+
+    AHIP(hipSetDevice(smol_internal_ctx_device(ctx)));
+    hipStream_t st = static_cast<hipStream_t>(smol_attn_ctx_stream(ctx));
+    AdParams p;
+    memset(&p, 0, offsetof(AdParams, tiles));
+    p.x = x;
+    p.x_bf16 = x_dtype == SMOL_ATTN_BF16;
+    p.vec = in_dim % 8 == 0 && ((uintptr_t)x & 15) == 0;
+    p.in_dim = in_dim;
+    p.out_dim = out_dim;
+    p.seq = seq;
+    p.a = set->a; p.ra = set->ra; p.kp = set->kp;
+    p.b = set->b; p.np = set->np; p.rp = set->rp;
+    p.scale = set->scale;
+    p.rank = set->rank;
+    p.n_tiles = n_tiles;
+    /* a step a wave at least, and no more workgroups than fill the device */
+    const int steps = set->kp / 32, cus = smol_internal_ctx_cus(ctx);
+    int chunks = std::max(1, std::min({cus / n_tiles, (steps + AD_NW - 1) / AD_NW, 16}));
+    p.chunk = (steps + chunks - 1) / chunks;
+    p.n_chunks = (steps + p.chunk - 1) / p.chunk;
+    const size_t tb = ((size_t)p.n_chunks * n_tiles * 16 * set->ra * 4 + 255) & ~(size_t)255;
+    const bool ybf = y_dtype == SMOL_ATTN_BF16;
+    void *work;
+    if (int rc = smol_internal_work(ctx, tb + (ybf ? (size_t)seq * out_dim * 4 : 0), &work)) return rc;
+    p.t = static_cast<float *>(work);
+    float *base = ybf ? reinterpret_cast<float *>(static_cast<char *>(work) + tb) : static_cast<float *>(y);
+    p.base = base;
+    p.y = y;
+    p.y_bf16 = ybf;
+    if (n_tiles <= AD_ARG_TILES) {
+        memcpy(p.tiles, tiles.data(), n_tiles * sizeof(AdTile));
+    } else {
+        const void *dev;
+        if (int rc = smol_internal_upload(ctx, tiles.data(), n_tiles * sizeof(AdTile), &dev)) return rc;
+        p.tiles_dev = static_cast<const AdTile *>(dev);
+    }
+    if (int rc = smol_linear_dev(ctx, base, SMOL_ATTN_F32, x, x_dtype, w, bias, seq, in_dim, out_dim)) return rc;
+    hipEvent_t e0 = nullptr, e1 = nullptr;
+    smol_internal_timing_events(ctx, AD_TIMING_KIND, &e0, &e1);
+    if (e0) AHIP(hipEventRecord(e0, st));
+    const unsigned in_blocks = (unsigned)n_tiles * p.n_chunks;
+    const int nt = set->ra / 16;
+    if (nt <= 1) launch_in<1>(p, in_blocks, st);
+    else if (nt <= 2) launch_in<2>(p, in_blocks, st);
+    else if (nt <= 4) launch_in<4>(p, in_blocks, st);
+    else launch_in<8>(p, in_blocks, st);
+    AHIP(hipGetLastError());
+    if (ybf && bare) {
+        const long long n = (long long)seq * out_dim;
+        hipLaunchKernelGGL(k_adapt_bare, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (uint16_t *)y, base, n);
+    }
+    const unsigned out_blocks = (unsigned)n_tiles * ((out_dim + AD_OUT * AD_NW - 1) / (AD_OUT * AD_NW));
+    switch (set->rp / 32) {
+    case 1: hipLaunchKernelGGL(k_adapt_out<1>, dim3(out_blocks), dim3(AD_TPB), 0, st, p); break;
+    case 2: hipLaunchKernelGGL(k_adapt_out<2>, dim3(out_blocks), dim3(AD_TPB), 0, st, p); break;
+    default: hipLaunchKernelGGL(k_adapt_out<4>, dim3(out_blocks), dim3(AD_TPB), 0, st, p); break;
+    }
+    AHIP(hipGetLastError());
+    if (e1) AHIP(hipEventRecord(e1, st));
+    return SMOL_ATTN_OK;
+}

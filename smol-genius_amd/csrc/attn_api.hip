@@ -1860,8 +1860,25 @@ static int check_capture(smol_attn_ctx *ctx, const char *what, bool grows) {
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     HIP_TRY(hipStreamIsCapturing(ctx->stream, &cs));
     if (cs == hipStreamCaptureStatusNone) return 0;
-    return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%s under stream capture (run the call once before, with at most %d sequences)",
-                what, SH_ARG_SEQS);
+    return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%s under stream capture (run the call once before; batches past the kernel "
+                "arguments' tables cannot be captured)", what);
+}
+
+/* for adapters.hip: `bytes` of the context's workspace, and a table's upload
+ * (both hold until the context's next call) */
+extern "C" int smol_internal_work(smol_attn_ctx *ctx, size_t bytes, void **p) {
+    int rc;
+    if ((rc = check_capture(ctx, "workspace growth", bytes > ctx->work.cap))) return rc;
+    if ((rc = dev_reserve(ctx->work, bytes, ctx->stream))) return rc;
+    *p = ctx->work.p;
+    return 0;
+}
+extern "C" int smol_internal_upload(smol_attn_ctx *ctx, const void *host, size_t bytes, const void **dev) {
+    int rc;
+    if ((rc = check_capture(ctx, "a batch's table", true))) return rc;
+    if ((rc = upload_desc(ctx, host, bytes))) return rc;
+    *dev = ctx->desc.p;
+    return 0;
 }
 
 /* cache growth and the table's, refused under capture */

@@ -102,6 +102,9 @@ SIGNATURES = [
     ("smol_linear_dev", [_vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int], _c_int),
     ("smol_linear_qkv_dev", [_vp, _vp, _vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _c_int, _c_int, _c_int,
                              _c_int], _c_int),
+    ("smol_adapters_create", [_vp, _c_int, _c_int, _c_int, _vp, _vp, _IP, _FP, ctypes.POINTER(_vp)], _c_int),
+    ("smol_adapters_destroy", [_vp], _c_int),
+    ("smol_linear_adapters_dev", [_vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _vp, _IP], _c_int),
     ("smol_linear_ops_dev", [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp], _c_int),
     ("smol_rms_norm_dev", [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_float], _c_int),
     ("smol_bf16_rms_norm_dev", [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_float], _c_int),
@@ -856,6 +859,61 @@ def linear(ctx, x, w, bias=None, out=None, out_bf16=False):
     b = _dev(bias, "bias") if bias is not None else None
     _check(load().smol_linear_dev(ctx.h, _dev(out, "out"), BF16 if out_bf16 else F32, _dev(x, "x"),
                                   _dtype_code(x), _wbits(w, "w"), b, seq, in_dim, out_dim), "smol_linear_dev")
+    return out
+
+
+class Adapters:
+    """Low-rank adapters of one projection (smol_adapters): (a [rank, in], b [out, rank], scale) each, device bf16
+    tensors (or their bits as int16), copied into the set at creation."""
+
+    def __init__(self, ctx, adapters):
+        import torch
+        bits = (torch.bfloat16, torch.int16, torch.uint16)
+        adapters = list(adapters)
+        if not adapters:
+            raise SmolAttnError("no adapters")
+        a0, b0, _ = adapters[0]
+        if a0.dim() != 2 or b0.dim() != 2:
+            raise SmolAttnError("a is [rank, in], b [out, rank]")
+        self.ctx, self.in_dim, self.out_dim, n = ctx, a0.shape[1], b0.shape[0], len(adapters)
+        av, bv, ranks, scales = (_vp * n)(), (_vp * n)(), (_c_int * n)(), (_c_float * n)()
+        for i, (a, b, scale) in enumerate(adapters):
+            ranks[i], scales[i] = a.shape[0], scale
+            av[i] = _on(ctx, a, bits, (a.shape[0], self.in_dim), "a")
+            bv[i] = _on(ctx, b, bits, (self.out_dim, a.shape[0]), "b")
+        self.n = n
+        self.h = _vp()
+        _check(load().smol_adapters_create(ctx.h, n, self.in_dim, self.out_dim, av, bv, ranks, scales, ctypes.byref(self.h)),
+               "smol_adapters_create")
+        _live.add(self)
+
+    def close(self):
+        if self.h:
+            load().smol_adapters_destroy(self.h)
+            self.h = _vp()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def linear_adapters(ctx, x, w, adapters, ids, bias=None, out=None, out_bf16=False):
+    """y = x W^T (+ bias) with adapter ids[s] of `adapters` (-1: none) for row s (smol_linear_adapters_dev). ids: host
+    numbers [seq]. Returns y [seq, out], float32, or the truncated bf16 bits as int16 when out_bf16."""
+    import torch
+    seq, in_dim, out_dim = x.shape[0], adapters.in_dim, adapters.out_dim
+    xp = _on(ctx, x, (torch.float32, torch.bfloat16), (seq, in_dim), "x")
+    wp = _on(ctx, w, (torch.bfloat16, torch.int16, torch.uint16), (out_dim, in_dim), "w")
+    bp = None if bias is None else _on(ctx, bias, (torch.float32,), (out_dim,), "bias")
+    dt = torch.int16 if out_bf16 else torch.float32
+    if out is None:
+        out = torch.empty((seq, out_dim), dtype=dt, device=x.device)
+    i, ip = _host_ints(ids, seq, "ids")
+    _check(load().smol_linear_adapters_dev(ctx.h, _on(ctx, out, (dt,), (seq, out_dim), "out"), BF16 if out_bf16 else F32, xp,
+                                           _dtype_code(x), wp, bp, seq, in_dim, out_dim, adapters.h, ip),
+           "smol_linear_adapters_dev")
     return out
 
 
