@@ -277,8 +277,8 @@ SMOL_ATTN_API int smol_attn_decode_noalloc(smol_attn_ctx *ctx, smol_kv_cache *kv
  *
  * Common to the two decode steps below. The new token of sequence i is used
  * in fp32 by the call that appends it and stored as bf16 (nearest even). The
- * scores of a row are a 24-bit split of Q against the cache's bf16 bits, the
- * probabilities carry 16 bits into P.V, everything else is fp32; there is no
+ * products are fp32 Q and fp32 probabilities, each split into three bf16 parts
+ * (24 bits), with the cache's bf16 bits; everything else is fp32, and there is no
  * range limit. A cached row that holds NaN or infinity makes the outputs of the
  * sequences that see it NaN, and of no other; rows at or past a sequence's length are never used. A
  * sequence's result does not depend on what the cache holds elsewhere, but the

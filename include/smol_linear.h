@@ -75,9 +75,11 @@ SMOL_ATTN_API int smol_adapters_destroy(smol_adapters *set);
 /* y[s] = W x[s] (+ bias) + scale_a B_a (A_a x[s]) with a = ids[s], or without
  * the last term where ids[s] is -1: smol_linear_dev with an adapter a row.
  * ids: host array [seq]; rows of one adapter need not follow each other. The
- * shared product has smol_linear_dev's precision; A_a x and B_a (A_a x) are
- * fp32 sums of fp32 inputs (24 bits) and the exact bf16 weights, and a bf16 y is
- * truncated once, from the whole sum. y (16-byte aligned) overlaps neither x
+ * products are fp32 sums of fp32 inputs (24 bits) and the exact bf16 weights,
+ * except that the shared one of more than 64 rows is smol_linear_dev's (x to
+ * 2^-16); a bf16 y is truncated once, from the whole sum. An fp32 row of x that
+ * holds infinity may give NaN. A row's results do not depend on the other rows'
+ * values. y (16-byte aligned) overlaps neither x
  * nor W. Uses the context's workspace. Under stream capture the call must
  * have been made once before, with at most 40 groups of 16 rows that share an
  * adapter (SMOL_ATTN_ERR_UNSUPPORTED otherwise); the captured call keeps its

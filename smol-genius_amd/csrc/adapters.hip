@@ -3,17 +3,20 @@
  * for every row (smol_linear_adapters_dev): for row s with adapter a,
  *     y_s = W x_s + bias + scale_a B_a (A_a x_s),   A_a [rank][in], B_a [out][rank].
  *
- * The shared product is the library's own (linear.hip). The low-rank part is
- * two thin products over tiles of 16 rows that share an adapter (the host
+ * The low-rank part works on tiles of 16 rows that share an adapter (the host
  * sorts the rows; the rows of a tile need not follow each other):
- *   k_adapt_in   t^T = A x^T, the in_dim cut into chunks so that few tiles still
- *                fill the device; each chunk writes its own partial t, so the
- *                sum's order is fixed;
- *   k_adapt_out  adds scale B t to y: the chunks' t are summed as they are read.
- * Both run on v_mfma_f32_16x16x32_bf16 with the weights as the A operand, so a
- * lane holds four consecutive ranks (outputs) of one row and stores them
- * together. An fp32 x and t are split into three bf16 parts (24 bits), so the
- * low-rank part is as exact as an fp32 product of the bf16 weights.
+ *   k_adapt_in   t = A x, the in_dim cut into chunks so that few tiles still fill
+ *                the device; each chunk writes its own partial t, so the sum's
+ *                order is fixed.
+ * Up to AD_FEW rows the rest is one launch, k_adapt_few: W streams once from
+ * memory through the matrix cores against all rows (k_adapt_in's launch has
+ * laid x out as bf16 parts for it), the waves' sums meet in LDS, and scale B t
+ * and the bias join them there. More rows run the library's own product
+ * (linear.hip) and then k_adapt_out, which adds scale B t to it.
+ * All run on v_mfma_f32_16x16x32_bf16 with the weights as the A operand, so a
+ * lane holds four consecutive ranks (outputs) of one row. An fp32 x and t are
+ * split into three bf16 parts (24 bits), so these products are as exact as
+ * fp32 products of the bf16 weights.
  *
  * The weights of a set are packed once, at its creation: ranks padded with
  * zeros to the matrix instruction's sizes, so no load needs a bound.
@@ -41,6 +44,7 @@ namespace {
 constexpr int AD_MAX_RANK = 128;
 constexpr int AD_TPB = 256, AD_NW = AD_TPB / 64;
 constexpr int AD_ARG_TILES = 40;
+constexpr int AD_FEW = 64; /* rows that k_adapt_few takes */
 constexpr int AD_TIMING_KIND = 2;
 
 struct AdTile {
@@ -50,11 +54,15 @@ struct AdTile {
 
 struct AdParams {
     const void *x; int x_bf16; int vec;
+    const uint16_t *w; int w_vec; const float *bias;
+    uint16_t *xs;                    /* few rows: x as bf16 parts [part][row][kp], zeros past in_dim */
+    int in_blocks;                   /* workgroups of k_adapt_in on tiles; those behind them lay x out */
     int in_dim, out_dim, seq;
     const uint16_t *a; int ra, kp;   /* [adapter][ra][kp] */
     const uint16_t *b; int np, rp;   /* [adapter][np][rp] */
     const float *scale; const int *rank; /* [adapter] */
-    float *t; int n_tiles, n_chunks, chunk; /* [chunk][tile][16][ra]; chunk: 32-wide steps of in_dim */
+    float *t; int n_tiles, n_chunks, chunk; /* [chunk][seq][ra]; chunk: 32-wide steps of in_dim */
+    unsigned has[2];                 /* few rows: the rows that have an adapter */
     const float *base;               /* fp32 [seq][out] that the low-rank part is added to */
     void *y; int y_bf16;             /* fp32 y is base itself */
     const AdTile *tiles_dev;
@@ -73,15 +81,61 @@ __device__ __forceinline__ void ad_split3(const float *x, b8 &p0, b8 &p1, b8 &p2
     }
 }
 
+/* elements [k0, k0 + 8) of row `row` of x as bf16 parts, zeros past in_dim; vec: in_dim is a multiple of 8 and x
+ * aligned */
+template <bool XBF>
+__device__ __forceinline__ void ad_x8(const AdParams &p, long long row, int k0, b8 *xp) {
+    if constexpr (XBF) {
+        const uint16_t *x = (const uint16_t *)p.x + row * p.in_dim + k0;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (p.vec) {
+            if (k0 < p.in_dim) w = *reinterpret_cast<const uint4 *>(x);
+        } else {
+            uint32_t v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = k0 + i < p.in_dim ? x[i] : 0u;
+            w = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+        }
+        xp[0] = as_b8(w);
+    } else {
+        const float *x = (const float *)p.x + row * p.in_dim + k0;
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (p.vec) {
+            if (k0 < p.in_dim) {
+                const float4 u = *reinterpret_cast<const float4 *>(x), w = *reinterpret_cast<const float4 *>(x + 4);
+                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w; v[4] = w.x; v[5] = w.y; v[6] = w.z; v[7] = w.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (k0 + i < p.in_dim) v[i] = x[i];
+        }
+        ad_split3(v, xp[0], xp[1], xp[2]);
+    }
+}
+
 /* NT: rank tiles of 16 that the accumulators hold */
 template <int NT, bool XBF>
 __global__ __launch_bounds__(AD_TPB) void k_adapt_in(const AdParams p) {
+    constexpr int PARTS = XBF ? 1 : 3;
     __shared__ __attribute__((aligned(16))) float s_t[AD_NW * 16 * NT * 16];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
+    if ((int)blockIdx.x >= p.in_blocks) {
+        const long long e = (long long)(blockIdx.x - p.in_blocks) * AD_TPB + tid;
+        const int per = p.kp / 8, row = (int)(e / per), k0 = (int)(e - (long long)row * per) * 8;
+        if (row < p.seq) {
+            b8 xp[PARTS];
+            ad_x8<XBF>(p, row, k0, xp);
+#pragma unroll
+            for (int q = 0; q < PARTS; q++)
+                *reinterpret_cast<b8 *>(p.xs + ((long long)q * p.seq + row) * p.kp + k0) = xp[q];
+        }
+        return;
+    }
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tile = blockIdx.x % p.n_tiles, chunk = blockIdx.x / p.n_tiles;
     const AdTile *tl = (p.tiles_dev ? p.tiles_dev : p.tiles) + tile;
-    const int ad = tl->adapter, nt = (p.rank[ad] + 15) / 16;
+    const int ad = tl->adapter, n = tl->n, nt = (p.rank[ad] + 15) / 16;
     const long long row = tl->row[c];
     const uint16_t *a = p.a + ((long long)ad * p.ra + c) * p.kp + 8 * j;
     f4 acc[NT];
@@ -89,41 +143,16 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_in(const AdParams p) {
     for (int t = 0; t < NT; t++) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
     const int s1 = min((chunk + 1) * p.chunk, p.kp / 32);
     for (int s = chunk * p.chunk + wave; s < s1; s += AD_NW) {
-        const int k0 = 32 * s + 8 * j;
-        b8 xp[XBF ? 1 : 3];
-        if constexpr (XBF) {
-            const uint16_t *x = (const uint16_t *)p.x + row * p.in_dim + k0;
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (p.vec) {
-                if (k0 < p.in_dim) w = *reinterpret_cast<const uint4 *>(x);
-            } else {
-                uint32_t v[8];
+        b8 xp[PARTS], w[NT];
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = k0 + i < p.in_dim ? x[i] : 0u;
-                w = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
-            }
-            xp[0] = as_b8(w);
-        } else {
-            const float *x = (const float *)p.x + row * p.in_dim + k0;
-            float v[8];
-            if (p.vec) {
-                /* in_dim is a multiple of 8 */
-                const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                const float4 u = k0 < p.in_dim ? *reinterpret_cast<const float4 *>(x) : z;
-                const float4 w = k0 < p.in_dim ? *reinterpret_cast<const float4 *>(x + 4) : z;
-                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w; v[4] = w.x; v[5] = w.y; v[6] = w.z; v[7] = w.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = k0 + i < p.in_dim ? x[i] : 0.0f;
-            }
-            ad_split3(v, xp[0], xp[1], xp[2]);
-        }
+        for (int t = 0; t < NT; t++)
+            if (t < nt) w[t] = as_b8(*reinterpret_cast<const uint4 *>(a + (long long)t * 16 * p.kp + 32 * s));
+        ad_x8<XBF>(p, row, 32 * s + 8 * j, xp);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             if (t >= nt) break;
-            const b8 w = as_b8(*reinterpret_cast<const uint4 *>(a + (long long)t * 16 * p.kp + 32 * s));
 #pragma unroll
-            for (int q = XBF ? 0 : 2; q >= 0; q--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xp[q], acc[t], 0, 0, 0);
+            for (int q = PARTS - 1; q >= 0; q--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[t], xp[q], acc[t], 0, 0, 0);
         }
     }
     /* lane (c, j): ranks 16 t + 4 j .. + 3 of row c */
@@ -131,13 +160,136 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_in(const AdParams p) {
     for (int t = 0; t < NT; t++)
         *reinterpret_cast<f4 *>(s_t + ((wave * 16 + c) * NT + t) * 16 + 4 * j) = acc[t];
     __syncthreads();
-    float *out = p.t + ((long long)chunk * p.n_tiles + tile) * 16 * p.ra;
-    for (int e = tid; e < 16 * nt * 4; e += AD_TPB) {
+    for (int e = tid; e < n * nt * 4; e += AD_TPB) {
         const int r = e / (nt * 4), q = e - r * nt * 4;
         f4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < AD_NW; w++) sum += *reinterpret_cast<f4 *>(s_t + ((w * 16 + r) * NT) * 16 + 4 * q);
-        *reinterpret_cast<f4 *>(out + r * p.ra + 4 * q) = sum;
+        *reinterpret_cast<f4 *>(p.t + ((long long)chunk * p.seq + tl->row[r]) * p.ra + 4 * q) = sum;
+    }
+}
+
+/* scale t of row `row`, ranks [8 j', 8 j' + 8) of each 32-wide step, as bf16 parts: the chunks' partial sums, four at a
+ * time in flight */
+template <int KS>
+__device__ __forceinline__ void ad_t(const AdParams &p, long long row, int rank, float scale, bool live, int j, b8 (*tp)[3]) {
+    const long long step = (long long)p.seq * p.ra;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+        const int r = 32 * ks + 8 * j;
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        /* k_adapt_in writes whole tiles of 16 ranks */
+        if (live && r < ((rank + 15) & ~15)) {
+            const float *t = p.t + row * p.ra + r;
+            for (int q = 0; q < p.n_chunks; q += 4) {
+                f4 x[4], z[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (q + u < p.n_chunks) {
+                        x[u] = *reinterpret_cast<const f4 *>(t + (q + u) * step);
+                        z[u] = *reinterpret_cast<const f4 *>(t + (q + u) * step + 4);
+                    }
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (q + u < p.n_chunks) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            v[i] += x[u][i];
+                            v[4 + i] += z[u][i];
+                        }
+                    }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= scale;
+        ad_split3(v, tp[ks][0], tp[ks][1], tp[ks][2]);
+    }
+}
+
+/* Up to 16 RT rows against 16 outputs a workgroup. Its eight waves share in_dim out by 32-wide steps, each with US steps
+ * of W in flight; the sums of every wave are added in LDS in wave order, the adapters' tiles (one wave each) add their
+ * part, and each output is written once. */
+constexpr int FEW_NW = 8;
+template <int RT, bool XBF, int KS>
+__global__ __launch_bounds__(64 * FEW_NW) void k_adapt_few(const AdParams p) {
+    constexpr int PARTS = XBF ? 1 : 3, US = RT <= 2 ? 4 : 2, STR = 20;
+    __shared__ __attribute__((aligned(16))) float s_y[(FEW_NW + 1) * RT * 16 * STR];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int o0 = blockIdx.x * 16, steps = p.kp / 32;
+    const uint16_t *w = p.w + (long long)min(o0 + c, p.out_dim - 1) * p.in_dim + 8 * j;
+    f4 acc[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
+    auto load_w = [&](int s) __attribute__((always_inline)) {
+        const int k0 = 32 * s + 8 * j;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (p.w_vec) {
+            if (k0 < p.in_dim) v = *reinterpret_cast<const uint4 *>(w + 32 * s);
+        } else {
+            uint32_t x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = k0 + i < p.in_dim ? w[32 * s + i] : 0u;
+            v = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+        }
+        return v;
+    };
+    for (int s0 = wave; s0 < steps; s0 += FEW_NW * US) {
+        uint4 wv[US];
+        b8 xf[US][RT][PARTS];
+#pragma unroll
+        for (int u = 0; u < US; u++) {
+            const int s = s0 + u * FEW_NW;
+            wv[u] = s < steps ? load_w(s) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+#pragma unroll
+                for (int q = 0; q < PARTS; q++)
+                    xf[u][t][q] = as_b8(s < steps ? *reinterpret_cast<const uint4 *>(
+                                                        p.xs + ((long long)q * p.seq + min(16 * t + c, p.seq - 1)) * p.kp +
+                                                        32 * s + 8 * j)
+                                                  : make_uint4(0, 0, 0, 0));
+        }
+#pragma unroll
+        for (int u = 0; u < US; u++)
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+#pragma unroll
+                for (int q = PARTS - 1; q >= 0; q--)
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(wv[u]), xf[u][t][q], acc[t], 0, 0, 0);
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++) *reinterpret_cast<f4 *>(s_y + ((wave * RT + t) * 16 + c) * STR + 4 * j) = acc[t];
+    /* the low-rank part, by row, behind the waves' sums (rows without an adapter are not read there) */
+    float *s_low = s_y + FEW_NW * RT * 16 * STR;
+    for (int tile = wave; tile < p.n_tiles; tile += FEW_NW) {
+        const AdTile *tl = (p.tiles_dev ? p.tiles_dev : p.tiles) + tile;
+        const int ad = tl->adapter, rank = p.rank[ad], row = tl->row[c];
+        const bool live = c < tl->n;
+        const uint16_t *b = p.b + ((long long)ad * p.np + o0 + c) * p.rp + 8 * j;
+        b8 bw[KS], tp[KS][3];
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) bw[ks] = as_b8(*reinterpret_cast<const uint4 *>(b + 32 * ks));
+        ad_t<KS>(p, row, rank, p.scale[ad], live, j, tp);
+        f4 low = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int q = 2; q >= 0; q--) low = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw[ks], tp[ks][q], low, 0, 0, 0);
+        if (live) *reinterpret_cast<f4 *>(s_low + row * STR + 4 * j) = low;
+    }
+    __syncthreads();
+    for (int e = tid; e < p.seq * 16; e += 64 * FEW_NW) {
+        const int r = e / 16, o = e % 16;
+        if (o0 + o >= p.out_dim) continue;
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < FEW_NW; q++) v += s_y[(q * RT * 16 + r) * STR + o];
+        if (p.bias) v += p.bias[o0 + o];
+        if (p.has[r >> 5] >> (r & 31) & 1) v += s_low[r * STR + o];
+        const long long at = (long long)r * p.out_dim + o0 + o;
+        if (p.y_bf16) ((uint16_t *)p.y)[at] = (uint16_t)(__float_as_uint(v) >> 16);
+        else ((float *)p.y)[at] = v;
     }
 }
 
@@ -152,51 +304,54 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_out(const AdParams p) {
     if (o0 >= p.out_dim) return;
     const AdTile *tl = (p.tiles_dev ? p.tiles_dev : p.tiles) + tile;
     const int ad = tl->adapter, rank = p.rank[ad];
-    const float scale = p.scale[ad];
     const long long row = tl->row[c];
     const bool live = c < tl->n;
-    b8 tp[KS][3];
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-        const int r = 32 * ks + 8 * j;
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        /* k_adapt_in writes whole tiles of 16 ranks */
-        if (r < ((rank + 15) & ~15)) {
-            const float *t = p.t + (long long)tile * 16 * p.ra + c * p.ra + r;
-            for (int q = 0; q < p.n_chunks; q++, t += (long long)p.n_tiles * 16 * p.ra) {
-                const float4 x = *reinterpret_cast<const float4 *>(t), z = *reinterpret_cast<const float4 *>(t + 4);
-                v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += z.x; v[5] += z.y; v[6] += z.z; v[7] += z.w;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= scale;
-        ad_split3(v, tp[ks][0], tp[ks][1], tp[ks][2]);
-    }
+    constexpr int U = AD_OUT / 16;
+    const bool quads = (p.out_dim & 3) == 0;
+    f4 base[U];
+    b8 w[U][KS];
+    /* B has whole tiles of AD_OUT rows and 32 ranks; the sums that they join */
     const uint16_t *b = p.b + ((long long)ad * p.np + o0 + c) * p.rp + 8 * j;
 #pragma unroll
-    for (int u = 0; u < AD_OUT / 16; u++) {
+    for (int u = 0; u < U; u++) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) w[u][ks] = as_b8(*reinterpret_cast<const uint4 *>(b + (long long)16 * u * p.rp + 32 * ks));
         const int o = o0 + 16 * u + 4 * j;
-        if (o0 + 16 * u >= p.out_dim) break;
+        const long long at = row * p.out_dim + o;
+        if (quads) {
+            if (o < p.out_dim) base[u] = *reinterpret_cast<const f4 *>(p.base + at);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (o + i < p.out_dim) base[u][i] = p.base[at + i];
+        }
+    }
+    b8 tp[KS][3];
+    ad_t<KS>(p, row, rank, p.scale[ad], live, j, tp);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int o = o0 + 16 * u + 4 * j;
         f4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            if (32 * ks >= rank) break;
-            const b8 w = as_b8(*reinterpret_cast<const uint4 *>(b + (long long)16 * u * p.rp + 32 * ks));
+        for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-            for (int q = 2; q >= 0; q--) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, tp[ks][q], acc, 0, 0, 0);
-        }
+            for (int q = 2; q >= 0; q--) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u][ks], tp[ks][q], acc, 0, 0, 0);
         if (!live) continue;
         const long long at = row * p.out_dim + o;
-        if (!p.y_bf16 && (p.out_dim & 3) == 0 && o < p.out_dim) {
-            f4 *y = reinterpret_cast<f4 *>((float *)p.y + at);
-            *y = *reinterpret_cast<const f4 *>(p.base + at) + acc;
+        acc += base[u];
+        if (quads && o < p.out_dim) {
+            if (p.y_bf16)
+                *reinterpret_cast<uint2 *>((uint16_t *)p.y + at) =
+                    make_uint2(__float_as_uint(acc[0]) >> 16 | (__float_as_uint(acc[1]) & 0xFFFF0000u),
+                               __float_as_uint(acc[2]) >> 16 | (__float_as_uint(acc[3]) & 0xFFFF0000u));
+            else
+                *reinterpret_cast<f4 *>((float *)p.y + at) = acc;
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (o + i < p.out_dim) {
-                    const float v = p.base[at + i] + acc[i];
-                    if (p.y_bf16) ((uint16_t *)p.y)[at + i] = (uint16_t)(__float_as_uint(v) >> 16);
-                    else ((float *)p.y)[at + i] = v;
+                    if (p.y_bf16) ((uint16_t *)p.y)[at + i] = (uint16_t)(__float_as_uint(acc[i]) >> 16);
+                    else ((float *)p.y)[at + i] = acc[i];
                 }
         }
     }
@@ -209,12 +364,13 @@ __global__ __launch_bounds__(256) void k_adapt_bare(uint16_t *y, const float *ba
 }
 
 /* dst [rows][stride] = src [rows][cols], zeros behind; rows past src_rows are zeros */
-__global__ __launch_bounds__(256) void k_adapt_pack(uint16_t *dst, const uint16_t *src, int rows, int stride, int src_rows,
+template <typename T>
+__global__ __launch_bounds__(256) void k_adapt_pack(T *dst, const T *src, int rows, int stride, int src_rows,
                                                     int cols) {
     const long long n = (long long)rows * stride;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
         const int r = (int)(i / stride), q = (int)(i - (long long)r * stride);
-        dst[i] = r < src_rows && q < cols ? src[(long long)r * cols + q] : (uint16_t)0;
+        dst[i] = r < src_rows && q < cols ? src[(long long)r * cols + q] : (T)0;
     }
 }
 
@@ -241,9 +397,9 @@ struct smol_adapters {
 
 extern "C" int smol_adapters_destroy(smol_adapters *s) {
     if (!s) return SMOL_ATTN_OK;
-    hipSetDevice(s->device);
-    hipStreamSynchronize(s->stream);
-    if (s->mem) hipFree(s->mem);
+    (void)hipSetDevice(s->device);
+    (void)hipStreamSynchronize(s->stream);
+    if (s->mem) (void)hipFree(s->mem);
     delete s;
     return SMOL_ATTN_OK;
 }
@@ -278,7 +434,7 @@ extern "C" int smol_adapters_create(smol_attn_ctx *ctx, int n, int in_dim, int o
     hipError_t e = hipMalloc(&s->mem, ab + bb + 2 * sb);
     if (e != hipSuccess) {
         delete s;
-        hipGetLastError();
+        (void)hipGetLastError();
         return afail(e == hipErrorOutOfMemory ? SMOL_ATTN_ERR_NOMEM : SMOL_ATTN_ERR_DEVICE, "smol_adapters_create: device memory");
     }
     s->a = static_cast<uint16_t *>(s->mem);
@@ -288,7 +444,7 @@ extern "C" int smol_adapters_create(smol_attn_ctx *ctx, int n, int in_dim, int o
     for (int i = 0; i < n && e == hipSuccess; i++) {
         auto pack = [&](uint16_t *dst, const uint16_t *src, int rows, int stride, int src_rows, int cols) {
             const long long blocks = std::min<long long>(((long long)rows * stride + 255) / 256, 4096);
-            hipLaunchKernelGGL(k_adapt_pack, dim3((unsigned)blocks), dim3(256), 0, s->stream, dst, src, rows, stride, src_rows, cols);
+            hipLaunchKernelGGL(k_adapt_pack<uint16_t>, dim3((unsigned)blocks), dim3(256), 0, s->stream, dst, src, rows, stride, src_rows, cols);
         };
         pack(s->a + (size_t)i * s->ra * s->kp, a[i], s->ra, s->kp, rank[i], in_dim);
         pack(s->b + (size_t)i * s->np * s->rp, b[i], s->np, s->rp, out_dim, rank[i]);
@@ -304,6 +460,16 @@ extern "C" int smol_adapters_create(smol_attn_ctx *ctx, int n, int in_dim, int o
     }
     *out = s;
     return SMOL_ATTN_OK;
+}
+
+template <int RT, bool XBF>
+static void launch_few(const AdParams &p, int ks, hipStream_t st) {
+    const dim3 g((unsigned)((p.out_dim + 15) / 16)), b(64 * FEW_NW);
+    switch (ks) {
+    case 1: hipLaunchKernelGGL((k_adapt_few<RT, XBF, 1>), g, b, 0, st, p); break;
+    case 2: hipLaunchKernelGGL((k_adapt_few<RT, XBF, 2>), g, b, 0, st, p); break;
+    default: hipLaunchKernelGGL((k_adapt_few<RT, XBF, 4>), g, b, 0, st, p); break;
+    }
 }
 
 template <int NT>
@@ -380,12 +546,27 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
     int chunks = std::max(1, std::min({cus / n_tiles, (steps + AD_NW - 1) / AD_NW, 16}));
     p.chunk = (steps + chunks - 1) / chunks;
     p.n_chunks = (steps + p.chunk - 1) / p.chunk;
-    const size_t tb = ((size_t)p.n_chunks * n_tiles * 16 * set->ra * 4 + 255) & ~(size_t)255;
-    const bool ybf = y_dtype == SMOL_ATTN_BF16;
+    const bool ybf = y_dtype == SMOL_ATTN_BF16, few = seq <= AD_FEW;
+    /* more rows than k_adapt_few takes, and operands that the library's product cannot stage (16-byte pieces): x and W
+     * are copied with padded rows first */
+    const bool pad = !few && (in_dim % 8 != 0 || ((uintptr_t)x & 15) || ((uintptr_t)w & 15));
+    const int kp = set->kp, parts = p.x_bf16 ? 1 : 3;
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    const size_t tb = up((size_t)p.n_chunks * seq * set->ra * 4), yb = up(!few && ybf ? (size_t)seq * out_dim * 4 : 0);
+    const size_t xb = up(few ? (size_t)parts * seq * kp * 2 : pad ? (size_t)seq * kp * xs : 0);
     void *work;
-    if (int rc = smol_internal_work(ctx, tb + (ybf ? (size_t)seq * out_dim * 4 : 0), &work)) return rc;
+    if (int rc = smol_internal_work(ctx, tb + yb + xb + (pad ? (size_t)out_dim * kp * 2 : 0), &work)) return rc;
     p.t = static_cast<float *>(work);
-    float *base = ybf ? reinterpret_cast<float *>(static_cast<char *>(work) + tb) : static_cast<float *>(y);
+    float *base = yb ? reinterpret_cast<float *>(static_cast<char *>(work) + tb) : static_cast<float *>(y);
+    void *x_own = static_cast<char *>(work) + tb + yb;
+    uint16_t *w_own = reinterpret_cast<uint16_t *>(static_cast<char *>(work) + tb + yb + xb);
+    p.w = w;
+    p.w_vec = in_dim % 8 == 0 && ((uintptr_t)w & 15) == 0;
+    p.bias = bias;
+    p.xs = static_cast<uint16_t *>(x_own);
+    if (few)
+        for (int s = 0; s < seq; s++)
+            if (ids[s] >= 0) p.has[s >> 5] |= 1u << (s & 31);
     p.base = base;
     p.y = y;
     p.y_bf16 = ybf;
@@ -396,17 +577,51 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
         if (int rc = smol_internal_upload(ctx, tiles.data(), n_tiles * sizeof(AdTile), &dev)) return rc;
         p.tiles_dev = static_cast<const AdTile *>(dev);
     }
-    if (int rc = smol_linear_dev(ctx, base, SMOL_ATTN_F32, x, x_dtype, w, bias, seq, in_dim, out_dim)) return rc;
     hipEvent_t e0 = nullptr, e1 = nullptr;
-    smol_internal_timing_events(ctx, AD_TIMING_KIND, &e0, &e1);
-    if (e0) AHIP(hipEventRecord(e0, st));
-    const unsigned in_blocks = (unsigned)n_tiles * p.n_chunks;
+    if (few) {
+        smol_internal_timing_events(ctx, AD_TIMING_KIND, &e0, &e1);
+        if (e0) AHIP(hipEventRecord(e0, st));
+    } else {
+        const void *bx = x;
+        const uint16_t *bw = w;
+        int bk = in_dim;
+        if (pad) {
+            const unsigned pg = 2048;
+            if (p.x_bf16) hipLaunchKernelGGL(k_adapt_pack<uint16_t>, dim3(pg), dim3(256), 0, st, static_cast<uint16_t *>(x_own), (const uint16_t *)x, seq, kp, seq, in_dim);
+            else hipLaunchKernelGGL(k_adapt_pack<uint32_t>, dim3(pg), dim3(256), 0, st, static_cast<uint32_t *>(x_own), (const uint32_t *)x, seq, kp, seq, in_dim);
+            hipLaunchKernelGGL(k_adapt_pack<uint16_t>, dim3(pg), dim3(256), 0, st, w_own, w, out_dim, kp, out_dim, in_dim);
+            AHIP(hipGetLastError());
+            bx = x_own;
+            bw = w_own;
+            bk = kp;
+        }
+        if (int rc = smol_linear_dev(ctx, base, SMOL_ATTN_F32, bx, x_dtype, bw, bias, seq, bk, out_dim)) return rc;
+        smol_internal_timing_events(ctx, AD_TIMING_KIND, &e0, &e1);
+        if (e0) AHIP(hipEventRecord(e0, st));
+    }
+    p.in_blocks = n_tiles * p.n_chunks;
+    const unsigned in_blocks = (unsigned)p.in_blocks + (few ? ((unsigned)seq * (kp / 8) + AD_TPB - 1) / AD_TPB : 0);
     const int nt = set->ra / 16;
     if (nt <= 1) launch_in<1>(p, in_blocks, st);
     else if (nt <= 2) launch_in<2>(p, in_blocks, st);
     else if (nt <= 4) launch_in<4>(p, in_blocks, st);
     else launch_in<8>(p, in_blocks, st);
     AHIP(hipGetLastError());
+    if (few) {
+        const int ks = set->rp / 32;
+        if (p.x_bf16) {
+            if (seq <= 16) launch_few<1, true>(p, ks, st);
+            else if (seq <= 32) launch_few<2, true>(p, ks, st);
+            else launch_few<4, true>(p, ks, st);
+        } else {
+            if (seq <= 16) launch_few<1, false>(p, ks, st);
+            else if (seq <= 32) launch_few<2, false>(p, ks, st);
+            else launch_few<4, false>(p, ks, st);
+        }
+        AHIP(hipGetLastError());
+        if (e1) AHIP(hipEventRecord(e1, st));
+        return SMOL_ATTN_OK;
+    }
     if (ybf && bare) {
         const long long n = (long long)seq * out_dim;
         hipLaunchKernelGGL(k_adapt_bare, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (uint16_t *)y, base, n);

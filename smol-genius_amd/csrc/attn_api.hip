@@ -48,8 +48,10 @@ extern "C" int smol_launch_win(const WinParams *wp, int hd, int n_tiles, int max
                                hipEvent_t e1);
 extern "C" int smol_win_max_keys(int hd, int in_dtype, int precise);
 extern "C" int smol_shared_tile_rows(int hd, int rows);
+extern "C" int smol_shared_occupancy(int hd);
 extern "C" int smol_launch_shared(const ShParams *p, int hd, int tile_rows, int max_len, hipStream_t st, hipEvent_t e0,
                                   hipEvent_t e1);
+extern "C" int smol_evict_fused(int max_moves);
 extern "C" int smol_launch_evict(const EvictParams *p, int max_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
 extern "C" int smol_launch_to_bf16_trunc(const float *x, uint16_t *y, long long n, hipStream_t st);
 extern "C" int smol_launch_bf16_norm_rope(uint16_t *x, const float *w, uint16_t *x2, const float *w2, int H2,
@@ -1924,11 +1926,12 @@ static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int l
     sp.n_seq = n;
     /* what the window leaves */
     int p_first = 0, max_own = 0;
-    long long own_slabs = 0;
+    std::vector<int> own_slabs;
+    own_slabs.reserve(n);
     for (const ShSeq &q : seqs) {
         const int first = sp.window > 0 ? std::max(0, q.pos - sp.window + 1 - sp.p_len) & ~(SMOL_SLAB - 1) : 0;
         max_own = std::max(max_own, q.len - first);
-        own_slabs += (q.len - first + SMOL_SLAB - 1) / SMOL_SLAB;
+        own_slabs.push_back((q.len - first + SMOL_SLAB - 1) / SMOL_SLAB);
     }
     if (sp.window > 0 && sp.p_len > 0) {
         int lo = INT_MAX;
@@ -1936,15 +1939,26 @@ static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int l
         p_first = std::min(lo, sp.p_len) & ~(SMOL_SLAB - 1);
     }
     sp.p_first = p_first;
-    const int tile = smol_shared_tile_rows(hd, rows);
+    const int tile = getenv("SH_TILE") ? atoi(getenv("SH_TILE")) : smol_shared_tile_rows(hd, rows);
     const int p_slabs = (sp.p_len - p_first + SMOL_SLAB - 1) / SMOL_SLAB, own_max = (max_own + SMOL_SLAB - 1) / SMOL_SLAB;
     sp.n_rb = (rows + tile - 1) / tile;
     sp.s_rb = (G + 15) / 16;
-    /* equally long chunks of at least a slab a wave, as many as fill the device */
-    const long long units = (long long)Hkv * sp.n_rb * p_slabs + Hkv * (long long)sp.s_rb * own_slabs;
-    long long c = (units + 2LL * ctx->cu_count - 1) / (2LL * ctx->cu_count);
-    c = std::max(c, ((long long)std::max(p_slabs, own_max) + SH_MAX_SPLIT - 1) / SH_MAX_SPLIT);
-    c = std::max(4LL, (c + 3) & ~3LL);
+    long long units = (long long)Hkv * sp.n_rb * p_slabs;
+    for (int k : own_slabs) units += (long long)Hkv * sp.s_rb * k;
+    /* equally long chunks of at least a slab a wave: as short as lets every
+     * workgroup run at once, since each spends 6 us before its first slab and
+     * after its last */
+    const long long slots = (long long)ctx->cu_count * smol_shared_occupancy(hd);
+    const long long most = ((long long)std::max(p_slabs, own_max) + SH_MAX_SPLIT - 1) / SH_MAX_SPLIT;
+    auto workgroups = [&](long long c) {
+        long long w = (long long)Hkv * sp.n_rb * ((p_slabs + c - 1) / c);
+        for (int k : own_slabs) w += (long long)Hkv * sp.s_rb * std::max(1LL, (k + c - 1) / c);
+        return w;
+    };
+    long long c = std::max({4LL, most, (units + slots - 1) / slots});
+    c = (c + 3) & ~3LL;
+    for (int i = 0; i < 32 && c < std::max(p_slabs, own_max) && workgroups(c) > slots; i++) c += 4;
+    if (ctx->opt[SMOL_OPT_DEC_SLABS] > 0) c = std::max<long long>(most, (ctx->opt[SMOL_OPT_DEC_SLABS] + 3) & ~3);
     if (c > (INT_MAX >> 6)) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d rows", max_len);
     sp.p_chunk = sp.s_chunk = (int)c * SMOL_SLAB;
     sp.n_ps = (int)((p_slabs + c - 1) / c);
@@ -2133,9 +2147,10 @@ extern "C" int smol_kv_cache_evict(smol_kv_cache *kv, int layer, int n_seq, cons
     ep.mass = mass; ep.row_pos = row_pos; ep.mass_out = mass_out; ep.pos_out = pos_out; ep.m_stride = stride;
     ep.keep = keep; ep.first = first; ep.recent = recent;
     ep.max_moves = max_moves;
+    ep.fused = smol_evict_fused(max_moves);
     ep.n_seq = n_seq;
     WorkPlan wk;
-    const size_t o_mv = wk.take((size_t)pairs * 2 * max_moves * 4), o_n = wk.take((size_t)pairs * 4);
+    const size_t o_mv = wk.take(ep.fused ? 0 : (size_t)pairs * 2 * max_moves * 4), o_n = wk.take(ep.fused ? 0 : (size_t)pairs * 4);
     if ((rc = check_capture(ctx, "workspace growth", wk.bytes > ctx->work.cap))) return rc;
     if ((rc = dev_reserve(ctx->work, wk.bytes, ctx->stream))) return rc;
     ep.moves = (int *)((unsigned char *)ctx->work.p + o_mv);

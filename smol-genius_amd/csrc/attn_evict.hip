@@ -14,18 +14,24 @@
  * its digits (11, 11 and 10 bits) from histograms in LDS. Ties and the two
  * lists need counts in row order: each thread takes a run of consecutive rows
  * (an odd number of them, so the threads' LDS reads fall in different banks)
- * and one scan over the threads' counts gives every run its start.
- * k_evict_move then moves K rows in 16-byte pieces and V^T columns by element,
- * neighbouring rows in neighbouring lanes, since the rows of one slab share
- * the 64 bytes of a column.
+ * and one scan over the threads' counts gives every run its start. A few moves
+ * (EV_FUSED) are made by the same workgroup; more go to k_evict_move, which has
+ * a workgroup for every EV_MOVES of them. K rows move in 16-byte pieces, V^T
+ * columns by element with neighbouring rows in neighbouring lanes, since the
+ * rows of one slab share the 64 bytes of a column.
+ *
+ * What bounds it: the ranks are latency (loads, about a dozen barriers); the
+ * moves are memory traffic in pieces of 64 bytes. A moved row's V touches one
+ * such piece per column, so rows far apart cost 32 times their bytes: 8192 rows
+ * cut to 1024 read 3.7 MB of V^T a head for 0.2 MB of moved values.
  */
 #include "attn_device.h"
 
 namespace {
 
-constexpr int EV_TPB = 1024;
 constexpr int EV_BINS = 2048;
-constexpr int EV_MOVES = 32;       /* moves of a k_evict_move workgroup */
+constexpr int EV_MOVES = 32;  /* moves of a k_evict_move workgroup */
+constexpr int EV_FUSED = 256; /* moves that k_evict_select makes itself */
 
 __device__ __forceinline__ ShSeq ev_seq(const EvictParams &p, int i) {
     const int4 s = reinterpret_cast<const int4 *>(p.seqs_dev ? p.seqs_dev : p.seqs)[i];
@@ -40,48 +46,100 @@ __device__ __forceinline__ unsigned ev_rank(float m, int pos, int first, int fro
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-/* exclusive prefix sums over the workgroup's threads of (a, b); ta, tb: the totals */
-__device__ __forceinline__ void ev_scan2(int &a, int &b, int &ta, int &tb, int *s_part) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int ia = a, ib = b;
+/* inclusive sums over the lanes of a wave */
+__device__ __forceinline__ int ev_wave_sum(int v) {
 #pragma unroll
     for (int sh = 1; sh < 64; sh <<= 1) {
-        const int xa = __shfl_up(ia, sh), xb = __shfl_up(ib, sh);
-        if (lane >= sh) {
-            ia += xa;
-            ib += xb;
-        }
+        const int x = __shfl_up(v, sh);
+        if ((threadIdx.x & 63) >= sh) v += x;
     }
-    __syncthreads();
-    if (lane == 63) {
+    return v;
+}
+
+/* exclusive prefix sums of (a, b) over the TPB threads, through s_part [2][TPB / 64] of this scan's own */
+template <int TPB>
+__device__ __forceinline__ void ev_scan2(int &a, int &b, int *s_part) {
+    constexpr int NW = TPB / 64;
+    const int wave = threadIdx.x >> 6, ia = ev_wave_sum(a), ib = ev_wave_sum(b);
+    if ((threadIdx.x & 63) == 63) {
         s_part[wave] = ia;
-        s_part[16 + wave] = ib;
+        s_part[NW + wave] = ib;
     }
     __syncthreads();
     int oa = 0, ob = 0;
-    ta = tb = 0;
 #pragma unroll
-    for (int w = 0; w < EV_TPB / 64; w++) {
-        if (w == wave) {
-            oa = ta;
-            ob = tb;
+    for (int w = 0; w < NW; w++)
+        if (w < wave) {
+            oa += s_part[w];
+            ob += s_part[NW + w];
         }
-        ta += s_part[w];
-        tb += s_part[16 + w];
-    }
     a = oa + ia - a;
     b = ob + ib - b;
+}
+
+/* V^T elements and K pieces of n moves (dst, src: shared memory) by TPB threads, and their mass and position, MB moves at
+ * a time. All loads of a round go out before its first store (source and target could be the same row for all the
+ * compiler knows). */
+template <int TPB, int MB>
+__device__ __forceinline__ void ev_move(const EvictParams &p, const ShSeq &sq, int g, const int *dst, const int *src, int n) {
+    const int tid = threadIdx.x, hd = p.hd;
+    const long long at = ((long long)sq.slot * p.Hkv + g) * p.m_stride;
+    const long long base = (long long)sq.slot * p.c_slot_stride + (long long)g * p.cap * hd;
+    uint16_t *kc = p.kc + base, *vt = p.vtc + base;
+    constexpr int DS = TPB / MB, U = 128 / DS, KU = 2;
+    const int pieces = hd / 8;
+    for (int m0 = 0; m0 < n; m0 += MB) {
+        const int mn = min(MB, n - m0), m = m0 + tid % MB;
+        const bool mine = m < n;
+        uint4 kx[KU];
+#pragma unroll
+        for (int u = 0; u < KU; u++) {
+            const int e = tid + u * TPB;
+            if (e < mn * pieces) kx[u] = *reinterpret_cast<const uint4 *>(kc + (long long)src[m0 + e / pieces] * hd + e % pieces * 8);
+        }
+        float mass = 0.0f;
+        int pos = 0;
+        if (tid < mn) {
+            mass = p.mass[at + src[m0 + tid]];
+            pos = p.row_pos[at + src[m0 + tid]];
+        }
+        const int sm = mine ? src[m] : 0, dm = mine ? dst[m] : 0;
+        const long long so = (long long)(sm / SMOL_SLAB) * SMOL_SLAB * hd + sm % SMOL_SLAB;
+        const long long to = (long long)(dm / SMOL_SLAB) * SMOL_SLAB * hd + dm % SMOL_SLAB;
+        for (int d0 = tid / MB; d0 < hd; d0 += U * DS) {
+            uint16_t x[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) x[u] = mine && d0 + u * DS < hd ? vt[so + (d0 + u * DS) * SMOL_SLAB] : (uint16_t)0;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (mine && d0 + u * DS < hd) vt[to + (d0 + u * DS) * SMOL_SLAB] = x[u];
+        }
+#pragma unroll
+        for (int u = 0; u < KU; u++) {
+            const int e = tid + u * TPB;
+            if (e < mn * pieces) *reinterpret_cast<uint4 *>(kc + (long long)dst[m0 + e / pieces] * hd + e % pieces * 8) = kx[u];
+        }
+        for (int e = tid + KU * TPB; e < mn * pieces; e += TPB) /* head_dim 256 in few threads */
+            *reinterpret_cast<uint4 *>(kc + (long long)dst[m0 + e / pieces] * hd + e % pieces * 8) =
+                *reinterpret_cast<const uint4 *>(kc + (long long)src[m0 + e / pieces] * hd + e % pieces * 8);
+        if (tid < mn) {
+            p.mass_out[at + dst[m0 + tid]] = mass;
+            p.pos_out[at + dst[m0 + tid]] = pos;
+        }
+    }
 }
 
 } // namespace
 
 /* ROWS: the longest sequence whose ranks stay in LDS; 0: any, its ranks formed again at each reading */
-template <int ROWS>
-__global__ __launch_bounds__(EV_TPB) void k_evict_select(const EvictParams p) {
+template <int ROWS, int TPB>
+__global__ __launch_bounds__(TPB) void k_evict_select(const EvictParams p) {
     constexpr bool LDS = ROWS > 0;
+    constexpr int NW = TPB / 64, NB = EV_BINS / TPB, U = 8;
     __shared__ unsigned s_rank[LDS ? ROWS : 1];
-    __shared__ int s_hist[EV_BINS], s_part[32], s_found[3];
+    __shared__ int s_hist[3][EV_BINS], s_part[5][2 * NW], s_found[3][2];
     const int tid = threadIdx.x, pair = blockIdx.x, i = pair / p.Hkv, g = pair - i * p.Hkv;
+    const int lane = tid & 63, wave = tid >> 6;
     const ShSeq sq = ev_seq(p, i);
     const int n = sq.len, keep = p.keep, left = min(n, keep);
     const long long at = ((long long)sq.slot * p.Hkv + g) * p.m_stride;
@@ -91,9 +149,9 @@ __global__ __launch_bounds__(EV_TPB) void k_evict_select(const EvictParams p) {
     int *po = p.pos_out + at;
     const bool apart = p.mass_out != p.mass;
     if (n <= keep) {
-        if (tid == 0) p.n_moves[pair] = 0;
+        if (tid == 0 && !p.fused) p.n_moves[pair] = 0;
         if (apart)
-            for (int r = tid; r < n; r += EV_TPB) {
+            for (int r = tid; r < n; r += TPB) {
                 mo[r] = mass[r];
                 po[r] = pos[r];
             }
@@ -101,6 +159,46 @@ __global__ __launch_bounds__(EV_TPB) void k_evict_select(const EvictParams p) {
     }
     const int from = sq.pos - p.recent; /* sq.pos: one past the newest position */
     auto rank_at = [&](int r) { return LDS ? s_rank[r] : ev_rank(mass[r], pos[r], p.first, from); };
+    for (int b = tid; b < 3 * EV_BINS; b += TPB) s_hist[0][b] = 0;
+    __syncthreads();
+
+    /* adds one to the bin of every live lane; a wave whose rows share a bin adds them at once */
+    auto count = [&](int *hist, unsigned bin, bool live) __attribute__((always_inline)) {
+        const unsigned long long who = __ballot(live);
+        if (!who) return;
+        const int lead = __ffsll(who) - 1;
+        const unsigned b0 = __shfl(bin, lead);
+        if (__ballot(live && bin == b0) == who) {
+            if (lane == lead) atomicAdd(&hist[b0], __popcll(who));
+        } else if (live) {
+            atomicAdd(&hist[bin], 1);
+        }
+    };
+    /* the ranks and their first digits, U rows a thread in flight; the rows that stay in place are written where the
+     * arrays are apart (the holes are written again, later) */
+    for (int r0 = tid; r0 - tid < n; r0 += U * TPB) {
+        float m[U];
+        int q[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int r = min(r0 + u * TPB, n - 1);
+            m[u] = mass[r];
+            q[u] = pos[r];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int r = r0 + u * TPB;
+            if (r - tid >= n) break;
+            const unsigned v = ev_rank(m[u], q[u], p.first, from);
+            if (LDS && r < n) s_rank[r] = v;
+            count(s_hist[0], v >> 21, r < n);
+            if (apart && r < left) {
+                mo[r] = m[u];
+                po[r] = q[u];
+            }
+        }
+    }
+    __syncthreads();
 
     /* the keep-th largest rank, digit by digit */
     unsigned prefix = 0;
@@ -108,56 +206,44 @@ __global__ __launch_bounds__(EV_TPB) void k_evict_select(const EvictParams p) {
 #pragma unroll
     for (int pass = 0; pass < 3; pass++) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-        for (int b = tid; b < EV_BINS; b += EV_TPB) s_hist[b] = 0;
+        if (pass > 0) {
+            for (int r0 = 0; r0 < n; r0 += TPB) {
+                const int r = r0 + tid;
+                const unsigned v = r < n ? rank_at(r) : 0;
+                count(s_hist[pass], (v >> shift) & ((1u << bits) - 1),
+                      r < n && (v >> (shift + bits)) == (prefix >> (shift + bits)));
+            }
+            __syncthreads();
+        }
+        /* thread t holds NB bins, the highest first: the rows in the bins above them are the threads' before it */
+        int cnt[NB], sum = 0;
+#pragma unroll
+        for (int b = 0; b < NB; b++) sum += cnt[b] = s_hist[pass][EV_BINS - 1 - NB * tid - b];
+        const int incl = ev_wave_sum(sum);
+        if (lane == 63) s_part[pass][wave] = incl;
         __syncthreads();
-        for (int r0 = 0; r0 < n; r0 += EV_TPB) {
-            const int r = r0 + tid;
-            unsigned v = 0;
-            bool live = r < n;
-            if (live) {
-                if (LDS && pass == 0) {
-                    v = ev_rank(mass[r], pos[r], p.first, from);
-                    s_rank[r] = v;
-                } else {
-                    v = rank_at(r);
-                }
-                live = pass == 0 || (v >> (shift + bits)) == (prefix >> (shift + bits));
+        int above = incl - sum;
+#pragma unroll
+        for (int w = 0; w < NW; w++)
+            if (w < wave) above += s_part[pass][w];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            if (above < need && above + cnt[b] >= need) {
+                s_found[pass][0] = EV_BINS - 1 - NB * tid - b;
+                s_found[pass][1] = need - above;
             }
-            /* a wave whose rows share a bin adds them at once */
-            const unsigned bin = (v >> shift) & ((1u << bits) - 1);
-            const unsigned long long who = __ballot(live);
-            if (who) {
-                const int lead = __ffsll(who) - 1;
-                const unsigned b0 = __shfl(bin, lead);
-                if (__ballot(live && bin == b0) == who) {
-                    if ((tid & 63) == lead) atomicAdd(&s_hist[b0], __popcll(who));
-                } else if (live) {
-                    atomicAdd(&s_hist[bin], 1);
-                }
-            }
+            above += cnt[b];
         }
         __syncthreads();
-        /* thread t holds the bins 2 (1023 - t) + 1 and 2 (1023 - t): an exclusive scan counts the rows above them */
-        const int hi = 2 * (EV_TPB - 1 - tid) + 1;
-        const int ch = s_hist[hi], cl = s_hist[hi - 1];
-        int above = ch + cl, z = 0, ta, tb;
-        ev_scan2(above, z, ta, tb, s_part);
-        if (above < need && above + ch + cl >= need) {
-            const bool in_hi = above + ch >= need;
-            s_found[0] = in_hi ? hi : hi - 1;
-            s_found[1] = need - (in_hi ? above : above + ch);
-        }
-        __syncthreads();
-        prefix |= (unsigned)s_found[0] << shift;
-        need = s_found[1];
-        __syncthreads();
+        prefix |= (unsigned)s_found[pass][0] << shift;
+        need = s_found[pass][1];
     }
 
     /* rows above the threshold stay, and the lowest `need` rows at it */
-    const int per = ((n + EV_TPB - 1) / EV_TPB) | 1, b0 = min(n, tid * per), b1 = min(n, b0 + per);
-    int eq = 0, z = 0, te, tz;
+    const int per = ((n + TPB - 1) / TPB) | 1, b0 = min(n, tid * per), b1 = min(n, b0 + per);
+    int eq = 0, z = 0;
     for (int r = b0; r < b1; r++) eq += rank_at(r) == prefix;
-    ev_scan2(eq, z, te, tz, s_part);
+    ev_scan2<TPB>(eq, z, s_part[3]);
     auto walk = [&](auto f) __attribute__((always_inline)) {
         int e = eq;
         for (int r = b0; r < b1; r++) {
@@ -167,24 +253,32 @@ __global__ __launch_bounds__(EV_TPB) void k_evict_select(const EvictParams p) {
             f(r, kept);
         }
     };
-    int holes = 0, movers = 0, th, tm;
+    int holes = 0, movers = 0;
     walk([&](int r, bool kept) {
         holes += r < keep && !kept;
         movers += r >= keep && kept;
     });
-    ev_scan2(holes, movers, th, tm, s_part);
-    int *dst = p.moves + (long long)pair * 2 * p.max_moves, *src = dst + p.max_moves;
-    walk([&](int r, bool kept) {
-        if (r < keep && !kept) dst[holes++] = r;
-        if (r >= keep && kept) src[movers++] = r;
-    });
-    if (tid == 0) p.n_moves[pair] = th;
-    /* the rows that stay in place; k_evict_move writes the holes (in a launch behind this one) */
-    if (apart)
-        for (int r = tid; r < left; r += EV_TPB) {
-            mo[r] = mass[r];
-            po[r] = pos[r];
-        }
+    ev_scan2<TPB>(holes, movers, s_part[4]);
+    if (p.fused) {
+        walk([&](int r, bool kept) {
+            if (r < keep && !kept) s_hist[0][holes++] = r;
+            if (r >= keep && kept) s_hist[1][movers++] = r;
+        });
+    } else {
+        int *dst = p.moves + (long long)pair * 2 * p.max_moves, *src = dst + p.max_moves;
+        walk([&](int r, bool kept) {
+            if (r < keep && !kept) dst[holes++] = r;
+            if (r >= keep && kept) src[movers++] = r;
+        });
+    }
+    /* as many holes as movers; the last thread's counts are the totals */
+    if (tid == TPB - 1) {
+        if (p.fused) s_found[0][0] = holes;
+        else p.n_moves[pair] = holes;
+    }
+    if (!p.fused) return;
+    __syncthreads();
+    ev_move<TPB, TPB == 1024 ? 64 : 32>(p, sq, g, s_hist[0], s_hist[1], s_found[0][0]);
 }
 
 __global__ __launch_bounds__(256) void k_evict_move(const EvictParams p) {
@@ -193,52 +287,29 @@ __global__ __launch_bounds__(256) void k_evict_move(const EvictParams p) {
     const int total = p.n_moves[pair];
     if (m0 >= total) return;
     const int tid = threadIdx.x, i = pair / p.Hkv, g = pair - i * p.Hkv, n = min(EV_MOVES, total - m0);
-    const ShSeq sq = ev_seq(p, i);
-    const int *dst = p.moves + (long long)pair * 2 * p.max_moves + m0, *src = dst + p.max_moves;
-    const long long at = ((long long)sq.slot * p.Hkv + g) * p.m_stride;
     if (tid < n) {
-        const int d = dst[tid], s = src[tid];
-        s_dst[tid] = d;
-        s_src[tid] = s;
-        p.mass_out[at + d] = p.mass[at + s];
-        p.pos_out[at + d] = p.row_pos[at + s];
+        const int *dst = p.moves + (long long)pair * 2 * p.max_moves + m0 + tid;
+        s_dst[tid] = dst[0];
+        s_src[tid] = dst[p.max_moves];
     }
     __syncthreads();
-    const int hd = p.hd, pieces = hd / 8;
-    const long long base = (long long)sq.slot * p.c_slot_stride + (long long)g * p.cap * hd;
-    uint16_t *kc = p.kc + base, *vt = p.vtc + base;
-    for (int e = tid; e < n * pieces; e += 256) {
-        const int m = e / pieces, d0 = (e - m * pieces) * 8;
-        *reinterpret_cast<uint4 *>(kc + (long long)s_dst[m] * hd + d0) =
-            *reinterpret_cast<const uint4 *>(kc + (long long)s_src[m] * hd + d0);
-    }
-    const int m = tid % EV_MOVES;
-    if (m < n) {
-        const long long so = (long long)(s_src[m] / SMOL_SLAB) * SMOL_SLAB * hd + s_src[m] % SMOL_SLAB;
-        const long long to = (long long)(s_dst[m] / SMOL_SLAB) * SMOL_SLAB * hd + s_dst[m] % SMOL_SLAB;
-        /* eight loads in flight before the first store (source and target could be the same row for all the compiler
-         * knows) */
-        constexpr int DS = 256 / EV_MOVES;
-        for (int d0 = tid / EV_MOVES; d0 < hd; d0 += 8 * DS) {
-            uint16_t x[8];
-#pragma unroll
-            for (int u = 0; u < 8; u++) x[u] = d0 + u * DS < hd ? vt[so + (d0 + u * DS) * SMOL_SLAB] : (uint16_t)0;
-#pragma unroll
-            for (int u = 0; u < 8; u++)
-                if (d0 + u * DS < hd) vt[to + (d0 + u * DS) * SMOL_SLAB] = x[u];
-        }
-    }
+    ev_move<256, EV_MOVES>(p, ev_seq(p, i), g, s_dst, s_src, n);
 }
+
+extern "C" int smol_evict_fused(int max_moves) { return max_moves <= EV_FUSED; }
 
 /* max_rows: rows of the longest sequence */
 extern "C" int smol_launch_evict(const EvictParams *p, int max_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1) {
     const unsigned pairs = (unsigned)p->n_seq * p->Hkv;
-    if (max_rows <= 4096) hipExtLaunchKernelGGL((k_evict_select<4096>), dim3(pairs), dim3(EV_TPB), 0, st, e0, nullptr, 0, *p);
-    else if (max_rows <= 32768) hipExtLaunchKernelGGL((k_evict_select<32768>), dim3(pairs), dim3(EV_TPB), 0, st, e0, nullptr, 0, *p);
-    else hipExtLaunchKernelGGL((k_evict_select<0>), dim3(pairs), dim3(EV_TPB), 0, st, e0, nullptr, 0, *p);
+    const hipEvent_t e = p->fused ? e1 : nullptr;
+    /* 256 threads for up to 1024 rows: a barrier among four waves instead of sixteen */
+    if (max_rows <= 1024) hipExtLaunchKernelGGL((k_evict_select<1024, 256>), dim3(pairs), dim3(256), 0, st, e0, e, 0, *p);
+    else if (max_rows <= 8192) hipExtLaunchKernelGGL((k_evict_select<8192, 1024>), dim3(pairs), dim3(1024), 0, st, e0, e, 0, *p);
+    else if (max_rows <= 32768) hipExtLaunchKernelGGL((k_evict_select<32768, 1024>), dim3(pairs), dim3(1024), 0, st, e0, e, 0, *p);
+    else hipExtLaunchKernelGGL((k_evict_select<0, 1024>), dim3(pairs), dim3(1024), 0, st, e0, e, 0, *p);
     if (hipGetLastError() != hipSuccess) return -3;
+    if (p->fused) return 0;
     const unsigned blocks = pairs * (unsigned)((p->max_moves + EV_MOVES - 1) / EV_MOVES);
-    if (blocks == 0) return 0;
     hipExtLaunchKernelGGL(k_evict_move, dim3(blocks), dim3(256), 0, st, nullptr, e1, 0, *p);
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }

@@ -317,6 +317,7 @@ typedef struct {
     int *moves;                /* [pair][2 max_moves]: holes, then the rows that fill them */
     int *n_moves;              /* [pair] */
     int max_moves;
+    int fused;                 /* the selecting workgroup makes the moves (no list in memory) */
     int n_seq;
     const ShSeq *seqs_dev;     /* (slot, rows, end) of each sequence when n_seq > SH_ARG_SEQS */
     ShSeq seqs[SH_ARG_SEQS];

@@ -45,19 +45,18 @@ struct ShGeom {
 };
 
 constexpr int SH_NW = 4, SH_TPB = 64 * SH_NW;
-constexpr int Q_PARTS = 3;
+constexpr int Q_PARTS = 3, P_PARTS = 3;
 
 template <int HD, int NT>
 struct ShLds {
     using Gm = ShGeom<HD>;
-    static constexpr int TR = 16 * NT;
-    static constexpr int RAW = (TR + 1) * Gm::QSTR;               /* staged rows, the new key's behind them */
-    static constexpr int ROT = 16 * Gm::QSTR;                     /* an own-rows item's rotated rows */
-    static constexpr int CB = SH_NW * 16 * Gm::OSTR + 2 * (SH_NW + 1) * 16; /* a row tile's outputs of every wave */
-    static constexpr int UNI = RAW + ROT > CB ? RAW + ROT : CB;
+    static constexpr int TR = 16 * NT, CH8 = HD / 8;
+    static constexpr int RAW = (TR + 1) * Gm::QSTR;               /* the rows times the norm's weights, the new key's behind */
+    static constexpr int CB = SH_NW * 16 * Gm::OSTR + 2 * SH_NW * 16; /* a row tile's outputs of every wave, their m and l */
+    static constexpr int UNI = RAW > CB ? RAW : CB;
     static constexpr int FRAG = Q_PARTS * Gm::KS * NT * 256;      /* Q fragments: 16 bytes a lane */
-    static constexpr int SMALL = TR + 2 + 2 * Gm::HDP + 16;       /* 1 / rms, new key and value, new scores */
-    static constexpr int FLOATS = UNI + FRAG + ((SMALL + 3) & ~3);
+    static constexpr int SS = ((TR + 1) * CH8 + 3) & ~3;          /* a row's squares by chunk; then the new scores by chunk */
+    static constexpr int FLOATS = UNI + FRAG + SS + 2 * Gm::HDP;  /* the new key and value last */
 };
 
 __device__ __forceinline__ void ld8f(const float *a, float *v) {
@@ -135,10 +134,9 @@ __device__ __forceinline__ void sh_item(const ShParams &p, const ShItem &it, flo
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int G = p.G, R = it.R;
-    float *s_raw = smem, *s_rot = smem + L::RAW;
+    float *s_raw = smem;
     uint4 *s_frag = reinterpret_cast<uint4 *>(smem + L::UNI);
-    float *s_small = smem + L::UNI + L::FRAG;
-    float *s_rinv = s_small, *s_knew = s_small + TR + 2, *s_vnew = s_knew + HDP, *s_snew = s_vnew + HDP;
+    float *s_ss = smem + L::UNI + L::FRAG, *s_knew = s_ss + L::SS, *s_vnew = s_knew + HDP;
 
     /* ---- the slab pipeline's loads ---- */
     struct KRaw { uint4 k[2][KS]; };
@@ -181,124 +179,135 @@ __device__ __forceinline__ void sh_item(const ShParams &p, const ShItem &it, flo
     KRaw kr;
     VRaw vr;
 
-    /* ---- stage the rows: raw, 1 / rms, rotated and split into fragments ---- */
-    constexpr int CH8 = HD / 8, CHP = HDP / 8;
+    /* ---- stage the rows: normalised, rotated and split into fragments ----
+     * Thread chunks of 8 elements; every load of a chunk (its row, the table
+     * row, the weights) is issued before the first is used, and the first
+     * slab's behind them. */
+    constexpr int CH8 = HD / 8, HALF = HD / 2;
+    constexpr int NQ = ((TR + 1) * CH8 + SH_TPB - 1) / SH_TPB;
     const int n_rows = R + (it.with_new ? 1 : 0); /* row R: the new key */
     auto row_seq = [&](int r) { return it.prefix ? (it.row0 + r) / G : it.seq; };
     auto row_head = [&](int r) { return it.g * G + (it.prefix ? (it.row0 + r) % G : it.row0 + r); };
-    for (int e = tid; e < n_rows * CH8; e += SH_TPB) {
-        const int r = e / CH8, d0 = (e - r * CH8) * 8;
-        float v[8];
-        if (r < R) load8(p.q_in, p.in_dtype, (long long)row_seq(r) * p.Hq * HD + (long long)row_head(r) * HD + d0, v);
-        else load8(p.k_in, p.in_dtype, ((long long)it.seq * p.Hkv + it.g) * HD + d0, v);
-        st8f(s_raw + r * QSTR + d0, v);
+    const bool rope = p.rope_kind != SMOL_ROPE_OFF;
+    float x[NQ][8], cv[NQ][8], sn[NQ][8];
+    ShSeq own;
+    if (!it.prefix) own = sh_seq(p, it.seq);
+#pragma unroll
+    for (int u = 0; u < NQ; u++) {
+        const int e = tid + SH_TPB * u, r = e / CH8, d0 = (e - r * CH8) * 8;
+        if (e < n_rows * CH8) {
+            const int sq = r < R ? row_seq(r) : it.seq;
+            if (r < R) load8(p.q_in, p.in_dtype, (long long)sq * p.Hq * HD + (long long)row_head(r) * HD + d0, x[u]);
+            else load8(p.k_in, p.in_dtype, ((long long)sq * p.Hkv + it.g) * HD + d0, x[u]);
+            if (rope) {
+                const long long at = (long long)(it.prefix ? sh_seq(p, sq).pos : own.pos) * HD + d0;
+                ld8f(p.rope_cos + at, cv[u]);
+                ld8f(p.rope_sin + at, sn[u]);
+            }
+        }
     }
-    if (it.with_new && tid < CH8) {
-        float v[8];
-        load8(p.v_in, p.in_dtype, ((long long)it.seq * p.Hkv + it.g) * HD + tid * 8, v);
-        st8f(s_vnew + tid * 8, v);
-    }
+    float vn[8];
+    if (it.with_new && tid < CH8) load8(p.v_in, p.in_dtype, ((long long)it.seq * p.Hkv + it.g) * HD + tid * 8, vn);
     issue_k(k0, kr);
     issue_v(k0, vr);
-    __syncthreads();
-    auto row_dot8 = [&](const float *a, const float *b, int jj) __attribute__((always_inline)) {
-        float sd = 0.0f;
-#pragma unroll
-        for (int ci = 0; ci < (CH8 + 7) / 8; ci++) {
-            const int ch = jj + 8 * ci;
-            if (ch >= CH8) break;
-            float x[8], y[8];
-            ld8f(a + 8 * ch, x);
-            ld8f(b + 8 * ch, y);
-#pragma unroll
-            for (int i = 0; i < 8; i++) sd = fmaf(x[i], y[i], sd);
-        }
-        sd += __shfl_xor(sd, 1, 8);
-        sd += __shfl_xor(sd, 2, 8);
-        sd += __shfl_xor(sd, 4, 8);
-        return sd;
-    };
-    if (p.q_norm || p.k_norm) {
-#pragma unroll
-        for (int ri = 0; ri < (TR + 1 + SH_TPB / 8 - 1) / (SH_TPB / 8); ri++) {
-            const int r0 = ri * (SH_TPB / 8) + (tid >> 3), r = min(r0, n_rows - 1);
-            const float ss = row_dot8(s_raw + r * QSTR, s_raw + r * QSTR, tid & 7);
-            if (r0 < n_rows && (tid & 7) == 0) s_rinv[r] = 1.0f / sqrtf(ss / (float)HD + p.norm_eps);
-        }
-        __syncthreads();
+    /* rows past R are zero columns */
+    for (int e = tid; e < (TR - R) * 4 * KS * Q_PARTS; e += SH_TPB) {
+        const int r = R + e % (TR - R), w = e / (TR - R), ks = w / 4 % KS, q = w / (4 * KS);
+        s_frag[((q * KS + ks) * NT + (r >> 4)) * 64 + (w & 3) * 16 + (r & 15)] = make_uint4(0, 0, 0, 0);
     }
-    for (int e = tid; e < (TR + 1) * CHP; e += SH_TPB) {
-        const int r = e / CHP, d0 = (e - r * CHP) * 8;
-        /* rows [0, TR) are fragments (zeros past R), row TR stands for the new key */
-        const bool is_k = r == TR;
-        if (is_k && !it.with_new) break;
-        float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if ((is_k || r < R) && d0 < HD) {
-            const int lr = is_k ? R : r;
-            const float *row = s_raw + lr * QSTR;
-            const float *w = is_k ? p.k_norm : p.q_norm;
-            const float ri = w ? s_rinv[lr] : 1.0f;
-            float x[8];
-            ld8f(row + d0, x);
+    if constexpr (HDP > HD) /* and so are columns past head_dim */
+        for (int e = tid; e < R * (HDP - HD) / 8 * Q_PARTS; e += SH_TPB) {
+            const int r = e % R, w = e / R, d0 = HD + w % ((HDP - HD) / 8) * 8, q = w / ((HDP - HD) / 8);
+            s_frag[((q * KS + d0 / 32) * NT + (r >> 4)) * 64 + (d0 >> 3 & 3) * 16 + (r & 15)] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+    for (int u = 0; u < NQ; u++) {
+        const int e = tid + SH_TPB * u, r = e / CH8, d0 = (e - r * CH8) * 8;
+        if (e < n_rows * CH8) {
+            const float *w = r < R ? p.q_norm : p.k_norm;
             if (w) {
+                float ss = 0.0f, wv[8];
+                ld8f(w + d0, wv);
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = (x[i] * w[d0 + i]) * ri;
+                for (int i = 0; i < 8; i++) {
+                    ss = fmaf(x[u][i], x[u][i], ss);
+                    x[u][i] *= wv[i];
+                }
+                s_ss[e] = ss;
             }
-            if (p.rope_kind == SMOL_ROPE_OFF) {
+            st8f(s_raw + r * QSTR + d0, x[u]);
+        }
+    }
+    if (it.with_new && tid < CH8) st8f(s_vnew + tid * 8, vn);
+    __syncthreads();
 #pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = x[i];
+    for (int u = 0; u < NQ; u++) {
+        const int e = tid + SH_TPB * u, r = e / CH8, d0 = (e - r * CH8) * 8;
+        if (e < n_rows * CH8) {
+            const bool is_k = r >= R;
+            float ri = is_k ? 1.0f : p.qscale;
+            if (is_k ? p.k_norm != nullptr : p.q_norm != nullptr) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int i = 0; i < CH8; i++) ss += s_ss[r * CH8 + i];
+                ri *= 1.0f / sqrtf(ss / (float)HD + p.norm_eps);
+            }
+            float y[8];
+            if (!rope) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) y[i] = x[u][i];
+            } else if (p.rope_kind == SMOL_ROPE_INTERLEAVED_K) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    y[i] = fmaf(x[u][i], cv[u][i], -(x[u][i + 1] * sn[u][i]));
+                    y[i + 1] = fmaf(x[u][i + 1], cv[u][i + 1], x[u][i] * sn[u][i + 1]);
+                }
             } else {
-                const long long tr = (long long)sh_seq(p, is_k ? it.seq : row_seq(r)).pos * HD + d0;
-                float cv[8], sv[8];
-                ld8f(p.rope_cos + tr, cv);
-                ld8f(p.rope_sin + tr, sv);
-                if (p.rope_kind == SMOL_ROPE_INTERLEAVED_K) {
+                const float *row = s_raw + r * QSTR;
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        y[i] = x[i] * cv[i] - x[i + 1] * sv[i];
-                        y[i + 1] = x[i + 1] * cv[i + 1] + x[i] * sv[i + 1];
-                    }
-                } else {
-                    constexpr int HALF = HD / 2;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int d = d0 + i, pd = d < HALF ? d + HALF : d - HALF;
-                        const float pr = w ? (row[pd] * w[pd]) * ri : row[pd];
-                        y[i] = d < HALF ? fmaf(x[i], cv[i], -(pr * sv[i])) : fmaf(x[i], cv[i], pr * sv[i]);
-                    }
+                for (int i = 0; i < 8; i++) {
+                    const int d = d0 + i;
+                    const float pr = row[d < HALF ? d + HALF : d - HALF];
+                    y[i] = d < HALF ? fmaf(x[u][i], cv[u][i], -(pr * sn[u][i])) : fmaf(x[u][i], cv[u][i], pr * sn[u][i]);
                 }
             }
-        }
-        if (is_k) {
-            st8f(s_knew + d0, y);
-            continue;
-        }
 #pragma unroll
-        for (int i = 0; i < 8; i++) y[i] *= p.qscale;
-        if (it.with_new) st8f(s_rot + r * QSTR + d0, y);
-        b8 f[Q_PARTS];
-        split8x3(y, f[0], f[1], f[2]);
-        const int ks = d0 / 32, at = ((d0 >> 3) & 3) * 16 + (r & 15);
+            for (int i = 0; i < 8; i++) x[u][i] = y[i] * ri;
+            if (is_k) {
+                st8f(s_knew + d0, x[u]);
+            } else {
+                b8 f[Q_PARTS];
+                split8x3(x[u], f[0], f[1], f[2]);
+                const int ks = d0 / 32, at = ((d0 >> 3) & 3) * 16 + (r & 15);
 #pragma unroll
-        for (int q = 0; q < Q_PARTS; q++)
-            s_frag[((q * KS + ks) * NT + (r >> 4)) * 64 + at] = *reinterpret_cast<uint4 *>(&f[q]);
+                for (int q = 0; q < Q_PARTS; q++)
+                    s_frag[((q * KS + ks) * NT + (r >> 4)) * 64 + at] = *reinterpret_cast<uint4 *>(&f[q]);
+            }
+        }
     }
     __syncthreads();
     if (it.with_new) {
-        /* the new key's fp32 score of every row, and its row and the new value in the cache */
-        const int r = tid >> 3;
-        if (r < 16) {
-            const int rr = min(r, R - 1);
-            float sd = row_dot8(s_rot + rr * QSTR, s_knew, tid & 7);
-            if (p.cap2 > 0.0f) sd = p.cap2 * tanhf(sd / p.cap2);
-            if ((tid & 7) == 0) {
-                s_snew[r] = sd;
-                if (SC && r < R) p.logit_new[(long long)it.seq * p.Hq + row_head(r)] = sd;
+        /* the new key's fp32 score by chunks: row_new() sums them */
+#pragma unroll
+        for (int u = 0; u < NQ; u++) {
+            const int e = tid + SH_TPB * u, r = e / CH8, d0 = (e - r * CH8) * 8;
+            if (r < R) {
+                float kn[8], sd = 0.0f;
+                ld8f(s_knew + d0, kn);
+#pragma unroll
+                for (int i = 0; i < 8; i++) sd = fmaf(x[u][i], kn[i], sd);
+                s_ss[e] = sd;
             }
         }
     }
+    auto row_new = [&](int r) __attribute__((always_inline)) {
+        float sd = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CH8; i++) sd += s_ss[r * CH8 + i];
+        return p.cap2 > 0.0f ? p.cap2 * tanhf(sd / p.cap2) : sd;
+    };
 
-    /* ---- fragments, row ranges, state ---- */
+    /* ---- row ranges, state ---- */
     float m[NT], l[NT];
     f4 o[NT][DT];
     int lo[NT], lo_min = 1 << 30, lo_max = 0; /* window: the first key that a row sees */
@@ -408,8 +417,8 @@ __device__ __forceinline__ void sh_item(const ShParams &p, const ShItem &it, flo
                 ps += pv[e];
             }
             l[t] += ps;
-            b8 ph, pl;
-            split8(pv, ph, pl);
+            b8 pp[P_PARTS];
+            split8x3(pv, pp[0], pp[1], pp[2]);
             if (apart) {
                 /* a row must not meet 0 x inf: one row at a time, against
                  * the values that it sees */
@@ -418,17 +427,18 @@ __device__ __forceinline__ void sh_item(const ShParams &p, const ShItem &it, flo
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) {
                         const b8 v = as_b8(keep_keys8(vr.v[dt], k0 + 8 * j, lo_r, it.ke));
-                        f4 a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pl, f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                        a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph, a, 0, 0, 0);
+                        f4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int q = P_PARTS - 1; q >= 0; q--) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pp[q], a, 0, 0, 0);
                         if (c == r) o[t][dt] += a;
                     }
                 }
             } else {
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(vr.v[dt]), pl, o[t][dt], 0, 0, 0);
-                    o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(vr.v[dt]), ph, o[t][dt], 0, 0, 0);
-                }
+                for (int q = P_PARTS - 1; q >= 0; q--)
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++)
+                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(vr.v[dt]), pp[q], o[t][dt], 0, 0, 0);
             }
         }
         issue_v(k1, vr);
@@ -436,7 +446,7 @@ __device__ __forceinline__ void sh_item(const ShParams &p, const ShItem &it, flo
     }
 
     /* ---- the waves' states (and the new token's) join, one row tile at a time ---- */
-    float *cb = smem, *cm = smem + SH_NW * 16 * OSTR, *cl = cm + (SH_NW + 1) * 16;
+    float *cb = smem, *cm = smem + SH_NW * 16 * OSTR, *cl = cm + SH_NW * 16;
     for (int t = 0; t < NT; t++) {
         __syncthreads();
 #pragma unroll
@@ -455,14 +465,15 @@ __device__ __forceinline__ void sh_item(const ShParams &p, const ShItem &it, flo
         for (int e = tid; e < 16 * (HD / 4); e += SH_TPB) {
             const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
             if (t * 16 + r >= R) continue;
-            float mm = it.with_new ? s_snew[r] : -INFINITY;
+            const float s_new = it.with_new ? row_new(r) : -INFINITY;
+            float mm = s_new;
 #pragma unroll
             for (int w = 0; w < SH_NW; w++) mm = fmaxf(mm, cm[w * 16 + r]);
             const float mu = mm == -INFINITY ? 0.0f : mm;
             f4 acc = {0.f, 0.f, 0.f, 0.f};
             float ls = 0.0f;
             if (it.with_new) {
-                ls = __builtin_amdgcn_exp2f(s_snew[r] - mu);
+                ls = __builtin_amdgcn_exp2f(s_new - mu);
                 acc = *reinterpret_cast<f4 *>(s_vnew + d) * ls;
             }
 #pragma unroll
@@ -472,7 +483,10 @@ __device__ __forceinline__ void sh_item(const ShParams &p, const ShItem &it, flo
                 acc += f * *reinterpret_cast<f4 *>(cb + (w * 16 + r) * OSTR + d);
             }
             *reinterpret_cast<f4 *>(it.part_o + (long long)(t * 16 + r) * HD + d) = acc;
-            if (d == 0) *reinterpret_cast<float2 *>(it.part_ml + (t * 16 + r) * 2) = make_float2(mm, ls);
+            if (d == 0) {
+                *reinterpret_cast<float2 *>(it.part_ml + (t * 16 + r) * 2) = make_float2(mm, ls);
+                if (SC && it.with_new) p.logit_new[(long long)it.seq * p.Hq + row_head(r)] = s_new;
+            }
         }
     }
     if (it.with_new && it.row0 == 0) {
@@ -492,7 +506,7 @@ __device__ __forceinline__ void sh_item(const ShParams &p, const ShItem &it, flo
 } // namespace
 
 template <int HD, int NT, bool SC>
-__global__ __launch_bounds__(SH_TPB) void k_sh(const ShParams p) {
+__global__ __launch_bounds__(SH_TPB, HD <= 128 && NT <= 2 ? 2 : 1) void k_sh(const ShParams p) {
     __shared__ __attribute__((aligned(16))) float smem[ShLds<HD, NT>::FLOATS];
     const int b = blockIdx.x;
     ShItem it;
@@ -640,6 +654,11 @@ static int launch_hd(const ShParams *p, int nt, int max_len, hipStream_t st, hip
     const unsigned blocks = (unsigned)p->n_pblocks + (unsigned)p->n_ss * p->n_seq * p->Hkv * p->s_rb;
     if (p->mass) hipExtLaunchKernelGGL((k_sh<HD, 1, true>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
     else if (nt == 1) hipExtLaunchKernelGGL((k_sh<HD, 1, false>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
+    else if (nt == 4 && HD <= 128) {
+        if constexpr (HD <= 128) hipExtLaunchKernelGGL((k_sh<HD, 4, false>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
+    } else if (nt == 2 && HD == 256) {
+        if constexpr (HD == 256) hipExtLaunchKernelGGL((k_sh<HD, 2, false>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
+    }
     else if constexpr (HD <= 128) hipExtLaunchKernelGGL((k_sh<HD, 2, false>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
     else return -1;
     if (hipGetLastError() != hipSuccess) return -3;
@@ -651,6 +670,9 @@ static int launch_hd(const ShParams *p, int nt, int max_len, hipStream_t st, hip
 
 /* rows of a prefix item's tile at head_dim hd, for a batch of `rows` rows a kv head */
 extern "C" int smol_shared_tile_rows(int hd, int rows) { return rows <= 16 || hd > 128 ? 16 : 32; }
+
+/* workgroups of a compute unit at once (k_sh's launch bounds) */
+extern "C" int smol_shared_occupancy(int hd) { return hd <= 128 ? 2 : 1; }
 
 extern "C" int smol_launch_shared(const ShParams *p, int hd, int tile_rows, int max_len, hipStream_t st, hipEvent_t e0,
                                   hipEvent_t e1) {

@@ -11,6 +11,7 @@ The names mirror the reference's kernel API (common/kernels/smol_kernels.h):
 ``smol_sliding_window_attention_softcap``, ``smol_compute_rope_neox`` ... with
 the same argument meaning (``out`` is overwritten in place).
 """
+import array
 import atexit
 import ctypes
 import os
@@ -72,11 +73,11 @@ SIGNATURES = [
     ("smol_attn_decode_noalloc", [_vp, _vp, _c_int, _vp, _c_int, _IP, _IP, _vp, _vp, _vp, _c_int, _c_int,
                                   _c_float, _c_int, _c_float, _vp, _vp, _c_float, _vp], _c_int),
     # a batch on a shared prefix; a cache held to a budget
-    ("smol_attn_decode_shared", [_vp, _vp, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _IP, _IP, _vp, _vp, _vp, _c_int,
+    ("smol_attn_decode_shared", [_vp, _vp, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _c_int,
                                  _c_int, _c_float, _c_int, _c_float, _vp, _vp, _c_float, _vp], _c_int),
-    ("smol_attn_decode_scored", [_vp, _vp, _c_int, _vp, _c_int, _IP, _IP, _IP, _vp, _vp, _vp, _c_int, _c_int, _c_float,
+    ("smol_attn_decode_scored", [_vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_float,
                                  _c_float, _vp, _vp, _c_float, _vp, _vp, _c_int, _c_float, _vp], _c_int),
-    ("smol_kv_cache_evict", [_vp, _c_int, _c_int, _IP, _IP, _IP, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int],
+    ("smol_kv_cache_evict", [_vp, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int],
      _c_int),
     ("smol_kv_cache_pointers", [_vp, _c_int, ctypes.POINTER(_vp), ctypes.POINTER(_vp)], _c_int),
     ("smol_attn_apply_rope", [_vp, _vp, _vp, _IP, _c_int, _c_int], _c_int),
@@ -104,7 +105,7 @@ SIGNATURES = [
                              _c_int], _c_int),
     ("smol_adapters_create", [_vp, _c_int, _c_int, _c_int, _vp, _vp, _IP, _FP, ctypes.POINTER(_vp)], _c_int),
     ("smol_adapters_destroy", [_vp], _c_int),
-    ("smol_linear_adapters_dev", [_vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _vp, _IP], _c_int),
+    ("smol_linear_adapters_dev", [_vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp], _c_int),
     ("smol_linear_ops_dev", [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp], _c_int),
     ("smol_rms_norm_dev", [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_float], _c_int),
     ("smol_bf16_rms_norm_dev", [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_float], _c_int),
@@ -458,48 +459,56 @@ def decode(ctx, kv, layer, rope, slots, pos, q, k_new, v_new, n_heads, scale, wi
                        q_norm, k_norm, eps)()
 
 
-def _on(ctx, t, dtypes, shape, what):
-    """the address of a contiguous tensor of these dtypes and this shape on the context's device"""
-    if not t.is_cuda or t.device.index != ctx.device or not t.is_contiguous():
-        raise SmolAttnError("%s must be a contiguous tensor on device %d" % (what, ctx.device))
-    if t.dtype not in dtypes:
-        raise SmolAttnError("%s is %s" % (what, t.dtype))
-    if tuple(t.shape) != tuple(shape):
-        raise SmolAttnError("%s has shape %s, not %s" % (what, tuple(t.shape), tuple(shape)))
+def _on(ctx, t, dtype, shape, what):
+    """the address of a contiguous tensor of this dtype and shape on the context's device"""
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != ctx.device:
+        raise SmolAttnError("%s must be a contiguous %s tensor of shape %s on device %d, got %s %s on %s" % (
+            what, dtype, tuple(shape), ctx.device, t.dtype, tuple(t.shape), t.device))
     return t.data_ptr()
 
 
 def _host_ints(a, n, what):
-    a = np.ascontiguousarray(a, np.int32)
-    if a.shape != (n,):
-        raise SmolAttnError("%s: %d numbers are wanted, got shape %s" % (what, n, a.shape))
-    return a, a.ctypes.data_as(_IP)
+    """host numbers as C ints, and their address"""
+    if type(a) in (list, tuple):
+        # three times as fast as numpy's conversion of a short list
+        a = array.array("i", a)
+        if len(a) == n:
+            return a, a.buffer_info()[0]
+        shape = (len(a),)
+    else:
+        a = np.ascontiguousarray(a, np.int32)
+        shape = a.shape
+        if shape == (n,):
+            return a, a.__array_interface__["data"][0]
+    raise SmolAttnError("%s: %d numbers are wanted, got shape %s" % (what, n, shape))
 
 
 def _step_args(ctx, kv, q, k_new, v_new, n_heads, q_norm, k_norm, out):
     """what the two decode steps below share: addresses of q, k, v, the norms and out, and the dtype code"""
     import torch
-    n, hd, kvd = q.shape[0], kv.head_dim, kv.n_kv_heads * kv.head_dim
-    dt = _dtype_code(q)
-    ptrs = [_on(ctx, q, (q.dtype,), (n, n_heads * hd), "q")]
-    ptrs += [_on(ctx, t, (q.dtype,), (n, kvd), nm) for t, nm in ((k_new, "k_new"), (v_new, "v_new"))]
-    norms = [None if w is None else _on(ctx, w, (torch.float32,), (hd,), nm)
-             for w, nm in ((q_norm, "q_norm"), (k_norm, "k_norm"))]
+    f32 = torch.float32
+    dtype = q.dtype
+    dt = F32 if dtype is f32 else BF16 if dtype is torch.bfloat16 else _dtype_code(q)
+    n, hd = q.shape[0], kv.head_dim
+    rows, new = (n, n_heads * hd), (n, kv.n_kv_heads * hd)
     if out is None:
-        out = torch.empty((n, n_heads * hd), dtype=torch.float32, device=q.device)
-    return n, ptrs, dt, norms, out, _on(ctx, out, (torch.float32,), (n, n_heads * hd), "out")
+        out = torch.empty(rows, dtype=f32, device=q.device)
+    return (n, _on(ctx, q, dtype, rows, "q"), _on(ctx, k_new, dtype, new, "k_new"), _on(ctx, v_new, dtype, new, "v_new"), dt,
+            None if q_norm is None else _on(ctx, q_norm, f32, (hd,), "q_norm"),
+            None if k_norm is None else _on(ctx, k_norm, f32, (hd,), "k_norm"), out, _on(ctx, out, f32, rows, "out"))
 
 
 def decode_shared(ctx, prefix, prefix_slot, prefix_len, kv, layer, rope, slots, lens, q, k_new, v_new, n_heads, scale,
                   window=0, cap=0.0, out=None, q_norm=None, k_norm=None, eps=1e-6):
     """One decode step of sequences that share the first prefix_len positions, rows of `prefix` at prefix_slot; see
     smol_attn_decode_shared. lens: each sequence's own rows in `kv` before the step. Returns out [n, n_heads*hd]."""
-    n, ptrs, dt, norms, out, optr = _step_args(ctx, kv, q, k_new, v_new, n_heads, q_norm, k_norm, out)
-    sl, slp = _host_ints(slots, n, "slots")
-    le, lep = _host_ints(lens, n, "lens")
-    _check(load().smol_attn_decode_shared(ctx.h, prefix.h, prefix_slot, prefix_len, kv.h, layer, rope.h if rope else None, n,
-                                          slp, lep, *ptrs, dt, n_heads, scale, window, cap, *norms, eps, optr),
-           "smol_attn_decode_shared")
+    n, qp, kp, vp, dt, qw, kw, out, op = _step_args(ctx, kv, q, k_new, v_new, n_heads, q_norm, k_norm, out)
+    slots, sp = _host_ints(slots, n, "slots")
+    lens, lp = _host_ints(lens, n, "lens")
+    rc = load().smol_attn_decode_shared(ctx.h, prefix.h, prefix_slot, prefix_len, kv.h, layer, rope.h if rope else None, n, sp,
+                                        lp, qp, kp, vp, dt, n_heads, scale, window, cap, qw, kw, eps, op)
+    if rc:
+        _check(rc, "smol_attn_decode_shared")
     return out
 
 
@@ -507,8 +516,9 @@ def _score_arrays(ctx, kv, mass, row_pos):
     import torch
     if mass.dim() != 3:
         raise SmolAttnError("mass must be [slots, kv_heads, stride]")
-    shape = (kv.n_slots, kv.n_kv_heads, mass.shape[2])
-    return _on(ctx, mass, (torch.float32,), shape, "mass"), _on(ctx, row_pos, (torch.int32,), shape, "row_pos"), shape[2]
+    stride = mass.shape[2]
+    shape = (kv.n_slots, kv.n_kv_heads, stride)
+    return _on(ctx, mass, torch.float32, shape, "mass"), _on(ctx, row_pos, torch.int32, shape, "row_pos"), stride
 
 
 def decode_scored(ctx, kv, layer, rope, slots, rows, pos, q, k_new, v_new, n_heads, scale, mass, row_pos, decay=1.0,
@@ -516,13 +526,15 @@ def decode_scored(ctx, kv, layer, rope, slots, rows, pos, q, k_new, v_new, n_hea
     """One decode step that also adds each row's weight to mass [slots, kv_heads, stride] (float32) and notes the new
     row's position in row_pos (int32, same shape); see smol_attn_decode_scored. rows: rows in use, pos: the new
     tokens' positions. Returns out [n, n_heads*hd]."""
-    n, ptrs, dt, norms, out, optr = _step_args(ctx, kv, q, k_new, v_new, n_heads, q_norm, k_norm, out)
-    sl, slp = _host_ints(slots, n, "slots")
-    ro, rop = _host_ints(rows, n, "rows")
-    po, pop = _host_ints(pos, n, "pos")
-    mp, rp, stride = _score_arrays(ctx, kv, mass, row_pos)
-    _check(load().smol_attn_decode_scored(ctx.h, kv.h, layer, rope.h if rope else None, n, slp, rop, pop, *ptrs, dt, n_heads,
-                                          scale, cap, *norms, eps, mp, rp, stride, decay, optr), "smol_attn_decode_scored")
+    n, qp, kp, vp, dt, qw, kw, out, op = _step_args(ctx, kv, q, k_new, v_new, n_heads, q_norm, k_norm, out)
+    slots, sp = _host_ints(slots, n, "slots")
+    rows, rp = _host_ints(rows, n, "rows")
+    pos, pp = _host_ints(pos, n, "pos")
+    ma, ra, stride = _score_arrays(ctx, kv, mass, row_pos)
+    rc = load().smol_attn_decode_scored(ctx.h, kv.h, layer, rope.h if rope else None, n, sp, rp, pp, qp, kp, vp, dt, n_heads,
+                                        scale, cap, qw, kw, eps, ma, ra, stride, decay, op)
+    if rc:
+        _check(rc, "smol_attn_decode_scored")
     return out
 
 
@@ -532,18 +544,20 @@ def kv_evict(kv, layer, slots, rows, ends, mass, row_pos, keep, first=0, recent=
     ctx = kv.ctx
     if (mass_out is None) != (pos_out is None):
         raise SmolAttnError("mass_out and pos_out are given together")
-    if mass_out is None:
-        mass_out, pos_out = mass, row_pos
     n = len(slots)
-    sl, slp = _host_ints(slots, n, "slots")
-    ro, rop = _host_ints(rows, n, "rows")
-    en, enp = _host_ints(ends, n, "ends")
-    mp, rp, stride = _score_arrays(ctx, kv, mass, row_pos)
-    mo, po, stride_out = _score_arrays(ctx, kv, mass_out, pos_out)
-    if stride != stride_out:
-        raise SmolAttnError("mass_out has another stride than mass")
-    _check(load().smol_kv_cache_evict(kv.h, layer, n, slp, rop, enp, mp, rp, mo, po, stride, keep, first, recent),
-           "smol_kv_cache_evict")
+    slots, sp = _host_ints(slots, n, "slots")
+    rows, rp = _host_ints(rows, n, "rows")
+    ends, ep = _host_ints(ends, n, "ends")
+    ma, ra, stride = _score_arrays(ctx, kv, mass, row_pos)
+    if mass_out is None:
+        mass_out, pos_out, mo, po = mass, row_pos, ma, ra
+    else:
+        mo, po, stride_out = _score_arrays(ctx, kv, mass_out, pos_out)
+        if stride != stride_out:
+            raise SmolAttnError("mass_out has another stride than mass")
+    rc = load().smol_kv_cache_evict(kv.h, layer, n, sp, rp, ep, ma, ra, mo, po, stride, keep, first, recent)
+    if rc:
+        _check(rc, "smol_kv_cache_evict")
     return mass_out, pos_out
 
 
@@ -862,13 +876,18 @@ def linear(ctx, x, w, bias=None, out=None, out_bf16=False):
     return out
 
 
+def _bits(w):
+    """a bf16 weight's dtype: bfloat16, or 16-bit whole numbers that hold its bits"""
+    import torch
+    return w.dtype if w.dtype in (torch.bfloat16, torch.int16, torch.uint16) else torch.bfloat16
+
+
 class Adapters:
     """Low-rank adapters of one projection (smol_adapters): (a [rank, in], b [out, rank], scale) each, device bf16
     tensors (or their bits as int16), copied into the set at creation."""
 
     def __init__(self, ctx, adapters):
         import torch
-        bits = (torch.bfloat16, torch.int16, torch.uint16)
         adapters = list(adapters)
         if not adapters:
             raise SmolAttnError("no adapters")
@@ -879,8 +898,8 @@ class Adapters:
         av, bv, ranks, scales = (_vp * n)(), (_vp * n)(), (_c_int * n)(), (_c_float * n)()
         for i, (a, b, scale) in enumerate(adapters):
             ranks[i], scales[i] = a.shape[0], scale
-            av[i] = _on(ctx, a, bits, (a.shape[0], self.in_dim), "a")
-            bv[i] = _on(ctx, b, bits, (self.out_dim, a.shape[0]), "b")
+            av[i] = _on(ctx, a, _bits(a), (a.shape[0], self.in_dim), "a")
+            bv[i] = _on(ctx, b, _bits(b), (self.out_dim, a.shape[0]), "b")
         self.n = n
         self.h = _vp()
         _check(load().smol_adapters_create(ctx.h, n, self.in_dim, self.out_dim, av, bv, ranks, scales, ctypes.byref(self.h)),
@@ -904,16 +923,19 @@ def linear_adapters(ctx, x, w, adapters, ids, bias=None, out=None, out_bf16=Fals
     numbers [seq]. Returns y [seq, out], float32, or the truncated bf16 bits as int16 when out_bf16."""
     import torch
     seq, in_dim, out_dim = x.shape[0], adapters.in_dim, adapters.out_dim
-    xp = _on(ctx, x, (torch.float32, torch.bfloat16), (seq, in_dim), "x")
-    wp = _on(ctx, w, (torch.bfloat16, torch.int16, torch.uint16), (out_dim, in_dim), "w")
-    bp = None if bias is None else _on(ctx, bias, (torch.float32,), (out_dim,), "bias")
-    dt = torch.int16 if out_bf16 else torch.float32
+    xt = x.dtype
+    xd = F32 if xt is torch.float32 else BF16 if xt is torch.bfloat16 else _dtype_code(x)
+    xp = _on(ctx, x, xt, (seq, in_dim), "x")
+    wp = _on(ctx, w, _bits(w), (out_dim, in_dim), "w")
+    bp = None if bias is None else _on(ctx, bias, torch.float32, (out_dim,), "bias")
+    yt = torch.int16 if out_bf16 else torch.float32
     if out is None:
-        out = torch.empty((seq, out_dim), dtype=dt, device=x.device)
-    i, ip = _host_ints(ids, seq, "ids")
-    _check(load().smol_linear_adapters_dev(ctx.h, _on(ctx, out, (dt,), (seq, out_dim), "out"), BF16 if out_bf16 else F32, xp,
-                                           _dtype_code(x), wp, bp, seq, in_dim, out_dim, adapters.h, ip),
-           "smol_linear_adapters_dev")
+        out = torch.empty((seq, out_dim), dtype=yt, device=x.device)
+    ids, ip = _host_ints(ids, seq, "ids")
+    rc = load().smol_linear_adapters_dev(ctx.h, _on(ctx, out, yt, (seq, out_dim), "out"), BF16 if out_bf16 else F32, xp, xd, wp,
+                                         bp, seq, in_dim, out_dim, adapters.h, ip)
+    if rc:
+        _check(rc, "smol_linear_adapters_dev")
     return out
 
 

@@ -1,7 +1,7 @@
 """The projection with an adapter a row against its 64-bit form.
 
-Bounds, derived before any run. The shared product is smol_linear_dev's: fp32
-sums of exact products, x carried to 2^-16 on the GEMM path (two bf16 parts),
+Bounds, derived before any run. The shared product is an fp32 sum of exact
+products, x carried to 2^-16 on smol_linear_dev's GEMM path (two bf16 parts),
 so (2 (in + 1) 2^-24 + 2^-16) sum |x w| + 2^-22 |bias|. The low-rank part carries
 x and t whole (three bf16 parts): t is off by at most 2 (in + 20) 2^-24 sum |a x|
 (20: the chunks' and the waves' partial sums), and B t by that through |B| and
@@ -99,6 +99,11 @@ CASES = [
     dict(seq=33, k=72, n=129, ranks=[100, 2, 31, 32], bias=False),
     dict(seq=300, k=512, n=768, ranks=[16, 32, 48]),
     dict(seq=700, k=136, n=64, ranks=[8] * 60),
+    # the last rows of the one-launch form and the first past it, an in_dim that needs padded copies
+    dict(seq=32, k=2048, n=48, ranks=[16, 4]),
+    dict(seq=64, k=96, n=200, ranks=[20] * 50),
+    dict(seq=65, k=97, n=90, ranks=[12, 40]),
+    dict(seq=200, k=333, n=1001, ranks=[128, 8]),
 ]
 
 
@@ -117,29 +122,29 @@ def test_no_row_has_one(sa, ctx):
     assert torch.equal(y, sa.linear(ctx, t.dev[0], t.dev[1], t.dev[2]))
 
 
-def test_rows_do_not_meet(sa, ctx):
-    """a NaN row, and NaN weights of an adapter, reach their own rows only; the bare rows are the shared product's bits"""
-    t = Case(50, 256, 192, [8, 16, 24])
-    t.ids = [i % 4 - 1 for i in range(50)]
+@pytest.mark.parametrize("n", [9, 50, 130])
+def test_rows_do_not_meet(sa, ctx, n):
+    """a NaN row, and NaN weights of an adapter, reach their own rows only"""
+    t = Case(n, 256, 192, [8, 16, 24])
+    t.ids = [i % 4 - 1 for i in range(n)]
     clean = t.call(sa, ctx).clone()
-    base = sa.linear(ctx, *t.dev)
-    bare = [s for s in range(50) if t.ids[s] < 0]
-    assert torch.equal(clean[bare], base[bare])
+    t.check(clean)
     t.ab[1][0][3] = float("nan")
     t.to(sa, ctx)
     t.dev[0][6] = float("nan")
     y = t.call(sa, ctx)
-    hit = [s for s in range(50) if t.ids[s] == 1 or s == 6]
-    rest = [s for s in range(50) if s not in hit]
+    hit = [s for s in range(n) if t.ids[s] == 1 or s == 6]
+    rest = [s for s in range(n) if s not in hit]
     assert torch.isnan(y[hit]).all() and torch.equal(y[rest], clean[rest])
 
 
-def test_a_row_does_not_depend_on_the_order(sa, ctx):
+@pytest.mark.parametrize("n", [32, 64, 128])
+def test_a_row_does_not_depend_on_the_order(sa, ctx, n):
     """the same rows in another order, with the same number of rows an adapter: the same bits a row"""
-    t = Case(64, 512, 256, [16, 8])
-    t.ids = [s % 2 for s in range(64)]
+    t = Case(n, 512, 256, [16, 8])
+    t.ids = [s % 2 for s in range(n)]
     y = t.call(sa, ctx).clone()
-    perm = torch.arange(63, -1, -1)
+    perm = torch.arange(n - 1, -1, -1)
     t.dev = (t.dev[0][perm.cuda()].contiguous(),) + t.dev[1:]
     t.ids = [t.ids[int(i)] for i in perm]
     assert torch.equal(t.call(sa, ctx), y[perm.cuda()])
