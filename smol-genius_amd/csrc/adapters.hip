@@ -43,19 +43,26 @@ namespace {
 
 constexpr int AD_MAX_RANK = 128;
 constexpr int AD_TPB = 256, AD_NW = AD_TPB / 64;
-constexpr int AD_ARG_TILES = 40;
+constexpr int AD_ARG_TILES = 40, AD_ARG_RUNS = 400;
 constexpr int AD_FEW = 64; /* rows that k_adapt_few takes */
 constexpr int AD_TIMING_KIND = 2;
 
 struct AdTile {
-    int adapter, n;
+    int adapter, n, rank;
+    float scale;
     int row[16]; /* rows past n repeat the first */
+};
+/* a tile of rows that follow each other (prompts one after the other): more of them fit the kernel arguments */
+struct AdRun {
+    int row0;
+    short adapter, n;
 };
 
 struct AdParams {
     const void *x; int x_bf16; int vec;
     const uint16_t *w; int w_vec; const float *bias;
-    uint16_t *xs;                    /* few rows: x as bf16 parts [part][row][kp], zeros past in_dim */
+    uint16_t *xs;                    /* few rows: x as B fragments [16-row tile][32-wide step][part][lane][8], zeros past
+                                      * in_dim and seq */
     int in_blocks;                   /* workgroups of k_adapt_in on tiles; those behind them lay x out */
     int in_dim, out_dim, seq;
     const uint16_t *a; int ra, kp;   /* [adapter][ra][kp] */
@@ -66,8 +73,26 @@ struct AdParams {
     const float *base;               /* fp32 [seq][out] that the low-rank part is added to */
     void *y; int y_bf16;             /* fp32 y is base itself */
     const AdTile *tiles_dev;
-    AdTile tiles[AD_ARG_TILES];
+    int runs_only;                   /* the tiles are runs[] */
+    union {
+        AdTile tiles[AD_ARG_TILES];
+        AdRun runs[AD_ARG_RUNS];
+    };
 };
+
+struct AdAt {
+    int adapter, n, rank;
+    float scale;
+    int row; /* of this lane's column c */
+};
+__device__ __forceinline__ AdAt ad_at(const AdParams &p, int tile, int c) {
+    if (p.runs_only) {
+        const AdRun r = p.runs[tile];
+        return AdAt{r.adapter, r.n, p.rank[r.adapter], p.scale[r.adapter], r.row0 + (c < r.n ? c : 0)};
+    }
+    const AdTile *t = (p.tiles_dev ? p.tiles_dev : p.tiles) + tile;
+    return AdAt{t->adapter, t->n, t->rank, t->scale, t->row[c]};
+}
 
 __device__ __forceinline__ void ad_split3(const float *x, b8 &p0, b8 &p1, b8 &p2) {
 #pragma unroll
@@ -121,23 +146,22 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_in(const AdParams p) {
     __shared__ __attribute__((aligned(16))) float s_t[AD_NW * 16 * NT * 16];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
     if ((int)blockIdx.x >= p.in_blocks) {
-        const long long e = (long long)(blockIdx.x - p.in_blocks) * AD_TPB + tid;
-        const int per = p.kp / 8, row = (int)(e / per), k0 = (int)(e - (long long)row * per) * 8;
-        if (row < p.seq) {
-            b8 xp[PARTS];
-            ad_x8<XBF>(p, row, k0, xp);
+        /* a wave a fragment: lane (c, j) holds row c's elements 8 j .. + 7 of the step */
+        const int f = (blockIdx.x - p.in_blocks) * AD_NW + (tid >> 6), steps = p.kp / 32, t = f / steps, s = f - t * steps;
+        const int row = 16 * t + c;
+        if (t >= (p.seq + 15) / 16) return;
+        b8 xp[PARTS];
+        ad_x8<XBF>(p, min(row, p.seq - 1), row < p.seq ? 32 * s + 8 * j : p.kp, xp);
 #pragma unroll
-            for (int q = 0; q < PARTS; q++)
-                *reinterpret_cast<b8 *>(p.xs + ((long long)q * p.seq + row) * p.kp + k0) = xp[q];
-        }
+        for (int q = 0; q < PARTS; q++) *reinterpret_cast<b8 *>(p.xs + ((((long long)t * steps + s) * PARTS + q) * 64 + lane) * 8) = xp[q];
         return;
     }
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tile = blockIdx.x % p.n_tiles, chunk = blockIdx.x / p.n_tiles;
-    const AdTile *tl = (p.tiles_dev ? p.tiles_dev : p.tiles) + tile;
-    const int ad = tl->adapter, n = tl->n, nt = (p.rank[ad] + 15) / 16;
-    const long long row = tl->row[c];
-    const uint16_t *a = p.a + ((long long)ad * p.ra + c) * p.kp + 8 * j;
+    const AdAt tl = ad_at(p, tile, c);
+    const int n = tl.n, nt = (tl.rank + 15) / 16;
+    const long long row = tl.row;
+    const uint16_t *a = p.a + ((long long)tl.adapter * p.ra + c) * p.kp + 8 * j;
     f4 acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
@@ -165,7 +189,7 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_in(const AdParams p) {
         f4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < AD_NW; w++) sum += *reinterpret_cast<f4 *>(s_t + ((w * 16 + r) * NT) * 16 + 4 * q);
-        *reinterpret_cast<f4 *>(p.t + ((long long)chunk * p.seq + tl->row[r]) * p.ra + 4 * q) = sum;
+        *reinterpret_cast<f4 *>(p.t + ((long long)chunk * p.seq + ad_at(p, tile, r).row) * p.ra + 4 * q) = sum;
     }
 }
 
@@ -206,8 +230,8 @@ __device__ __forceinline__ void ad_t(const AdParams &p, long long row, int rank,
     }
 }
 
-/* Up to 16 RT rows against 16 outputs a workgroup. Its eight waves share in_dim out by 32-wide steps, each with US steps
- * of W in flight; the sums of every wave are added in LDS in wave order, the adapters' tiles (one wave each) add their
+/* Up to 16 RT rows against 16 outputs a workgroup. Its eight waves share in_dim out by runs of US 32-wide steps (whole cache lines of
+ * W's rows), a run in flight; the sums of every wave are added in LDS in wave order, the adapters' tiles (one wave each) add their
  * part, and each output is written once. */
 constexpr int FEW_NW = 8;
 template <int RT, bool XBF, int KS>
@@ -234,21 +258,22 @@ __global__ __launch_bounds__(64 * FEW_NW) void k_adapt_few(const AdParams p) {
         }
         return v;
     };
-    for (int s0 = wave; s0 < steps; s0 += FEW_NW * US) {
+    const int tiles_x = (p.seq + 15) / 16;
+    for (int s0 = wave * US; s0 < steps; s0 += FEW_NW * US) {
         uint4 wv[US];
         b8 xf[US][RT][PARTS];
 #pragma unroll
         for (int u = 0; u < US; u++) {
-            const int s = s0 + u * FEW_NW;
+            const int s = s0 + u;
             wv[u] = s < steps ? load_w(s) : make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int t = 0; t < RT; t++)
 #pragma unroll
                 for (int q = 0; q < PARTS; q++)
-                    xf[u][t][q] = as_b8(s < steps ? *reinterpret_cast<const uint4 *>(
-                                                        p.xs + ((long long)q * p.seq + min(16 * t + c, p.seq - 1)) * p.kp +
-                                                        32 * s + 8 * j)
-                                                  : make_uint4(0, 0, 0, 0));
+                    xf[u][t][q] = as_b8(s < steps && t < tiles_x
+                                            ? *reinterpret_cast<const uint4 *>(
+                                                  p.xs + ((((long long)t * steps + s) * PARTS + q) * 64 + lane) * 8)
+                                            : make_uint4(0, 0, 0, 0));
         }
 #pragma unroll
         for (int u = 0; u < US; u++)
@@ -263,14 +288,14 @@ __global__ __launch_bounds__(64 * FEW_NW) void k_adapt_few(const AdParams p) {
     /* the low-rank part, by row, behind the waves' sums (rows without an adapter are not read there) */
     float *s_low = s_y + FEW_NW * RT * 16 * STR;
     for (int tile = wave; tile < p.n_tiles; tile += FEW_NW) {
-        const AdTile *tl = (p.tiles_dev ? p.tiles_dev : p.tiles) + tile;
-        const int ad = tl->adapter, rank = p.rank[ad], row = tl->row[c];
-        const bool live = c < tl->n;
-        const uint16_t *b = p.b + ((long long)ad * p.np + o0 + c) * p.rp + 8 * j;
+        const AdAt tl = ad_at(p, tile, c);
+        const int row = tl.row;
+        const bool live = c < tl.n;
+        const uint16_t *b = p.b + ((long long)tl.adapter * p.np + o0 + c) * p.rp + 8 * j;
         b8 bw[KS], tp[KS][3];
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) bw[ks] = as_b8(*reinterpret_cast<const uint4 *>(b + 32 * ks));
-        ad_t<KS>(p, row, rank, p.scale[ad], live, j, tp);
+        ad_t<KS>(p, row, tl.rank, tl.scale, live, j, tp);
         f4 low = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < KS; ks++)
@@ -302,16 +327,15 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_out(const AdParams p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tile = blockIdx.x % p.n_tiles, o0 = (blockIdx.x / p.n_tiles * AD_NW + wave) * AD_OUT;
     if (o0 >= p.out_dim) return;
-    const AdTile *tl = (p.tiles_dev ? p.tiles_dev : p.tiles) + tile;
-    const int ad = tl->adapter, rank = p.rank[ad];
-    const long long row = tl->row[c];
-    const bool live = c < tl->n;
+    const AdAt tl = ad_at(p, tile, c);
+    const long long row = tl.row;
+    const bool live = c < tl.n;
     constexpr int U = AD_OUT / 16;
     const bool quads = (p.out_dim & 3) == 0;
     f4 base[U];
     b8 w[U][KS];
     /* B has whole tiles of AD_OUT rows and 32 ranks; the sums that they join */
-    const uint16_t *b = p.b + ((long long)ad * p.np + o0 + c) * p.rp + 8 * j;
+    const uint16_t *b = p.b + ((long long)tl.adapter * p.np + o0 + c) * p.rp + 8 * j;
 #pragma unroll
     for (int u = 0; u < U; u++) {
 #pragma unroll
@@ -327,7 +351,7 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_out(const AdParams p) {
         }
     }
     b8 tp[KS][3];
-    ad_t<KS>(p, row, rank, p.scale[ad], live, j, tp);
+    ad_t<KS>(p, row, tl.rank, tl.scale, live, j, tp);
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int o = o0 + 16 * u + 4 * j;
@@ -393,6 +417,8 @@ struct smol_adapters {
     uint16_t *a, *b;
     float *scale;
     int *rank;
+    std::vector<float> h_scale;
+    std::vector<int> h_rank;
 };
 
 extern "C" int smol_adapters_destroy(smol_adapters *s) {
@@ -425,6 +451,8 @@ extern "C" int smol_adapters_create(smol_attn_ctx *ctx, int n, int in_dim, int o
     s->in_dim = in_dim;
     s->out_dim = out_dim;
     s->max_rank = max_rank;
+    s->h_scale.assign(scale, scale + n);
+    s->h_rank.assign(rank, rank + n);
     s->ra = (max_rank + 15) & ~15;
     s->rp = (max_rank + 31) & ~31;
     s->kp = (int)(((long long)in_dim + 31) & ~31LL);
@@ -513,6 +541,7 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
         count[i] = 0;
     }
     std::vector<AdTile> tiles(n_tiles);
+    bool runs_only = set->n <= SHRT_MAX;
     for (int s = 0; s < seq; s++) {
         const int id = ids[s];
         if (id < 0) continue;
@@ -520,8 +549,11 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
         const int k = count[id]++ % 16;
         if (k == 0) {
             t.adapter = id;
+            t.rank = set->h_rank[id];
+            t.scale = set->h_scale[id];
             for (int i = 0; i < 16; i++) t.row[i] = s;
         }
+        runs_only &= s == t.row[0] + k;
         t.row[k] = s;
         t.n = k + 1;
     }
@@ -541,9 +573,10 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
     p.scale = set->scale;
     p.rank = set->rank;
     p.n_tiles = n_tiles;
-    /* a step a wave at least, and no more workgroups than fill the device */
+    /* a step a wave at least; more than a quarter of the device's compute units gains less than the further partial sums
+     * cost the reader (17 tiles of 1024: 8 chunks 16.0 us a call, 3 chunks 14.3) */
     const int steps = set->kp / 32, cus = smol_internal_ctx_cus(ctx);
-    int chunks = std::max(1, std::min({cus / n_tiles, (steps + AD_NW - 1) / AD_NW, 16}));
+    int chunks = std::max(1, std::min({cus / 4 / n_tiles, (steps + AD_NW - 1) / AD_NW, 16}));
     p.chunk = (steps + chunks - 1) / chunks;
     p.n_chunks = (steps + p.chunk - 1) / p.chunk;
     const bool ybf = y_dtype == SMOL_ATTN_BF16, few = seq <= AD_FEW;
@@ -553,7 +586,7 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
     const int kp = set->kp, parts = p.x_bf16 ? 1 : 3;
     auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     const size_t tb = up((size_t)p.n_chunks * seq * set->ra * 4), yb = up(!few && ybf ? (size_t)seq * out_dim * 4 : 0);
-    const size_t xb = up(few ? (size_t)parts * seq * kp * 2 : pad ? (size_t)seq * kp * xs : 0);
+    const size_t xb = up(few ? (size_t)parts * ((seq + 15) & ~15) * kp * 2 : pad ? (size_t)seq * kp * xs : 0);
     void *work;
     if (int rc = smol_internal_work(ctx, tb + yb + xb + (pad ? (size_t)out_dim * kp * 2 : 0), &work)) return rc;
     p.t = static_cast<float *>(work);
@@ -570,7 +603,10 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
     p.base = base;
     p.y = y;
     p.y_bf16 = ybf;
-    if (n_tiles <= AD_ARG_TILES) {
+    if (n_tiles > AD_ARG_TILES && n_tiles <= AD_ARG_RUNS && runs_only) {
+        p.runs_only = 1;
+        for (int i = 0; i < n_tiles; i++) p.runs[i] = {tiles[i].row[0], (short)tiles[i].adapter, (short)tiles[i].n};
+    } else if (n_tiles <= AD_ARG_TILES) {
         memcpy(p.tiles, tiles.data(), n_tiles * sizeof(AdTile));
     } else {
         const void *dev;
@@ -600,7 +636,7 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
         if (e0) AHIP(hipEventRecord(e0, st));
     }
     p.in_blocks = n_tiles * p.n_chunks;
-    const unsigned in_blocks = (unsigned)p.in_blocks + (few ? ((unsigned)seq * (kp / 8) + AD_TPB - 1) / AD_TPB : 0);
+    const unsigned in_blocks = (unsigned)p.in_blocks + (few ? ((unsigned)((seq + 15) / 16) * (kp / 32) + AD_NW - 1) / AD_NW : 0);
     const int nt = set->ra / 16;
     if (nt <= 1) launch_in<1>(p, in_blocks, st);
     else if (nt <= 2) launch_in<2>(p, in_blocks, st);
