@@ -166,18 +166,26 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_in(const AdParams p) {
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
     const int s1 = min((chunk + 1) * p.chunk, p.kp / 32);
-    for (int s = chunk * p.chunk + wave; s < s1; s += AD_NW) {
-        b8 xp[PARTS], w[NT];
+    constexpr int US = NT <= 4 ? 4 : 2; /* steps in flight */
+    for (int s0 = chunk * p.chunk + wave * US; s0 < s1; s0 += AD_NW * US) {
+        b8 xp[US][PARTS], w[US][NT];
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-            if (t < nt) w[t] = as_b8(*reinterpret_cast<const uint4 *>(a + (long long)t * 16 * p.kp + 32 * s));
-        ad_x8<XBF>(p, row, 32 * s + 8 * j, xp);
+        for (int u = 0; u < US; u++) {
+            const bool live = s0 + u < s1;
+            const int k0 = live ? 32 * (s0 + u) : 0;
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            if (t >= nt) break;
-#pragma unroll
-            for (int q = PARTS - 1; q >= 0; q--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[t], xp[q], acc[t], 0, 0, 0);
+            for (int t = 0; t < NT; t++)
+                if (t < nt) w[u][t] = as_b8(*reinterpret_cast<const uint4 *>(a + (long long)t * 16 * p.kp + k0));
+            ad_x8<XBF>(p, row, live ? k0 + 8 * j : p.kp, xp[u]); /* past the chunk: zeros */
         }
+#pragma unroll
+        for (int u = 0; u < US; u++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                if (t >= nt) break;
+#pragma unroll
+                for (int q = PARTS - 1; q >= 0; q--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u][t], xp[u][q], acc[t], 0, 0, 0);
+            }
     }
     /* lane (c, j): ranks 16 t + 4 j .. + 3 of row c */
 #pragma unroll
@@ -320,28 +328,46 @@ __global__ __launch_bounds__(64 * FEW_NW) void k_adapt_few(const AdParams p) {
 
 constexpr int AD_OUT = 64; /* outputs of a k_adapt_out wave */
 
-/* KS: 32-wide steps over the rank */
+/* y = base + scale B t for a tile's rows and 256 outputs. The products leave the matrix cores with a row's outputs spread
+ * over lanes 16 apart; they pass through LDS so that base and y move as whole lines (16 rows of 1 KB). Bound by base and y.
+ * KS: 32-wide steps over the rank */
 template <int KS>
 __global__ __launch_bounds__(AD_TPB) void k_adapt_out(const AdParams p) {
+    constexpr int W = AD_OUT * AD_NW, STR = W + 4, U = AD_OUT / 16, NB = 16 * W / 4 / AD_TPB;
+    __shared__ __attribute__((aligned(16))) float s_d[16 * STR];
+    __shared__ int s_row[16];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int tile = blockIdx.x % p.n_tiles, o0 = (blockIdx.x / p.n_tiles * AD_NW + wave) * AD_OUT;
-    if (o0 >= p.out_dim) return;
+    const int tile = blockIdx.x % p.n_tiles, w0 = blockIdx.x / p.n_tiles * W, o0 = w0 + wave * AD_OUT;
     const AdAt tl = ad_at(p, tile, c);
     const long long row = tl.row;
-    const bool live = c < tl.n;
-    constexpr int U = AD_OUT / 16;
-    const bool quads = (p.out_dim & 3) == 0;
-    f4 base[U];
-    b8 w[U][KS];
-    /* B has whole tiles of AD_OUT rows and 32 ranks; the sums that they join */
-    const uint16_t *b = p.b + ((long long)tl.adapter * p.np + o0 + c) * p.rp + 8 * j;
+    if (tid < 16) s_row[tid] = tl.row;
+    const bool live = c < tl.n, mine = o0 < p.out_dim; /* B has whole tiles of AD_OUT rows and 32 ranks */
+    b8 w[U][KS], tp[KS][3];
+    const uint16_t *b = p.b + ((long long)tl.adapter * p.np + (mine ? o0 : 0) + c) * p.rp + 8 * j;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
+    for (int u = 0; u < U; u++)
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) w[u][ks] = as_b8(*reinterpret_cast<const uint4 *>(b + (long long)16 * u * p.rp + 32 * ks));
-        const int o = o0 + 16 * u + 4 * j;
-        const long long at = row * p.out_dim + o;
+    ad_t<KS>(p, row, tl.rank, tl.scale, live, j, tp);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int q = 2; q >= 0; q--) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u][ks], tp[ks][q], acc, 0, 0, 0);
+        *reinterpret_cast<f4 *>(s_d + c * STR + wave * AD_OUT + 16 * u + 4 * j) = acc;
+    }
+    __syncthreads();
+    /* a wave a row at a time, a lane four outputs */
+    const bool quads = (p.out_dim & 3) == 0;
+    f4 base[NB];
+#pragma unroll
+    for (int u = 0; u < NB; u++) {
+        const int e = tid + u * AD_TPB, r = e / (W / 4), o = w0 + e % (W / 4) * 4;
+        if (r >= tl.n) continue;
+        const long long at = (long long)s_row[r] * p.out_dim + o;
         if (quads) {
             if (o < p.out_dim) base[u] = *reinterpret_cast<const f4 *>(p.base + at);
         } else {
@@ -350,32 +376,25 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_out(const AdParams p) {
                 if (o + i < p.out_dim) base[u][i] = p.base[at + i];
         }
     }
-    b8 tp[KS][3];
-    ad_t<KS>(p, row, tl.rank, tl.scale, live, j, tp);
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int o = o0 + 16 * u + 4 * j;
-        f4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-            for (int q = 2; q >= 0; q--) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u][ks], tp[ks][q], acc, 0, 0, 0);
-        if (!live) continue;
-        const long long at = row * p.out_dim + o;
-        acc += base[u];
+    for (int u = 0; u < NB; u++) {
+        const int e = tid + u * AD_TPB, r = e / (W / 4), o = w0 + e % (W / 4) * 4;
+        if (r >= tl.n) continue;
+        const long long at = (long long)s_row[r] * p.out_dim + o;
+        const f4 v = base[u] + *reinterpret_cast<const f4 *>(s_d + r * STR + o - w0);
         if (quads && o < p.out_dim) {
             if (p.y_bf16)
                 *reinterpret_cast<uint2 *>((uint16_t *)p.y + at) =
-                    make_uint2(__float_as_uint(acc[0]) >> 16 | (__float_as_uint(acc[1]) & 0xFFFF0000u),
-                               __float_as_uint(acc[2]) >> 16 | (__float_as_uint(acc[3]) & 0xFFFF0000u));
+                    make_uint2(__float_as_uint(v[0]) >> 16 | (__float_as_uint(v[1]) & 0xFFFF0000u),
+                               __float_as_uint(v[2]) >> 16 | (__float_as_uint(v[3]) & 0xFFFF0000u));
             else
-                *reinterpret_cast<f4 *>((float *)p.y + at) = acc;
+                *reinterpret_cast<f4 *>((float *)p.y + at) = v;
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (o + i < p.out_dim) {
-                    if (p.y_bf16) ((uint16_t *)p.y)[at + i] = (uint16_t)(__float_as_uint(acc[i]) >> 16);
-                    else ((float *)p.y)[at + i] = acc[i];
+                    if (p.y_bf16) ((uint16_t *)p.y)[at + i] = (uint16_t)(__float_as_uint(v[i]) >> 16);
+                    else ((float *)p.y)[at + i] = v[i];
                 }
         }
     }
@@ -576,7 +595,7 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
     /* a step a wave at least; more than a quarter of the device's compute units gains less than the further partial sums
      * cost the reader (17 tiles of 1024: 8 chunks 16.0 us a call, 3 chunks 14.3) */
     const int steps = set->kp / 32, cus = smol_internal_ctx_cus(ctx);
-    int chunks = std::max(1, std::min({cus / 4 / n_tiles, (steps + AD_NW - 1) / AD_NW, 16}));
+    const int chunks = std::max(1, std::min({n_tiles > 32 ? cus / n_tiles : cus / 4 / n_tiles, (steps + AD_NW - 1) / AD_NW, 16}));
     p.chunk = (steps + chunks - 1) / chunks;
     p.n_chunks = (steps + p.chunk - 1) / p.chunk;
     const bool ybf = y_dtype == SMOL_ATTN_BF16, few = seq <= AD_FEW;

@@ -48,6 +48,7 @@ extern "C" int smol_launch_win(const WinParams *wp, int hd, int n_tiles, int max
                                hipEvent_t e1);
 extern "C" int smol_win_max_keys(int hd, int in_dtype, int precise);
 extern "C" int smol_shared_tile_rows(int hd, int rows);
+extern "C" int smol_shared_own_rows(void);
 extern "C" int smol_shared_occupancy(int hd);
 extern "C" int smol_launch_shared(const ShParams *p, int hd, int tile_rows, int max_len, hipStream_t st, hipEvent_t e0,
                                   hipEvent_t e1);
@@ -1939,30 +1940,34 @@ static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int l
         p_first = std::min(lo, sp.p_len) & ~(SMOL_SLAB - 1);
     }
     sp.p_first = p_first;
-    const int tile = getenv("SH_TILE") ? atoi(getenv("SH_TILE")) : smol_shared_tile_rows(hd, rows);
+    const int tile = smol_shared_tile_rows(hd, rows);
     const int p_slabs = (sp.p_len - p_first + SMOL_SLAB - 1) / SMOL_SLAB, own_max = (max_own + SMOL_SLAB - 1) / SMOL_SLAB;
     sp.n_rb = (rows + tile - 1) / tile;
-    sp.s_rb = (G + 15) / 16;
-    long long units = (long long)Hkv * sp.n_rb * p_slabs;
-    for (int k : own_slabs) units += (long long)Hkv * sp.s_rb * k;
-    /* equally long chunks of at least a slab a wave: as short as lets every
-     * workgroup run at once, since each spends 6 us before its first slab and
-     * after its last */
+    sp.s_rb = (G + smol_shared_own_rows() - 1) / smol_shared_own_rows();
+    /* Chunks of equal length, a slab a wave at least, as short as leaves a
+     * prefix item for three compute units of four at most, and own-rows items
+     * that fit beside them (with room for the XCDs' uneven shares). A workgroup spends 5 to 8 us besides its slabs, so more of them
+     * cost more than they spread (head_dim 128, 16 sequences on 4096: 8, 16, 32
+     * slabs a chunk 22 / 20 / 24 us a call; 64 on 16384: 16, 32, 64 77 / 66 / 73). */
     const long long slots = (long long)ctx->cu_count * smol_shared_occupancy(hd);
-    const long long most = ((long long)std::max(p_slabs, own_max) + SH_MAX_SPLIT - 1) / SH_MAX_SPLIT;
-    auto workgroups = [&](long long c) {
-        long long w = (long long)Hkv * sp.n_rb * ((p_slabs + c - 1) / c);
-        for (int k : own_slabs) w += (long long)Hkv * sp.s_rb * std::max(1LL, (k + c - 1) / c);
-        return w;
+    auto chunk = [&](int longest, long long limit, auto workgroups) {
+        const int least = std::max(4, (longest + SH_MAX_SPLIT - 1) / SH_MAX_SPLIT), forced = ctx->opt[SMOL_OPT_DEC_SLABS];
+        long long c = (std::max(least, forced) + 3) & ~3;
+        if (forced <= 0)
+            while (c < longest && workgroups(c) > limit) c += std::max(4LL, (c / 8) & ~3LL);
+        return (int)c;
     };
-    long long c = std::max({4LL, most, (units + slots - 1) / slots});
-    c = (c + 3) & ~3LL;
-    for (int i = 0; i < 32 && c < std::max(p_slabs, own_max) && workgroups(c) > slots; i++) c += 4;
-    if (ctx->opt[SMOL_OPT_DEC_SLABS] > 0) c = std::max<long long>(most, (ctx->opt[SMOL_OPT_DEC_SLABS] + 3) & ~3);
-    if (c > (INT_MAX >> 6)) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d rows", max_len);
-    sp.p_chunk = sp.s_chunk = (int)c * SMOL_SLAB;
-    sp.n_ps = (int)((p_slabs + c - 1) / c);
-    sp.n_ss = std::max(1, (int)((own_max + c - 1) / c));
+    auto p_items = [&](long long c) { return (long long)Hkv * sp.n_rb * ((p_slabs + c - 1) / c); };
+    const int cp = chunk(p_slabs, ctx->cu_count * 3 / 4, p_items);
+    const int cs = chunk(own_max, p_slabs ? (slots - p_items(cp)) * 3 / 4 : slots, [&](long long c) {
+        long long w = 0;
+        for (int k : own_slabs) w += std::max(1LL, (k + c - 1) / c);
+        return w * Hkv * sp.s_rb;
+    });
+    sp.p_chunk = cp * SMOL_SLAB;
+    sp.s_chunk = cs * SMOL_SLAB;
+    sp.n_ps = (p_slabs + cp - 1) / cp;
+    sp.n_ss = std::max(1, (own_max + cs - 1) / cs);
     const long long pblocks = ((long long)Hkv * sp.n_ps + 7) / 8 * 8 * sp.n_rb;
     const long long sblocks = (long long)sp.n_ss * n * Hkv * sp.s_rb;
     if (pblocks + sblocks > INT_MAX / 2 || (long long)n * sp.Hq + (long long)n * Hkv * (max_len / 1024 + 1) > INT_MAX / 2)

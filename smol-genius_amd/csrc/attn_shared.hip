@@ -13,61 +13,59 @@
  * n_seq x G rows of a kv head with its P keys, read once for all of them,
  * and each sequence's own rows are a product of G rows.
  *
- * Work split. A workgroup of four waves is one item: either (kv head, a tile
- * of 16 NT rows of the batch, a chunk of the prefix) or (sequence, kv head, a
- * chunk of its own rows). Its waves take 32-key slabs in turn, K and V^T
- * fragments straight from the cache into registers, as k_dec
- * (attn_decode.hip) does; their (m, l, O) join in LDS and go to the workspace,
- * and k_sh_merge joins an output row's chunks. Items need no table: the
- * chunks are equally long, so a workgroup finds its item from its number, and
- * only the sequences' (slot, length, position) travel with the call.
+ * Work split. A workgroup of four waves is one item: a chunk of the prefix
+ * against a block of the batch's rows of a kv head, or a chunk of a
+ * sequence's own rows against its G rows. Items need no table: the chunks are
+ * equally long, so a workgroup finds its item from its number, and only the
+ * sequences' (slot, length, position) travel with the call. Each item leaves
+ * (m, l, O) of its rows in the workspace, and k_sh_merge joins a row's chunks.
+ *   Narrow items (own rows; a prefix against at most 32 rows): all waves hold
+ *     the same 16 rows and take 32-key slabs in turn, K and V^T fragments
+ *     straight from the cache into registers; their states join in LDS. Bound
+ *     by memory.
+ *   Wide items (a prefix against more rows): the waves hold 16 rows each, 64
+ *     together, and share every slab, which transfers bring into a ring in LDS
+ *     in the order that its fragments are read without bank conflicts. Bound
+ *     by the matrix cores: three products for one (below).
+ *
+ * Every lane loads, normalises and rotates exactly the elements of Q that its
+ * fragments hold (row c, dims 32 ks + 8 j ..), so the prologue is one round of
+ * loads without LDS or a barrier.
  *
  * Precision. K and V are the cache's bf16 bits. The fp32 side of each product
  * is split into bf16 parts that the matrix cores take exactly: Q into three
- * (24 bits, all of fp32), the probabilities into two (16 bits: at most 2^-16 of
- * each probability is lost, and their errors are independent).
- * The new token's key and value are used in fp32 by the step that appends
- * them and rounded to nearest bf16 in the cache. Softmax state, sums and the
- * join are fp32.
+ * (24 bits, all of fp32), and so are the probabilities (two parts lose up to
+ * 2^-16 of each, which measured 1.3e-6 of a row's norm where fp32 forms are
+ * off by 5e-7). The new token's key and value are used in fp32 by the step
+ * that appends them and rounded to nearest bf16 in the cache. Softmax state,
+ * sums and the join are fp32.
  */
 #include "attn_device.h"
 
 namespace {
 
+constexpr int SH_NW = 4, SH_TPB = 64 * SH_NW;
+constexpr int Q_PARTS = 3, P_PARTS = 3;
+
 template <int HD>
 struct ShGeom {
     static constexpr int KS = (HD + 31) / 32; /* 32-wide d chunks of a K fragment */
     static constexpr int DT = (HD + 15) / 16; /* 16-wide d tiles of the output */
-    static constexpr int HDP = KS * 32;
-    static constexpr int QSTR = HDP + 4;      /* LDS row of a staged row */
+    static constexpr int HALF = HD / 2;
     static constexpr int OSTR = DT * 16 + 4;  /* LDS row of a wave's output */
     static constexpr unsigned SLAB_BYTES = SMOL_SLAB * HD * 2;
-};
-
-constexpr int SH_NW = 4, SH_TPB = 64 * SH_NW;
-constexpr int Q_PARTS = 3, P_PARTS = 3;
-
-template <int HD, int NT>
-struct ShLds {
-    using Gm = ShGeom<HD>;
-    static constexpr int TR = 16 * NT, CH8 = HD / 8;
-    static constexpr int RAW = (TR + 1) * Gm::QSTR;               /* the rows times the norm's weights, the new key's behind */
-    static constexpr int CB = SH_NW * 16 * Gm::OSTR + 2 * SH_NW * 16; /* a row tile's outputs of every wave, their m and l */
-    static constexpr int UNI = RAW > CB ? RAW : CB;
-    static constexpr int FRAG = Q_PARTS * Gm::KS * NT * 256;      /* Q fragments: 16 bytes a lane */
-    static constexpr int SS = ((TR + 1) * CH8 + 3) & ~3;          /* a row's squares by chunk; then the new scores by chunk */
-    static constexpr int FLOATS = UNI + FRAG + SS + 2 * Gm::HDP;  /* the new key and value last */
+    static constexpr bool POW2 = (HD & (HD - 1)) == 0; /* half a head is whole steps */
+    static constexpr bool WIDE = HD == 64 || HD == 128; /* the sizes that have wide items */
+    static constexpr int WS = 2;                       /* slabs of a wide item's step */
+    static constexpr int STAGES = 2;
+    static constexpr int CB_BYTES = (SH_NW * 16 * OSTR + 2 * SH_NW * 16) * 4; /* the waves' outputs, their m and l */
+    static constexpr int RING_BYTES = WIDE ? STAGES * WS * 2 * (int)SLAB_BYTES : 0;
 };
 
 __device__ __forceinline__ void ld8f(const float *a, float *v) {
     const float4 x = *reinterpret_cast<const float4 *>(a), y = *reinterpret_cast<const float4 *>(a + 4);
     v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
 }
-__device__ __forceinline__ void st8f(float *a, const float *v) {
-    *reinterpret_cast<float4 *>(a) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4 *>(a + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
-
 /* x = p0 + p1 + p2 in bf16: each part is what the parts before it leave,
  * rounded to nearest, so three carry all 24 bits of x */
 __device__ __forceinline__ void split8x3(const float *x, b8 &p0, b8 &p1, b8 &p2) {
@@ -90,11 +88,15 @@ __device__ __forceinline__ uint4 keep_keys8(uint4 v, int k, int lo, int hi) {
     return make_uint4(keep_keys(v.x, k, lo, hi), keep_keys(v.y, k + 2, lo, hi), keep_keys(v.z, k + 4, lo, hi),
                       keep_keys(v.w, k + 6, lo, hi));
 }
-__device__ __forceinline__ bool any_not_finite(uint4 v) {
+/* bit e: element e of the eight is not finite */
+__device__ __forceinline__ unsigned not_finite8(uint4 v) {
     const unsigned a[4] = {v.x, v.y, v.z, v.w};
-    bool bad = false;
+    unsigned bad = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) bad |= (a[i] & 0x7F80u) == 0x7F80u || (a[i] & 0x7F800000u) == 0x7F800000u;
+    for (int i = 0; i < 4; i++) {
+        bad |= (a[i] & 0x7F80u) == 0x7F80u ? 1u << 2 * i : 0u;
+        bad |= (a[i] & 0x7F800000u) == 0x7F800000u ? 2u << 2 * i : 0u;
+    }
     return bad;
 }
 
@@ -111,8 +113,95 @@ __device__ __forceinline__ int sh_own_chunks(const ShParams &p, const ShSeq &q) 
     return max(1, (q.len - sh_own_first(p, q) + p.s_chunk - 1) / p.s_chunk);
 }
 
-/* One item. NT row tiles of 16; rows r < R: sequence and head by `prefix`.
- * Keys [kb, ke) of the region at kbase / vbase (region_bytes each). */
+/* Elements [32 ks + 8 j, + 8) of a row for every ks, normalised (w: the norm's weights or null) and rotated to position
+ * `pos`, the lanes j = 0 .. 3 (16 apart) of a column holding one row together; all of them call this. next(): what is
+ * requested behind the row's own loads (a compute unit returns data in the order of its requests: the first slab in
+ * front of them held the rows back by its whole transfer, 12 us instead of 5 with every compute unit streaming). */
+template <int HD, class F>
+__device__ __forceinline__ void sh_row(const ShParams &p, const void *x_in, long long row, const float *w, int pos, int j,
+                                       float (&x)[ShGeom<HD>::KS][8], F next) {
+    constexpr int KS = ShGeom<HD>::KS, HALF = ShGeom<HD>::HALF, KH = KS / 2;
+    constexpr bool POW2 = ShGeom<HD>::POW2;
+    const bool neox = p.rope_kind == SMOL_ROPE_NEOX_K, inter = p.rope_kind == SMOL_ROPE_INTERLEAVED_K;
+    const float *ct = p.rope_cos + (long long)pos * HD, *st = p.rope_sin + (long long)pos * HD;
+    float cv[KH][8], sn[KH][8]; /* the table repeats a row's first half in its second (NeoX) */
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+        const int d0 = 32 * ks + 8 * j;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[ks][i] = 0.0f;
+        if (HD % 32 == 0 || d0 < HD) load8(x_in, p.in_dtype, row + d0, x[ks]);
+    }
+    if (POW2 && neox) {
+#pragma unroll
+        for (int ks = 0; ks < KH; ks++) {
+            ld8f(ct + 32 * ks + 8 * j, cv[ks]);
+            ld8f(st + 32 * ks + 8 * j, sn[ks]);
+        }
+    }
+    next();
+    float ri = 1.0f;
+    if (__any(w != nullptr)) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss = fmaf(x[ks][i], x[ks][i], ss);
+        ri = 1.0f / sqrtf(row_sum4(ss) / (float)HD + p.norm_eps);
+        if (w) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const int d0 = 32 * ks + 8 * j;
+                if (HD % 32 == 0 || d0 < HD) {
+                    float wv[8];
+                    ld8f(w + d0, wv);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[ks][i] = x[ks][i] * wv[i] * ri;
+                }
+            }
+        }
+    }
+    if (POW2 && neox) {
+        /* the partner half a head away is this lane's own */
+#pragma unroll
+        for (int ks = 0; ks < KH; ks++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float a = x[ks][i], b = x[ks + KH][i];
+                x[ks][i] = fmaf(a, cv[ks][i], -(b * sn[ks][i]));
+                x[ks + KH][i] = fmaf(b, cv[ks][i], a * sn[ks][i]);
+            }
+    } else if (inter || neox) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const int d0 = 32 * ks + 8 * j;
+            if (HD % 32 != 0 && d0 >= HD) continue;
+            float c8[8], s8[8];
+            ld8f(ct + d0, c8);
+            ld8f(st + d0, s8);
+            if (inter) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float a = x[ks][i], b = x[ks][i + 1];
+                    x[ks][i] = fmaf(a, c8[i], -(b * s8[i]));
+                    x[ks][i + 1] = fmaf(b, c8[i + 1], a * s8[i + 1]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int d = d0 + i, pd = d < HALF ? d + HALF : d - HALF;
+                    float pr = p.in_dtype == SMOL_IN_BF16 ? bf16_to_f32(((const uint16_t *)x_in)[row + pd])
+                                                          : ((const float *)x_in)[row + pd];
+                    if (w) pr = pr * w[pd] * ri;
+                    const float t = pr * s8[i];
+                    x[ks][i] = fmaf(x[ks][i], c8[i], d < HALF ? -t : t);
+                }
+            }
+        }
+    }
+}
+
+/* One item: R rows against the keys [kb, ke) of the region at kc / vtc */
 struct ShItem {
     bool prefix;
     int g;              /* kv head */
@@ -126,21 +215,180 @@ struct ShItem {
     float *part_o, *part_ml; /* of its row 0 */
 };
 
-template <int HD, int NT, bool SC>
-__device__ __forceinline__ void sh_item(const ShParams &p, const ShItem &it, float *smem) {
+/* A wave's 16 rows: their fragments, the first key that each may see, and the softmax state */
+template <int HD>
+struct ShRows {
+    static constexpr int KS = ShGeom<HD>::KS, DT = ShGeom<HD>::DT;
+    b8 q[Q_PARTS][KS];
+    int lo, lo_min, lo_max;
+    float m, l;
+    f4 o[DT];
+};
+
+constexpr int OWN_ROWS = 15; /* heads of an own-rows item: the 16th column holds the new key */
+
+/* Column c: row r0 + c of the item, if it has one; its fp32 elements stay in y. The column behind an own-rows item's last
+ * row holds the new key (normalised and rotated, not scaled), which takes no part in the products. */
+template <int HD, class F>
+__device__ __forceinline__ void sh_rows(const ShParams &p, const ShItem &it, int r0, int c, int j, ShRows<HD> &w,
+                                        float (&y)[ShGeom<HD>::KS][8], F next) {
+    constexpr int KS = ShGeom<HD>::KS, DT = ShGeom<HD>::DT;
+    const bool live = r0 + c < it.R, is_k = it.with_new && c == it.R;
+    const int r = live ? r0 + c : 0;
+    const int seq = it.prefix ? (it.row0 + r) / p.G : it.seq;
+    const int head = it.g * p.G + (it.prefix ? (it.row0 + r) % p.G : it.row0 + r);
+    const int pos = sh_seq(p, seq).pos;
+    sh_row<HD>(p, is_k ? p.k_in : p.q_in, is_k ? ((long long)seq * p.Hkv + it.g) * HD : ((long long)seq * p.Hq + head) * HD,
+               is_k ? p.k_norm : p.q_norm, pos, j, y, next);
+    const float f = live ? p.qscale : 1.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            y[ks][i] *= f;
+            z[i] = live ? y[ks][i] : 0.0f;
+        }
+        split8x3(z, w.q[0][ks], w.q[1][ks], w.q[2][ks]);
+    }
+    w.lo = w.lo_min = w.lo_max = 0;
+    if (p.window > 0) {
+        const int lo = max(0, pos - p.window + 1 - (it.prefix ? 0 : p.p_len));
+        w.lo = live ? lo : 0;
+        w.lo_max = w.lo;
+        w.lo_min = live ? lo : 1 << 30;
+#pragma unroll
+        for (int sh = 1; sh < 16; sh <<= 1) {
+            w.lo_max = max(w.lo_max, __shfl_xor(w.lo_max, sh));
+            w.lo_min = min(w.lo_min, __shfl_xor(w.lo_min, sh));
+        }
+        w.lo_max = __builtin_amdgcn_readfirstlane(w.lo_max);
+        w.lo_min = __builtin_amdgcn_readfirstlane(w.lo_min);
+    }
+    w.m = -INFINITY;
+    w.l = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) w.o[dt] = f4{0.f, 0.f, 0.f, 0.f};
+}
+
+/* S^T = K.Q^T of one slab: the small parts of Q first */
+template <int HD>
+__device__ __forceinline__ void sh_qk(const ShRows<HD> &w, const uint4 (&k)[2][ShGeom<HD>::KS], f4 (&s)[2]) {
+    s[0] = s[1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = Q_PARTS - 1; q >= 0; q--)
+#pragma unroll
+        for (int ks = 0; ks < ShGeom<HD>::KS; ks++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(k[h][ks]), w.q[q][ks], s[h], 0, 0, 0);
+}
+
+/* The scores of NS slabs from key k0 on: capped, kept (logits: where this lane's go, or null), and -inf for keys that a row
+ * does not see; nan: whether a row sees a value that is no number among those taken out */
+template <int HD, int NS, bool SC>
+__device__ __forceinline__ bool sh_mask(const ShParams &p, const ShRows<HD> &w, int k0, int ke, int j, f4 (&s)[NS][2],
+                                        uint4 (&v)[NS][ShGeom<HD>::DT], float *logits) {
+    constexpr int DT = ShGeom<HD>::DT;
+    if (p.cap2 > 0.0f) {
+#pragma unroll
+        for (int u = 0; u < NS; u++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[u][h][i] = p.cap2 * tanhf(s[u][h][i] / p.cap2);
+    }
+    if (SC && logits) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) *reinterpret_cast<f4 *>(logits + 4 * h) = s[0][h];
+    }
+    /* keys that some row does not see: their scores and, since 0 x inf is no number, their values */
+    const bool low = k0 < w.lo_max;
+    bool nan = false;
+    if (low || k0 + NS * SMOL_SLAB > ke) {
+#pragma unroll
+        for (int u = 0; u < NS; u++) {
+            const int ku = k0 + u * SMOL_SLAB + 8 * j;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int key = ku + e;
+                s[u][e >> 2][e & 3] = key >= w.lo && key < ke ? s[u][e >> 2][e & 3] : -INFINITY;
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) v[u][dt] = keep_keys8(v[u][dt], ku, w.lo_min, ke);
+            if (low && w.lo_min < w.lo_max) {
+                /* rows see different keys here: a key with a value that is not finite is taken out for all of them,
+                 * and the rows that see it get a sum that is no number */
+                unsigned bad = 0;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) bad |= not_finite8(v[u][dt]);
+                if (__any(bad != 0)) {
+#pragma unroll
+                    for (int sh = 1; sh < 16; sh <<= 1) bad |= __shfl_xor(bad, sh);
+                    const uint4 keep = make_uint4((bad & 1 ? 0u : 0xFFFFu) | (bad & 2 ? 0u : 0xFFFF0000u),
+                                                  (bad & 4 ? 0u : 0xFFFFu) | (bad & 8 ? 0u : 0xFFFF0000u),
+                                                  (bad & 16 ? 0u : 0xFFFFu) | (bad & 32 ? 0u : 0xFFFF0000u),
+                                                  (bad & 64 ? 0u : 0xFFFFu) | (bad & 128 ? 0u : 0xFFFF0000u));
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++)
+                        v[u][dt] = make_uint4(v[u][dt].x & keep.x, v[u][dt].y & keep.y, v[u][dt].z & keep.z, v[u][dt].w & keep.w);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) nan |= (bad >> e & 1) != 0 && ku + e >= w.lo;
+                }
+            }
+        }
+    }
+    return nan;
+}
+
+/* softmax of NS slabs and O^T += V^T.P^T */
+template <int HD, int NS>
+__device__ __forceinline__ void sh_pv(ShRows<HD> &w, const f4 (&s)[NS][2], const uint4 (&v)[NS][ShGeom<HD>::DT], bool nan) {
+    constexpr int DT = ShGeom<HD>::DT;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < NS; u++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, s[u][e >> 2][e & 3]);
+    mx = row_max4(mx);
+    const bool need = mx > w.m + LAZY_T;
+    if (__any(need)) {
+        const float m_new = need ? mx : w.m;
+        const float alpha = need ? __builtin_amdgcn_exp2f(w.m - m_new) : 1.0f;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) w.o[dt] *= alpha;
+        w.l *= alpha;
+        w.m = m_new;
+    }
+    const float m_use = w.m == -INFINITY ? 0.0f : w.m;
+    float ps = nan ? __builtin_nanf("") : 0.0f;
+    b8 pp[NS][P_PARTS];
+#pragma unroll
+    for (int u = 0; u < NS; u++) {
+        float pv[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            pv[e] = __builtin_amdgcn_exp2f(s[u][e >> 2][e & 3] - m_use);
+            ps += pv[e];
+        }
+        split8x3(pv, pp[u][0], pp[u][1], pp[u][2]);
+    }
+    w.l += ps;
+#pragma unroll
+    for (int u = 0; u < NS; u++)
+#pragma unroll
+        for (int q = P_PARTS - 1; q >= 0; q--)
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+                w.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(v[u][dt]), pp[u][q], w.o[dt], 0, 0, 0);
+}
+
+/* At most 16 rows, the same in every wave; the waves take the slabs in turn */
+template <int HD, bool SC>
+__device__ __forceinline__ void sh_narrow(const ShParams &p, const ShItem &it, char *smem) {
     using Gm = ShGeom<HD>;
-    using L = ShLds<HD, NT>;
-    constexpr int KS = Gm::KS, DT = Gm::DT, HDP = Gm::HDP, QSTR = Gm::QSTR, OSTR = Gm::OSTR, TR = 16 * NT;
+    constexpr int KS = Gm::KS, DT = Gm::DT, OSTR = Gm::OSTR;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int G = p.G, R = it.R;
-    float *s_raw = smem;
-    uint4 *s_frag = reinterpret_cast<uint4 *>(smem + L::UNI);
-    float *s_ss = smem + L::UNI + L::FRAG, *s_knew = s_ss + L::SS, *s_vnew = s_knew + HDP;
-
-    /* ---- the slab pipeline's loads ---- */
-    struct KRaw { uint4 k[2][KS]; };
-    struct VRaw { uint4 v[DT]; };
     const int kt_row = 8 * (c >> 2) + (c & 3);
     unsigned vo_k[2][KS], vo_v[DT];
 #pragma unroll
@@ -155,8 +403,9 @@ __device__ __forceinline__ void sh_item(const ShParams &p, const ShItem &it, flo
         const int d = 16 * dt + c;
         vo_v[dt] = (HD % 16 == 0 || d < HD) ? (unsigned)((d * SMOL_SLAB + 8 * j) * 2) : OOB_OFF;
     }
+    uint4 k[2][KS], v[1][DT];
     /* a slab at or past ke has an empty range: its loads return zeros */
-    auto issue_k = [&](int k0, KRaw &r) __attribute__((always_inline)) {
+    auto issue_k = [&](int k0) __attribute__((always_inline)) {
         const bool live = k0 < it.ke;
         const rsrc_t rs = make_rsrc(it.kc, live ? it.region_bytes : 0);
         const unsigned so = live ? (unsigned)(k0 / SMOL_SLAB) * Gm::SLAB_BYTES : 0u;
@@ -164,353 +413,230 @@ __device__ __forceinline__ void sh_item(const ShParams &p, const ShItem &it, flo
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
-                r.k[t][ks] = HD % 32 == 0 ? bload(rs, vo_k[0][0], so + (unsigned)((4 * t * HD + 32 * ks) * 2))
-                                          : bload(rs, vo_k[t][ks], so);
+                k[t][ks] = HD % 32 == 0 ? bload(rs, vo_k[0][0], so + (unsigned)((4 * t * HD + 32 * ks) * 2))
+                                        : bload(rs, vo_k[t][ks], so);
     };
-    auto issue_v = [&](int k0, VRaw &r) __attribute__((always_inline)) {
+    auto issue_v = [&](int k0) __attribute__((always_inline)) {
         const bool live = k0 < it.ke;
         const rsrc_t rs = make_rsrc(it.vtc, live ? it.region_bytes : 0);
         const unsigned so = live ? (unsigned)(k0 / SMOL_SLAB) * Gm::SLAB_BYTES : 0u;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
-            r.v[dt] = HD % 16 == 0 ? bload(rs, vo_v[0], so + (unsigned)(16 * dt * SMOL_SLAB * 2)) : bload(rs, vo_v[dt], so);
+            v[0][dt] = HD % 16 == 0 ? bload(rs, vo_v[0], so + (unsigned)(16 * dt * SMOL_SLAB * 2)) : bload(rs, vo_v[dt], so);
     };
     int k0 = it.kb + wave * SMOL_SLAB;
-    KRaw kr;
-    VRaw vr;
-
-    /* ---- stage the rows: normalised, rotated and split into fragments ----
-     * Thread chunks of 8 elements; every load of a chunk (its row, the table
-     * row, the weights) is issued before the first is used, and the first
-     * slab's behind them. */
-    constexpr int CH8 = HD / 8, HALF = HD / 2;
-    constexpr int NQ = ((TR + 1) * CH8 + SH_TPB - 1) / SH_TPB;
-    const int n_rows = R + (it.with_new ? 1 : 0); /* row R: the new key */
-    auto row_seq = [&](int r) { return it.prefix ? (it.row0 + r) / G : it.seq; };
-    auto row_head = [&](int r) { return it.g * G + (it.prefix ? (it.row0 + r) % G : it.row0 + r); };
-    const bool rope = p.rope_kind != SMOL_ROPE_OFF;
-    float x[NQ][8], cv[NQ][8], sn[NQ][8];
-    ShSeq own;
-    if (!it.prefix) own = sh_seq(p, it.seq);
+    ShRows<HD> w;
+    /* the new token is the last wave's, which has the fewest slabs: its key and value wait in LDS until the slabs are done */
+    const bool add_new = it.with_new && wave == SH_NW - 1;
+    float *s_kn = reinterpret_cast<float *>(smem + Gm::CB_BYTES), *s_vn = s_kn + KS * 32;
+    const long long new_row = ((long long)it.seq * p.Hkv + it.g) * HD;
+    {
+        float y[KS][8], vn[(HD + 63) / 64];
+        sh_rows<HD>(p, it, 0, c, j, w, y, [&]() __attribute__((always_inline)) {
+            if (add_new) {
 #pragma unroll
-    for (int u = 0; u < NQ; u++) {
-        const int e = tid + SH_TPB * u, r = e / CH8, d0 = (e - r * CH8) * 8;
-        if (e < n_rows * CH8) {
-            const int sq = r < R ? row_seq(r) : it.seq;
-            if (r < R) load8(p.q_in, p.in_dtype, (long long)sq * p.Hq * HD + (long long)row_head(r) * HD + d0, x[u]);
-            else load8(p.k_in, p.in_dtype, ((long long)sq * p.Hkv + it.g) * HD + d0, x[u]);
-            if (rope) {
-                const long long at = (long long)(it.prefix ? sh_seq(p, sq).pos : own.pos) * HD + d0;
-                ld8f(p.rope_cos + at, cv[u]);
-                ld8f(p.rope_sin + at, sn[u]);
+                for (int u = 0; u < (HD + 63) / 64; u++)
+                    if (HD % 64 == 0 || 64 * u + lane < HD)
+                        vn[u] = p.in_dtype == SMOL_IN_BF16 ? bf16_to_f32(((const uint16_t *)p.v_in)[new_row + 64 * u + lane])
+                                                           : ((const float *)p.v_in)[new_row + 64 * u + lane];
             }
-        }
-    }
-    float vn[8];
-    if (it.with_new && tid < CH8) load8(p.v_in, p.in_dtype, ((long long)it.seq * p.Hkv + it.g) * HD + tid * 8, vn);
-    issue_k(k0, kr);
-    issue_v(k0, vr);
-    /* rows past R are zero columns */
-    for (int e = tid; e < (TR - R) * 4 * KS * Q_PARTS; e += SH_TPB) {
-        const int r = R + e % (TR - R), w = e / (TR - R), ks = w / 4 % KS, q = w / (4 * KS);
-        s_frag[((q * KS + ks) * NT + (r >> 4)) * 64 + (w & 3) * 16 + (r & 15)] = make_uint4(0, 0, 0, 0);
-    }
-    if constexpr (HDP > HD) /* and so are columns past head_dim */
-        for (int e = tid; e < R * (HDP - HD) / 8 * Q_PARTS; e += SH_TPB) {
-            const int r = e % R, w = e / R, d0 = HD + w % ((HDP - HD) / 8) * 8, q = w / ((HDP - HD) / 8);
-            s_frag[((q * KS + d0 / 32) * NT + (r >> 4)) * 64 + (d0 >> 3 & 3) * 16 + (r & 15)] = make_uint4(0, 0, 0, 0);
-        }
+            issue_k(k0);
+            if (HD <= 128) issue_v(k0); /* at 256 the rows' registers leave no room for both */
+        });
+        if (add_new) {
 #pragma unroll
-    for (int u = 0; u < NQ; u++) {
-        const int e = tid + SH_TPB * u, r = e / CH8, d0 = (e - r * CH8) * 8;
-        if (e < n_rows * CH8) {
-            const float *w = r < R ? p.q_norm : p.k_norm;
-            if (w) {
-                float ss = 0.0f, wv[8];
-                ld8f(w + d0, wv);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    ss = fmaf(x[u][i], x[u][i], ss);
-                    x[u][i] *= wv[i];
+            for (int ks = 0; ks < KS; ks++)
+                if (c == it.R) {
+                    *reinterpret_cast<f4 *>(s_kn + 32 * ks + 8 * j) = f4{y[ks][0], y[ks][1], y[ks][2], y[ks][3]};
+                    *reinterpret_cast<f4 *>(s_kn + 32 * ks + 8 * j + 4) = f4{y[ks][4], y[ks][5], y[ks][6], y[ks][7]};
                 }
-                s_ss[e] = ss;
-            }
-            st8f(s_raw + r * QSTR + d0, x[u]);
+#pragma unroll
+            for (int u = 0; u < (HD + 63) / 64; u++)
+                if (64 * u + lane < KS * 32) s_vn[64 * u + lane] = HD % 64 == 0 || 64 * u + lane < HD ? vn[u] : 0.0f;
         }
     }
-    if (it.with_new && tid < CH8) st8f(s_vnew + tid * 8, vn);
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < NQ; u++) {
-        const int e = tid + SH_TPB * u, r = e / CH8, d0 = (e - r * CH8) * 8;
-        if (e < n_rows * CH8) {
-            const bool is_k = r >= R;
-            float ri = is_k ? 1.0f : p.qscale;
-            if (is_k ? p.k_norm != nullptr : p.q_norm != nullptr) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int i = 0; i < CH8; i++) ss += s_ss[r * CH8 + i];
-                ri *= 1.0f / sqrtf(ss / (float)HD + p.norm_eps);
-            }
-            float y[8];
-            if (!rope) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = x[u][i];
-            } else if (p.rope_kind == SMOL_ROPE_INTERLEAVED_K) {
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    y[i] = fmaf(x[u][i], cv[u][i], -(x[u][i + 1] * sn[u][i]));
-                    y[i + 1] = fmaf(x[u][i + 1], cv[u][i + 1], x[u][i] * sn[u][i + 1]);
-                }
-            } else {
-                const float *row = s_raw + r * QSTR;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int d = d0 + i;
-                    const float pr = row[d < HALF ? d + HALF : d - HALF];
-                    y[i] = d < HALF ? fmaf(x[u][i], cv[u][i], -(pr * sn[u][i])) : fmaf(x[u][i], cv[u][i], pr * sn[u][i]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[u][i] = y[i] * ri;
-            if (is_k) {
-                st8f(s_knew + d0, x[u]);
-            } else {
-                b8 f[Q_PARTS];
-                split8x3(x[u], f[0], f[1], f[2]);
-                const int ks = d0 / 32, at = ((d0 >> 3) & 3) * 16 + (r & 15);
-#pragma unroll
-                for (int q = 0; q < Q_PARTS; q++)
-                    s_frag[((q * KS + ks) * NT + (r >> 4)) * 64 + at] = *reinterpret_cast<uint4 *>(&f[q]);
-            }
-        }
-    }
-    __syncthreads();
-    if (it.with_new) {
-        /* the new key's fp32 score by chunks: row_new() sums them */
-#pragma unroll
-        for (int u = 0; u < NQ; u++) {
-            const int e = tid + SH_TPB * u, r = e / CH8, d0 = (e - r * CH8) * 8;
-            if (r < R) {
-                float kn[8], sd = 0.0f;
-                ld8f(s_knew + d0, kn);
-#pragma unroll
-                for (int i = 0; i < 8; i++) sd = fmaf(x[u][i], kn[i], sd);
-                s_ss[e] = sd;
-            }
-        }
-    }
-    auto row_new = [&](int r) __attribute__((always_inline)) {
-        float sd = 0.0f;
-#pragma unroll
-        for (int i = 0; i < CH8; i++) sd += s_ss[r * CH8 + i];
-        return p.cap2 > 0.0f ? p.cap2 * tanhf(sd / p.cap2) : sd;
-    };
-
-    /* ---- row ranges, state ---- */
-    float m[NT], l[NT];
-    f4 o[NT][DT];
-    int lo[NT], lo_min = 1 << 30, lo_max = 0; /* window: the first key that a row sees */
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        m[t] = -INFINITY;
-        l[t] = 0.0f;
-        lo[t] = 0;
-        if (p.window > 0) {
-            const int r = t * 16 + c;
-            if (r < R) lo[t] = max(0, sh_seq(p, row_seq(r)).pos - p.window + 1 - (it.prefix ? 0 : p.p_len));
-            lo_max = max(lo_max, lo[t]);
-            lo_min = min(lo_min, r < R ? lo[t] : 1 << 30);
-        }
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) o[t][dt] = f4{0.f, 0.f, 0.f, 0.f};
-    }
-    if (p.window > 0) {
-#pragma unroll
-        for (int sh = 1; sh < 16; sh <<= 1) {
-            lo_max = max(lo_max, __shfl_xor(lo_max, sh));
-            lo_min = min(lo_min, __shfl_xor(lo_min, sh));
-        }
-        lo_max = __builtin_amdgcn_readfirstlane(lo_max);
-        lo_min = __builtin_amdgcn_readfirstlane(lo_min);
-    } else {
-        lo_min = 0;
-    }
-
-    /* ---- the wave's slabs ---- */
+    if (HD > 128) issue_v(k0);
+    float *logits = SC && c < it.R
+                        ? p.logits + ((long long)it.seq * p.Hq + it.g * p.G + it.row0 + c) * p.l_stride + 8 * j : nullptr;
     while (k0 < it.ke) {
-        /* Q's fragments are read from LDS in every slab: kept in registers
-         * they would take 48 NT of them at head_dim 128 (the fence keeps the
-         * compiler from moving the reads in front of the loop) */
-        asm volatile("" ::: "memory");
-        f4 sacc[NT][2];
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            sacc[t][0] = sacc[t][1] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int q = Q_PARTS - 1; q >= 0; q--)
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    const b8 f = as_b8(s_frag[((q * KS + ks) * NT + t) * 64 + lane]);
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        sacc[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(kr.k[h][ks]), f, sacc[t][h], 0, 0, 0);
-                }
-        }
+        f4 s[1][2];
+        sh_qk<HD>(w, k, s[0]);
         const int k1 = k0 + SMOL_SLAB * SH_NW;
-        issue_k(k1, kr);
-        /* keys of the slab that some row does not see */
-        const bool low = k0 < lo_max, tail = k0 + SMOL_SLAB > it.ke;
-        bool apart = false; /* a value that is not finite in a slab whose rows see different keys */
-        if (low || tail) {
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) vr.v[dt] = keep_keys8(vr.v[dt], k0 + 8 * j, lo_min, it.ke);
-            if (low && lo_min < lo_max) {
-                bool bad = false;
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++) bad |= any_not_finite(vr.v[dt]);
-                apart = __any(bad);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            float sv[8];
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) sv[4 * h + i] = sacc[t][h][i];
-            if (p.cap2 > 0.0f) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) sv[e] = p.cap2 * tanhf(sv[e] / p.cap2);
-            }
-            if constexpr (SC) {
-                if (c < R) {
-                    float *lg = p.logits + ((long long)it.seq * p.Hq + row_head(c)) * p.l_stride + k0 + 8 * j;
-                    st8f(lg, sv);
-                }
-            }
-            if (low || tail) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int key = k0 + 8 * j + e;
-                    sv[e] = key >= lo[t] && key < it.ke ? sv[e] : -INFINITY;
-                }
-            }
-            float mx = sv[0];
-#pragma unroll
-            for (int e = 1; e < 8; e++) mx = fmaxf(mx, sv[e]);
-            mx = row_max4(mx);
-            const bool need = mx > m[t] + LAZY_T;
-            if (__any(need)) {
-                const float m_new = need ? mx : m[t];
-                const float alpha = need ? __builtin_amdgcn_exp2f(m[t] - m_new) : 1.0f;
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++) o[t][dt] *= alpha;
-                l[t] *= alpha;
-                m[t] = m_new;
-            }
-            const float m_use = m[t] == -INFINITY ? 0.0f : m[t];
-            float pv[8], ps = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                pv[e] = __builtin_amdgcn_exp2f(sv[e] - m_use);
-                ps += pv[e];
-            }
-            l[t] += ps;
-            b8 pp[P_PARTS];
-            split8x3(pv, pp[0], pp[1], pp[2]);
-            if (apart) {
-                /* a row must not meet 0 x inf: one row at a time, against
-                 * the values that it sees */
-                for (int r = 0; r < 16; r++) {
-                    const int lo_r = __builtin_amdgcn_readlane(lo[t], r);
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) {
-                        const b8 v = as_b8(keep_keys8(vr.v[dt], k0 + 8 * j, lo_r, it.ke));
-                        f4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int q = P_PARTS - 1; q >= 0; q--) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pp[q], a, 0, 0, 0);
-                        if (c == r) o[t][dt] += a;
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int q = P_PARTS - 1; q >= 0; q--)
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++)
-                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(vr.v[dt]), pp[q], o[t][dt], 0, 0, 0);
-            }
-        }
-        issue_v(k1, vr);
+        issue_k(k1);
+        const bool nan = sh_mask<HD, 1, SC>(p, w, k0, it.ke, j, s, v, SC && logits ? logits + k0 : nullptr);
+        sh_pv<HD, 1>(w, s, v, nan);
+        issue_v(k1);
         k0 = k1;
     }
-
-    /* ---- the waves' states (and the new token's) join, one row tile at a time ---- */
-    float *cb = smem, *cm = smem + SH_NW * 16 * OSTR, *cl = cm + SH_NW * 16;
-    for (int t = 0; t < NT; t++) {
-        __syncthreads();
+    float lt = row_sum4(w.l);
+    if (add_new) {
+        /* the new token: its fp32 score of every row (the three parts hold the row whole), its share of the state, its
+         * bf16 row in the cache */
+        float sd = 0.0f;
 #pragma unroll
-        for (int tt = 0; tt < NT; tt++)
-            if (tt == t) {
-                const float lt = row_sum4(l[tt]);
-                if (j == 0) {
-                    cm[wave * 16 + c] = m[tt];
-                    cl[wave * 16 + c] = lt;
-                }
+        for (int ks = 0; ks < KS; ks++) {
+            float kn[8];
+            ld8f(s_kn + 32 * ks + 8 * j, kn);
+            /* (formed here: in front of the slab loop the fp32 rows would hold registers through it) */
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-                    *reinterpret_cast<f4 *>(cb + (wave * 16 + c) * OSTR + 16 * dt + 4 * j) = o[tt][dt];
-            }
-        __syncthreads();
-        for (int e = tid; e < 16 * (HD / 4); e += SH_TPB) {
-            const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
-            if (t * 16 + r >= R) continue;
-            const float s_new = it.with_new ? row_new(r) : -INFINITY;
-            float mm = s_new;
+            for (int q = 0; q < Q_PARTS; q++) asm volatile("" : "+v"(w.q[q][ks]));
 #pragma unroll
-            for (int w = 0; w < SH_NW; w++) mm = fmaxf(mm, cm[w * 16 + r]);
-            const float mu = mm == -INFINITY ? 0.0f : mm;
-            f4 acc = {0.f, 0.f, 0.f, 0.f};
-            float ls = 0.0f;
-            if (it.with_new) {
-                ls = __builtin_amdgcn_exp2f(s_new - mu);
-                acc = *reinterpret_cast<f4 *>(s_vnew + d) * ls;
-            }
+            for (int i = 0; i < 8; i++) sd = fmaf(((float)w.q[0][ks][i] + (float)w.q[1][ks][i]) + (float)w.q[2][ks][i], kn[i], sd);
+        }
+        sd = row_sum4(sd);
+        if (p.cap2 > 0.0f) sd = p.cap2 * tanhf(sd / p.cap2);
+        if (SC && j == 0 && c < it.R) p.logit_new[(long long)it.seq * p.Hq + it.g * p.G + it.row0 + c] = sd;
+        const float mm = fmaxf(w.m, sd), mu = mm == -INFINITY ? 0.0f : mm;
+        const float alpha = __builtin_amdgcn_exp2f(w.m - mu), pn = __builtin_amdgcn_exp2f(sd - mu);
+        lt = fmaf(lt, alpha, pn);
+        w.m = mm;
 #pragma unroll
-            for (int w = 0; w < SH_NW; w++) {
-                const float f = __builtin_amdgcn_exp2f(cm[w * 16 + r] - mu);
-                ls += f * cl[w * 16 + r];
-                acc += f * *reinterpret_cast<f4 *>(cb + (w * 16 + r) * OSTR + d);
+        for (int dt = 0; dt < DT; dt++) w.o[dt] = w.o[dt] * alpha + *reinterpret_cast<const f4 *>(s_vn + 16 * dt + 4 * j) * pn;
+        if (it.row0 == 0) {
+            const ShSeq sq = sh_seq(p, it.seq);
+            const long long base = (long long)sq.slot * p.c_slot_stride + (long long)it.g * p.cap * HD;
+            if (lane < HD / 8) {
+                float kn[8];
+                ld8f(s_kn + 8 * lane, kn);
+                *reinterpret_cast<uint4 *>(p.kc + base + (long long)sq.len * HD + 8 * lane) = pack_bf16x8(kn);
             }
-            *reinterpret_cast<f4 *>(it.part_o + (long long)(t * 16 + r) * HD + d) = acc;
-            if (d == 0) {
-                *reinterpret_cast<float2 *>(it.part_ml + (t * 16 + r) * 2) = make_float2(mm, ls);
-                if (SC && it.with_new) p.logit_new[(long long)it.seq * p.Hq + row_head(r)] = s_new;
-            }
+            uint16_t *vt = p.vtc + base + (long long)(sq.len / SMOL_SLAB) * SMOL_SLAB * HD + sq.len % SMOL_SLAB;
+            for (int d = lane; d < HD; d += 64) vt[(long long)d * SMOL_SLAB] = f32_to_bf16(s_vn[d]);
         }
     }
-    if (it.with_new && it.row0 == 0) {
-        const ShSeq sq = sh_seq(p, it.seq);
-        for (int d0 = tid * 8; d0 < HD; d0 += SH_TPB * 8) {
-            const long long base = (long long)sq.slot * p.c_slot_stride + (long long)it.g * p.cap * HD;
-            float y[8];
-            ld8f(s_knew + d0, y);
-            *reinterpret_cast<uint4 *>(p.kc + base + (long long)sq.len * HD + d0) = pack_bf16x8(y);
-            uint16_t *vt = p.vtc + base + (long long)(sq.len / SMOL_SLAB) * SMOL_SLAB * HD + sq.len % SMOL_SLAB;
+
+    /* the waves' states join */
+    float *cb = reinterpret_cast<float *>(smem), *cm = cb + SH_NW * 16 * OSTR, *cl = cm + SH_NW * 16;
+    if (j == 0) {
+        cm[wave * 16 + c] = w.m;
+        cl[wave * 16 + c] = lt;
+    }
 #pragma unroll
-            for (int i = 0; i < 8; i++) vt[(long long)(d0 + i) * SMOL_SLAB] = f32_to_bf16(s_vnew[d0 + i]);
+    for (int dt = 0; dt < DT; dt++) *reinterpret_cast<f4 *>(cb + (wave * 16 + c) * OSTR + 16 * dt + 4 * j) = w.o[dt];
+    __syncthreads();
+    for (int e = tid; e < it.R * (HD / 4); e += SH_TPB) {
+        const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < SH_NW; q++) mm = fmaxf(mm, cm[q * 16 + r]);
+        const float mu = mm == -INFINITY ? 0.0f : mm;
+        f4 acc = {0.f, 0.f, 0.f, 0.f};
+        float ls = 0.0f;
+#pragma unroll
+        for (int q = 0; q < SH_NW; q++) {
+            const float f = __builtin_amdgcn_exp2f(cm[q * 16 + r] - mu);
+            ls = fmaf(f, cl[q * 16 + r], ls);
+            acc += f * *reinterpret_cast<f4 *>(cb + (q * 16 + r) * OSTR + d);
         }
+        *reinterpret_cast<f4 *>(it.part_o + (long long)r * HD + d) = acc;
+        if (d == 0) *reinterpret_cast<float2 *>(it.part_ml + r * 2) = make_float2(mm, ls);
+    }
+}
+
+/* 64 rows of the batch, 16 a wave, against slabs that all waves share through LDS. The ring's 16-byte pieces are placed
+ * so that the eight lanes that LDS serves together (rows c .. c + 7 of one j) fall in different columns of its 128-byte
+ * lines: piece q of K row r at q ^ ((r & 3) | (r >> 3 & 1) << 2), piece j of V^T row d at j ^ (d >> 1 & 3). A transfer
+ * writes its lanes' pieces one after the other, so it is the lanes' source addresses that are permuted. */
+template <int HD>
+__device__ __forceinline__ void sh_wide(const ShParams &p, const ShItem &it, char *smem) {
+    using Gm = ShGeom<HD>;
+    constexpr int KS = Gm::KS, DT = Gm::DT, STAGES = Gm::STAGES, WS = Gm::WS, PC = HD / 8; /* PC: 16-byte pieces of a K row */
+    constexpr int PART = Gm::SLAB_BYTES / 1024, ND = 2 * PART / SH_NW; /* 1 KB transfers of a slab's K (V^T); a wave's of a slab */
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = (it.ke - it.kb + SMOL_SLAB - 1) / SMOL_SLAB, first = it.kb / SMOL_SLAB;
+    const rsrc_t rk = make_rsrc(it.kc, it.region_bytes), rv = make_rsrc(it.vtc, it.region_bytes);
+    const unsigned lds0 = (unsigned)(size_t)smem;
+    /* transfer t of a slab (K's first): lane l's piece at 16 l */
+    unsigned voff[ND];
+#pragma unroll
+    for (int u = 0; u < ND; u++) {
+        const int t = wave * ND + u, piece = t % PART * 64 + lane;
+        if (t < PART) {
+            const int r = piece / PC, q = piece % PC;
+            voff[u] = (unsigned)((r * PC + (q ^ ((r & 3) | (r >> 3 & 1) << 2))) * 16);
+        } else {
+            const int d = piece / 4, q = piece % 4;
+            voff[u] = (unsigned)((d * 4 + (q ^ (d >> 1 & 3))) * 16);
+        }
+    }
+    auto fetch = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < WS; s++) {
+            /* past the last slab the last one again: every step has the same number of transfers in flight */
+            const unsigned so = (unsigned)(first + min(i * WS + s, n - 1)) * Gm::SLAB_BYTES;
+            const unsigned at = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)((i % STAGES) * WS + s) * 2 * Gm::SLAB_BYTES + wave * ND * 1024);
+#pragma unroll
+            for (int u = 0; u < ND; u++) dma_1k(wave * ND + u < PART ? rk : rv, voff[u], so, at + u * 1024);
+        }
+    };
+    ShRows<HD> w;
+    {
+        float y[KS][8];
+        sh_rows<HD>(p, it, 16 * wave, c, j, w, y, []() {});
+    }
+    /* the compiler's own loads are done before the first transfer, so vmcnt counts transfers alone from here on */
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++) fetch(i);
+    const int kt_row = 8 * (c >> 2) + (c & 3), ksw = (c & 3) | (c >> 2 & 1) << 2;
+    const int n_steps = (n + WS - 1) / WS;
+    for (int i = 0; i < n_steps; i++) {
+        /* this wave's part of step i has landed (later ones may be on their way); then everybody's has, and nobody
+         * still reads the stage that the next transfers overwrite */
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * WS * ND) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        fetch(i + STAGES - 1);
+        const char *sk = smem + (i % STAGES) * WS * 2 * Gm::SLAB_BYTES;
+        f4 s[WS][2];
+        uint4 v[WS][DT];
+#pragma unroll
+        for (int u = 0; u < WS; u++) {
+            uint4 k[2][KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) /* rows kt_row + 4 t: the swizzle's bits are c's */
+                    k[t][ks] = *reinterpret_cast<const uint4 *>(sk + u * 2 * Gm::SLAB_BYTES +
+                                                                ((kt_row + 4 * t) * PC + ((4 * ks + j) ^ ksw)) * 16);
+            sh_qk<HD>(w, k, s[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < WS; u++)
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                const int d = 16 * dt + c;
+                v[u][dt] = *reinterpret_cast<const uint4 *>(sk + (2 * u + 1) * Gm::SLAB_BYTES + (d * 4 + (j ^ (d >> 1 & 3))) * 16);
+            }
+        /* a slab past the last one repeats it; its keys are past ke */
+        const bool nan = sh_mask<HD, WS, false>(p, w, it.kb + i * WS * SMOL_SLAB, it.ke, j, s, v, nullptr);
+        sh_pv<HD, WS>(w, s, v, nan);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); /* no transfer outlives the workgroup */
+    const float lt = row_sum4(w.l);
+    const int r = 16 * wave + c;
+    if (r < it.R) {
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) *reinterpret_cast<f4 *>(it.part_o + (long long)r * HD + 16 * dt + 4 * j) = w.o[dt];
+        if (j == 0) *reinterpret_cast<float2 *>(it.part_ml + r * 2) = make_float2(w.m, lt);
     }
 }
 
 } // namespace
 
-template <int HD, int NT, bool SC>
-__global__ __launch_bounds__(SH_TPB, HD <= 128 && NT <= 2 ? 2 : 1) void k_sh(const ShParams p) {
-    __shared__ __attribute__((aligned(16))) float smem[ShLds<HD, NT>::FLOATS];
+/* KIND: what the call's prefix items are */
+enum { SH_NARROW, SH_WIDE, SH_SCORED };
+template <int HD, int KIND>
+__global__ __launch_bounds__(SH_TPB, HD <= 128 ? 2 : 1) void k_sh(const ShParams p) {
+    using Gm = ShGeom<HD>;
+    constexpr int NARROW = Gm::CB_BYTES + 2 * Gm::KS * 32 * 4; /* the waves' states, the new key and value */
+    constexpr int LDS = KIND == SH_WIDE && Gm::RING_BYTES > NARROW ? Gm::RING_BYTES : NARROW;
+    constexpr int ROWS = KIND == SH_WIDE ? 16 * SH_NW : 16;
+    __shared__ __attribute__((aligned(1024))) char smem[LDS];
     const int b = blockIdx.x;
     ShItem it;
-    if (NT > 1 || !SC) {
+    if constexpr (KIND != SH_SCORED) {
         if (b < p.n_pblocks) {
             /* workgroups b and b + 8 share an L2: the row blocks of one chunk follow each other there */
             const int rb = (b / 8) % p.n_rb, u = (b / (8 * p.n_rb)) * 8 + b % 8;
@@ -518,8 +644,8 @@ __global__ __launch_bounds__(SH_TPB, HD <= 128 && NT <= 2 ? 2 : 1) void k_sh(con
             if (sp >= p.n_ps) return;
             it.prefix = true;
             it.g = g;
-            it.row0 = rb * 16 * NT;
-            it.R = min(16 * NT, p.n_seq * p.G - it.row0);
+            it.row0 = rb * ROWS;
+            it.R = min(ROWS, p.n_seq * p.G - it.row0);
             it.seq = 0;
             it.kb = p.p_first + sp * p.p_chunk;
             it.ke = min(p.p_len, it.kb + p.p_chunk);
@@ -530,7 +656,8 @@ __global__ __launch_bounds__(SH_TPB, HD <= 128 && NT <= 2 ? 2 : 1) void k_sh(con
             const long long row = ((long long)sp * p.Hkv + g) * p.n_seq * p.G + it.row0;
             it.part_o = p.p_o + row * HD;
             it.part_ml = p.p_ml + row * 2;
-            sh_item<HD, NT, false>(p, it, smem);
+            if constexpr (KIND == SH_WIDE) sh_wide<HD>(p, it, smem);
+            else sh_narrow<HD, false>(p, it, smem);
             return;
         }
     }
@@ -541,8 +668,8 @@ __global__ __launch_bounds__(SH_TPB, HD <= 128 && NT <= 2 ? 2 : 1) void k_sh(con
     if (sp >= sh_own_chunks(p, sq)) return;
     it.prefix = false;
     it.g = g;
-    it.row0 = srb * 16;
-    it.R = min(16, p.G - it.row0);
+    it.row0 = srb * OWN_ROWS;
+    it.R = min(OWN_ROWS, p.G - it.row0);
     it.seq = i;
     it.kb = sh_own_first(p, sq) + sp * p.s_chunk;
     it.ke = min(sq.len, it.kb + p.s_chunk);
@@ -554,7 +681,7 @@ __global__ __launch_bounds__(SH_TPB, HD <= 128 && NT <= 2 ? 2 : 1) void k_sh(con
     const long long row = (((long long)i * p.Hkv + g) * p.n_ss + sp) * p.G + it.row0;
     it.part_o = p.s_o + row * HD;
     it.part_ml = p.s_ml + row * 2;
-    sh_item<HD, 1, SC>(p, it, smem);
+    sh_narrow<HD, KIND == SH_SCORED>(p, it, smem);
 }
 
 /* Joins the chunks of the output rows, one workgroup a row (a sequence's
@@ -616,25 +743,31 @@ __global__ __launch_bounds__(256) void k_sh_merge(const ShParams p) {
     const ShSeq sq = sh_seq(p, i);
     if (chunk * MASS_KEYS > sq.len) return;
     const int ns = sh_own_chunks(p, sq);
-    float acc[MASS_KEYS / 256] = {};
+    constexpr int KU = MASS_KEYS / 256;
+    float acc[KU] = {};
+    const int lane = tid & 63;
+    const float *ml0 = p.s_ml + ((((long long)i * p.Hkv + g) * p.n_ss) * p.G) * 2;
     for (int h = 0; h < p.G; h++) {
+        const long long row = (long long)i * p.Hq + g * p.G + h;
+        float x[KU];
+#pragma unroll
+        for (int u = 0; u < KU; u++) {
+            const int key = chunk * MASS_KEYS + u * 256 + tid;
+            x[u] = key < sq.len ? p.logits[row * p.l_stride + key] : key == sq.len ? p.logit_new[row] : 0.0f;
+        }
         /* every wave finds (m, l) by itself: the same order, so the same bits in each */
-        const float *ml = p.s_ml + ((((long long)i * p.Hkv + g) * p.n_ss) * p.G + h) * 2;
-        const int lane = tid & 63;
-        const float2 x = lane < ns ? *reinterpret_cast<const float2 *>(ml + (long long)lane * p.G * 2)
-                                   : make_float2(-INFINITY, 0.0f);
-        float M = x.x;
+        const float2 ml = lane < ns ? *reinterpret_cast<const float2 *>(ml0 + ((long long)lane * p.G + h) * 2)
+                                    : make_float2(-INFINITY, 0.0f);
+        float M = ml.x;
+#pragma unroll
         for (int sh = 1; sh < 64; sh <<= 1) M = fmaxf(M, __shfl_xor(M, sh));
         const float mu = M == -INFINITY ? 0.0f : M;
-        float Ls = lane < ns ? __builtin_amdgcn_exp2f(x.x - mu) * x.y : 0.0f;
-        for (int sh = 1; sh < 64; sh <<= 1) Ls += __shfl_xor(Ls, sh);
-        const long long row = (long long)i * p.Hq + g * p.G + h;
+        float Ls = lane < ns ? __builtin_amdgcn_exp2f(ml.x - mu) * ml.y : 0.0f;
 #pragma unroll
-        for (int u = 0; u < MASS_KEYS / 256; u++) {
-            const int key = chunk * MASS_KEYS + u * 256 + tid;
-            if (key <= sq.len)
-                acc[u] += __builtin_amdgcn_exp2f((key < sq.len ? p.logits[row * p.l_stride + key] : p.logit_new[row]) - mu) / Ls;
-        }
+        for (int sh = 1; sh < 64; sh <<= 1) Ls += __shfl_xor(Ls, sh);
+        const float rl = 1.0f / Ls;
+#pragma unroll
+        for (int u = 0; u < KU; u++) acc[u] = fmaf(__builtin_amdgcn_exp2f(x[u] - mu), rl, acc[u]);
     }
     float *mass = p.mass + ((long long)sq.slot * p.Hkv + g) * p.m_stride;
 #pragma unroll
@@ -650,16 +783,11 @@ __global__ __launch_bounds__(256) void k_sh_merge(const ShParams p) {
 }
 
 template <int HD>
-static int launch_hd(const ShParams *p, int nt, int max_len, hipStream_t st, hipEvent_t e0, hipEvent_t e1) {
+static int launch_hd(const ShParams *p, int tile_rows, int max_len, hipStream_t st, hipEvent_t e0, hipEvent_t e1) {
     const unsigned blocks = (unsigned)p->n_pblocks + (unsigned)p->n_ss * p->n_seq * p->Hkv * p->s_rb;
-    if (p->mass) hipExtLaunchKernelGGL((k_sh<HD, 1, true>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
-    else if (nt == 1) hipExtLaunchKernelGGL((k_sh<HD, 1, false>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
-    else if (nt == 4 && HD <= 128) {
-        if constexpr (HD <= 128) hipExtLaunchKernelGGL((k_sh<HD, 4, false>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
-    } else if (nt == 2 && HD == 256) {
-        if constexpr (HD == 256) hipExtLaunchKernelGGL((k_sh<HD, 2, false>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
-    }
-    else if constexpr (HD <= 128) hipExtLaunchKernelGGL((k_sh<HD, 2, false>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
+    if (p->mass) hipExtLaunchKernelGGL((k_sh<HD, SH_SCORED>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
+    else if (tile_rows == 16) hipExtLaunchKernelGGL((k_sh<HD, SH_NARROW>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
+    else if constexpr (ShGeom<HD>::WIDE) hipExtLaunchKernelGGL((k_sh<HD, SH_WIDE>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
     else return -1;
     if (hipGetLastError() != hipSuccess) return -3;
     unsigned mb = (unsigned)p->n_seq * p->Hq;
@@ -668,22 +796,27 @@ static int launch_hd(const ShParams *p, int nt, int max_len, hipStream_t st, hip
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }
 
-/* rows of a prefix item's tile at head_dim hd, for a batch of `rows` rows a kv head */
-extern "C" int smol_shared_tile_rows(int hd, int rows) { return rows <= 16 || hd > 128 ? 16 : 32; }
+/* rows of a prefix item at head_dim hd, for a batch of `rows` rows a kv head: 64 for a wide item. Wide items read K and
+ * V once for 64 rows where narrow ones do for 16 (64 sequences on 16384, head_dim 128, 128 rows a kv head: 71 us a call,
+ * 93 with narrow ones; 32 rows on 4096: 20 either way). Not at 256, where a wave's state leaves one workgroup a compute
+ * unit and its steps do not overlap (192 rows on 8191: 38 us, 31 narrow). */
+extern "C" int smol_shared_tile_rows(int hd, int rows) { return rows <= 32 || (hd != 64 && hd != 128) ? 16 : 16 * SH_NW; }
+
+/* heads of an own-rows item */
+extern "C" int smol_shared_own_rows(void) { return OWN_ROWS; }
 
 /* workgroups of a compute unit at once (k_sh's launch bounds) */
 extern "C" int smol_shared_occupancy(int hd) { return hd <= 128 ? 2 : 1; }
 
 extern "C" int smol_launch_shared(const ShParams *p, int hd, int tile_rows, int max_len, hipStream_t st, hipEvent_t e0,
                                   hipEvent_t e1) {
-    const int nt = tile_rows / 16;
     switch (hd) {
-    case 64: return launch_hd<64>(p, nt, max_len, st, e0, e1);
-    case 72: return launch_hd<72>(p, nt, max_len, st, e0, e1);
-    case 80: return launch_hd<80>(p, nt, max_len, st, e0, e1);
-    case 96: return launch_hd<96>(p, nt, max_len, st, e0, e1);
-    case 128: return launch_hd<128>(p, nt, max_len, st, e0, e1);
-    case 256: return launch_hd<256>(p, nt, max_len, st, e0, e1);
+    case 64: return launch_hd<64>(p, tile_rows, max_len, st, e0, e1);
+    case 72: return launch_hd<72>(p, tile_rows, max_len, st, e0, e1);
+    case 80: return launch_hd<80>(p, tile_rows, max_len, st, e0, e1);
+    case 96: return launch_hd<96>(p, tile_rows, max_len, st, e0, e1);
+    case 128: return launch_hd<128>(p, tile_rows, max_len, st, e0, e1);
+    case 256: return launch_hd<256>(p, tile_rows, max_len, st, e0, e1);
     default: return -1;
     }
 }

@@ -203,6 +203,16 @@ SHARED = [
     # more rows a kv head than one tile, an odd number of them
     dict(hq=8, hkv=1, hd=256, lens=[200, 0, 31, 77, 5], prefix=1000, inter=True, bf16=True, cap=30.0),
     dict(hq=12, hkv=4, hd=128, lens=list(range(0, 46, 2)), prefix=700, cap=50.0),
+    # more than 32 rows a kv head: 64 rows share the prefix's slabs, a last block of one row, less than a slab
+    dict(hq=8, hkv=2, hd=128, lens=list(range(0, 34, 2)) + [100], prefix=1000),
+    dict(hq=8, hkv=2, hd=64, lens=[i % 7 for i in range(33)], prefix=77, norm=False, inter=True),
+    dict(hq=13, hkv=1, hd=64, lens=[1, 0, 5, 9, 40], prefix=5, cap=20.0),
+    dict(hq=8, hkv=1, hd=256, lens=[0, 3, 64, 10, 7, 9, 200, 1, 5], prefix=523, inter=True, cap=30.0),
+    dict(hq=8, hkv=1, hd=128, lens=[0, 10, 40, 200, 33, 7, 8, 9, 100], prefix=300, window=150),
+    dict(hq=15, hkv=5, hd=96, lens=[2] * 12, prefix=200, bf16=True),
+    # fifteen heads a kv head, and sixteen: the new key takes the sixteenth column
+    dict(hq=15, hkv=1, hd=64, lens=[40, 0, 3], prefix=90),
+    dict(hq=16, hkv=1, hd=72, lens=[40, 0], prefix=31, inter=True),
     # more heads a kv head than one tile
     dict(hq=34, hkv=2, hd=64, lens=[40, 0, 3], prefix=90),
     dict(hq=20, hkv=1, hd=256, lens=[10, 50], prefix=33, norm=False, inter=True),
@@ -273,9 +283,10 @@ def test_shared_stale_and_foreign_rows(sa, ctx):
     assert torch.equal(out[[0, 2]], clean[[0, 2]]) and not torch.isfinite(out[1]).any()
 
 
-def test_shared_window_keeps_rows_apart(sa, ctx):
+@pytest.mark.parametrize("heads", [(4, 2, 64), (28, 2, 64), (12, 3, 96)])
+def test_shared_window_keeps_rows_apart(sa, ctx, heads):
     """a value that is not finite, in a prefix row that one sequence's window has left and another's has not"""
-    s = Shared(sa, ctx, 4, 2, 64, [0, 30, 60], 200, window=100)
+    s = Shared(sa, ctx, *heads, [0, 30, 60], 200, window=100)
     clean = s.call().clone()
     # rows seen: from 101, 131 and 161 on
     s.pre.v[s.p_slot, :, 140] = float("nan")
