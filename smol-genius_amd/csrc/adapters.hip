@@ -80,6 +80,8 @@ struct AdParams {
     };
 };
 
+static_assert(sizeof(AdParams) <= 4096, "kernel arguments");
+
 struct AdAt {
     int adapter, n, rank;
     float scale;

@@ -1917,7 +1917,10 @@ static int check_slots(const smol_kv_cache *kv, int n_seq, const int *slots, con
  * (pk, pvt, pcap, p_len) and what the call's options set are filled in. */
 static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int layer, const std::vector<ShSeq> &seqs,
                       int max_len) {
-    const int hd = kv->hd, Hkv = kv->n_kv, n = (int)seqs.size(), G = sp.Hq / Hkv, rows = n * G;
+    static_assert(sizeof(ShParams) <= 4096 && sizeof(EvictParams) <= 4096, "kernel arguments");
+    const int hd = kv->hd, Hkv = kv->n_kv, n = (int)seqs.size(), G = sp.Hq / Hkv;
+    if ((long long)n * sp.Hq > INT_MAX / 4) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d sequences of %d heads", n, sp.Hq);
+    const int rows = n * G;
     sp.kc = kv->k + (size_t)layer * kv_layer_elems(kv);
     sp.vtc = kv->vt + (size_t)layer * kv_layer_elems(kv);
     sp.c_slot_stride = (long long)kv_slot_elems(kv);
@@ -2092,6 +2095,9 @@ extern "C" int smol_attn_decode_scored(smol_attn_ctx *ctx, smol_kv_cache *kv, in
     if (((uintptr_t)mass | (uintptr_t)row_pos) & 3) return fail(SMOL_ATTN_ERR_ARG, "mass/row_pos must be 4-byte aligned");
     if (!(decay >= 0.0f) || decay > FLT_MAX) return fail(SMOL_ATTN_ERR_ARG, "decay %g", (double)decay);
     if (max_len >= stride) return fail(SMOL_ATTN_ERR_ARG, "row %d in mass rows of %d", max_len, stride);
+    const size_t bytes = (size_t)kv->n_slots * kv->n_kv * stride * 4;
+    if ((const char *)mass < (const char *)row_pos + bytes && (const char *)row_pos < (const char *)mass + bytes)
+        return fail(SMOL_ATTN_ERR_ARG, "mass and row_pos overlap");
     for (int i = 0; i < n_seq; i++) {
         if (pos[i] < 0 || pos[i] > INT_MAX - 64) return fail(SMOL_ATTN_ERR_ARG, "pos %d", pos[i]);
         max_pos = std::max(max_pos, pos[i]);

@@ -297,6 +297,19 @@ def test_shared_window_keeps_rows_apart(sa, ctx, heads):
     assert not torch.isfinite(out[0]).any() and not torch.isfinite(out[1]).any()
 
 
+@pytest.mark.parametrize("hd,inter", [(64, False), (72, True), (128, False), (256, True)])
+def test_shared_weights_off_sixteen_bytes(sa, ctx, hd, inter):
+    """norm weights that begin four bytes into a buffer (their alignment is a float's)"""
+    s = Shared(sa, ctx, 4, 2, hd, [30, 0, 65], 77, inter=inter)
+    out = s.call().clone()
+    for i, w in enumerate((s.qw, s.kw)):
+        buf = torch.zeros(hd + 1, device="cuda")
+        buf[1:] = w.cuda()
+        s.dev[1][i] = buf[1:]
+        assert buf[1:].data_ptr() % 16 == 4
+    assert torch.equal(out, s.call())
+
+
 def test_shared_grows_the_cache(sa, ctx):
     s = Shared(sa, ctx, 4, 2, 64, [63, 10], 50)
     assert s.own.kv.capacity == 64
@@ -467,6 +480,8 @@ def test_scored_refusals(sa, ctx):
         with pytest.raises(sa.SmolAttnError):
             s.call(m, p)
         setattr(s, field, keep)
+    with pytest.raises(sa.SmolAttnError, match="overlap"):
+        s.call(m, m.view(torch.int32))
     assert torch.equal(good, s.call(m, p))
 
 
