@@ -44,7 +44,11 @@ namespace {
 constexpr int AD_MAX_RANK = 128;
 constexpr int AD_TPB = 256, AD_NW = AD_TPB / 64;
 constexpr int AD_ARG_TILES = 40, AD_ARG_RUNS = 400;
-constexpr int AD_FEW = 64; /* rows that k_adapt_few takes */
+/* Rows that k_adapt_few takes. It keeps fp32 x at 24 bits and is two launches instead of three or four; against the library's
+ * product and k_adapt_out (kernel time, fp32 x, rank 16): 1024 -> 4096 16 rows 10.6 us against 14.2, 32 rows 12.2 against 14.6,
+ * 64 rows 15.5 against 16.2; 2048 -> 1024, where its workgroups are few, 64 rows 19.4 against 15.8. It re-reads x for every 16
+ * outputs, so it only loses more beyond. */
+constexpr int AD_FEW = 64;
 constexpr int AD_TIMING_KIND = 2;
 
 struct AdTile {
@@ -240,13 +244,19 @@ __device__ __forceinline__ void ad_t(const AdParams &p, long long row, int rank,
     }
 }
 
-/* Up to 16 RT rows against 16 outputs a workgroup. Its eight waves share in_dim out by runs of US 32-wide steps (whole cache lines of
+/* Up to 16 RT rows against 16 outputs a workgroup. Its waves share in_dim out by runs of US 32-wide steps (whole cache lines of
  * W's rows), a run in flight; the sums of every wave are added in LDS in wave order, the adapters' tiles (one wave each) add their
  * part, and each output is written once. */
-constexpr int FEW_NW = 8;
+template <int RT, bool XBF>
+struct Few {
+    /* sixteen waves, eight where their sums fill more LDS than their loads gain (1024 -> 4096, fp32 x: 16 rows 6.3 us against 7.0
+     * with eight, 32 rows 7.5 against 8.2, 64 rows 11.9 against 10.9; bf16 x: 64 rows 7.3 against 8.2) */
+    static constexpr int NW = RT == 4 && !XBF ? 8 : 16;
+    static constexpr int US = RT == 1 || (RT == 2 && XBF) ? 4 : 2;
+};
 template <int RT, bool XBF, int KS>
-__global__ __launch_bounds__(64 * FEW_NW) void k_adapt_few(const AdParams p) {
-    constexpr int PARTS = XBF ? 1 : 3, US = RT <= 2 ? 4 : 2, STR = 20;
+__global__ __launch_bounds__((64 * Few<RT, XBF>::NW)) void k_adapt_few(const AdParams p) {
+    constexpr int FEW_NW = Few<RT, XBF>::NW, PARTS = XBF ? 1 : 3, US = Few<RT, XBF>::US, STR = 20;
     __shared__ __attribute__((aligned(16))) float s_y[(FEW_NW + 1) * RT * 16 * STR];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -268,6 +278,10 @@ __global__ __launch_bounds__(64 * FEW_NW) void k_adapt_few(const AdParams p) {
         }
         return v;
     };
+    /* columns past the last row take the last row's x: results that no one reads, without reading their padding */
+    int xo[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) xo[t] = (16 * j + max(0, min(c, p.seq - 1 - 16 * t))) * 8;
     const int tiles_x = (p.seq + 15) / 16;
     for (int s0 = wave * US; s0 < steps; s0 += FEW_NW * US) {
         uint4 wv[US];
@@ -282,7 +296,7 @@ __global__ __launch_bounds__(64 * FEW_NW) void k_adapt_few(const AdParams p) {
                 for (int q = 0; q < PARTS; q++)
                     xf[u][t][q] = as_b8(s < steps && t < tiles_x
                                             ? *reinterpret_cast<const uint4 *>(
-                                                  p.xs + ((((long long)t * steps + s) * PARTS + q) * 64 + lane) * 8)
+                                                  p.xs + (((long long)t * steps + s) * PARTS + q) * 512 + xo[t])
                                             : make_uint4(0, 0, 0, 0));
         }
 #pragma unroll
@@ -513,7 +527,7 @@ extern "C" int smol_adapters_create(smol_attn_ctx *ctx, int n, int in_dim, int o
 
 template <int RT, bool XBF>
 static void launch_few(const AdParams &p, int ks, hipStream_t st) {
-    const dim3 g((unsigned)((p.out_dim + 15) / 16)), b(64 * FEW_NW);
+    const dim3 g((unsigned)((p.out_dim + 15) / 16)), b(64 * Few<RT, XBF>::NW);
     switch (ks) {
     case 1: hipLaunchKernelGGL((k_adapt_few<RT, XBF, 1>), g, b, 0, st, p); break;
     case 2: hipLaunchKernelGGL((k_adapt_few<RT, XBF, 2>), g, b, 0, st, p); break;
@@ -594,8 +608,10 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
     p.scale = set->scale;
     p.rank = set->rank;
     p.n_tiles = n_tiles;
-    /* a step a wave at least; more than a quarter of the device's compute units gains less than the further partial sums
-     * cost the reader (17 tiles of 1024: 8 chunks 16.0 us a call, 3 chunks 14.3) */
+    /* A step a wave at least. Few tiles: workgroups for a quarter of the compute units, since every chunk is another partial
+     * sum for each of the readers (64 rows of 2048 and 1024: a quarter, half, all of them 19.4, 20.2, 22.6 and 15.5, 16.4,
+     * 16.4 us in both kernels). Many tiles (more rows than k_adapt_few takes) have few readers a row: all compute units
+     * (1536 rows: k_adapt_in 4.8 us, a quarter of them 6.1). */
     const int steps = set->kp / 32, cus = smol_internal_ctx_cus(ctx);
     const int chunks = std::max(1, std::min({n_tiles > 32 ? cus / n_tiles : cus / 4 / n_tiles, (steps + AD_NW - 1) / AD_NW, 16}));
     p.chunk = (steps + chunks - 1) / chunks;

@@ -1948,10 +1948,13 @@ static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int l
     sp.n_rb = (rows + tile - 1) / tile;
     sp.s_rb = (G + smol_shared_own_rows() - 1) / smol_shared_own_rows();
     /* Chunks of equal length, a slab a wave at least, as short as leaves a
-     * prefix item for three compute units of four at most, and own-rows items
-     * that fit beside them (with room for the XCDs' uneven shares). A workgroup spends 5 to 8 us besides its slabs, so more of them
-     * cost more than they spread (head_dim 128, 16 sequences on 4096: 8, 16, 32
-     * slabs a chunk 22 / 20 / 24 us a call; 64 on 16384: 16, 32, 64 77 / 66 / 73). */
+     * prefix item for three compute units of four at most - for all of them if
+     * the own rows are little work - and own-rows items that fit beside them
+     * (with room for the XCDs' uneven shares). A workgroup spends 5 to 8 us
+     * besides its slabs, so more of them cost more than they spread (head_dim
+     * 128, 16 sequences on 4096: 8, 16, 32 slabs a chunk 22 / 20 / 24 us a
+     * call; 64 on 16384: 16, 32, 64 77 / 66 / 73; without own rows there 16,
+     * 32, 48 44 / 38 / 45). */
     const long long slots = (long long)ctx->cu_count * smol_shared_occupancy(hd);
     auto chunk = [&](int longest, long long limit, auto workgroups) {
         const int least = std::max(4, (longest + SH_MAX_SPLIT - 1) / SH_MAX_SPLIT), forced = ctx->opt[SMOL_OPT_DEC_SLABS];
@@ -1961,7 +1964,8 @@ static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int l
         return (int)c;
     };
     auto p_items = [&](long long c) { return (long long)Hkv * sp.n_rb * ((p_slabs + c - 1) / c); };
-    const int cp = chunk(p_slabs, ctx->cu_count * 3 / 4, p_items);
+    const long long own_work = std::accumulate(own_slabs.begin(), own_slabs.end(), 0LL) * sp.s_rb;
+    const int cp = chunk(p_slabs, 4 * own_work <= (long long)p_slabs * sp.n_rb ? ctx->cu_count : ctx->cu_count * 3 / 4, p_items);
     const int cs = chunk(own_max, p_slabs ? (slots - p_items(cp)) * 3 / 4 : slots, [&](long long c) {
         long long w = 0;
         for (int k : own_slabs) w += std::max(1LL, (k + c - 1) / c);

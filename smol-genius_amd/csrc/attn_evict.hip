@@ -31,7 +31,11 @@ namespace {
 
 constexpr int EV_BINS = 2048;
 constexpr int EV_MOVES = 32;  /* moves of a k_evict_move workgroup */
-constexpr int EV_FUSED = 256; /* moves that k_evict_select makes itself */
+constexpr int EV_TPB = 1024;  /* threads of k_evict_select (256: 11.5 us for 300 rows cut to 256, 1024: 10) */
+/* Moves that k_evict_select makes itself, which saves a launch (2.4 us) and a start-up: head_dim 128, 16 sequences of 8 kv heads,
+ * 32 moves 19.3 us against 28.7 in two kernels, 128 moves 38.6 against 43.2, 256 moves 56.2 against 55.2; one sequence, 128 moves
+ * 21.3 against 20.6, 256 moves 30.2 against 22.2. */
+constexpr int EV_FUSED = 128;
 
 __device__ __forceinline__ ShSeq ev_seq(const EvictParams &p, int i) {
     const int4 s = reinterpret_cast<const int4 *>(p.seqs_dev ? p.seqs_dev : p.seqs)[i];
@@ -132,8 +136,9 @@ __device__ __forceinline__ void ev_move(const EvictParams &p, const ShSeq &sq, i
 } // namespace
 
 /* ROWS: the longest sequence whose ranks stay in LDS; 0: any, its ranks formed again at each reading */
-template <int ROWS, int TPB>
-__global__ __launch_bounds__(TPB) void k_evict_select(const EvictParams p) {
+template <int ROWS>
+__global__ __launch_bounds__(EV_TPB) void k_evict_select(const EvictParams p) {
+    constexpr int TPB = EV_TPB;
     constexpr bool LDS = ROWS > 0;
     constexpr int NW = TPB / 64, NB = EV_BINS / TPB, U = 8;
     __shared__ unsigned s_rank[LDS ? ROWS : 1];
@@ -278,7 +283,7 @@ __global__ __launch_bounds__(TPB) void k_evict_select(const EvictParams p) {
     }
     if (!p.fused) return;
     __syncthreads();
-    ev_move<TPB, TPB == 1024 ? 64 : 32>(p, sq, g, s_hist[0], s_hist[1], s_found[0][0]);
+    ev_move<TPB, EV_MOVES>(p, sq, g, s_hist[0], s_hist[1], s_found[0][0]);
 }
 
 __global__ __launch_bounds__(256) void k_evict_move(const EvictParams p) {
@@ -302,11 +307,10 @@ extern "C" int smol_evict_fused(int max_moves) { return max_moves <= EV_FUSED; }
 extern "C" int smol_launch_evict(const EvictParams *p, int max_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1) {
     const unsigned pairs = (unsigned)p->n_seq * p->Hkv;
     const hipEvent_t e = p->fused ? e1 : nullptr;
-    /* 256 threads for up to 1024 rows: a barrier among four waves instead of sixteen */
-    if (max_rows <= 1024) hipExtLaunchKernelGGL((k_evict_select<1024, 256>), dim3(pairs), dim3(256), 0, st, e0, e, 0, *p);
-    else if (max_rows <= 8192) hipExtLaunchKernelGGL((k_evict_select<8192, 1024>), dim3(pairs), dim3(1024), 0, st, e0, e, 0, *p);
-    else if (max_rows <= 32768) hipExtLaunchKernelGGL((k_evict_select<32768, 1024>), dim3(pairs), dim3(1024), 0, st, e0, e, 0, *p);
-    else hipExtLaunchKernelGGL((k_evict_select<0, 1024>), dim3(pairs), dim3(1024), 0, st, e0, e, 0, *p);
+    const dim3 g(pairs), b(EV_TPB);
+    if (max_rows <= 8192) hipExtLaunchKernelGGL(k_evict_select<8192>, g, b, 0, st, e0, e, 0, *p);
+    else if (max_rows <= 32768) hipExtLaunchKernelGGL(k_evict_select<32768>, g, b, 0, st, e0, e, 0, *p);
+    else hipExtLaunchKernelGGL(k_evict_select<0>, g, b, 0, st, e0, e, 0, *p);
     if (hipGetLastError() != hipSuccess) return -3;
     if (p->fused) return 0;
     const unsigned blocks = pairs * (unsigned)((p->max_moves + EV_MOVES - 1) / EV_MOVES);

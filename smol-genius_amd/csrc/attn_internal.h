@@ -294,7 +294,7 @@ typedef struct {
     float qscale;              /* scale * log2 e */
     float *out; int Hq, Hkv, G;
     int window; float cap2;    /* window > 0: positions > pos - window; cap2 > 0: softcap in log2 units */
-    /* the items: n_pblocks workgroups of (prefix chunk, row block, kv head), then (chunk, sequence, kv head, 16 heads) */
+    /* the items: n_pblocks workgroups of (prefix chunk, row block, kv head), then (chunk, sequence, kv head, 15 heads) */
     int n_pblocks, n_rb, n_ps, p_chunk, n_ss, s_chunk, s_rb;
     int p_first;               /* the prefix chunks' first key (a window leaves out what lies before), a slab's start */
     float *p_o; float *p_ml;   /* [prefix chunk][kv][n_seq G] outputs [hd] and (m, l) */

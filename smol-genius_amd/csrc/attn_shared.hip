@@ -717,16 +717,28 @@ __global__ __launch_bounds__(256) void k_sh_merge(const ShParams p) {
             return k < p.n_ps ? (((long long)k * p.Hkv + g) * p.n_seq + i) * p.G + h
                               : (((long long)i * p.Hkv + g) * p.n_ss + (k - p.n_ps)) * p.G + h;
         };
+        /* the first chunks' outputs are on their way while the weights are formed */
+        constexpr int PRE = 4;
+        const int q = tid / GL, d = (tid - q * GL) * 4;
+        f4 pre[PRE];
+#pragma unroll
+        for (int u = 0; u < PRE; u++) {
+            const int k = q + u * NG;
+            pre[u] = f4{0.f, 0.f, 0.f, 0.f};
+            if (d < HD && k < n) pre[u] = *reinterpret_cast<const f4 *>((k < p.n_ps ? p.p_o : p.s_o) + row_of(k) * HD + d);
+        }
         float2 ml = make_float2(-INFINITY, 0.0f);
         if (tid < n) ml = *reinterpret_cast<const float2 *>((tid < p.n_ps ? p.p_ml : p.s_ml) + row_of(tid) * 2);
         const float M = block_max(ml.x), mu = M == -INFINITY ? 0.0f : M;
         const float w = tid < n ? __builtin_amdgcn_exp2f(ml.x - mu) : 0.0f;
         if (tid < n) s_w[tid] = w;
         const float L = block_sum(tid < n ? w * ml.y : 0.0f);
-        const int q = tid / GL, d = (tid - q * GL) * 4;
         f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < PRE; u++)
+            if (q + u * NG < n) acc += s_w[q + u * NG] * pre[u];
         if (d < HD)
-            for (int k = q; k < n; k += NG)
+            for (int k = q + PRE * NG; k < n; k += NG)
                 acc += s_w[k] * *reinterpret_cast<const f4 *>((k < p.n_ps ? p.p_o : p.s_o) + row_of(k) * HD + d);
         *reinterpret_cast<f4 *>(s_red + tid * 4) = acc;
         __syncthreads();
