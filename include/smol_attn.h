@@ -280,10 +280,10 @@ SMOL_ATTN_API int smol_attn_decode_noalloc(smol_attn_ctx *ctx, smol_kv_cache *kv
  * products are fp32 Q and fp32 probabilities, each split into three bf16 parts
  * (24 bits), with the cache's bf16 bits; everything else is fp32, and there is no
  * range limit. A cached row that holds NaN or infinity makes the outputs of the
- * sequences that see it NaN, and of no other; rows at or past a sequence's length are never used. A
- * sequence's result does not depend on what the cache holds elsewhere, but the
- * order of its sums follows the batch's shape. Slots are host arrays, each
- * slot at most once. Calls grow the cache, the table and the context's
+ * sequences that see it NaN, and of no other; rows at or past a sequence's
+ * length are never used. A sequence's result does not depend on what the cache
+ * holds elsewhere, but the order of its sums follows the batch's shape. Slots
+ * are host arrays, each slot at most once. Calls grow the cache, the table and the context's
  * workspace as needed. Under stream capture they may not grow anything and
  * take at most 128 sequences (SMOL_ATTN_ERR_UNSUPPORTED otherwise: run the
  * call once before the capture); the captured call keeps the slots, lengths

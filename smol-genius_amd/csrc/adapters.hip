@@ -20,6 +20,14 @@
  *
  * The weights of a set are packed once, at its creation: ranks padded with
  * zeros to the matrix instruction's sizes, so no load needs a bound.
+ *
+ * Measured on an MI355X: 3 rows of 1024 -> 2048, rank 8: k_adapt_in 4.2 us and
+ * k_adapt_few 5.6, two launches of little more than a launch's own time; 32
+ * rows of 1024 -> 4096, fp32, rank 16: 4.6 + 7.6 us (W's 8.4 MB; the bf16 parts
+ * of x, read again by every workgroup from L2, are 50 MB); 3 rows of 4096 ->
+ * 4096: 4.6 + 11 us (33.6 MB of W at 3.0 TB/s). 1536 rows of 1024 -> 2048,
+ * bf16, rank 32: 4.9 us, the library's product 20.5, k_adapt_out 8 us (26 MB,
+ * 3.3 TB/s).
  */
 #include "attn_device.h"
 

@@ -1,7 +1,7 @@
 /*
  * attn_shared.hip - one decode step for a batch that shares a long prefix
  * (k_sh), and the step that also adds up the weight of every cached row
- * (k_sh with SC); the rows that received little are taken out by
+ * (k_sh as SH_SCORED); the rows that received little are taken out by
  * attn_evict.hip.
  *
  * Mathematics. Sequence i has own cache rows [0, l_i), the new token (row
@@ -26,7 +26,20 @@
  *   Wide items (a prefix against more rows): the waves hold 16 rows each, 64
  *     together, and share every slab, which transfers bring into a ring in LDS
  *     in the order that its fragments are read without bank conflicts. Bound
- *     by the matrix cores: three products for one (below).
+ *     by the matrix cores and the softmax between their products, one after
+ *     the other in a wave: three products for one (below).
+ *
+ * Measured on an MI355X (kernel time, head_dim 128, 16 heads over 8):
+ * 4 sequences on 500 8.5 us and 16 on 4096 17.4 us (33 MB, 2.0 TB/s; the first
+ * load waits for the sequences' table and Q, 3 to 5 us, and a wave has one to
+ * four slabs); 64 on 16384 59 us (212 MB, 3.7 TB/s, matrix cores busy 27%;
+ * a wide item 0.85 us a slab). head_dim 256, 8 heads over 1, 24 on 8191: 26.5 us,
+ * one workgroup a compute unit, 2.6 us a wave's slab. Scored: 16 sequences of
+ * 3000 to 4160 rows 56 us (244 MB, 4.4 TB/s). k_sh_merge 4 to 7 us, a launch's
+ * and two round trips' time. Taken and left: one more launch instead of a join
+ * by the last workgroup, whose fences cost 1 us at 4 sequences and 24 us at 64;
+ * scores of the next slab beside the softmax of this one, 53 us against 45
+ * for 64 on 16384 without own rows.
  *
  * Every lane loads, normalises and rotates exactly the elements of Q that its
  * fragments hold (row c, dims 32 ks + 8 j ..), so the prologue is one round of
@@ -534,9 +547,10 @@ __device__ __forceinline__ void sh_narrow(const ShParams &p, const ShItem &it, c
 }
 
 /* 64 rows of the batch, 16 a wave, against slabs that all waves share through LDS. The ring's 16-byte pieces are placed
- * so that the eight lanes that LDS serves together (rows c .. c + 7 of one j) fall in different columns of its 128-byte
- * lines: piece q of K row r at q ^ ((r & 3) | (r >> 3 & 1) << 2), piece j of V^T row d at j ^ (d >> 1 & 3). A transfer
- * writes its lanes' pieces one after the other, so it is the lanes' source addresses that are permuted. */
+ * so that the sixteen lanes that LDS serves together (c 0..3 and 12..15 of one j, c 4..11 of the next) fall in different
+ * columns of its 256-byte lines: piece q of K row r at q ^ c(r) with the lane c that reads the row (c / 2 at head_dim 64,
+ * whose lines hold two rows), piece j of V^T row d at j ^ (d >> 1 & 3); the conflict counter reads 0. A transfer writes its
+ * lanes' pieces one after the other, so it is the lanes' source addresses that are permuted. */
 template <int HD>
 __device__ __forceinline__ void sh_wide(const ShParams &p, const ShItem &it, char *smem) {
     using Gm = ShGeom<HD>;
@@ -554,7 +568,7 @@ __device__ __forceinline__ void sh_wide(const ShParams &p, const ShItem &it, cha
         const int t = wave * ND + u, piece = t % PART * 64 + lane;
         if (t < PART) {
             const int r = piece / PC, q = piece % PC;
-            voff[u] = (unsigned)((r * PC + (q ^ ((r & 3) | (r >> 3 & 1) << 2))) * 16);
+            voff[u] = (unsigned)((r * PC + (q ^ (HD == 128 ? (r & 3) | (r >> 3 & 3) << 2 : (r >> 1 & 1) | (r >> 3 & 3) << 1))) * 16);
         } else {
             const int d = piece / 4, q = piece % 4;
             voff[u] = (unsigned)((d * 4 + (q ^ (d >> 1 & 3))) * 16);
@@ -579,7 +593,7 @@ __device__ __forceinline__ void sh_wide(const ShParams &p, const ShItem &it, cha
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
     for (int i = 0; i < STAGES - 1; i++) fetch(i);
-    const int kt_row = 8 * (c >> 2) + (c & 3), ksw = (c & 3) | (c >> 2 & 1) << 2;
+    const int kt_row = 8 * (c >> 2) + (c & 3), ksw = HD == 128 ? c : c >> 1;
     const int n_steps = (n + WS - 1) / WS;
     for (int i = 0; i < n_steps; i++) {
         /* this wave's part of step i has landed (later ones may be on their way); then everybody's has, and nobody
