@@ -288,7 +288,10 @@ SMOL_ATTN_API int smol_attn_decode_noalloc(smol_attn_ctx *ctx, smol_kv_cache *kv
  * take at most 128 sequences (SMOL_ATTN_ERR_UNSUPPORTED otherwise: run the
  * call once before the capture); the captured call keeps the slots, lengths
  * and positions that it was made with, and it uses the context's workspace, so
- * its replays are ordered with the context's other calls by the caller. */
+ * its replays are ordered with the context's other calls by the caller. It also
+ * keeps the addresses of the cache and the table: reserve both beforehand, for
+ * growth after the capture leaves the graph with freed memory. Calls grow a
+ * table to 4194304 positions at most (SMOL_ATTN_ERR_UNSUPPORTED past that). */
 
 /* One decode step of n_seq sequences that all continue the same prefix:
  * positions [0, prefix_len) are the rows of (layer, prefix_slot) of the cache

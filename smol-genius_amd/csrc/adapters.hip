@@ -567,6 +567,8 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
         return afail(SMOL_ATTN_ERR_UNSUPPORTED, "smol_linear_adapters_dev: sizes beyond the supported range");
     if ((const char *)x < (const char *)y + (size_t)seq * out_dim * ys && (const char *)y < (const char *)x + (size_t)seq * in_dim * xs)
         return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: y overlaps x");
+    if ((const char *)w < (const char *)y + (size_t)seq * out_dim * ys && (const char *)y < (const char *)w + (size_t)out_dim * in_dim * 2)
+        return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: y overlaps W");
     /* the rows by adapter, tiles of at most 16 */
     std::vector<int> count(set->n, 0);
     int bare = 0;

@@ -50,8 +50,8 @@ extern "C" int smol_win_max_keys(int hd, int in_dtype, int precise);
 extern "C" int smol_shared_tile_rows(int hd, int rows);
 extern "C" int smol_shared_own_rows(void);
 extern "C" int smol_shared_occupancy(int hd);
-extern "C" int smol_launch_shared(const ShParams *p, int hd, int tile_rows, int max_len, hipStream_t st, hipEvent_t e0,
-                                  hipEvent_t e1);
+extern "C" int smol_shared_mass_chunks(long long pairs, int max_len);
+extern "C" int smol_launch_shared(const ShParams *p, int hd, int tile_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
 extern "C" int smol_evict_fused(int max_moves);
 extern "C" int smol_launch_evict(const EvictParams *p, int max_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
 extern "C" int smol_launch_to_bf16_trunc(const float *x, uint16_t *y, long long n, hipStream_t st);
@@ -1884,16 +1884,25 @@ extern "C" int smol_internal_upload(smol_attn_ctx *ctx, const void *host, size_t
     return 0;
 }
 
-/* cache growth and the table's, refused under capture */
+/* cache growth and the table's, refused under capture, where a head's rows
+ * would pass what 31 bits address, and where a table (built on the host) would
+ * take gigabytes */
+constexpr int ROPE_GROW_MAX = 1 << 22;
 static int reserve_step(smol_attn_ctx *ctx, smol_kv_cache *kv, int rows, const smol_rope_table *rope, int hd, int positions) {
     int rc;
+    long long grown = kv->cap;
+    while (grown < rows) grown *= 2;
+    if (grown * hd * 2 > 0x7FFF0000LL) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d rows of head_dim %d a slot", rows, hd);
+    if (rope && positions > std::max(rope->cap, ROPE_GROW_MAX))
+        return fail(SMOL_ATTN_ERR_UNSUPPORTED, "position %d past the RoPE table's %d (tables grow to %d)", positions - 1,
+                    rope->cap, ROPE_GROW_MAX);
     if ((rc = check_capture(ctx, "cache growth", rows > kv->cap))) return rc;
     if ((rc = check_capture(ctx, "RoPE table growth", rope && positions > rope->cap))) return rc;
     if ((rc = smol_kv_cache_reserve(kv, rows))) return rc;
     return check_rope(ctx, rope, hd, positions);
 }
 
-/* one head's rows of a slot are addressed with 31 bits */
+/* one head's rows of a slot are addressed with 31 bits (a cache may have been created with more) */
 static int check_region(const smol_kv_cache *kv) {
     return (long long)kv->cap * kv->hd * 2 <= 0x7FFF0000LL
                ? 0 : fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d rows of head_dim %d a slot", kv->cap, kv->hd);
@@ -1915,7 +1924,7 @@ static int check_slots(const smol_kv_cache *kv, int n_seq, const int *slots, con
 
 /* Plans and launches k_sh and k_sh_merge. sp: the sequences, the prefix
  * (pk, pvt, pcap, p_len) and what the call's options set are filled in. */
-static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int layer, const std::vector<ShSeq> &seqs,
+static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int layer, std::vector<ShSeq> &seqs,
                       int max_len) {
     static_assert(sizeof(ShParams) <= 4096 && sizeof(EvictParams) <= 4096, "kernel arguments");
     const int hd = kv->hd, Hkv = kv->n_kv, n = (int)seqs.size(), G = sp.Hq / Hkv;
@@ -1966,7 +1975,13 @@ static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int l
     auto p_items = [&](long long c) { return (long long)Hkv * sp.n_rb * ((p_slabs + c - 1) / c); };
     const long long own_work = std::accumulate(own_slabs.begin(), own_slabs.end(), 0LL) * sp.s_rb;
     const int cp = chunk(p_slabs, 4 * own_work <= (long long)p_slabs * sp.n_rb ? ctx->cu_count : ctx->cu_count * 3 / 4, p_items);
-    const int cs = chunk(own_max, p_slabs ? (slots - p_items(cp)) * 3 / 4 : slots, [&](long long c) {
+    /* More sequences than that are an item each at least: a quarter more than those beside a prefix, twice as many
+     * without one, so that a long sequence among short ones is not one item (100 rows in 99 sequences, 16000 in one:
+     * 51 us a call, 218 as one item; 64 on 2000, 8000 own rows in one, 50 in the others: 31 and 110; 100 sequences of 50 to
+     * 6400 rows, no prefix: a quarter, half, all of them more 163 / 147 / 139; 128 of up to 1023 on 2000: 65 / 68 / 72). */
+    const long long own_least = (long long)n * Hkv * sp.s_rb;
+    const long long own_limit = p_slabs ? std::max((slots - p_items(cp)) * 3 / 4, own_least * 5 / 4) : std::max(slots, own_least * 2);
+    const int cs = chunk(own_max, own_limit, [&](long long c) {
         long long w = 0;
         for (int k : own_slabs) w += std::max(1LL, (k + c - 1) / c);
         return w * Hkv * sp.s_rb;
@@ -1976,8 +1991,18 @@ static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int l
     sp.n_ps = (p_slabs + cp - 1) / cp;
     sp.n_ss = std::max(1, (own_max + cs - 1) / cs);
     const long long pblocks = ((long long)Hkv * sp.n_ps + 7) / 8 * 8 * sp.n_rb;
-    const long long sblocks = (long long)sp.n_ss * n * Hkv * sp.s_rb;
-    if (pblocks + sblocks > INT_MAX / 2 || (long long)n * sp.Hq + (long long)n * Hkv * (max_len / 1024 + 1) > INT_MAX / 2)
+    /* Own chunks by number of the chunk, n_ss for each sequence, cost an empty workgroup wherever a sequence has
+     * fewer; counted through, a workgroup looks its sequence up (0.7 us): where that leaves out 1000 of them (1.1 us). */
+    long long own = 0;
+    for (int i = 0; i < n; i++) {
+        seqs[i].item0 = (int)own;
+        own += std::max(1, (own_slabs[i] + cs - 1) / cs);
+    }
+    const bool through = ((long long)sp.n_ss * n - own) * Hkv * sp.s_rb >= 1000;
+    sp.n_own = through ? (int)own : 0;
+    sp.m_chunks = smol_shared_mass_chunks((long long)n * Hkv, max_len);
+    const long long sblocks = (through ? own : (long long)sp.n_ss * n) * Hkv * sp.s_rb;
+    if (pblocks + sblocks > INT_MAX / 2 || (long long)n * sp.Hq + (long long)n * Hkv * sp.m_chunks > INT_MAX / 2)
         return fail(SMOL_ATTN_ERR_UNSUPPORTED, "decode call too large (%d sequences)", n);
     sp.n_pblocks = (int)pblocks;
 
@@ -2006,7 +2031,7 @@ static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int l
         sp.seqs_dev = (const ShSeq *)ctx->desc.p;
     }
     const int mk = timing_begin(ctx, 1);
-    rc = smol_launch_shared(&sp, hd, tile, max_len, ctx->stream, mark_a(ctx, mk), mark_b(ctx, mk));
+    rc = smol_launch_shared(&sp, hd, tile, ctx->stream, mark_a(ctx, mk), mark_b(ctx, mk));
     if (rc)
         return fail(rc == -1 ? SMOL_ATTN_ERR_UNSUPPORTED : SMOL_ATTN_ERR_DEVICE, "k_sh launch (hd %d): %s", hd,
                     rc == -1 ? "unsupported configuration" : hipGetErrorString(hipGetLastError()));

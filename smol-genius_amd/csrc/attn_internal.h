@@ -282,7 +282,7 @@ typedef struct {
     int slot;      /* cache slot of the sequence's own rows */
     int len;       /* own rows in the cache: the new token becomes row len */
     int pos;       /* position of the new token (RoPE row, window) */
-    int pad;
+    int item0;     /* k_sh: own chunks of the sequences before it */
 } ShSeq;
 
 typedef struct {
@@ -296,6 +296,8 @@ typedef struct {
     int window; float cap2;    /* window > 0: positions > pos - window; cap2 > 0: softcap in log2 units */
     /* the items: n_pblocks workgroups of (prefix chunk, row block, kv head), then (chunk, sequence, kv head, 15 heads) */
     int n_pblocks, n_rb, n_ps, p_chunk, n_ss, s_chunk, s_rb;
+    int n_own;                 /* own chunks of all sequences, one after the other; 0: n_ss of each, by chunk, some of them empty */
+    int m_chunks;              /* workgroups of a (sequence, kv head) that add its weights up */
     int p_first;               /* the prefix chunks' first key (a window leaves out what lies before), a slab's start */
     float *p_o; float *p_ml;   /* [prefix chunk][kv][n_seq G] outputs [hd] and (m, l) */
     float *s_o; float *s_ml;   /* [sequence][kv][own chunk][G] */

@@ -55,9 +55,12 @@
  */
 #include "attn_device.h"
 
+#include <algorithm>
+
 namespace {
 
 constexpr int SH_NW = 4, SH_TPB = 64 * SH_NW;
+constexpr int MASS_KEYS = 1024; /* rows whose weights a k_sh_merge workgroup adds up at a time */
 constexpr int Q_PARTS = 3, P_PARTS = 3;
 
 template <int HD>
@@ -116,6 +119,16 @@ __device__ __forceinline__ unsigned not_finite8(uint4 v) {
 __device__ __forceinline__ ShSeq sh_seq(const ShParams &p, int i) {
     const int4 s = reinterpret_cast<const int4 *>(p.seqs_dev ? p.seqs_dev : p.seqs)[i];
     return ShSeq{s.x, s.y, s.z, s.w};
+}
+/* the sequence that own chunk u belongs to, when they are counted through: every wave compares 64 starts at a time */
+__device__ __forceinline__ int sh_seq_of(const ShParams &p, int u) {
+    const ShSeq *q = p.seqs_dev ? p.seqs_dev : p.seqs;
+    int n = 0;
+    for (int b = 0; b < p.n_seq; b += 64) {
+        const int i = b + (threadIdx.x & 63);
+        n += __popcll(__ballot(i < p.n_seq && q[min(i, p.n_seq - 1)].item0 <= u));
+    }
+    return __builtin_amdgcn_readfirstlane(n - 1);
 }
 
 /* the first of a sequence's own rows that its window leaves, down to a slab */
@@ -676,9 +689,10 @@ __global__ __launch_bounds__(SH_TPB, HD <= 128 ? 2 : 1) void k_sh(const ShParams
         }
     }
     const int a = b - p.n_pblocks;
-    const int srb = a % p.s_rb, g = (a / p.s_rb) % p.Hkv, i = (a / (p.s_rb * p.Hkv)) % p.n_seq;
-    const int sp = a / (p.s_rb * p.Hkv * p.n_seq);
+    const int srb = a % p.s_rb, g = (a / p.s_rb) % p.Hkv, u = a / (p.s_rb * p.Hkv);
+    const int i = p.n_own ? sh_seq_of(p, u) : u % p.n_seq;
     const ShSeq sq = sh_seq(p, i);
+    const int sp = p.n_own ? u - sq.item0 : u / p.n_seq;
     if (sp >= sh_own_chunks(p, sq)) return;
     it.prefix = false;
     it.g = g;
@@ -700,10 +714,9 @@ __global__ __launch_bounds__(SH_TPB, HD <= 128 ? 2 : 1) void k_sh(const ShParams
 
 /* Joins the chunks of the output rows, one workgroup a row (a sequence's
  * head): (m, l) of every chunk first, then the outputs, as many chunks at a
- * time as there are lanes for. With mass (k_sh's SC): the workgroups behind
+ * time as there are lanes for. With mass (SH_SCORED): the workgroups behind
  * those add the weights exp2(s - m) / l of MASS_KEYS cached rows of a
  * (sequence, kv head), from the scores that k_sh left, in the heads' order. */
-constexpr int MASS_KEYS = 1024;
 
 template <int HD>
 __global__ __launch_bounds__(256) void k_sh_merge(const ShParams p) {
@@ -764,60 +777,61 @@ __global__ __launch_bounds__(256) void k_sh_merge(const ShParams p) {
         }
         return;
     }
-    const int a = blockIdx.x - n_out, pair = a % (p.n_seq * p.Hkv), chunk = a / (p.n_seq * p.Hkv);
+    const int a = blockIdx.x - n_out, pair = a % (p.n_seq * p.Hkv);
     const int i = pair / p.Hkv, g = pair - i * p.Hkv;
     const ShSeq sq = sh_seq(p, i);
-    if (chunk * MASS_KEYS > sq.len) return;
     const int ns = sh_own_chunks(p, sq);
     constexpr int KU = MASS_KEYS / 256;
-    float acc[KU] = {};
     const int lane = tid & 63;
     const float *ml0 = p.s_ml + ((((long long)i * p.Hkv + g) * p.n_ss) * p.G) * 2;
-    for (int h = 0; h < p.G; h++) {
-        const long long row = (long long)i * p.Hq + g * p.G + h;
-        float x[KU];
+    for (long long k0 = (long long)(a / (p.n_seq * p.Hkv)) * MASS_KEYS; k0 <= sq.len; k0 += (long long)p.m_chunks * MASS_KEYS) {
+        float acc[KU] = {};
+        for (int h = 0; h < p.G; h++) {
+            const long long row = (long long)i * p.Hq + g * p.G + h;
+            float x[KU];
+#pragma unroll
+            for (int u = 0; u < KU; u++) {
+                const long long key = k0 + u * 256 + tid;
+                x[u] = key < sq.len ? p.logits[row * p.l_stride + key] : key == sq.len ? p.logit_new[row] : 0.0f;
+            }
+            /* every wave finds (m, l) by itself: the same order, so the same bits in each */
+            const float2 ml = lane < ns ? *reinterpret_cast<const float2 *>(ml0 + ((long long)lane * p.G + h) * 2)
+                                        : make_float2(-INFINITY, 0.0f);
+            float M = ml.x;
+#pragma unroll
+            for (int sh = 1; sh < 64; sh <<= 1) M = fmaxf(M, __shfl_xor(M, sh));
+            const float mu = M == -INFINITY ? 0.0f : M;
+            float Ls = lane < ns ? __builtin_amdgcn_exp2f(ml.x - mu) * ml.y : 0.0f;
+#pragma unroll
+            for (int sh = 1; sh < 64; sh <<= 1) Ls += __shfl_xor(Ls, sh);
+            const float rl = 1.0f / Ls;
+#pragma unroll
+            for (int u = 0; u < KU; u++) acc[u] = fmaf(__builtin_amdgcn_exp2f(x[u] - mu), rl, acc[u]);
+        }
+        float *mass = p.mass + ((long long)sq.slot * p.Hkv + g) * p.m_stride;
 #pragma unroll
         for (int u = 0; u < KU; u++) {
-            const int key = chunk * MASS_KEYS + u * 256 + tid;
-            x[u] = key < sq.len ? p.logits[row * p.l_stride + key] : key == sq.len ? p.logit_new[row] : 0.0f;
-        }
-        /* every wave finds (m, l) by itself: the same order, so the same bits in each */
-        const float2 ml = lane < ns ? *reinterpret_cast<const float2 *>(ml0 + ((long long)lane * p.G + h) * 2)
-                                    : make_float2(-INFINITY, 0.0f);
-        float M = ml.x;
-#pragma unroll
-        for (int sh = 1; sh < 64; sh <<= 1) M = fmaxf(M, __shfl_xor(M, sh));
-        const float mu = M == -INFINITY ? 0.0f : M;
-        float Ls = lane < ns ? __builtin_amdgcn_exp2f(ml.x - mu) * ml.y : 0.0f;
-#pragma unroll
-        for (int sh = 1; sh < 64; sh <<= 1) Ls += __shfl_xor(Ls, sh);
-        const float rl = 1.0f / Ls;
-#pragma unroll
-        for (int u = 0; u < KU; u++) acc[u] = fmaf(__builtin_amdgcn_exp2f(x[u] - mu), rl, acc[u]);
-    }
-    float *mass = p.mass + ((long long)sq.slot * p.Hkv + g) * p.m_stride;
-#pragma unroll
-    for (int u = 0; u < MASS_KEYS / 256; u++) {
-        const int key = chunk * MASS_KEYS + u * 256 + tid;
-        if (key < sq.len) {
-            mass[key] = p.decay == 0.0f ? acc[u] : fmaf(mass[key], p.decay, acc[u]);
-        } else if (key == sq.len) {
-            mass[key] = acc[u];
-            p.row_pos[((long long)sq.slot * p.Hkv + g) * p.m_stride + key] = sq.pos;
+            const long long key = k0 + u * 256 + tid;
+            if (key < sq.len) {
+                mass[key] = p.decay == 0.0f ? acc[u] : fmaf(mass[key], p.decay, acc[u]);
+            } else if (key == sq.len) {
+                mass[key] = acc[u];
+                p.row_pos[((long long)sq.slot * p.Hkv + g) * p.m_stride + key] = sq.pos;
+            }
         }
     }
 }
 
 template <int HD>
-static int launch_hd(const ShParams *p, int tile_rows, int max_len, hipStream_t st, hipEvent_t e0, hipEvent_t e1) {
-    const unsigned blocks = (unsigned)p->n_pblocks + (unsigned)p->n_ss * p->n_seq * p->Hkv * p->s_rb;
+static int launch_hd(const ShParams *p, int tile_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1) {
+    const unsigned blocks = (unsigned)p->n_pblocks + (unsigned)(p->n_own ? p->n_own : p->n_ss * p->n_seq) * p->Hkv * p->s_rb;
     if (p->mass) hipExtLaunchKernelGGL((k_sh<HD, SH_SCORED>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
     else if (tile_rows == 16) hipExtLaunchKernelGGL((k_sh<HD, SH_NARROW>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
     else if constexpr (ShGeom<HD>::WIDE) hipExtLaunchKernelGGL((k_sh<HD, SH_WIDE>), dim3(blocks), dim3(SH_TPB), 0, st, e0, nullptr, 0, *p);
     else return -1;
     if (hipGetLastError() != hipSuccess) return -3;
     unsigned mb = (unsigned)p->n_seq * p->Hq;
-    if (p->mass) mb += (unsigned)p->n_seq * p->Hkv * (max_len / MASS_KEYS + 1);
+    if (p->mass) mb += (unsigned)p->n_seq * p->Hkv * p->m_chunks;
     hipExtLaunchKernelGGL((k_sh_merge<HD>), dim3(mb), dim3(256), 0, st, nullptr, e1, 0, *p);
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }
@@ -831,18 +845,23 @@ extern "C" int smol_shared_tile_rows(int hd, int rows) { return rows <= 32 || (h
 /* heads of an own-rows item */
 extern "C" int smol_shared_own_rows(void) { return OWN_ROWS; }
 
+/* workgroups for the weights of one (sequence, kv head), of `pairs`: one for every MASS_KEYS rows of the longest, but no
+ * more than 4096 in all or one each, for most are empty where one sequence is long (1000 empty ones cost 1.1 us) */
+extern "C" int smol_shared_mass_chunks(long long pairs, int max_len) {
+    return (int)std::min<long long>(max_len / MASS_KEYS + 1, std::max(1LL, 4096 / pairs));
+}
+
 /* workgroups of a compute unit at once (k_sh's launch bounds) */
 extern "C" int smol_shared_occupancy(int hd) { return hd <= 128 ? 2 : 1; }
 
-extern "C" int smol_launch_shared(const ShParams *p, int hd, int tile_rows, int max_len, hipStream_t st, hipEvent_t e0,
-                                  hipEvent_t e1) {
+extern "C" int smol_launch_shared(const ShParams *p, int hd, int tile_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1) {
     switch (hd) {
-    case 64: return launch_hd<64>(p, tile_rows, max_len, st, e0, e1);
-    case 72: return launch_hd<72>(p, tile_rows, max_len, st, e0, e1);
-    case 80: return launch_hd<80>(p, tile_rows, max_len, st, e0, e1);
-    case 96: return launch_hd<96>(p, tile_rows, max_len, st, e0, e1);
-    case 128: return launch_hd<128>(p, tile_rows, max_len, st, e0, e1);
-    case 256: return launch_hd<256>(p, tile_rows, max_len, st, e0, e1);
+    case 64: return launch_hd<64>(p, tile_rows, st, e0, e1);
+    case 72: return launch_hd<72>(p, tile_rows, st, e0, e1);
+    case 80: return launch_hd<80>(p, tile_rows, st, e0, e1);
+    case 96: return launch_hd<96>(p, tile_rows, st, e0, e1);
+    case 128: return launch_hd<128>(p, tile_rows, st, e0, e1);
+    case 256: return launch_hd<256>(p, tile_rows, st, e0, e1);
     default: return -1;
     }
 }

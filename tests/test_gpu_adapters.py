@@ -215,3 +215,87 @@ def test_refusals(sa, ctx):
                                             t.set.h, ids.ctypes.data_as(ctypes.POINTER(ctypes.c_int)))
     assert rc == -1
     assert torch.equal(t.call(sa, ctx), y)
+    # y over the weights
+    wy = torch.zeros(48 * 64 + 6 * 48, dtype=torch.float32, device="cuda")
+    rc = sa.load().smol_linear_adapters_dev(ctx.h, wy.data_ptr(), 0, x.data_ptr(), 0, wy.data_ptr() + 256, None, 6, 64, 48,
+                                            t.set.h, ids.ctypes.data_as(ctypes.POINTER(ctypes.c_int)))
+    assert rc == -1
+    assert torch.equal(y, t.call(sa, ctx))
+
+
+def test_captured_runs(sa):
+    """prompts one after the other: more tiles than the arguments' table holds, captured as runs"""
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        c2 = sa.Context(0)
+        t = Case(180, 64, 80, [8] * 60, ids=[s // 3 for s in range(180)])
+        out = torch.empty(180, 80, device="cuda")
+        t.call(sa, c2, out=out)
+        st.synchronize()
+        t.check(out)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st, capture_error_mode="thread_local"):
+            t.call(sa, c2, out=out)
+        for r in range(3):
+            t.dev[0].normal_()
+            g.replay()
+            st.synchronize()
+            got = out.clone()
+            t.call(sa, c2, out=out)
+            st.synchronize()
+            assert torch.equal(got, out)
+    st.synchronize()
+    del t, g
+    c2.close()
+
+
+def test_serving_steps(sa, ctx):
+    """decode steps of a batch whose requests share a prompt and have adapters of their own: the projections' outputs are the
+    attention's inputs and its output the last projection's; every stage against its 64-bit form on the inputs it got"""
+    from test_gpu_shared import attend, err, table, turned
+    n, dim, hq, hkv, hd, P = 5, 192, 8, 4, 64, 70
+    ids = [2, -1, 0, 2, 1]
+    cases = [Case(n, dim, h * hd, [8, 16, 4], ids=ids, bias=b, seed=10 + i)
+             for i, (h, b) in enumerate(((hq, True), (hkv, True), (hkv, False)))]
+    last = Case(n, hq * hd, dim, [8, 16, 4], ids=ids, bias=False, seed=20)
+    for t in cases + [last]:
+        t.to(sa, ctx)
+    pre, kv = sa.KVCache(ctx, 1, 1, hkv, hd, 128), sa.KVCache(ctx, 1, n, hkv, hd, 64)
+    kt, vt = pre.views(0)
+    torch.manual_seed(3)
+    kt.normal_()
+    vt.normal_()
+    pk, pv = kt[0].cpu().double(), vt[0].transpose(-1, -2).reshape(hkv, -1, hd).cpu().double()
+    rope = sa.RopeTable(ctx, hd, 1e4)
+    lens = [0] * n
+    own = [[] for _ in range(n)]
+    for step in range(3):
+        x = torch.randn(n, dim)
+        for t in cases:
+            t.x = x
+            t.dev = (x.cuda(),) + t.dev[1:]
+        q, k, v = (t.call(sa, ctx) for t in cases)
+        for t, y in zip(cases, (q, k, v)):
+            t.check(y)
+        att = sa.decode_shared(ctx, pre, 0, P, kv, 0, rope, list(range(n)), lens, q, k, v, hq, hd ** -0.5)
+        rows = table(sa, hd, 1e4, False, [P + l for l in lens])
+        q64 = turned(q.cpu().view(n, hq, hd), None, rows, False).view(n, hkv, hq // hkv, hd)
+        k64 = turned(k.cpu().view(n, hkv, hd), None, rows, False)
+        v64 = v.cpu().double().view(n, hkv, hd)
+        got = att.cpu().double().view(n, hkv, hq // hkv, hd)
+        for i in range(n):
+            for h in range(hkv):
+                kk = torch.cat([pk[h, :P]] + [r[0][h:h + 1] for r in own[i]] + [k64[i, h:h + 1]])
+                vv = torch.cat([pv[h, :P]] + [r[1][h:h + 1] for r in own[i]] + [v64[i, h:h + 1]])
+                o, _, w, a = attend(q64[i, h], kk, vv, hd ** -0.5, 0.0)
+                assert ((got[i, h] - o).abs() <= 2 * err(hd, a) * w + 2.0 ** -22 * o.abs()).all(), (step, i, h)
+            # the rows as the cache holds them
+            rk, rv = (torch.from_numpy(b.view(np.int16)).view(torch.bfloat16).double().view(hkv, hd)
+                      for b in kv.read(0, i, lens[i], 1))
+            own[i].append((rk, rv))
+        last.x = att.cpu()
+        last.dev = (att,) + last.dev[1:]
+        last.check(last.call(sa, ctx))
+        lens = [l + 1 for l in lens]
+    pre.close()
+    kv.close()

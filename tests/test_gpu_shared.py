@@ -244,6 +244,19 @@ def test_shared_long_prefix(sa, ctx):
     assert torch.equal(a, s.call())
 
 
+@pytest.mark.parametrize("c", [
+    dict(hq=4, hkv=2, hd=64, lens=[3] * 30 + [4000] + [i % 50 for i in range(30)], prefix=100),
+    dict(hq=8, hkv=2, hd=128, lens=[20] * 140 + [3000], prefix=64, window=700),
+    dict(hq=20, hkv=1, hd=80, lens=[2900] + [40] * 64, prefix=0),
+], ids=["61", "141-window", "65-no-prefix"])
+def test_shared_one_long_among_short(sa, ctx, c):
+    """one sequence's own rows are many chunks, the others' one each"""
+    s = Shared(sa, ctx, **c)
+    a = s.call().clone()
+    s.check(a)
+    assert torch.equal(a, s.call())
+
+
 def test_shared_equals_decode(sa, ctx):
     """the batch's step on a shared prefix is the decode step of sequences that hold the prefix themselves"""
     s = Shared(sa, ctx, 8, 4, 128, [40, 0, 5], 333)
@@ -465,6 +478,45 @@ def test_scored_long(sa, ctx):
     s.check(s.call(m, p), m, p)
 
 
+def test_scored_one_long_among_short(sa, ctx):
+    s = Scored(sa, ctx, 2, 2, 64, [5] * 70 + [6000], gap=1)
+    m, p = s.arrays()
+    s.check(s.call(m, p), m, p)
+
+
+@pytest.mark.parametrize("long", [1100, 4100])
+def test_scored_many_pairs(sa, ctx, long):
+    """more (sequence, kv head) pairs than there are workgroups to add weights up: each takes several runs of rows. The data
+    is made on the device; the longest sequences and some others are checked"""
+    n, hkv, hq, hd = 4200 * 1100 // long // 8, 8, 16, 64
+    rows = [long if i in (0, n - 1) else i % 70 for i in range(n)]
+    kv = sa.KVCache(ctx, 1, n, hkv, hd, long + 1)
+    torch.manual_seed(5)
+    kt, vt = kv.views(0)
+    kt.normal_()
+    vt.normal_()
+    q, k, v = (torch.randn(n, h * hd, device="cuda") for h in (hq, hkv, hkv))
+    mass = torch.rand(n, hkv, long + 3, device="cuda")
+    row_pos = torch.zeros(n, hkv, long + 3, dtype=torch.int32, device="cuda")
+    had = mass.clone()
+    out = sa.decode_scored(ctx, kv, 0, None, list(range(n)), rows, rows, q, k, v, hq, hd ** -0.5, mass, row_pos, decay=0.5)
+    assert torch.isfinite(out).all()
+    for i in (0, 1, 69, n // 2, n - 1):
+        r = rows[i]
+        assert torch.equal(mass[i, :, r + 1:], had[i, :, r + 1:]) and (row_pos[i, :, r] == r).all()
+        for h in range(hkv):
+            kk = torch.cat([kt[i, h, :r].double(), k[i].view(hkv, hd)[h:h + 1].double()])
+            vv = torch.cat([vt[i, h].transpose(1, 2).reshape(-1, hd)[:r].double(), v[i].view(hkv, hd)[h:h + 1].double()])
+            o, p, pv, a = attend(q[i].view(hkv, 2, hd)[h].double(), kk, vv, hd ** -0.5, 0.0)
+            e = err(hd, a)
+            assert ((out[i].view(hkv, 2, hd)[h] - o).abs() <= 2 * e * pv + 2.0 ** -22 * o.abs()).all()
+            w = p.sum(0)
+            old = 0.5 * had[i, h, :r + 1].double()
+            old[r] = 0.0
+            assert ((mass[i, h, :r + 1] - old - w).abs() <= 2 * e * w + 5 * 2.0 ** -24 * (old + w)).all()
+    kv.close()
+
+
 def test_scored_refusals(sa, ctx):
     s = Scored(sa, ctx, 4, 2, 64, [10, 5])
     m, p = s.arrays()
@@ -482,6 +534,17 @@ def test_scored_refusals(sa, ctx):
         setattr(s, field, keep)
     with pytest.raises(sa.SmolAttnError, match="overlap"):
         s.call(m, m.view(torch.int32))
+    # tables do not grow to any position, nor caches to any length: neither loops nor allocates
+    keep = s.pos
+    for far in (2 ** 22, 2 ** 30 + 1, 2 ** 31 - 70):
+        s.pos = [far, 3]
+        with pytest.raises(sa.SmolAttnError, match="table"):
+            s.call(m, p)
+    s.pos = keep
+    (q, k, v), (qw, kw_) = s.dev
+    for far in (2 ** 24, 2 ** 30 + 1, 2 ** 31 - 70):
+        with pytest.raises(sa.SmolAttnError, match="rows"):
+            sa.decode_shared(ctx, s.own.kv, s.slots[0], 0, s.own.kv, 1, None, [s.slots[1]], [far], q[:1], k[:1], v[:1], 4, 0.1)
     assert torch.equal(good, s.call(m, p))
 
 
