@@ -150,7 +150,9 @@ __device__ __forceinline__ void sh_row(const ShParams &p, const void *x_in, long
     constexpr bool POW2 = ShGeom<HD>::POW2;
     const bool neox = p.rope_kind == SMOL_ROPE_NEOX_K, inter = p.rope_kind == SMOL_ROPE_INTERLEAVED_K;
     const float *ct = p.rope_cos + (long long)pos * HD, *st = p.rope_sin + (long long)pos * HD;
-    float cv[KH][8], sn[KH][8]; /* the table repeats a row's first half in its second (NeoX) */
+    /* the norm's weights and the table's row are requested with the row: behind the first slab they would wait for it */
+    float wv[KS][8];
+    float cv[KH][8], sn[KH][8]; /* the table repeats a row's first half in its second (NeoX), or every value (interleaved) */
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) {
         const int d0 = 32 * ks + 8 * j;
@@ -158,11 +160,28 @@ __device__ __forceinline__ void sh_row(const ShParams &p, const void *x_in, long
         for (int i = 0; i < 8; i++) x[ks][i] = 0.0f;
         if (HD % 32 == 0 || d0 < HD) load8(x_in, p.in_dtype, row + d0, x[ks]);
     }
+    if (w) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+            if (HD % 32 == 0 || 32 * ks + 8 * j < HD) ld8f(w + 32 * ks + 8 * j, wv[ks]);
+    }
     if (POW2 && neox) {
 #pragma unroll
         for (int ks = 0; ks < KH; ks++) {
             ld8f(ct + 32 * ks + 8 * j, cv[ks]);
             ld8f(st + 32 * ks + 8 * j, sn[ks]);
+        }
+    } else if (POW2 && inter) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            float c8[8], s8[8];
+            ld8f(ct + 32 * ks + 8 * j, c8);
+            ld8f(st + 32 * ks + 8 * j, s8);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                cv[ks / 2][ks % 2 * 4 + i] = c8[2 * i];
+                sn[ks / 2][ks % 2 * 4 + i] = s8[2 * i];
+            }
         }
     }
     next();
@@ -179,10 +198,8 @@ __device__ __forceinline__ void sh_row(const ShParams &p, const void *x_in, long
             for (int ks = 0; ks < KS; ks++) {
                 const int d0 = 32 * ks + 8 * j;
                 if (HD % 32 == 0 || d0 < HD) {
-                    float wv[8];
-                    ld8f(w + d0, wv);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[ks][i] = x[ks][i] * wv[i] * ri;
+                    for (int i = 0; i < 8; i++) x[ks][i] = x[ks][i] * wv[ks][i] * ri;
                 }
             }
         }
@@ -196,6 +213,15 @@ __device__ __forceinline__ void sh_row(const ShParams &p, const void *x_in, long
                 const float a = x[ks][i], b = x[ks + KH][i];
                 x[ks][i] = fmaf(a, cv[ks][i], -(b * sn[ks][i]));
                 x[ks + KH][i] = fmaf(b, cv[ks][i], a * sn[ks][i]);
+            }
+    } else if (POW2 && inter) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float a = x[ks][2 * i], b = x[ks][2 * i + 1], c = cv[ks / 2][ks % 2 * 4 + i], d = sn[ks / 2][ks % 2 * 4 + i];
+                x[ks][2 * i] = fmaf(a, c, -(b * d));
+                x[ks][2 * i + 1] = fmaf(b, c, a * d);
             }
     } else if (inter || neox) {
 #pragma unroll
