@@ -31,15 +31,15 @@
  *
  * Measured on an MI355X (kernel time, head_dim 128, 16 heads over 8):
  * 4 sequences on 500 8.5 us and 16 on 4096 17.4 us (33 MB, 2.0 TB/s; the first
- * load waits for the sequences' table and Q, 3 to 5 us, and a wave has one to
- * four slabs); 64 on 16384 59 us (212 MB, 3.7 TB/s, matrix cores busy 27%;
- * a wide item 0.85 us a slab). head_dim 256, 8 heads over 1, 24 on 8191: 26.5 us,
+ * load waits for the sequences' table, a row and its turn, 3 to 5 us, and a
+ * wave has one to four slabs); 64 on 16384 59 us (212 MB, 3.7 TB/s, matrix cores busy 27%;
+ * a wide item 0.85 us a slab). head_dim 256, 8 heads over 1, 24 on 8191: 24.6 us,
  * one workgroup a compute unit, 2.6 us a wave's slab. Scored: 16 sequences of
  * 3000 to 4160 rows 56 us (244 MB, 4.4 TB/s). k_sh_merge 4 to 7 us, a launch's
- * and two round trips' time. Taken and left: one more launch instead of a join
- * by the last workgroup, whose fences cost 1 us at 4 sequences and 24 us at 64;
- * scores of the next slab beside the softmax of this one, 53 us against 45
- * for 64 on 16384 without own rows.
+ * and two round trips' time. Tried and not kept: a join by the last workgroup
+ * instead of that launch, whose fences cost 1 us more at 4 sequences and 24 us
+ * at 64; scores of the next slab beside the softmax of this one, a slab a step, 42.5
+ * us a call against 38.2 for 64 on 16384 without own rows.
  *
  * Every lane loads, normalises and rotates exactly the elements of Q that its
  * fragments hold (row c, dims 32 ks + 8 j ..), so the prologue is one round of
