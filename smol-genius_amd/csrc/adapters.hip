@@ -8,6 +8,8 @@
  *   k_adapt_in   t = A x, the in_dim cut into chunks so that few tiles still fill
  *                the device; each chunk writes its own partial t, so the sum's
  *                order is fixed.
+ * A few rows with few ranks run in one launch, k_adapt_one, whose workgroups
+ * each form t themselves.
  * Up to AD_FEW rows the rest is one launch, k_adapt_few: W streams once from
  * memory through the matrix cores against all rows (k_adapt_in's launch has
  * laid x out as bf16 parts for it), the waves' sums meet in LDS, and scale B t
@@ -21,8 +23,7 @@
  * The weights of a set are packed once, at its creation: ranks padded with
  * zeros to the matrix instruction's sizes, so no load needs a bound.
  *
- * Measured on an MI355X: 3 rows of 1024 -> 2048, rank 8: k_adapt_in 4.2 us and
- * k_adapt_few 5.6, two launches of little more than a launch's own time; 32
+ * Measured on an MI355X: 3 rows of 1024 -> 2048, rank 8: k_adapt_one 8.2 us; 32
  * rows of 1024 -> 4096, fp32, rank 16: 4.6 + 7.6 us (W's 8.4 MB; the bf16 parts
  * of x, read again by every workgroup from L2, are 50 MB); 3 rows of 4096 ->
  * 4096: 4.6 + 11 us (33.6 MB of W at 3.0 TB/s). 1536 rows of 1024 -> 2048,
@@ -252,6 +253,16 @@ __device__ __forceinline__ void ad_t(const AdParams &p, long long row, int rank,
     }
 }
 
+/* elements [8 j, 8 j + 8) of step s of W's row (w: its element 8 j), zeros past in_dim */
+__device__ __forceinline__ uint4 ad_w8(const AdParams &p, const uint16_t *w, int s, int j) {
+    const int k0 = 32 * s + 8 * j;
+    if (p.w_vec) return k0 < p.in_dim ? *reinterpret_cast<const uint4 *>(w + 32 * s) : make_uint4(0, 0, 0, 0);
+    uint32_t x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = k0 + i < p.in_dim ? w[32 * s + i] : 0u;
+    return make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+}
+
 /* Up to 16 RT rows against 16 outputs a workgroup. Its waves share in_dim out by runs of US 32-wide steps (whole cache lines of
  * W's rows), a run in flight; the sums of every wave are added in LDS in wave order, the adapters' tiles (one wave each) add their
  * part, and each output is written once. */
@@ -273,19 +284,6 @@ __global__ __launch_bounds__((64 * Few<RT, XBF>::NW)) void k_adapt_few(const AdP
     f4 acc[RT];
 #pragma unroll
     for (int t = 0; t < RT; t++) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
-    auto load_w = [&](int s) __attribute__((always_inline)) {
-        const int k0 = 32 * s + 8 * j;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (p.w_vec) {
-            if (k0 < p.in_dim) v = *reinterpret_cast<const uint4 *>(w + 32 * s);
-        } else {
-            uint32_t x[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = k0 + i < p.in_dim ? w[32 * s + i] : 0u;
-            v = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
-        }
-        return v;
-    };
     /* columns past the last row take the last row's x: results that no one reads, without reading their padding */
     int xo[RT];
 #pragma unroll
@@ -297,7 +295,7 @@ __global__ __launch_bounds__((64 * Few<RT, XBF>::NW)) void k_adapt_few(const AdP
 #pragma unroll
         for (int u = 0; u < US; u++) {
             const int s = s0 + u;
-            wv[u] = s < steps ? load_w(s) : make_uint4(0, 0, 0, 0);
+            wv[u] = s < steps ? ad_w8(p, w, s, j) : make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int t = 0; t < RT; t++)
 #pragma unroll
@@ -344,6 +342,117 @@ __global__ __launch_bounds__((64 * Few<RT, XBF>::NW)) void k_adapt_few(const AdP
         for (int q = 0; q < FEW_NW; q++) v += s_y[(q * RT * 16 + r) * STR + o];
         if (p.bias) v += p.bias[o0 + o];
         if (p.has[r >> 5] >> (r & 31) & 1) v += s_low[r * STR + o];
+        const long long at = (long long)r * p.out_dim + o0 + o;
+        if (p.y_bf16) ((uint16_t *)p.y)[at] = (uint16_t)(__float_as_uint(v) >> 16);
+        else ((float *)p.y)[at] = v;
+    }
+}
+
+/* Up to 16 rows with up to ONE_SLOTS tiles of 16 ranks among their adapters, all in one launch: every workgroup (16 outputs)
+ * forms A x of those tiles by itself, for all rows, beside its outputs of W x. Its waves share in_dim out; their sums meet in
+ * LDS in wave order, t is split there for B. What a workgroup reads again of A and x bounds it, so only little of both
+ * (ONE_WORK, in_dim times 4 for a slot and 1 for a row; kernel time here and in two launches, whatever out_dim up to 4096: one
+ * row and slot of 1024 6.9 and 9.6 us, of 4096 13.9 and 13.9; three and three of 1024 8.2 and 9.7, of 2048 12.0 and 11.4; four
+ * rows and slots of 1024 10.7 and 11.3, of 2048 15.9 and 14.1; 16 rows and four slots of 512 9.1 and 9.2, of 1024 12.4 and 10.1;
+ * a second launch costs the host 2.4 us besides). */
+constexpr int ONE_SLOTS = 4, ONE_NW = 16;
+constexpr long long ONE_WORK = 20480;
+template <bool XBF>
+__global__ __launch_bounds__(64 * ONE_NW) void k_adapt_one(const AdParams p) {
+    constexpr int PARTS = XBF ? 1 : 3, US = 2, STR = 20, NS = 1 + ONE_SLOTS, TSTR = ONE_SLOTS * 16 + 4;
+    __shared__ __attribute__((aligned(16))) float s_y[ONE_NW * NS * 16 * STR], s_t[16 * TSTR], s_low[16 * STR];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int o0 = blockIdx.x * 16, steps = p.kp / 32;
+    const uint16_t *w = p.w + (long long)min(o0 + c, p.out_dim - 1) * p.in_dim + 8 * j;
+    /* slot q: tile q's first ranks, and so on: the tiles' slots follow each other */
+    const uint16_t *a[ONE_SLOTS];
+    int n_slots = 0;
+#pragma unroll
+    for (int q = 0; q < ONE_SLOTS; q++) a[q] = p.a;
+    for (int t = 0; t < p.n_tiles; t++)
+        for (int r = 0; r < p.tiles[t].rank; r += 16, n_slots++)
+#pragma unroll
+            for (int q = 0; q < ONE_SLOTS; q++)
+                if (q == n_slots) a[q] = p.a + ((long long)p.tiles[t].adapter * p.ra + r + c) * p.kp + 8 * j;
+    const long long row = min(c, p.seq - 1); /* columns past the last row: results that no one reads */
+    f4 acc[NS];
+#pragma unroll
+    for (int q = 0; q < NS; q++) acc[q] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = wave * US; s0 < steps; s0 += ONE_NW * US) {
+        uint4 wv[US];
+        b8 xp[US][PARTS], av[US][ONE_SLOTS];
+#pragma unroll
+        for (int u = 0; u < US; u++) {
+            const bool live = s0 + u < steps;
+            const int s = live ? s0 + u : 0;
+            wv[u] = ad_w8(p, w, s, j);
+#pragma unroll
+            for (int q = 0; q < ONE_SLOTS; q++)
+                if (q < n_slots) av[u][q] = as_b8(*reinterpret_cast<const uint4 *>(a[q] + 32 * s));
+            ad_x8<XBF>(p, row, live ? 32 * s + 8 * j : p.kp, xp[u]); /* past the last step: zeros */
+        }
+#pragma unroll
+        for (int u = 0; u < US; u++)
+#pragma unroll
+            for (int q = PARTS - 1; q >= 0; q--) {
+                acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(wv[u]), xp[u][q], acc[0], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < ONE_SLOTS; t++)
+                    if (t < n_slots) acc[1 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av[u][t], xp[u][q], acc[1 + t], 0, 0, 0);
+            }
+    }
+#pragma unroll
+    for (int q = 0; q < NS; q++)
+        if (q <= n_slots) *reinterpret_cast<f4 *>(s_y + ((wave * NS + q) * 16 + c) * STR + 4 * j) = acc[q];
+    __syncthreads();
+    /* t of every row and slot: a thread a rank */
+    for (int e = tid; e < n_slots * 256; e += 64 * ONE_NW) {
+        const int q = e / 256, r = e / 16 % 16, k = e % 16;
+        float v = 0.0f;
+#pragma unroll
+        for (int u = 0; u < ONE_NW; u++) v += s_y[((u * NS + 1 + q) * 16 + r) * STR + k];
+        s_t[r * TSTR + q * 16 + k] = v;
+    }
+    __syncthreads();
+    /* B t by tile, a wave each */
+    for (int tile = wave; tile < p.n_tiles; tile += ONE_NW) {
+        int slot = 0;
+        for (int t = 0; t < tile; t++) slot += (p.tiles[t].rank + 15) / 16;
+        const AdAt tl = ad_at(p, tile, c);
+        const uint16_t *b = p.b + ((long long)tl.adapter * p.np + o0 + c) * p.rp + 8 * j;
+        f4 low = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < ONE_SLOTS / 2; ks++) {
+            if (32 * ks >= tl.rank) break;
+            const int r = 32 * ks + 8 * j;
+            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (r < ((tl.rank + 15) & ~15)) {
+                const f4 x = *reinterpret_cast<const f4 *>(s_t + tl.row * TSTR + slot * 16 + r);
+                const f4 y = *reinterpret_cast<const f4 *>(s_t + tl.row * TSTR + slot * 16 + r + 4);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    v[i] = x[i] * tl.scale;
+                    v[4 + i] = y[i] * tl.scale;
+                }
+            }
+            b8 tp[3];
+            ad_split3(v, tp[0], tp[1], tp[2]);
+            const b8 bw = as_b8(*reinterpret_cast<const uint4 *>(b + 32 * ks));
+#pragma unroll
+            for (int q = 2; q >= 0; q--) low = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw, tp[q], low, 0, 0, 0);
+        }
+        if (c < tl.n) *reinterpret_cast<f4 *>(s_low + tl.row * STR + 4 * j) = low;
+    }
+    __syncthreads();
+    for (int e = tid; e < p.seq * 16; e += 64 * ONE_NW) {
+        const int r = e / 16, o = e % 16;
+        if (o0 + o >= p.out_dim) continue;
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < ONE_NW; q++) v += s_y[(q * NS * 16 + r) * STR + o];
+        if (p.bias) v += p.bias[o0 + o];
+        if (p.has[0] >> r & 1) v += s_low[r * STR + o];
         const long long at = (long long)r * p.out_dim + o0 + o;
         if (p.y_bf16) ((uint16_t *)p.y)[at] = (uint16_t)(__float_as_uint(v) >> 16);
         else ((float *)p.y)[at] = v;
@@ -627,6 +736,9 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
     p.chunk = (steps + chunks - 1) / chunks;
     p.n_chunks = (steps + p.chunk - 1) / p.chunk;
     const bool ybf = y_dtype == SMOL_ATTN_BF16, few = seq <= AD_FEW;
+    int slots = 0;
+    for (const AdTile &t : tiles) slots += (t.rank + 15) / 16;
+    const bool one = seq <= 16 && slots <= ONE_SLOTS && (4LL * slots + seq) * in_dim <= ONE_WORK;
     /* more rows than k_adapt_few takes, and operands that the library's product cannot stage (16-byte pieces): x and W
      * are copied with padded rows first */
     const bool pad = !few && (in_dim % 8 != 0 || ((uintptr_t)x & 15) || ((uintptr_t)w & 15));
@@ -681,6 +793,14 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
         if (int rc = smol_linear_dev(ctx, base, SMOL_ATTN_F32, bx, x_dtype, bw, bias, seq, bk, out_dim)) return rc;
         smol_internal_timing_events(ctx, AD_TIMING_KIND, &e0, &e1);
         if (e0) AHIP(hipEventRecord(e0, st));
+    }
+    if (one) {
+        const dim3 g((unsigned)((out_dim + 15) / 16)), b(64 * ONE_NW);
+        if (p.x_bf16) hipLaunchKernelGGL(k_adapt_one<true>, g, b, 0, st, p);
+        else hipLaunchKernelGGL(k_adapt_one<false>, g, b, 0, st, p);
+        AHIP(hipGetLastError());
+        if (e1) AHIP(hipEventRecord(e1, st));
+        return SMOL_ATTN_OK;
     }
     p.in_blocks = n_tiles * p.n_chunks;
     const unsigned in_blocks = (unsigned)p.in_blocks + (few ? ((unsigned)((seq + 15) / 16) * (kp / 32) + AD_NW - 1) / AD_NW : 0);

@@ -103,6 +103,13 @@ CASES = [
     dict(seq=32, k=2048, n=48, ranks=[16, 4]),
     dict(seq=64, k=96, n=200, ranks=[20] * 50),
     dict(seq=65, k=97, n=90, ranks=[12, 40]),
+    # few rows and ranks, one launch: four tiles of ranks, a set whose largest rank no row uses, the last sizes and the next
+    dict(seq=16, k=256, n=100, ranks=[17, 20]),
+    dict(seq=5, k=333, n=65, ranks=[64]),
+    dict(seq=4, k=1000, n=48, ranks=[16, 16, 16, 16], ids=[3, 1, 0, 2]),
+    dict(seq=3, k=96, n=40, ranks=[128, 8, 33], ids=[2, -1, 1]),
+    dict(seq=16, k=1024, n=33, ranks=[16], bare=0.0),
+    dict(seq=16, k=1032, n=33, ranks=[16], bare=0.0),
     dict(seq=200, k=333, n=1001, ranks=[128, 8]),
 ]
 
@@ -138,7 +145,7 @@ def test_rows_do_not_meet(sa, ctx, n):
     assert torch.isnan(y[hit]).all() and torch.equal(y[rest], clean[rest])
 
 
-@pytest.mark.parametrize("n", [32, 64, 128])
+@pytest.mark.parametrize("n", [8, 32, 64, 128])
 def test_a_row_does_not_depend_on_the_order(sa, ctx, n):
     """the same rows in another order, with the same number of rows an adapter: the same bits a row"""
     t = Case(n, 512, 256, [16, 8])
