@@ -116,7 +116,7 @@ SMOL_ATTN_API int smol_attn_ctx_timing_read(smol_attn_ctx *ctx, double *ms, int 
 #define SMOL_OPT_FB_LISTS 1       /* -1: one k_attn_fb workgroup per tile, or per piece of one whose keys are split
                                    * (no lists) */
 #define SMOL_OPT_FB_NT 2          /* 2: two row tiles per k_attn_fb wave */
-#define SMOL_OPT_DEC_SLABS 3      /* k_dec: 32-key slabs per workgroup (0: by call size) */
+#define SMOL_OPT_DEC_SLABS 3      /* k_dec, k_sh: 32-key slabs per workgroup (0: by call size) */
 #define SMOL_OPT_DEC_WAVES 4      /* k_dec: 4 or 8 waves per workgroup (0: by shape) */
 #define SMOL_OPT_DEC_SPLIT 5      /* k_dec: -1 keeps every (sequence, kv head) in one workgroup */
 #define SMOL_OPT_XCD_CHECK 6      /* read only: 1 when workgroups b and b + n_xcc were seen on one XCD at

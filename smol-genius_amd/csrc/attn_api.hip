@@ -1966,7 +1966,8 @@ static int run_shared(smol_attn_ctx *ctx, ShParams &sp, smol_kv_cache *kv, int l
      * 32, 48 44 / 38 / 45). */
     const long long slots = (long long)ctx->cu_count * smol_shared_occupancy(hd);
     auto chunk = [&](int longest, long long limit, auto workgroups) {
-        const int least = std::max(4, (longest + SH_MAX_SPLIT - 1) / SH_MAX_SPLIT), forced = ctx->opt[SMOL_OPT_DEC_SLABS];
+        const int least = std::max(4, (longest + SH_MAX_SPLIT - 1) / SH_MAX_SPLIT);
+        const int forced = std::min(ctx->opt[SMOL_OPT_DEC_SLABS], std::max(longest, 4));
         long long c = (std::max(least, forced) + 3) & ~3;
         if (forced <= 0)
             while (c < longest && workgroups(c) > limit) c += std::max(4LL, (c / 8) & ~3LL);

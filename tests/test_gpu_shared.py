@@ -257,6 +257,19 @@ def test_shared_one_long_among_short(sa, ctx, c):
     assert torch.equal(a, s.call())
 
 
+@pytest.mark.parametrize("slabs", [-5, 1, 4, 7, 64, 2 ** 30, 2 ** 31 - 1])
+def test_forced_slabs(sa, slabs):
+    c2 = sa.Context(0)
+    c2.set_option(sa.OPT_DEC_SLABS, slabs)
+    s = Shared(sa, c2, 8, 2, 128, [3, 700, 0, 64] * 3, 1100, window=900)
+    s.check(s.call())
+    z = Scored(sa, c2, 4, 2, 64, [900, 0, 33])
+    m, p = z.arrays()
+    z.check(z.call(m, p), m, p)
+    del s, z
+    c2.close()
+
+
 def test_shared_equals_decode(sa, ctx):
     """the batch's step on a shared prefix is the decode step of sequences that hold the prefix themselves"""
     s = Shared(sa, ctx, 8, 4, 128, [40, 0, 5], 333)
