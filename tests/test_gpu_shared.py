@@ -749,6 +749,33 @@ def test_budgeted_stream(sa, ctx):
     ctx.synchronize()
 
 
+def test_slots_past_32_bits(sa, ctx):
+    """the last slots of a cache of more than 4 GB hold, give and lose the same rows as those of a small one"""
+    hkv, hq, hd, rows, P = 8, 16, 128, 200, 300
+    torch.manual_seed(4)
+    K, V = (torch.randn(2, hkv, 320, hd, device="cuda").to(torch.bfloat16) for _ in range(2))
+    q, k, v = (torch.randn(1, h * hd, device="cuda") for h in (hq, hkv, hkv))
+    got = []
+    for n_slots, cap in ((2, 320), (40, 65536)):
+        kv = sa.KVCache(ctx, 1, n_slots, hkv, hd, cap)
+        assert n_slots == 2 or n_slots * hkv * kv.capacity * hd * 2 > 2 ** 32
+        kt, vt = kv.views(0)
+        kt[-2:, :, :320] = K
+        vt[-2:, :, :10] = V.view(2, hkv, 10, 32, hd).transpose(-1, -2)
+        a, b = n_slots - 2, n_slots - 1
+        out = [sa.decode_shared(ctx, kv, b, P, kv, 0, None, [a], [rows], q, k, v, hq, hd ** -0.5)]
+        mass = torch.zeros(n_slots, hkv, 320, device="cuda")
+        pos = torch.arange(320, dtype=torch.int32, device="cuda").expand(n_slots, hkv, 320).contiguous()
+        out.append(sa.decode_scored(ctx, kv, 0, None, [b], [P], [P], q, k, v, hq, hd ** -0.5, mass, pos))
+        sa.kv_evict(kv, 0, [b], [P + 1], [P + 1], mass, pos, 100, recent=10)
+        out += [mass[b, :, :100].clone(), pos[b, :, :100].clone(), kt[-2:, :, :320].clone(), vt[-2:, :, :10].clone()]
+        assert (kt[:-2].count_nonzero() + vt[:-2].count_nonzero()).item() == 0
+        got.append(out)
+        kv.close()
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
 def test_captured_steps_replay(sa):
     """a shared step, a scored step and an eviction in one graph, replayed with other inputs in the same buffers and
     eager work between the replays; growth under capture is refused"""
