@@ -543,10 +543,9 @@ __global__ __launch_bounds__(256) void k_adapt_bare(uint16_t *y, const float *ba
 template <typename T>
 __global__ __launch_bounds__(256) void k_adapt_pack(T *dst, const T *src, int rows, int stride, int src_rows,
                                                     int cols) {
-    const long long n = (long long)rows * stride;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const int r = (int)(i / stride), q = (int)(i - (long long)r * stride);
-        dst[i] = r < src_rows && q < cols ? src[(long long)r * cols + q] : (T)0;
+    for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+        const T *s = src + (long long)r * cols;
+        for (int q = threadIdx.x; q < stride; q += 256) dst[(long long)r * stride + q] = r < src_rows && q < cols ? s[q] : (T)0;
     }
 }
 
@@ -623,8 +622,7 @@ extern "C" int smol_adapters_create(smol_attn_ctx *ctx, int n, int in_dim, int o
     s->rank = reinterpret_cast<int *>(static_cast<char *>(s->mem) + ab + bb + sb);
     for (int i = 0; i < n && e == hipSuccess; i++) {
         auto pack = [&](uint16_t *dst, const uint16_t *src, int rows, int stride, int src_rows, int cols) {
-            const long long blocks = std::min<long long>(((long long)rows * stride + 255) / 256, 4096);
-            hipLaunchKernelGGL(k_adapt_pack<uint16_t>, dim3((unsigned)blocks), dim3(256), 0, s->stream, dst, src, rows, stride, src_rows, cols);
+            hipLaunchKernelGGL(k_adapt_pack<uint16_t>, dim3((unsigned)std::min(rows, 4096)), dim3(256), 0, s->stream, dst, src, rows, stride, src_rows, cols);
         };
         pack(s->a + (size_t)i * s->ra * s->kp, a[i], s->ra, s->kp, rank[i], in_dim);
         pack(s->b + (size_t)i * s->np * s->rp, b[i], s->np, s->rp, out_dim, rank[i]);
@@ -781,10 +779,10 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
         const uint16_t *bw = w;
         int bk = in_dim;
         if (pad) {
-            const unsigned pg = 2048;
-            if (p.x_bf16) hipLaunchKernelGGL(k_adapt_pack<uint16_t>, dim3(pg), dim3(256), 0, st, static_cast<uint16_t *>(x_own), (const uint16_t *)x, seq, kp, seq, in_dim);
-            else hipLaunchKernelGGL(k_adapt_pack<uint32_t>, dim3(pg), dim3(256), 0, st, static_cast<uint32_t *>(x_own), (const uint32_t *)x, seq, kp, seq, in_dim);
-            hipLaunchKernelGGL(k_adapt_pack<uint16_t>, dim3(pg), dim3(256), 0, st, w_own, w, out_dim, kp, out_dim, in_dim);
+            const unsigned xg = (unsigned)std::min(seq, 4096), wg = (unsigned)std::min(out_dim, 4096);
+            if (p.x_bf16) hipLaunchKernelGGL(k_adapt_pack<uint16_t>, dim3(xg), dim3(256), 0, st, static_cast<uint16_t *>(x_own), (const uint16_t *)x, seq, kp, seq, in_dim);
+            else hipLaunchKernelGGL(k_adapt_pack<uint32_t>, dim3(xg), dim3(256), 0, st, static_cast<uint32_t *>(x_own), (const uint32_t *)x, seq, kp, seq, in_dim);
+            hipLaunchKernelGGL(k_adapt_pack<uint16_t>, dim3(wg), dim3(256), 0, st, w_own, w, out_dim, kp, out_dim, in_dim);
             AHIP(hipGetLastError());
             bx = x_own;
             bw = w_own;

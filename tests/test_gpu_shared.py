@@ -478,6 +478,8 @@ class Scored:
     dict(hq=3, hkv=3, hd=72, rows=[129, 64]),
     dict(hq=20, hkv=1, hd=96, rows=[40, 500], decay=0.0, cap=50.0),
     dict(hq=2, hkv=1, hd=64, rows=[i % 40 for i in range(130)]),
+    # more heads a kv head than the weights' workgroups hold at once
+    dict(hq=520, hkv=1, hd=64, rows=[40, 0]),
 ], ids=lambda c: "%d-%d-%d-%s" % (c["hq"], c["hkv"], c["hd"], "_".join(map(str, c["rows"][:4]))))
 def test_scored(sa, ctx, c):
     s = Scored(sa, ctx, **c)
