@@ -81,9 +81,9 @@ SMOL_ATTN_API int smol_adapters_destroy(smol_adapters *set);
  * holds infinity may give NaN. A row's results do not depend on the other rows'
  * values. y (16-byte aligned) overlaps neither x nor W. Uses the context's
  * workspace. Under stream capture the call must have been made once before,
- * with at most 40 groups of up to 16 rows that share an adapter, or 400 of
- * rows that also follow each other (SMOL_ATTN_ERR_UNSUPPORTED otherwise); the
- * captured call keeps its ids. */
+ * with at most 40 groups of up to 16 rows that share an adapter (or, for a bf16
+ * y of more than 64 rows, have none), or 400 of rows that also follow each
+ * other (SMOL_ATTN_ERR_UNSUPPORTED otherwise); the captured call keeps its ids. */
 SMOL_ATTN_API int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype, const void *x, int x_dtype,
                                            const uint16_t *w, const float *bias, int seq, int in_dim, int out_dim,
                                            const smol_adapters *set, const int *ids);

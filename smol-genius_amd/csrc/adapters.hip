@@ -61,7 +61,7 @@ constexpr int AD_FEW = 64;
 constexpr int AD_TIMING_KIND = 2;
 
 struct AdTile {
-    int adapter, n, rank;
+    int adapter, n, rank; /* adapter -1: rows without one, whose product k_adapt_out truncates */
     float scale;
     int row[16]; /* rows past n repeat the first */
 };
@@ -82,6 +82,7 @@ struct AdParams {
     const uint16_t *b; int np, rp;   /* [adapter][np][rp] */
     const float *scale; const int *rank; /* [adapter] */
     float *t; int n_tiles, n_chunks, chunk; /* [chunk][seq][ra]; chunk: 32-wide steps of in_dim */
+    int n_out;                       /* tiles of k_adapt_out: behind the n_tiles those without an adapter */
     unsigned has[2];                 /* few rows: the rows that have an adapter */
     const float *base;               /* fp32 [seq][out] that the low-rank part is added to */
     void *y; int y_bf16;             /* fp32 y is base itself */
@@ -103,7 +104,8 @@ struct AdAt {
 __device__ __forceinline__ AdAt ad_at(const AdParams &p, int tile, int c) {
     if (p.runs_only) {
         const AdRun r = p.runs[tile];
-        return AdAt{r.adapter, r.n, p.rank[r.adapter], p.scale[r.adapter], r.row0 + (c < r.n ? c : 0)};
+        const int row = r.row0 + (c < r.n ? c : 0);
+        return r.adapter < 0 ? AdAt{-1, r.n, 0, 0.0f, row} : AdAt{r.adapter, r.n, p.rank[r.adapter], p.scale[r.adapter], row};
     }
     const AdTile *t = (p.tiles_dev ? p.tiles_dev : p.tiles) + tile;
     return AdAt{t->adapter, t->n, t->rank, t->scale, t->row[c]};
@@ -471,26 +473,31 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_out(const AdParams p) {
     __shared__ int s_row[16];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int tile = blockIdx.x % p.n_tiles, w0 = blockIdx.x / p.n_tiles * W, o0 = w0 + wave * AD_OUT;
+    const int tile = blockIdx.x % p.n_out, w0 = blockIdx.x / p.n_out * W, o0 = w0 + wave * AD_OUT;
     const AdAt tl = ad_at(p, tile, c);
     const long long row = tl.row;
     if (tid < 16) s_row[tid] = tl.row;
     const bool live = c < tl.n, mine = o0 < p.out_dim; /* B has whole tiles of AD_OUT rows and 32 ranks */
-    b8 w[U][KS], tp[KS][3];
-    const uint16_t *b = p.b + ((long long)tl.adapter * p.np + (mine ? o0 : 0) + c) * p.rp + 8 * j;
+    if (tl.adapter < 0) {
+        /* what adds nothing to any value, its sign included */
+        for (int e = tid; e < 16 * STR; e += AD_TPB) s_d[e] = -0.0f;
+    } else {
+        b8 w[U][KS], tp[KS][3];
+        const uint16_t *b = p.b + ((long long)tl.adapter * p.np + (mine ? o0 : 0) + c) * p.rp + 8 * j;
 #pragma unroll
-    for (int u = 0; u < U; u++)
+        for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) w[u][ks] = as_b8(*reinterpret_cast<const uint4 *>(b + (long long)16 * u * p.rp + 32 * ks));
-    ad_t<KS>(p, row, tl.rank, tl.scale, live, j, tp);
+            for (int ks = 0; ks < KS; ks++) w[u][ks] = as_b8(*reinterpret_cast<const uint4 *>(b + (long long)16 * u * p.rp + 32 * ks));
+        ad_t<KS>(p, row, tl.rank, tl.scale, live, j, tp);
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        f4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < U; u++) {
+            f4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
+            for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-            for (int q = 2; q >= 0; q--) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u][ks], tp[ks][q], acc, 0, 0, 0);
-        *reinterpret_cast<f4 *>(s_d + c * STR + wave * AD_OUT + 16 * u + 4 * j) = acc;
+                for (int q = 2; q >= 0; q--) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u][ks], tp[ks][q], acc, 0, 0, 0);
+            *reinterpret_cast<f4 *>(s_d + c * STR + wave * AD_OUT + 16 * u + 4 * j) = acc;
+        }
     }
     __syncthreads();
     /* a wave a row at a time, a lane four outputs */
@@ -531,12 +538,6 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_out(const AdParams p) {
                 }
         }
     }
-}
-
-/* rows without an adapter, bf16 y: the shared product alone, truncated */
-__global__ __launch_bounds__(256) void k_adapt_bare(uint16_t *y, const float *base, long long n) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) y[i] = (uint16_t)(__float_as_uint(base[i]) >> 16);
 }
 
 /* dst [rows][stride] = src [rows][cols], zeros behind; rows past src_rows are zeros */
@@ -677,7 +678,7 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
     if ((const char *)w < (const char *)y + (size_t)seq * out_dim * ys && (const char *)y < (const char *)w + (size_t)out_dim * in_dim * 2)
         return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: y overlaps W");
     /* the rows by adapter, tiles of at most 16 */
-    std::vector<int> count(set->n, 0);
+    std::vector<int> count(set->n + 1, 0);
     int bare = 0;
     for (int s = 0; s < seq; s++) {
         if (ids[s] < -1 || ids[s] >= set->n) return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: an id outside the set");
@@ -685,24 +686,28 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
         else count[ids[s]]++;
     }
     if (bare == seq) return smol_linear_dev(ctx, y, y_dtype, x, x_dtype, w, bias, seq, in_dim, out_dim);
-    std::vector<int> first(set->n, 0);
+    /* rows without one are k_adapt_out's too where y is not the product itself */
+    const bool casts = bare && y_dtype == SMOL_ATTN_BF16 && seq > AD_FEW;
+    std::vector<int> first(set->n + 1, 0);
     int n_tiles = 0;
     for (int i = 0; i < set->n; i++) {
         first[i] = n_tiles;
         n_tiles += (count[i] + 15) / 16;
         count[i] = 0;
     }
-    std::vector<AdTile> tiles(n_tiles);
+    const int n_out = n_tiles + (casts ? (bare + 15) / 16 : 0);
+    first[set->n] = n_tiles;
+    std::vector<AdTile> tiles(n_out);
     bool runs_only = set->n <= SHRT_MAX;
     for (int s = 0; s < seq; s++) {
-        const int id = ids[s];
-        if (id < 0) continue;
+        if (ids[s] < 0 && !casts) continue;
+        const int id = ids[s] < 0 ? set->n : ids[s];
         AdTile &t = tiles[first[id] + count[id] / 16];
         const int k = count[id]++ % 16;
         if (k == 0) {
-            t.adapter = id;
-            t.rank = set->h_rank[id];
-            t.scale = set->h_scale[id];
+            t.adapter = ids[s];
+            t.rank = ids[s] < 0 ? 0 : set->h_rank[id];
+            t.scale = ids[s] < 0 ? 0.0f : set->h_scale[id];
             for (int i = 0; i < 16; i++) t.row[i] = s;
         }
         runs_only &= s == t.row[0] + k;
@@ -725,6 +730,7 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
     p.scale = set->scale;
     p.rank = set->rank;
     p.n_tiles = n_tiles;
+    p.n_out = n_out;
     /* A step a wave at least. Few tiles: workgroups for a quarter of the compute units, since every chunk is another partial
      * sum for each of the readers (64 rows of 2048 and 1024: a quarter, half, all of them 19.4, 20.2, 22.6 and 15.5, 16.4,
      * 16.4 us in both kernels). Many tiles (more rows than k_adapt_few takes) have few readers a row: all compute units
@@ -760,14 +766,14 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
     p.base = base;
     p.y = y;
     p.y_bf16 = ybf;
-    if (n_tiles > AD_ARG_TILES && n_tiles <= AD_ARG_RUNS && runs_only) {
+    if (n_out > AD_ARG_TILES && n_out <= AD_ARG_RUNS && runs_only) {
         p.runs_only = 1;
-        for (int i = 0; i < n_tiles; i++) p.runs[i] = {tiles[i].row[0], (short)tiles[i].adapter, (short)tiles[i].n};
-    } else if (n_tiles <= AD_ARG_TILES) {
-        memcpy(p.tiles, tiles.data(), n_tiles * sizeof(AdTile));
+        for (int i = 0; i < n_out; i++) p.runs[i] = {tiles[i].row[0], (short)tiles[i].adapter, (short)tiles[i].n};
+    } else if (n_out <= AD_ARG_TILES) {
+        memcpy(p.tiles, tiles.data(), n_out * sizeof(AdTile));
     } else {
         const void *dev;
-        if (int rc = smol_internal_upload(ctx, tiles.data(), n_tiles * sizeof(AdTile), &dev)) return rc;
+        if (int rc = smol_internal_upload(ctx, tiles.data(), n_out * sizeof(AdTile), &dev)) return rc;
         p.tiles_dev = static_cast<const AdTile *>(dev);
     }
     hipEvent_t e0 = nullptr, e1 = nullptr;
@@ -823,11 +829,7 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
         if (e1) AHIP(hipEventRecord(e1, st));
         return SMOL_ATTN_OK;
     }
-    if (ybf && bare) {
-        const long long n = (long long)seq * out_dim;
-        hipLaunchKernelGGL(k_adapt_bare, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (uint16_t *)y, base, n);
-    }
-    const unsigned out_blocks = (unsigned)n_tiles * ((out_dim + AD_OUT * AD_NW - 1) / (AD_OUT * AD_NW));
+    const unsigned out_blocks = (unsigned)n_out * ((out_dim + AD_OUT * AD_NW - 1) / (AD_OUT * AD_NW));
     switch (set->rp / 32) {
     case 1: hipLaunchKernelGGL(k_adapt_out<1>, dim3(out_blocks), dim3(AD_TPB), 0, st, p); break;
     case 2: hipLaunchKernelGGL(k_adapt_out<2>, dim3(out_blocks), dim3(AD_TPB), 0, st, p); break;

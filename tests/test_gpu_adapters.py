@@ -129,6 +129,22 @@ def test_no_row_has_one(sa, ctx):
     assert torch.equal(y, sa.linear(ctx, t.dev[0], t.dev[1], t.dev[2]))
 
 
+@pytest.mark.parametrize("seq,k,n", [(65, 64, 48), (130, 96, 257), (1000, 72, 300)])
+def test_bare_rows_among_others(sa, ctx, seq, k, n):
+    """a bf16 y of many rows: those without an adapter are smol_linear_dev's bits, whatever the adapters hold"""
+    t = Case(seq, k, n, [8, 16], bf16=True, bare=0.4)
+    y = t.call(sa, ctx, True)
+    t.check(y, True)
+    z = sa.linear(ctx, t.dev[0], t.dev[1], t.dev[2], out_bf16=True)
+    bare = [s for s in range(seq) if t.ids[s] < 0]
+    assert bare and torch.equal(y[bare], z[bare])
+    for a, b, _ in t.ab:
+        a.fill_(float("nan"))
+        b.fill_(float("inf"))
+    t.to(sa, ctx)
+    assert torch.equal(t.call(sa, ctx, True)[bare], z[bare])
+
+
 @pytest.mark.parametrize("n", [9, 50, 130])
 def test_rows_do_not_meet(sa, ctx, n):
     """a NaN row, and NaN weights of an adapter, reach their own rows only"""
