@@ -254,15 +254,15 @@ def _inputs(c, seed):
     return d
 
 
-_kept = {}  # the library, the context and the position tables that a program makes once
+_kept = {}  # the context and the position tables that a program makes once
 
 
 def _sa():
+    import importlib
+    sa = importlib.import_module("smol-genius_amd.smol_attn")
     if "ctx" not in _kept:
-        import importlib
-        _kept["sa"] = importlib.import_module("smol-genius_amd.smol_attn")
-        _kept["ctx"] = _kept["sa"].Context(0)
-    return _kept["sa"], _kept["ctx"]
+        _kept["ctx"] = sa.Context(0)
+    return sa, _kept["ctx"]
 
 
 def _cache(sa, ctx, k, v):
