@@ -279,9 +279,11 @@ SMOL_ATTN_API int smol_attn_decode_noalloc(smol_attn_ctx *ctx, smol_kv_cache *kv
  * in fp32 by the call that appends it and stored as bf16 (nearest even). The
  * products are fp32 Q and fp32 probabilities, each split into three bf16 parts
  * (24 bits), with the cache's bf16 bits; everything else is fp32, and there is no
- * range limit. A cached row that holds NaN or infinity makes the outputs of the
- * sequences that see it NaN, and of no other; rows at or past a sequence's
- * length are never used. A sequence's result does not depend on what the cache
+ * range limit but fp32's own (values of V below 2^96, for they are summed before
+ * they are divided). A visible row, cached or new, whose key or value holds a NaN
+ * or infinity, be it in one element, makes NaN of all outputs of the heads that
+ * read it, and of no other; a key also of their weights (a value leaves these
+ * alone). Rows at or past a sequence's length are never used. A sequence's result does not depend on what the cache
  * holds elsewhere, but the order of its sums follows the batch's shape. Slots
  * are host arrays, each slot at most once. Calls grow the cache, the table and the context's
  * workspace as needed. Under stream capture they may not grow anything and

@@ -336,18 +336,29 @@ __device__ __forceinline__ void sh_qk(const ShRows<HD> &w, const uint4 (&k)[2][S
 }
 
 /* The scores of NS slabs from key k0 on: capped, kept (logits: where this lane's go, or null), and -inf for keys that a row
- * does not see; nan: whether a row sees a value that is no number among those taken out */
+ * does not see; nan: whether a row sees a value that is no number among those taken out. odd becomes the largest of the
+ * scores' bits as whole numbers: MINUS_INF or more with a score of -inf (or of +inf and a cap, which makes a number of it), and
+ * with no finite score. */
+constexpr unsigned MINUS_INF = 0xFF800000u;
 template <int HD, int NS, bool SC>
 __device__ __forceinline__ bool sh_mask(const ShParams &p, const ShRows<HD> &w, int k0, int ke, int j, f4 (&s)[NS][2],
-                                        uint4 (&v)[NS][ShGeom<HD>::DT], float *logits) {
+                                        uint4 (&v)[NS][ShGeom<HD>::DT], float *logits, unsigned &odd) {
     constexpr int DT = ShGeom<HD>::DT;
+#pragma unroll
+    for (int u = 0; u < NS; u++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) odd = max(odd, __float_as_uint(s[u][e >> 2][e & 3]));
+    asm volatile("" : "+v"(odd)); /* formed here: later, the scores as they were would hold registers */
     if (p.cap2 > 0.0f) {
 #pragma unroll
         for (int u = 0; u < NS; u++)
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) s[u][h][i] = p.cap2 * tanhf(s[u][h][i] / p.cap2);
+                for (int i = 0; i < 4; i++) {
+                    odd = max(odd, s[u][h][i] == INFINITY ? MINUS_INF : 0u);
+                    s[u][h][i] = p.cap2 * tanhf(s[u][h][i] / p.cap2);
+                }
     }
     if (SC && logits) {
 #pragma unroll
@@ -434,6 +445,29 @@ __device__ __forceinline__ void sh_pv(ShRows<HD> &w, const f4 (&s)[NS][2], const
                 w.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(v[u][dt]), pp[u][q], w.o[dt], 0, 0, 0);
 }
 
+/* Rows that see a key with an element that is not finite become NaN. Such a key's scores are not finite, for every row: NaN and
+ * +inf go through the softmax, but -inf has no weight and a cap makes numbers of both. A finite product past fp32's range gives
+ * them too. So the keys [k0, ke), a slab every `step`, are read again where odd tells of such a score. (A value that is not
+ * finite shows in its dimension of the sum: k_sh_merge.) */
+template <int HD>
+__device__ __forceinline__ void sh_spoil(const ShItem &it, ShRows<HD> &w, unsigned odd, int k0, int step) {
+    constexpr int PC = HD / 8;
+    if (!__any(odd >= MINUS_INF)) return;
+    const rsrc_t rs = make_rsrc(it.kc, it.region_bytes);
+#pragma unroll 1
+    for (; k0 < it.ke; k0 += step) {
+        unsigned bad = 0; /* bit r: row r of the slab */
+#pragma unroll 1
+        for (int i = threadIdx.x & 63; i < SMOL_SLAB * PC; i += 64)
+            if (not_finite8(bload(rs, i * 16, (unsigned)(k0 / SMOL_SLAB) * ShGeom<HD>::SLAB_BYTES))) bad |= 1u << i / PC;
+#pragma unroll
+        for (int sh = 1; sh < 64; sh <<= 1) bad |= __shfl_xor(bad, sh);
+        const int lo = max(0, w.lo - k0), hi = min(SMOL_SLAB, it.ke - k0);
+        const unsigned seen = lo < hi ? (~0u >> (SMOL_SLAB - hi)) & (~0u << lo) : 0u;
+        if (bad & seen) w.l = __builtin_nanf("");
+    }
+}
+
 /* At most 16 rows, the same in every wave; the waves take the slabs in turn */
 template <int HD, bool SC>
 __device__ __forceinline__ void sh_narrow(const ShParams &p, const ShItem &it, char *smem) {
@@ -510,21 +544,23 @@ __device__ __forceinline__ void sh_narrow(const ShParams &p, const ShItem &it, c
     if (HD > 128) issue_v(k0);
     float *logits = SC && c < it.R
                         ? p.logits + ((long long)it.seq * p.Hq + it.g * p.G + it.row0 + c) * p.l_stride + 8 * j : nullptr;
+    unsigned odd = 0;
     while (k0 < it.ke) {
         f4 s[1][2];
         sh_qk<HD>(w, k, s[0]);
         const int k1 = k0 + SMOL_SLAB * SH_NW;
         issue_k(k1);
-        const bool nan = sh_mask<HD, 1, SC>(p, w, k0, it.ke, j, s, v, SC && logits ? logits + k0 : nullptr);
+        const bool nan = sh_mask<HD, 1, SC>(p, w, k0, it.ke, j, s, v, SC && logits ? logits + k0 : nullptr, odd);
         sh_pv<HD, 1>(w, s, v, nan);
         issue_v(k1);
         k0 = k1;
     }
+    sh_spoil<HD>(it, w, odd, it.kb + wave * SMOL_SLAB, SMOL_SLAB * SH_NW);
     float lt = row_sum4(w.l);
     if (add_new) {
         /* the new token: its fp32 score of every row (the three parts hold the row whole), its share of the state, its
          * bf16 row in the cache */
-        float sd = 0.0f;
+        float sd = 0.0f, z = 0.0f; /* z: zero, or NaN with an element of the key that is not finite */
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
             float kn[8];
@@ -533,9 +569,12 @@ __device__ __forceinline__ void sh_narrow(const ShParams &p, const ShItem &it, c
 #pragma unroll
             for (int q = 0; q < Q_PARTS; q++) asm volatile("" : "+v"(w.q[q][ks]));
 #pragma unroll
-            for (int i = 0; i < 8; i++) sd = fmaf(((float)w.q[0][ks][i] + (float)w.q[1][ks][i]) + (float)w.q[2][ks][i], kn[i], sd);
+            for (int i = 0; i < 8; i++) {
+                sd = fmaf(((float)w.q[0][ks][i] + (float)w.q[1][ks][i]) + (float)w.q[2][ks][i], kn[i], sd);
+                z = fmaf(kn[i], 0.0f, z);
+            }
         }
-        sd = row_sum4(sd);
+        sd = row_sum4(sd) + row_sum4(z);
         if (p.cap2 > 0.0f) sd = p.cap2 * tanhf(sd / p.cap2);
         if (SC && j == 0 && c < it.R) p.logit_new[(long long)it.seq * p.Hq + it.g * p.G + it.row0 + c] = sd;
         const float mm = fmaxf(w.m, sd), mu = mm == -INFINITY ? 0.0f : mm;
@@ -634,6 +673,7 @@ __device__ __forceinline__ void sh_wide(const ShParams &p, const ShItem &it, cha
     for (int i = 0; i < STAGES - 1; i++) fetch(i);
     const int kt_row = 8 * (c >> 2) + (c & 3), ksw = HD == 128 ? c : c >> 1;
     const int n_steps = (n + WS - 1) / WS;
+    unsigned odd = 0;
     for (int i = 0; i < n_steps; i++) {
         /* this wave's part of step i has landed (later ones may be on their way); then everybody's has, and nobody
          * still reads the stage that the next transfers overwrite */
@@ -663,10 +703,11 @@ __device__ __forceinline__ void sh_wide(const ShParams &p, const ShItem &it, cha
                 v[u][dt] = *reinterpret_cast<const uint4 *>(sk + (2 * u + 1) * Gm::SLAB_BYTES + (d * 4 + (j ^ (d >> 1 & 3))) * 16);
             }
         /* a slab past the last one repeats it; its keys are past ke */
-        const bool nan = sh_mask<HD, WS, false>(p, w, it.kb + i * WS * SMOL_SLAB, it.ke, j, s, v, nullptr);
+        const bool nan = sh_mask<HD, WS, false>(p, w, it.kb + i * WS * SMOL_SLAB, it.ke, j, s, v, nullptr, odd);
         sh_pv<HD, WS>(w, s, v, nan);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); /* no transfer outlives the workgroup */
+    sh_spoil<HD>(it, w, odd, it.kb, SMOL_SLAB);
     const float lt = row_sum4(w.l);
     const int r = 16 * wave + c;
     if (r < it.R) {
@@ -802,7 +843,9 @@ __global__ __launch_bounds__(256) void k_sh_merge(const ShParams p) {
             f4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < NG; k++) sum += *reinterpret_cast<const f4 *>(s_red + (k * GL + tid) * 4);
-            *reinterpret_cast<f4 *>(p.out + ((long long)i * p.Hq + head) * HD + tid * 4) = sum / L;
+            /* a value that is not finite reached its dimension: the whole row becomes NaN (its threads are one wave) */
+            const float z = ((sum[0] - sum[0]) + (sum[1] - sum[1])) + ((sum[2] - sum[2]) + (sum[3] - sum[3]));
+            *reinterpret_cast<f4 *>(p.out + ((long long)i * p.Hq + head) * HD + tid * 4) = sum / (__any(z != 0.0f) ? __builtin_nanf("") : L);
         }
         return;
     }
