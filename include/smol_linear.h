@@ -77,8 +77,9 @@ SMOL_ATTN_API int smol_adapters_destroy(smol_adapters *set);
  * ids: host array [seq]; rows of one adapter need not follow each other. The
  * products are fp32 sums of fp32 inputs (24 bits) and the exact bf16 weights,
  * except that the shared one of more than 64 rows is smol_linear_dev's (x to
- * 2^-16), and so is a call whose ids are all -1; a bf16 y is truncated once, from the whole sum. An fp32 row of x that
- * holds infinity may give NaN. A row's results do not depend on the other rows'
+ * 2^-16), and so is a call whose ids are all -1; a bf16 y is truncated once, from the whole sum. Infinities in x
+ * give what these products and sums give: an infinity where all terms agree, NaN where they do not or where one meets a zero
+ * weight (A x is such a term of each output, in fp32). A row's results do not depend on the other rows'
  * values. y (16-byte aligned) overlaps neither x nor W. Uses the context's
  * workspace. Under stream capture the call must have been made once before,
  * with at most 40 groups of up to 16 rows that share an adapter (or, for a bf16

@@ -111,12 +111,16 @@ __device__ __forceinline__ AdAt ad_at(const AdParams &p, int tile, int c) {
     return AdAt{t->adapter, t->n, t->rank, t->scale, t->row[c]};
 }
 
+/* x = p0 + p1 + p2 in bf16, each part what the parts before it leave, rounded to nearest: 24 bits. The first two are held to
+ * bf16's largest finite value: a finite x beyond it would round to infinity, and inf - inf is no number. An infinite x so goes
+ * into p2 whole, beside finite parts of its sign, and its products are infinities of the right sign. */
 __device__ __forceinline__ void ad_split3(const float *x, b8 &p0, b8 &p1, b8 &p2) {
+    constexpr float BF16_MAX = 3.3895313892515355e38f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const __bf16 a = (__bf16)x[i];
+        const __bf16 a = (__bf16)__builtin_amdgcn_fmed3f(x[i], -BF16_MAX, BF16_MAX);
         const float r = x[i] - (float)a;
-        const __bf16 b = (__bf16)r;
+        const __bf16 b = (__bf16)__builtin_amdgcn_fmed3f(r, -BF16_MAX, BF16_MAX);
         p0[i] = a;
         p1[i] = b;
         p2[i] = (__bf16)(r - (float)b);
@@ -219,7 +223,7 @@ __global__ __launch_bounds__(AD_TPB) void k_adapt_in(const AdParams p) {
 }
 
 /* scale t of row `row`, ranks [8 j', 8 j' + 8) of each 32-wide step, as bf16 parts: the chunks' partial sums, four at a
- * time in flight */
+ * time in flight. Ranks past the adapter's are zeros: an infinite x makes NaN of the padding's 0 x there */
 template <int KS>
 __device__ __forceinline__ void ad_t(const AdParams &p, long long row, int rank, float scale, bool live, int j, b8 (*tp)[3]) {
     const long long step = (long long)p.seq * p.ra;
@@ -250,7 +254,7 @@ __device__ __forceinline__ void ad_t(const AdParams &p, long long row, int rank,
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= scale;
+        for (int i = 0; i < 8; i++) v[i] = r + i < rank ? v[i] * scale : 0.0f;
         ad_split3(v, tp[ks][0], tp[ks][1], tp[ks][2]);
     }
 }
@@ -433,9 +437,9 @@ __global__ __launch_bounds__(64 * ONE_NW) void k_adapt_one(const AdParams p) {
                 const f4 x = *reinterpret_cast<const f4 *>(s_t + tl.row * TSTR + slot * 16 + r);
                 const f4 y = *reinterpret_cast<const f4 *>(s_t + tl.row * TSTR + slot * 16 + r + 4);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    v[i] = x[i] * tl.scale;
-                    v[4 + i] = y[i] * tl.scale;
+                for (int i = 0; i < 4; i++) { /* ranks past the adapter's: as in ad_t */
+                    v[i] = r + i < tl.rank ? x[i] * tl.scale : 0.0f;
+                    v[4 + i] = r + 4 + i < tl.rank ? y[i] * tl.scale : 0.0f;
                 }
             }
             b8 tp[3];
