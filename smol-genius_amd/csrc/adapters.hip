@@ -667,7 +667,7 @@ extern "C" int smol_linear_adapters_dev(smol_attn_ctx *ctx, void *y, int y_dtype
     if (!ctx) return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: null context");
     if ((x_dtype != SMOL_ATTN_F32 && x_dtype != SMOL_ATTN_BF16) || (y_dtype != SMOL_ATTN_F32 && y_dtype != SMOL_ATTN_BF16))
         return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: dtype");
-    if (!set || !ids) return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: null adapters or ids");
+    if (!set || (!ids && seq != 0)) return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: null adapters or ids");
     if (set->ctx != ctx) return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: adapters of another context");
     if (seq < 0 || in_dim != set->in_dim || out_dim != set->out_dim)
         return afail(SMOL_ATTN_ERR_ARG, "smol_linear_adapters_dev: sizes differ from the adapters'");
