@@ -80,7 +80,7 @@ SMOL_ATTN_API int smol_adapters_destroy(smol_adapters *set);
  * 2^-16), and so is a call whose ids are all -1; a bf16 y is truncated once, from the whole sum. Infinities in x
  * give what these products and sums give: an infinity where all terms agree, NaN where they do not or where one meets a zero
  * weight (A x is such a term of each output, in fp32). A row's results do not depend on the other rows'
- * values. y (16-byte aligned) overlaps neither x nor W. Uses the context's
+ * values, but the order of its sums follows the number of rows and how the ids share them out. y (16-byte aligned) overlaps neither x nor W. Uses the context's
  * workspace. Under stream capture the call must have been made once before,
  * with at most 40 groups of up to 16 rows that share an adapter (or, for a bf16
  * y of more than 64 rows, have none), or 400 of rows that also follow each

@@ -27,8 +27,8 @@
  * rows of 1024 -> 4096, fp32, rank 16: 4.6 + 7.6 us (W's 8.4 MB; the bf16 parts
  * of x, read again by every workgroup from L2, are 50 MB); 3 rows of 4096 ->
  * 4096: 4.6 + 11 us (33.6 MB of W at 3.0 TB/s). 1536 rows of 1024 -> 2048,
- * bf16, rank 32: 4.9 us, the library's product 20.5, k_adapt_out 8 us (26 MB,
- * 3.3 TB/s).
+ * bf16, rank 32: 4.9 us, the library's product 20.5, k_adapt_out 8.5 us (26 MB,
+ * 3.1 TB/s).
  */
 #include "attn_device.h"
 
@@ -55,8 +55,10 @@ constexpr int AD_TPB = 256, AD_NW = AD_TPB / 64;
 constexpr int AD_ARG_TILES = 40, AD_ARG_RUNS = 400;
 /* Rows that k_adapt_few takes. It keeps fp32 x at 24 bits and is two launches instead of three or four; against the library's
  * product and k_adapt_out (kernel time, fp32 x, rank 16): 1024 -> 4096 16 rows 10.6 us against 14.2, 32 rows 12.2 against 14.6,
- * 64 rows 15.5 against 16.2; 2048 -> 1024, where its workgroups are few, 64 rows 19.4 against 15.8. It re-reads x for every 16
- * outputs, so it only loses more beyond. */
+ * 64 rows 15.5 against 16.2; 2048 -> 1024, where its workgroups are few, 64 rows 19.4 against 15.8, which the 24 bits cost
+ * there. A bf16 x, a call of 64 rows here and one of 65 the other way: 1024 -> 1024 11.2 us and 15.2, 2048 -> 1024 12.7 and
+ * 15.6, 1024 -> 4096 11.3 and 15.7, 1024 -> 6144 15.0 and 16.2. It re-reads x for every 16 outputs, so it only loses more
+ * beyond. */
 constexpr int AD_FEW = 64;
 constexpr int AD_TIMING_KIND = 2;
 

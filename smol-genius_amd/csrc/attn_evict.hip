@@ -25,7 +25,7 @@
  * such piece per column, so rows far apart cost 32 times their bytes: 8192 rows
  * cut to 1024 read 1.8 MB of V^T a head for 0.2 MB of moved values.
  * Measured on an MI355X (head_dim 128, 8 kv heads): 16 sequences, 4160 rows cut
- * to 4096, 23.7 us in k_evict_select, 12 of them for the ranks; 32 sequences,
+ * to 4096, 26 us in k_evict_select, 12 of them for the ranks; 32 sequences,
  * 8192 cut to 1024, 18 us and 156 us in k_evict_move for 703 MB of traffic
  * (4.5 TB/s; a large copy reaches 4.7).
  */

@@ -30,10 +30,10 @@
  *     the other in a wave: three products for one (below).
  *
  * Measured on an MI355X (kernel time, head_dim 128, 16 heads over 8):
- * 4 sequences on 500 8.5 us and 16 on 4096 17.4 us (33 MB, 2.0 TB/s; the first
+ * 4 sequences on 500 8.8 us and 16 on 4096 18.1 us (36 MB, 2.0 TB/s; the first
  * load waits for the sequences' table, a row and its turn, 3 to 5 us, and a
- * wave has one to four slabs); 64 on 16384 59 us (212 MB, 3.7 TB/s, matrix cores busy 27%;
- * a wide item 0.85 us a slab). head_dim 256, 8 heads over 1, 24 on 8191: 24.6 us,
+ * wave has one to four slabs); 64 on 16384 60 us (212 MB, 3.7 TB/s, matrix cores busy 26%;
+ * a wide item 0.85 us a slab). head_dim 256, 8 heads over 1, 24 on 8191: 25.8 us,
  * one workgroup a compute unit, 2.6 us a wave's slab. Scored: 16 sequences of
  * 3000 to 4160 rows 56 us (244 MB, 4.4 TB/s). k_sh_merge 4 to 7 us, a launch's
  * and two round trips' time. Tried and not kept: a join by the last workgroup
@@ -917,7 +917,9 @@ static int launch_hd(const ShParams *p, int tile_rows, hipStream_t st, hipEvent_
 /* rows of a prefix item at head_dim hd, for a batch of `rows` rows a kv head: 64 for a wide item. Wide items read K and
  * V once for 64 rows where narrow ones do for 16 (64 sequences on 16384, head_dim 128, 128 rows a kv head: 71 us a call,
  * 93 with narrow ones; 32 rows on 4096: 20 either way). Not at 256, where a wave's state leaves one workgroup a compute
- * unit and its steps do not overlap (192 rows on 8191: 38 us, 31 narrow). */
+ * unit and its steps do not overlap (192 rows on 8191: 38 us, 31 narrow). 72, 80 and 96 have narrow items alone: the ring's
+ * layout wants rows of 8 or 16 pieces, and slabs that the waves' 1 KB transfers share out evenly (192 rows of 4 kv heads on
+ * 4096, a call: 20.8, 21.5 and 24.8 us narrow; 15.3 and 20.6 wide at 64 and 128). */
 extern "C" int smol_shared_tile_rows(int hd, int rows) { return rows <= 32 || (hd != 64 && hd != 128) ? 16 : 16 * SH_NW; }
 
 /* heads of an own-rows item */
