@@ -476,6 +476,13 @@ def _host_ints(a, n, what):
             return a, a.buffer_info()[0]
         shape = (len(a),)
     else:
+        a = np.asarray(a)
+        if a.dtype != np.int32 and a.size:
+            # as array.array does for a list; a cast alone would wrap or cut
+            if a.dtype.kind not in "biu":
+                raise TypeError("%s: whole numbers are wanted, got %s" % (what, a.dtype))
+            if a.max() > 2 ** 31 - 1 or a.min() < -2 ** 31:
+                raise OverflowError("%s: a number that no C int holds" % what)
         a = np.ascontiguousarray(a, np.int32)
         shape = a.shape
         if shape == (n,):
