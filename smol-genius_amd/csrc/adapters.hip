@@ -594,6 +594,9 @@ extern "C" int smol_adapters_create(smol_attn_ctx *ctx, int n, int in_dim, int o
     *out = nullptr;
     if (n <= 0 || in_dim <= 0 || out_dim <= 0 || !a || !b || !rank || !scale)
         return afail(SMOL_ATTN_ERR_ARG, "smol_adapters_create: sizes or null arrays");
+    /* what no call of one row could take; the padded sizes stay below 31 bits */
+    if (in_dim > INT_MAX / 4 || out_dim > INT_MAX / 4 || (long long)out_dim * in_dim > (1LL << 40))
+        return afail(SMOL_ATTN_ERR_UNSUPPORTED, "smol_adapters_create: sizes beyond the supported range");
     int max_rank = 0;
     for (int i = 0; i < n; i++) {
         if (rank[i] < 1 || rank[i] > AD_MAX_RANK) return afail(SMOL_ATTN_ERR_UNSUPPORTED, "smol_adapters_create: a rank outside 1 .. 128");
