@@ -66,6 +66,8 @@ extern "C" {
 #define SMOL_ATTN_ERR_RANGE (-6) /* a value left the fp16 staging's range (see Numerics) */
 #define SMOL_ATTN_ERR_TIMEOUT (-7) /* a decode split-K merge gave up waiting for its splits; the
                                     * rows it merges are NaN (reported by synchronize) */
+#define SMOL_ATTN_ERR_PAGE (-8)    /* a call on a paged cache met a page number, a length or a row range that is none
+                                    * (reported by synchronize) */
 
 /* element type of the Q / K / V inputs */
 #define SMOL_ATTN_F32 0
@@ -93,8 +95,9 @@ SMOL_ATTN_API int smol_attn_ctx_create(int device, void *stream, smol_attn_ctx *
 SMOL_ATTN_API int smol_attn_ctx_destroy(smol_attn_ctx *ctx);
 /* waits for the context's stream; returns SMOL_ATTN_ERR_TIMEOUT when a
  * decode merge since the last synchronize gave up waiting for its splits,
- * else SMOL_ATTN_ERR_RANGE when a call raised the range flag (both flags are
- * cleared) */
+ * else SMOL_ATTN_ERR_PAGE when a call on a paged cache met a number out of
+ * range, else SMOL_ATTN_ERR_RANGE when a call raised the range flag (the flags
+ * are cleared) */
 SMOL_ATTN_API int smol_attn_ctx_synchronize(smol_attn_ctx *ctx);
 SMOL_ATTN_API void *smol_attn_ctx_stream(smol_attn_ctx *ctx);
 
@@ -346,6 +349,96 @@ SMOL_ATTN_API int smol_attn_decode_scored(smol_attn_ctx *ctx, smol_kv_cache *kv,
 SMOL_ATTN_API int smol_kv_cache_evict(smol_kv_cache *kv, int layer, int n_seq, const int *slots, const int *rows,
                                       const int *ends, const float *mass, const int *row_pos, float *mass_out,
                                       int *pos_out, int stride, int keep, int first, int recent);
+
+/* ---- a KV cache in pages ------------------------------------------------------
+ * No counterparts in the reference. A slot of smol_kv_cache takes the rows of
+ * the longest sequence; a pool of pages takes what the sequences hold. A page
+ * has SMOL_PAGE_ROWS rows of every kv head of one layer. Which pages a sequence
+ * has, in order, says a table of the caller's: `table` [n_seq][stride], device
+ * ints, row r of sequence i being row r % SMOL_PAGE_ROWS of page
+ * table[i][r / SMOL_PAGE_ROWS]. The same numbers serve every layer. Entries for
+ * rows that a call neither reads nor writes are not looked at. Several sequences
+ * may read one page (a common prefix); a page that a call writes to belongs to
+ * one sequence of the call.
+ *
+ * Tables, lengths, positions and row ranges are device arrays, so a captured
+ * call replays with what they hold by then. The kernels check them: a page
+ * number outside the pool, a length past the table's or the RoPE table's end,
+ * a row range that is none are not followed; what they would give is NaN, what
+ * they would write is not written, and the next smol_attn_ctx_synchronize
+ * returns SMOL_ATTN_ERR_PAGE. Work is enqueued on the context's stream. A call
+ * grows the RoPE table to stride * SMOL_PAGE_ROWS positions (4194304 at most)
+ * and the context's workspace; under stream capture it may not
+ * (SMOL_ATTN_ERR_UNSUPPORTED: run the call once before), its replays are
+ * ordered with the context's other calls by the caller, and growth after the
+ * capture leaves the graph with freed memory. n_seq at most 65535, alignment 16
+ * bytes for rows, 4 for numbers.
+ *
+ * Types. SMOL_PAGES_BF16: rows rounded to nearest even. SMOL_PAGES_INT8: a row of
+ * a kv head, K's and V's each, is 8-bit codes times a scale of its own:
+ * s = amax / 127 with amax the row's largest magnitude, code = rint(x * (127 / amax))
+ * (nearest even), so an element is off by at most s / 2; a row with amax below
+ * 2^-90 is zeros, and one with a NaN or infinity gets a NaN for its scale: it
+ * stands for NaN. */
+#define SMOL_PAGE_ROWS 64
+#define SMOL_PAGES_BF16 1
+#define SMOL_PAGES_INT8 2
+typedef struct smol_kv_pages smol_kv_pages;
+
+/* a pool of n_pages pages for each of n_layers layers, zero-filled; it does not grow */
+SMOL_ATTN_API int smol_kv_pages_create(smol_attn_ctx *ctx, int n_layers, int n_pages, int n_kv_heads, int head_dim, int type,
+                                       smol_kv_pages **out);
+/* waits for the context's stream, then frees the pool (before its context) */
+SMOL_ATTN_API int smol_kv_pages_destroy(smol_kv_pages *pages);
+/* device addresses of one layer, for callers that copy, move or fill pages. With e = 16 (int8) or 8 (bf16) elements in 16 bytes:
+ *   *k       [n_pages][n_kv_heads][ceil(head_dim / e)][64][e], a row's last e padded with zeros
+ *   *v       int8 [n_pages][n_kv_heads][head_dim][64]: row 16 t + 4 g + i of the page at 16 g + 4 t + i;
+ *            bf16 [n_pages][n_kv_heads][2][head_dim][32]: row 32 h + 16 t + 4 g + i in half h at 8 g + 4 t + i
+ *   *scales  fp32 [n_pages][n_kv_heads][2][64], K's rows and V's (never negative); NULL for bf16
+ *   *bounds  bf16 [n_pages][n_kv_heads][2][head_dim]: the lowest and the highest stored value of K's rows, rounded outward;
+ *            smol_attn_decode_paged_top chooses by them. A call that writes a page's row 0 starts its bounds anew, any other
+ *            widens them, so rows that were written over may still count. */
+SMOL_ATTN_API int smol_kv_pages_pointers(const smol_kv_pages *pages, int layer, void **k, void **v, float **scales,
+                                         uint16_t **bounds);
+
+/* Writes rows of a ragged batch: rows starts[i] .. starts[i + 1] - 1 of k_new, v_new [rows][n_kv_heads * head_dim] (dtype
+ * SMOL_ATTN_F32 or _BF16) are positions pos[i], pos[i] + 1, .. of sequence i, K normalised (k_norm [head_dim], NULL: not) and
+ * rotated (rope NULL: not) in fp32 as smol_attn_decode_qknorm's. starts [n_seq + 1], pos [n_seq]: device ints, starts not
+ * falling; a sequence may have no rows. */
+SMOL_ATTN_API int smol_kv_pages_append(smol_kv_pages *pages, int layer, const smol_rope_table *rope, int n_seq, const int *table,
+                                       int stride, const int *starts, const int *pos, int rows, const void *k_new,
+                                       const void *v_new, int dtype, const float *k_norm, float eps);
+/* The values that rows stand for, into k_out, v_out [rows][n_kv_heads * head_dim] of dtype (bf16: nearest even); starts and pos
+ * as above. What a chunk of a prompt attends to with smol_attn_causal, for one use. Rows between the sequences' ranges are left
+ * as they were. */
+SMOL_ATTN_API int smol_kv_pages_read(smol_kv_pages *pages, int layer, int n_seq, const int *table, int stride, const int *starts,
+                                     const int *pos, int rows, void *k_out, void *v_out, int dtype);
+
+/* One decode step: sequence i has len[i] rows (device ints); its new token gets row and position len[i], for which its table
+ * has a page. out[i] is the attention of q[i] over its rows and the new token; norm, RoPE, window, cap and layouts as for
+ * smol_attn_decode_qknorm (NULL norm weights skip a norm). A negative len[i] is no sequence: nothing of it is read or written,
+ * out[i] stays (a batch padded to a captured size).
+ * The new token is used in fp32. bf16 pools: products as of smol_attn_decode_shared. int8 pools: Q and the weights as 24-bit
+ * whole numbers against their row's (their page's) largest, products with the codes exact, sums fp32; the 8 bits of the cache
+ * are all that is lost. A visible row that is not finite, be it in one element, makes NaN of all outputs of the heads that
+ * read it, and of no other; rows at or past a sequence's length are never used. A sequence's result does not depend on the
+ * pages that hold its rows; the order of its sums follows the batch's lengths. */
+SMOL_ATTN_API int smol_attn_decode_paged(smol_attn_ctx *ctx, smol_kv_pages *pages, int layer, const smol_rope_table *rope,
+                                         int n_seq, const int *table, int stride, const int *len, const void *q,
+                                         const void *k_new, const void *v_new, int dtype, int n_heads, float scale, int window,
+                                         float cap, const float *q_norm, const float *k_norm, float eps, float *out);
+/* The same over at most `top` pages of each sequence and kv head. Of the ceil(len / 64) pages that hold rows, the first `first`
+ * and the last `recent` (at least 1) stay; the others by the larger
+ *   sum over the heads h of the kv head and over d of max(scale q_h[d] lo[d], scale q_h[d] hi[d]),
+ * q normalised and rotated, lo and hi the page's bounds, all in 64 bits: no page whose rows all score lower than another's can
+ * be chosen before it on a single head. NaN counts above infinity, ties go to the lower page; first + recent <= top. chosen:
+ * device ints [n_seq][n_kv_heads][top], the chosen pages' places in the sequence (0 the first), ascending, -1 behind the
+ * last; NULL: not wanted. */
+SMOL_ATTN_API int smol_attn_decode_paged_top(smol_attn_ctx *ctx, smol_kv_pages *pages, int layer, const smol_rope_table *rope,
+                                             int n_seq, const int *table, int stride, const int *len, int top, int first,
+                                             int recent, const void *q, const void *k_new, const void *v_new, int dtype,
+                                             int n_heads, float scale, float cap, const float *q_norm, const float *k_norm,
+                                             float eps, int *chosen, float *out);
 
 /* Causal attention on flat device arrays, no cache and no RoPE: the device
  * form of smol_causal_attention (attention.c:153-170). K, V: [seq_k][n_kv*hd]. */

@@ -25,6 +25,7 @@
 #include <algorithm>
 #include <atomic>
 #include <mutex>
+#include <new>
 #include <numeric>
 #include <queue>
 #include <vector>
@@ -32,6 +33,7 @@
 #include "../../include/smol_attn.h"
 #include "../../include/smol_kernels_attn.h"
 #include "attn_internal.h"
+#include "paged_plan.h"
 
 extern "C" int smol_launch_prep(const PrepParams *pp, int n_blocks, hipStream_t st, hipEvent_t ev0, hipEvent_t ev1);
 extern "C" int smol_launch_decode(const DecParams *dp, int hd, int rows, int nw, hipStream_t st, hipEvent_t ev0,
@@ -54,6 +56,9 @@ extern "C" int smol_shared_mass_chunks(long long pairs, int max_len);
 extern "C" int smol_launch_shared(const ShParams *p, int hd, int tile_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
 extern "C" int smol_evict_fused(int max_moves);
 extern "C" int smol_launch_evict(const EvictParams *p, int max_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
+extern "C" int smol_paged_occupancy(int hd, int codes);
+extern "C" int smol_launch_paged(const PgParams *p, int hd, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
+extern "C" int smol_launch_pages(const PgRunParams *p, int hd, int write, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
 extern "C" int smol_launch_to_bf16_trunc(const float *x, uint16_t *y, long long n, hipStream_t st);
 extern "C" int smol_launch_bf16_norm_rope(uint16_t *x, const float *w, uint16_t *x2, const float *w2, int H2,
                                           float eps, const float *cos_t, const float *sin_t, int pos0, int seq, int H,
@@ -225,11 +230,12 @@ struct smol_attn_ctx {
     DevBuf work;   /* a call's own arrays: Q scratch, staged K and V, partials (WorkPlan) */
     DevBuf out32; /* fp32 result of a call whose output is bf16 */
     DevBuf dec_part; /* k_dec partial slots and flags */
-    /* flags, 256 bytes of pinned host memory that kernels write to (only when
+    /* flags, 384 bytes of pinned host memory that kernels write to (only when
      * there is something to report) and the host reads without a copy: word 0
      * is set when fp16 staging overflows, word 32 (its own 128-byte line) by
-     * a k_dec merger that gave up waiting for its splits; synchronize reads
-     * and clears both */
+     * a k_dec merger that gave up waiting for its splits, word 64 by a kernel
+     * of the paged cache that met a page number or a length that is none;
+     * synchronize reads and clears them */
     int *range_flag = nullptr;
     hipEvent_t mark = nullptr; /* smol_internal_mark */
     /* kernel arguments of k_dec and k_attn_win, built in place per context
@@ -447,10 +453,14 @@ static int take_flags(smol_attn_ctx *ctx) {
     int flag[SMOL_FLAG_WORDS] = {};
     flag[0] = f[0];
     flag[SMOL_FLAG_MERGE] = f[SMOL_FLAG_MERGE];
-    f[0] = f[SMOL_FLAG_MERGE] = 0;
+    flag[SMOL_FLAG_PAGE] = f[SMOL_FLAG_PAGE];
+    f[0] = f[SMOL_FLAG_MERGE] = f[SMOL_FLAG_PAGE] = 0;
     if (flag[SMOL_FLAG_MERGE])
         return fail(SMOL_ATTN_ERR_TIMEOUT, "a decode split-K merge gave up waiting for its splits (the affected "
                     "rows are NaN)");
+    if (flag[SMOL_FLAG_PAGE])
+        return fail(SMOL_ATTN_ERR_PAGE, "a page number, a length or a row range of a paged cache call was out of range (the "
+                    "affected outputs are NaN, the affected rows not written)");
     if (flag[0])
         return fail(SMOL_ATTN_ERR_RANGE, "a staged Q, K or V value was not finite or reached 65520 in magnitude "
                     "(fp16 staging of the prefill and bidirectional kernels)");
@@ -2218,6 +2228,233 @@ extern "C" int smol_kv_cache_pointers(const smol_kv_cache *kv, int layer, void *
     *k = kv->k + (size_t)layer * kv_layer_elems(kv);
     *vt = kv->vt + (size_t)layer * kv_layer_elems(kv);
     return SMOL_ATTN_OK;
+}
+
+/* ------------------------------------------------------- a cache in pages */
+
+struct smol_kv_pages {
+    smol_attn_ctx *ctx;
+    int device;
+    hipStream_t stream;
+    int n_layers, n_pages, n_kv, hd, type;
+    unsigned char *mem = nullptr;
+    size_t k_bytes, v_bytes, s_bytes, b_bytes; /* of one layer, each a multiple of 256 */
+    size_t layer_bytes() const { return k_bytes + v_bytes + s_bytes + b_bytes; }
+};
+
+extern "C" int smol_kv_pages_create(smol_attn_ctx *ctx, int n_layers, int n_pages, int n_kv, int hd, int type,
+                                    smol_kv_pages **out) {
+    if (!ctx || !out) return fail(SMOL_ATTN_ERR_ARG, "NULL argument");
+    *out = nullptr;
+    if (n_layers <= 0 || n_pages <= 0 || n_kv <= 0) return fail(SMOL_ATTN_ERR_ARG, "pool of %d layers, %d pages, %d heads", n_layers, n_pages, n_kv);
+    if (n_kv > 65535) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d kv heads", n_kv);
+    if (!hd_supported(hd)) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "head_dim %d", hd);
+    if (type != SMOL_PAGES_BF16 && type != SMOL_PAGES_INT8) return fail(SMOL_ATTN_ERR_ARG, "page type %d", type);
+    const bool codes = type == SMOL_PAGES_INT8;
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    const size_t at = (size_t)n_pages * n_kv;
+    smol_kv_pages proto{ctx, ctx->device, ctx->stream, n_layers, n_pages, n_kv, hd, type};
+    proto.k_bytes = up(at * ((codes ? (hd + 15) / 16 : hd / 8) * PG_ROWS * 16));
+    proto.v_bytes = up(at * PG_ROWS * hd * (codes ? 1 : 2));
+    proto.s_bytes = codes ? up(at * 2 * PG_ROWS * 4) : 0;
+    proto.b_bytes = up(at * 2 * hd * 2);
+    if (proto.layer_bytes() > ((size_t)1 << 46) / n_layers)
+        return fail(SMOL_ATTN_ERR_NOMEM, "pool of %d layers of %zu bytes", n_layers, proto.layer_bytes());
+    const int rc = set_device(ctx);
+    if (rc) return rc;
+    const size_t bytes = proto.layer_bytes() * n_layers;
+    void *mem = nullptr;
+    hipError_t e = hipMalloc(&mem, bytes);
+    if (e == hipSuccess) e = hipMemsetAsync(mem, 0, bytes, ctx->stream);
+    if (e != hipSuccess) {
+        if (mem) hipFree(mem);
+        hipGetLastError();
+        return fail(e == hipErrorOutOfMemory ? SMOL_ATTN_ERR_NOMEM : SMOL_ATTN_ERR_DEVICE, "kv pages (%zu bytes): %s", bytes,
+                    hipGetErrorString(e));
+    }
+    smol_kv_pages *kp = new (std::nothrow) smol_kv_pages(proto);
+    if (!kp) {
+        hipFree(mem);
+        return fail(SMOL_ATTN_ERR_NOMEM, "kv pages: no host memory");
+    }
+    kp->mem = (unsigned char *)mem;
+    *out = kp;
+    return SMOL_ATTN_OK;
+}
+
+extern "C" int smol_kv_pages_destroy(smol_kv_pages *kp) {
+    if (!kp) return SMOL_ATTN_OK;
+    hipSetDevice(kp->device);
+    hipStreamSynchronize(kp->stream);
+    hipFree(kp->mem);
+    delete kp;
+    return SMOL_ATTN_OK;
+}
+
+extern "C" int smol_kv_pages_pointers(const smol_kv_pages *kp, int layer, void **k, void **v, float **scales, uint16_t **bounds) {
+    if (!kp || !k || !v || !scales || !bounds) return fail(SMOL_ATTN_ERR_ARG, "NULL argument");
+    if (layer < 0 || layer >= kp->n_layers) return fail(SMOL_ATTN_ERR_ARG, "layer %d out of range", layer);
+    unsigned char *m = kp->mem + kp->layer_bytes() * layer;
+    *k = m;
+    *v = m + kp->k_bytes;
+    *scales = kp->s_bytes ? (float *)(m + kp->k_bytes + kp->v_bytes) : nullptr;
+    *bounds = (uint16_t *)(m + kp->k_bytes + kp->v_bytes + kp->s_bytes);
+    return SMOL_ATTN_OK;
+}
+
+constexpr long long PG_MAX_BLOCKS = (1 << 24) - 1; /* a grid's threads along one axis: below 2^32 */
+
+/* what all calls on a pool check and hand to the kernels; the table of positions grows to what the page table can hold */
+static int paged_pool(smol_kv_pages *kp, int layer, const smol_rope_table *rope, int n_seq, const int *table, int stride, PgPool &pp) {
+    if (!kp) return fail(SMOL_ATTN_ERR_ARG, "pool is NULL");
+    smol_attn_ctx *ctx = kp->ctx;
+    if (layer < 0 || layer >= kp->n_layers) return fail(SMOL_ATTN_ERR_ARG, "layer %d out of range", layer);
+    if (n_seq <= 0 || n_seq > 65535 || !table || stride <= 0 || stride > INT_MAX / (2 * PG_ROWS))
+        return fail(SMOL_ATTN_ERR_ARG, "bad batch: %d sequences, page table rows of %d", n_seq, stride);
+    if ((uintptr_t)table & 3) return fail(SMOL_ATTN_ERR_ARG, "page table must be 4-byte aligned");
+    memset(&pp, 0, sizeof pp);
+    pp.positions = INT_MAX;
+    pp.rope_kind = SMOL_ROPE_OFF;
+    int rc;
+    if (rope) {
+        if (rope->ctx != ctx) return fail(SMOL_ATTN_ERR_ARG, "rope table belongs to another context");
+        if (rope->hd != kp->hd) return fail(SMOL_ATTN_ERR_ARG, "rope table head_dim %d != %d", rope->hd, kp->hd);
+        const int need = (int)std::min<long long>((long long)stride * PG_ROWS, ROPE_GROW_MAX);
+        if ((rc = check_capture(ctx, "RoPE table growth", need > rope->cap))) return rc;
+        if ((rc = smol_rope_table_ensure(const_cast<smol_rope_table *>(rope), need))) return rc;
+        pp.rope_cos = rope->cos_d;
+        pp.rope_sin = rope->sin_d;
+        pp.rope_kind = rope->type == SMOL_ROPE_INTERLEAVED ? SMOL_ROPE_INTERLEAVED_K : SMOL_ROPE_NEOX_K;
+        pp.positions = rope->cap;
+    }
+    if ((rc = set_device(ctx))) return rc;
+    void *k, *v;
+    smol_kv_pages_pointers(kp, layer, &k, &v, &pp.scales, &pp.bounds);
+    pp.k = (unsigned char *)k;
+    pp.v = (unsigned char *)v;
+    pp.n_pages = kp->n_pages;
+    pp.Hkv = kp->n_kv;
+    pp.codes = kp->type == SMOL_PAGES_INT8;
+    pp.table = table;
+    pp.stride = stride;
+    pp.n_seq = n_seq;
+    pp.flag = ctx->range_flag + SMOL_FLAG_PAGE;
+    return 0;
+}
+
+static int paged_run(smol_kv_pages *kp, int layer, const smol_rope_table *rope, int n_seq, const int *table, int stride, const int *starts,
+                     const int *pos, int rows, int dtype, const void *a, const void *b, bool write, PgRunParams &rp) {
+    if (!kp) return fail(SMOL_ATTN_ERR_ARG, "pool is NULL");
+    if (dtype != SMOL_ATTN_F32 && dtype != SMOL_ATTN_BF16) return fail(SMOL_ATTN_ERR_ARG, "dtype %d", dtype);
+    if (!starts || !pos || rows < 0) return fail(SMOL_ATTN_ERR_ARG, "bad batch of %d rows", rows);
+    if (((uintptr_t)starts | (uintptr_t)pos) & 3) return fail(SMOL_ATTN_ERR_ARG, "starts and pos must be 4-byte aligned");
+    if (rows > 0 && (!a || !b)) return fail(SMOL_ATTN_ERR_ARG, "NULL tensor");
+    if (pg_max_run_pages(n_seq, rows) > PG_MAX_BLOCKS) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d rows", rows);
+    int rc;
+    if ((rc = check_aligned(a, b))) return rc;
+    if ((rc = paged_pool(kp, layer, rope, n_seq, table, stride, rp.p))) return rc;
+    if (rows == 0) return SMOL_ATTN_OK;
+    rp.starts = starts;
+    rp.pos = pos;
+    rp.rows = rows;
+    rp.dtype = dtype;
+    const int mk = timing_begin(kp->ctx, 2);
+    rc = smol_launch_pages(&rp, kp->hd, write, kp->ctx->stream, mark_a(kp->ctx, mk), mark_b(kp->ctx, mk));
+    if (rc) return fail(SMOL_ATTN_ERR_DEVICE, "paged rows (hd %d): %s", kp->hd, hipGetErrorString(hipGetLastError()));
+    return SMOL_ATTN_OK;
+}
+
+extern "C" int smol_kv_pages_append(smol_kv_pages *kp, int layer, const smol_rope_table *rope, int n_seq, const int *table, int stride,
+                                    const int *starts, const int *pos, int rows, const void *k_new, const void *v_new, int dtype,
+                                    const float *k_norm, float eps) {
+    PgRunParams rp = {};
+    const int rc = check_norm(nullptr, k_norm, eps, 1);
+    if (rc) return rc;
+    rp.k_in = k_new;
+    rp.v_in = v_new;
+    rp.k_norm = k_norm;
+    rp.norm_eps = eps;
+    return paged_run(kp, layer, rope, n_seq, table, stride, starts, pos, rows, dtype, k_new, v_new, true, rp);
+}
+
+extern "C" int smol_kv_pages_read(smol_kv_pages *kp, int layer, int n_seq, const int *table, int stride, const int *starts,
+                                  const int *pos, int rows, void *k_out, void *v_out, int dtype) {
+    PgRunParams rp = {};
+    rp.k_out = k_out;
+    rp.v_out = v_out;
+    if (kp && rows > 0 && k_out && v_out) {
+        const size_t bytes = (size_t)rows * kp->n_kv * kp->hd * (dtype == SMOL_ATTN_BF16 ? 2 : 4);
+        if ((const char *)k_out < (const char *)v_out + bytes && (const char *)v_out < (const char *)k_out + bytes)
+            return fail(SMOL_ATTN_ERR_ARG, "k_out and v_out overlap");
+    }
+    return paged_run(kp, layer, nullptr, n_seq, table, stride, starts, pos, rows, dtype, k_out, v_out, false, rp);
+}
+
+static int decode_paged(smol_attn_ctx *ctx, smol_kv_pages *kp, int layer, const smol_rope_table *rope, int n_seq, const int *table,
+                        int stride, const int *len, int top, int first, int recent, const void *q, const void *k_new, const void *v_new,
+                        int dtype, int n_heads, float scale, int window, float cap, const float *q_norm, const float *k_norm, float eps,
+                        int *chosen, float *out) {
+    static_assert(sizeof(PgParams) <= 1024, "kernel arguments");
+    if (!kp) return fail(SMOL_ATTN_ERR_ARG, "pool is NULL");
+    int rc = check_common(ctx, dtype, n_heads, kp->n_kv, kp->hd, q, out);
+    if (rc) return rc;
+    if ((rc = check_norm(q_norm, k_norm, eps, 1))) return rc;
+    if (kp->ctx != ctx) return fail(SMOL_ATTN_ERR_ARG, "pool belongs to another context");
+    if (!len || !k_new || !v_new) return fail(SMOL_ATTN_ERR_ARG, "NULL tensor");
+    if (((uintptr_t)len | (uintptr_t)chosen) & 3) return fail(SMOL_ATTN_ERR_ARG, "len and chosen must be 4-byte aligned");
+    if ((rc = check_aligned(k_new, v_new))) return rc;
+    PgParams pg = {};
+    if ((rc = paged_pool(kp, layer, rope, n_seq, table, stride, pg.p))) return rc;
+    const int Hkv = kp->n_kv, G = n_heads / Hkv, hd = kp->hd;
+    pg.len = len;
+    pg.q_in = q; pg.k_in = k_new; pg.v_in = v_new; pg.in_dtype = dtype;
+    pg.q_norm = q_norm; pg.k_norm = k_norm; pg.norm_eps = eps;
+    pg.qscale = (float)(scale * LOG2E_D);
+    pg.scale = scale;
+    pg.out = out; pg.Hq = n_heads; pg.G = G;
+    pg.window = window;
+    pg.cap2 = cap > 0.0f ? (float)(cap * LOG2E_D) : 0.0f;
+    pg.tiles = (G + 15) / 16;
+    pg.top = top; pg.first = first; pg.recent = recent;
+    if (top > 0 && (long long)n_seq * ((stride + 63) / 64) > PG_MAX_BLOCKS)
+        return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d sequences, page table rows of %d", n_seq, stride);
+    if (pg.tiles > 65535) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d heads a kv head", G);
+    pg.slots = std::max(1, ctx->cu_count * smol_paged_occupancy(hd, pg.p.codes) / (Hkv * pg.tiles));
+    const long long items = pg_max_chunks(n_seq, pg.slots);
+    pg.max_items = (int)items;
+    WorkPlan wk;
+    const size_t o_o = wk.take((size_t)items * n_heads * hd * 4), o_ml = wk.take((size_t)items * n_heads * 8);
+    const size_t o_list = wk.take(top > 0 && !chosen ? (size_t)n_seq * Hkv * top * 4 : 0);
+    const size_t o_score = wk.take(top > 0 ? (size_t)n_seq * Hkv * stride * 8 : 0);
+    if ((rc = check_capture(ctx, "workspace growth", wk.bytes > ctx->work.cap))) return rc;
+    if ((rc = dev_reserve(ctx->work, wk.bytes, ctx->stream))) return rc;
+    unsigned char *w = (unsigned char *)ctx->work.p;
+    pg.part_o = (float *)(w + o_o);
+    pg.part_ml = (float *)(w + o_ml);
+    pg.list = chosen ? chosen : (int *)(w + o_list);
+    pg.score = (double *)(w + o_score);
+    const int mk = timing_begin(ctx, 1);
+    rc = smol_launch_paged(&pg, hd, ctx->stream, mark_a(ctx, mk), mark_b(ctx, mk));
+    if (rc) return fail(SMOL_ATTN_ERR_DEVICE, "paged decode (hd %d): %s", hd, hipGetErrorString(hipGetLastError()));
+    return SMOL_ATTN_OK;
+}
+
+extern "C" int smol_attn_decode_paged(smol_attn_ctx *ctx, smol_kv_pages *kp, int layer, const smol_rope_table *rope, int n_seq,
+                                      const int *table, int stride, const int *len, const void *q, const void *k_new,
+                                      const void *v_new, int dtype, int n_heads, float scale, int window, float cap,
+                                      const float *q_norm, const float *k_norm, float eps, float *out) {
+    return decode_paged(ctx, kp, layer, rope, n_seq, table, stride, len, 0, 0, 0, q, k_new, v_new, dtype, n_heads, scale, window, cap,
+                        q_norm, k_norm, eps, nullptr, out);
+}
+
+extern "C" int smol_attn_decode_paged_top(smol_attn_ctx *ctx, smol_kv_pages *kp, int layer, const smol_rope_table *rope, int n_seq,
+                                          const int *table, int stride, const int *len, int top, int first, int recent,
+                                          const void *q, const void *k_new, const void *v_new, int dtype, int n_heads, float scale,
+                                          float cap, const float *q_norm, const float *k_norm, float eps, int *chosen, float *out) {
+    if (top <= 0 || first < 0 || recent < 1 || first > top - recent || top > INT_MAX / (2 * PG_ROWS))
+        return fail(SMOL_ATTN_ERR_ARG, "%d pages, the first %d and the last %d among them", top, first, recent);
+    return decode_paged(ctx, kp, layer, rope, n_seq, table, stride, len, top, first, recent, q, k_new, v_new, dtype, n_heads, scale, 0,
+                        cap, q_norm, k_norm, eps, chosen, out);
 }
 
 extern "C" int smol_attn_causal(smol_attn_ctx *ctx, const void *q, const void *k, const void *v,

@@ -214,8 +214,9 @@ typedef struct {
 #define DEC_ARG_ITEMS 320     /* workgroup items passed in the kernel arguments */
 #define DEC_SPIN_LIMIT (1 << 22) /* flag polls before a merger gives up (writes NaN rows and raises
                                     the context's merge flag) */
-#define SMOL_FLAG_WORDS 64       /* ints of a context's flags (256 bytes of pinned host memory) */
+#define SMOL_FLAG_WORDS 96       /* ints of a context's flags (384 bytes of pinned host memory) */
 #define SMOL_FLAG_MERGE 32       /* word of the merge flag: its own 128-byte line */
+#define SMOL_FLAG_PAGE 64        /* word of the page flag, likewise */
 
 /* one workgroup of the grid (index = blockIdx.x); seq < 0: nothing to do.
  * A group's rows are cut into row blocks of at most DEC_RB(hd) rows; each
@@ -324,6 +325,53 @@ typedef struct {
     const ShSeq *seqs_dev;     /* (slot, rows, end) of each sequence when n_seq > SH_ARG_SEQS */
     ShSeq seqs[SH_ARG_SEQS];
 } EvictParams;
+
+/* ---- paged.hip: a cache in pages ----
+ * One layer of a pool, for page p and kv head g (sizes in bytes: e = 16 codes or 8 bf16 values are 16 bytes):
+ *   K       [page][kv][ceil(hd / e)][64][16]  16-byte pieces of the rows, a row's last one padded with zeros: one
+ *                                             load of a wave takes four pieces of 16 rows, 256 contiguous bytes each
+ *   V       codes [page][kv][hd][64], bf16 [page][kv][2][hd][32]: rows along the line in the order of pg_order
+ *   scales  fp32 [page][kv][2][64], K's and V's rows (codes)
+ *   bounds  bf16 [page][kv][2][hd], lows and highs of K's rows */
+typedef struct {
+    unsigned char *k, *v; float *scales; uint16_t *bounds;
+    int n_pages, Hkv, codes;
+    const int *table; int stride;     /* [n_seq][stride] page numbers */
+    int n_seq;
+    const float *rope_cos; const float *rope_sin; int rope_kind;
+    int positions;                    /* rows of the RoPE table (INT_MAX without one) */
+    int *flag;                        /* set to 1 where a page number or a length is none */
+} PgPool;
+
+/* k_pg_append, k_pg_read: rows [starts[i], starts[i + 1]) of a ragged batch are positions pos[i] .. of sequence i */
+typedef struct {
+    PgPool p;
+    const int *starts; const int *pos;
+    int rows;
+    const void *k_in; const void *v_in; int dtype;
+    const float *k_norm; float norm_eps;
+    void *k_out; void *v_out;
+} PgRunParams;
+
+/* k_pg, k_pg_merge, k_pg_score, k_pg_select: a decode step */
+typedef struct {
+    PgPool p;
+    const int *len;                   /* [n_seq] cached rows; the new token becomes row len */
+    const void *q_in; const void *k_in; const void *v_in; int in_dtype;
+    const float *q_norm; const float *k_norm; float norm_eps;
+    float qscale;                     /* scale * log2 e */
+    double scale;
+    float *out; int Hq, G;
+    int window; float cap2;           /* window > 0: positions > len - window; cap2 > 0: softcap in log2 units */
+    int slots;                        /* whole chunks at most (pg_chunk) */
+    int max_items;                    /* workgroups a kv head and tile of heads */
+    int tiles;                        /* tiles of 16 heads of a kv head */
+    float *part_o; float *part_ml;    /* [kv][max_items][G]: outputs [hd], (m, l) */
+    /* top > 0: at most that many pages of each (sequence, kv head), which `list` names in ascending order */
+    int top, first, recent;
+    int *list;                        /* [n_seq][kv][top], -1 behind the last */
+    double *score;                    /* [n_seq][kv][stride] */
+} PgParams;
 
 /* ---- k_gemm (gemm.hip), k_gemm_rs (gemm_rs.hip) and k_gemm_sw (gemm_sw.hip): the projections on bf16 MFMA ---- */
 #define GEMM_CFGS 8 /* their tile configurations (smol_gemm_tile) */

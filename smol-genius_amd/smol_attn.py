@@ -24,6 +24,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SMOL_ATTN_LIB") or os.path.join(HERE, "libsmol_attn.so")
 
 F32, BF16 = 0, 1
+INT8 = 2  # SMOL_PAGES_INT8, beside BF16 for the pages of a pool
+PAGE_ROWS = 64  # SMOL_PAGE_ROWS
 ROPE_NONE, ROPE_NEOX, ROPE_INTERLEAVED = -1, 0, 1
 
 _c_int, _c_float, _vp = ctypes.c_int, ctypes.c_float, ctypes.c_void_p
@@ -80,6 +82,17 @@ SIGNATURES = [
     ("smol_kv_cache_evict", [_vp, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int],
      _c_int),
     ("smol_kv_cache_pointers", [_vp, _c_int, ctypes.POINTER(_vp), ctypes.POINTER(_vp)], _c_int),
+    # a KV cache in pages
+    ("smol_kv_pages_create", [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.POINTER(_vp)], _c_int),
+    ("smol_kv_pages_destroy", [_vp], _c_int),
+    ("smol_kv_pages_pointers", [_vp, _c_int, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_vp)],
+     _c_int),
+    ("smol_kv_pages_append", [_vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _c_int, _vp, _vp, _c_int, _vp, _c_float], _c_int),
+    ("smol_kv_pages_read", [_vp, _c_int, _c_int, _vp, _c_int, _vp, _vp, _c_int, _vp, _vp, _c_int], _c_int),
+    ("smol_attn_decode_paged", [_vp, _vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_float, _c_int,
+                                _c_float, _vp, _vp, _c_float, _vp], _c_int),
+    ("smol_attn_decode_paged_top", [_vp, _vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp,
+                                    _c_int, _c_int, _c_float, _c_float, _vp, _vp, _c_float, _vp, _vp], _c_int),
     ("smol_attn_apply_rope", [_vp, _vp, _vp, _IP, _c_int, _c_int], _c_int),
     ("smol_attn_norm_rope", [_vp, _vp, _vp, _vp, _c_float, _IP, _c_int, _c_int, _c_int], _c_int),
     ("smol_attn_norm_rope_bf16", [_vp, _vp, _vp, _vp, _c_float, _c_int, _c_int, _c_int, _c_int], _c_int),
@@ -162,8 +175,14 @@ class SmolAttnTimeoutError(SmolAttnError):
     splits since the last synchronize; the rows it merged are NaN."""
 
 
+class SmolAttnPageError(SmolAttnError):
+    """SMOL_ATTN_ERR_PAGE: a call on a paged cache since the last synchronize
+    met a page number, a length or a row range that is none."""
+
+
 ERR_RANGE = -6  # SMOL_ATTN_ERR_RANGE
 ERR_TIMEOUT = -7  # SMOL_ATTN_ERR_TIMEOUT
+ERR_PAGE = -8  # SMOL_ATTN_ERR_PAGE
 
 
 def load(path=LIB_PATH):
@@ -193,7 +212,7 @@ def load(path=LIB_PATH):
 
 def _check(rc, what):
     if rc != 0:
-        cls = {ERR_RANGE: SmolAttnRangeError, ERR_TIMEOUT: SmolAttnTimeoutError}.get(rc, SmolAttnError)
+        cls = {ERR_RANGE: SmolAttnRangeError, ERR_TIMEOUT: SmolAttnTimeoutError, ERR_PAGE: SmolAttnPageError}.get(rc, SmolAttnError)
         raise cls("%s failed (%d): %s" % (what, rc, load().smol_attn_last_error().decode()))
 
 
@@ -304,11 +323,11 @@ def rope_fill_host(pos0, n_pos, head_dim, theta, rope_type=ROPE_NEOX):
 
 
 class _DeviceMemory:
-    """16-bit device memory of a handle, in the form that torch.as_tensor takes"""
+    """Device memory of a handle, in the form that torch.as_tensor takes"""
 
-    def __init__(self, owner, ptr, shape):
+    def __init__(self, owner, ptr, shape, typestr="<i2"):
         self.owner = owner
-        self.__cuda_array_interface__ = dict(shape=shape, typestr="<i2", data=(ptr, False), version=2)
+        self.__cuda_array_interface__ = dict(shape=shape, typestr=typestr, data=(ptr, False), version=2)
 
 
 class KVCache:
@@ -566,6 +585,130 @@ def kv_evict(kv, layer, slots, rows, ends, mass, row_pos, keep, first=0, recent=
     if rc:
         _check(rc, "smol_kv_cache_evict")
     return mass_out, pos_out
+
+
+class KVPages:
+    """A pool of pages of PAGE_ROWS rows (smol_kv_pages): BF16 rows or INT8 codes with a scale a row and kv head."""
+
+    def __init__(self, ctx, n_layers, n_pages, n_kv_heads, head_dim, page_type=BF16):
+        self.ctx = ctx
+        self.h = ctypes.c_void_p()
+        _check(load().smol_kv_pages_create(ctx.h, n_layers, n_pages, n_kv_heads, head_dim, page_type, ctypes.byref(self.h)),
+               "smol_kv_pages_create")
+        self.n_layers, self.n_pages, self.n_kv_heads, self.head_dim, self.page_type = n_layers, n_pages, n_kv_heads, head_dim, page_type
+        _live.add(self)
+
+    def views(self, layer):
+        """One layer as torch views of the pool's own memory: K [pages, kv_heads, ceil(head_dim / e), 64, e] with e = 16 (int8)
+        or 8 (bfloat16), V int8 [pages, kv_heads, head_dim, 64] or bfloat16 [pages, kv_heads, 2, head_dim, 32], scales float32
+        [pages, kv_heads, 2, 64] (None for BF16) and bounds bfloat16 [pages, kv_heads, 2, head_dim]; the order of rows along V's
+        lines is smol_kv_pages_pointers'. Work on them is ordered with the context's stream by the caller."""
+        import torch
+        k, v, s, b = _vp(), _vp(), _vp(), _vp()
+        _check(load().smol_kv_pages_pointers(self.h, layer, ctypes.byref(k), ctypes.byref(v), ctypes.byref(s), ctypes.byref(b)),
+               "smol_kv_pages_pointers")
+        np_, nk, hd, codes = self.n_pages, self.n_kv_heads, self.head_dim, self.page_type == INT8
+        e = 16 if codes else 8
+
+        def view(p, shape, typestr):
+            t = torch.as_tensor(_DeviceMemory(self, p.value, shape, typestr), device="cuda:%d" % self.ctx.device)
+            return t.view(torch.bfloat16) if typestr == "<i2" else t
+        row = "|i1" if codes else "<i2"
+        return (view(k, (np_, nk, -(-hd // e), PAGE_ROWS, e), row),
+                view(v, (np_, nk, hd, PAGE_ROWS) if codes else (np_, nk, 2, hd, PAGE_ROWS // 2), row),
+                view(s, (np_, nk, 2, PAGE_ROWS), "<f4") if codes else None, view(b, (np_, nk, 2, hd), "<i2"))
+
+    def close(self):
+        if self.h:
+            load().smol_kv_pages_destroy(self.h)
+            self.h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _page_table(ctx, table):
+    import torch
+    if table.dim() != 2:
+        raise SmolAttnError("table must be [sequences, pages]")
+    n, stride = table.shape
+    return n, stride, _on(ctx, table, torch.int32, (n, stride), "table")
+
+
+def pages_append(pages, layer, rope, table, starts, pos, k_new, v_new, k_norm=None, eps=1e-6):
+    """Writes rows starts[i] .. starts[i + 1] - 1 of k_new and v_new [rows, kv_heads*hd] to the positions pos[i] .. of sequence i;
+    see smol_kv_pages_append. table [n, stride], starts [n + 1], pos [n]: device int32."""
+    import torch
+    ctx, hd = pages.ctx, pages.head_dim
+    n, stride, tp = _page_table(ctx, table)
+    dtype, rows = k_new.dtype, k_new.shape[0]
+    dt = F32 if dtype is torch.float32 else BF16 if dtype is torch.bfloat16 else _dtype_code(k_new)
+    shape = (rows, pages.n_kv_heads * hd)
+    rc = load().smol_kv_pages_append(pages.h, layer, rope.h if rope else None, n, tp, stride,
+                                     _on(ctx, starts, torch.int32, (n + 1,), "starts"), _on(ctx, pos, torch.int32, (n,), "pos"),
+                                     rows, _on(ctx, k_new, dtype, shape, "k_new"), _on(ctx, v_new, dtype, shape, "v_new"), dt,
+                                     None if k_norm is None else _on(ctx, k_norm, torch.float32, (hd,), "k_norm"), eps)
+    if rc:
+        _check(rc, "smol_kv_pages_append")
+
+
+def pages_read(pages, layer, table, starts, pos, rows, dtype=None, k_out=None, v_out=None):
+    """The values of the rows at positions pos[i] .. of the sequences, starts[i + 1] - starts[i] of each, as k, v
+    [rows, kv_heads*hd] of dtype (float32 or bfloat16, the default); see smol_kv_pages_read."""
+    import torch
+    ctx = pages.ctx
+    n, stride, tp = _page_table(ctx, table)
+    if dtype is None:
+        dtype = torch.bfloat16 if k_out is None else k_out.dtype
+    shape = (rows, pages.n_kv_heads * pages.head_dim)
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=dtype, device=table.device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=dtype, device=table.device)
+    dt = F32 if dtype is torch.float32 else BF16 if dtype is torch.bfloat16 else _dtype_code(k_out)
+    rc = load().smol_kv_pages_read(pages.h, layer, n, tp, stride, _on(ctx, starts, torch.int32, (n + 1,), "starts"),
+                                   _on(ctx, pos, torch.int32, (n,), "pos"), rows, _on(ctx, k_out, dtype, shape, "k_out"),
+                                   _on(ctx, v_out, dtype, shape, "v_out"), dt)
+    if rc:
+        _check(rc, "smol_kv_pages_read")
+    return k_out, v_out
+
+
+def decode_paged(ctx, pages, layer, rope, table, lens, q, k_new, v_new, n_heads, scale, window=0, cap=0.0, out=None, q_norm=None,
+                 k_norm=None, eps=1e-6):
+    """One decode step over a paged cache: lens (device int32 [n]) rows of each sequence before the step, -1 for no sequence; see
+    smol_attn_decode_paged. Returns out [n, n_heads*hd]."""
+    import torch
+    n, qp, kp, vp, dt, qw, kw, out, op = _step_args(ctx, pages, q, k_new, v_new, n_heads, q_norm, k_norm, out)
+    stride = table.shape[1]
+    rc = load().smol_attn_decode_paged(ctx.h, pages.h, layer, rope.h if rope else None, n,
+                                       _on(ctx, table, torch.int32, (n, stride), "table"), stride,
+                                       _on(ctx, lens, torch.int32, (n,), "lens"), qp, kp, vp, dt, n_heads, scale, window, cap, qw,
+                                       kw, eps, op)
+    if rc:
+        _check(rc, "smol_attn_decode_paged")
+    return out
+
+
+def decode_paged_top(ctx, pages, layer, rope, table, lens, q, k_new, v_new, n_heads, scale, top, first=1, recent=1, cap=0.0,
+                     out=None, chosen=None, q_norm=None, k_norm=None, eps=1e-6):
+    """decode_paged over the `top` pages of each sequence and kv head whose bounds promise the largest scores, the first and the
+    recent ones among them; see smol_attn_decode_paged_top. Returns out and chosen (int32 [n, kv_heads, top])."""
+    import torch
+    n, qp, kp, vp, dt, qw, kw, out, op = _step_args(ctx, pages, q, k_new, v_new, n_heads, q_norm, k_norm, out)
+    stride, shape = table.shape[1], (n, pages.n_kv_heads, top)
+    if chosen is None:
+        chosen = torch.empty(shape, dtype=torch.int32, device=q.device)
+    rc = load().smol_attn_decode_paged_top(ctx.h, pages.h, layer, rope.h if rope else None, n,
+                                           _on(ctx, table, torch.int32, (n, stride), "table"), stride,
+                                           _on(ctx, lens, torch.int32, (n,), "lens"), top, first, recent, qp, kp, vp, dt, n_heads,
+                                           scale, cap, qw, kw, eps, _on(ctx, chosen, torch.int32, shape, "chosen"), op)
+    if rc:
+        _check(rc, "smol_attn_decode_paged_top")
+    return out, chosen
 
 
 def causal(ctx, q, k, v, seq_q, seq_k, n_heads, n_kv_heads, head_dim, scale, q_offset, window=0, cap=0.0,
