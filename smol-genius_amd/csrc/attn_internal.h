@@ -351,6 +351,7 @@ typedef struct {
     const void *k_in; const void *v_in; int dtype;
     const float *k_norm; float norm_eps;
     void *k_out; void *v_out;
+    int heads;                        /* kv heads of a workgroup */
 } PgRunParams;
 
 /* k_pg, k_pg_merge, k_pg_score, k_pg_select: a decode step */

@@ -154,10 +154,18 @@ __device__ __forceinline__ PgScale pg_scale(unsigned amax_bits) {
     if (a < PG_TINY) return {0.0f, 0.0f};
     return {a / 127.0f, 127.0f / a};
 }
-__device__ __forceinline__ int pg_code(float x, float inv) {
-    /* inv 0 with an infinite x is no number: 0, its scale tells */
-    const float y = rintf(x * inv);
-    return y == y ? (int)fminf(fmaxf(y, -127.0f), 127.0f) : 0;
+/* x inv, at most 127 in magnitude, plus 1.5 2^23: rounded to a whole number, whose two's complement is the low byte; what is no number
+ * (inv 0 with an infinite x) leaves a zero there, and the row's scale tells */
+#define PG_MAGIC 12582912.0f
+__device__ __forceinline__ float pg_code(float x, float inv) {
+#pragma clang fp contract(off) /* the fp32 product is what is rounded, as in the formula */
+    return x * inv + PG_MAGIC;
+}
+/* the codes of four, packed */
+__device__ __forceinline__ unsigned pg_pack4(float a, float b, float c, float d) {
+    const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x0c0c0400u);
+    const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(d), __float_as_uint(c), 0x0c0c0400u);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 /* the next bf16 at or below / above x (a NaN stays one) */
 __device__ __forceinline__ uint16_t bf16_down(float x) {
@@ -192,10 +200,11 @@ __device__ void pg_store_row(const PgPool &p, int page, int g, int r, const floa
     for (int d = lane; d < HD; d += 64) {
         float kept;
         if (CODES) {
-            const int c = pg_code(x[d], sc.inv);
-            kept = (float)c * sc.s;
-            if (KEY) ((signed char *)base)[((d >> 4) * PG_ROWS + r) * 16 + (d & 15)] = (signed char)c;
-            else ((signed char *)base)[d * PG_ROWS + pg_order(r, true)] = (signed char)c;
+            const float y = pg_code(x[d], sc.inv);
+            const unsigned char c = (unsigned char)__float_as_uint(y);
+            kept = (y - PG_MAGIC) * sc.s;
+            if (KEY) base[((d >> 4) * PG_ROWS + r) * 16 + (d & 15)] = c;
+            else base[d * PG_ROWS + pg_order(r, true)] = c;
         } else {
             const uint16_t b = bf16_of(x[d]);
             kept = bf16_to_f32(b);
@@ -1070,215 +1079,535 @@ __device__ __forceinline__ bool pg_find_run(const PgRunParams &p, int u, PgRun &
 }
 } // namespace
 
-template <int HD, bool CODES>
-__global__ __launch_bounds__(PG_TPB) void k_pg_append(const PgRunParams p) {
-    constexpr int XS = HD + 1; /* odd: columns without bank conflicts */
-    __shared__ float s_x[PG_ROWS * XS];
-    __shared__ float s_inv[PG_ROWS];
-    const int tid = threadIdx.x, kvh = blockIdx.y;
-    PgRun run;
-    if (!pg_find_run(p, blockIdx.x, run)) return;
-    const int page = p.p.table[(long long)run.seq * p.p.stride + run.page];
-    if (pg_bad_page(page, p.p.n_pages)) {
-        if (tid == 0) *p.p.flag = 1;
-        return;
+namespace {
+/* minimum and maximum that pass a NaN over, without the extra instruction that quiets a signalling one first */
+__device__ __forceinline__ float min_num(float a, float b) {
+    float r;
+    asm("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ float max_num(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+/* a lane's value from the other half of its 16 lanes */
+__device__ __forceinline__ float ror8(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, true));
+}
+
+/* Sixteen values a lane (f of two: their minimum or maximum) over the rows of a wave, LR lanes each, by halves: the upper and the
+ * lower 32 lanes swap eight values each and keep eight, the lanes 16 apart four of those. Value e + 4 b4 + 8 b5 of the lanes with
+ * bits 4 and 5 of b4 and b5 is left in v[e]: 28 instructions where a full exchange takes 16 times six. */
+template <int LR, class F>
+__device__ __forceinline__ void rows_join(float (&v)[16], F f) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[e]), __float_as_uint(v[e + 8]), false, false);
+        v[e] = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
     }
-    const int n = run.r1 - run.r0;
-    const long long at = (long long)page * p.p.Hkv + kvh;
-    unsigned char *kb = p.p.k + at * PgBytes<HD, CODES>::K, *vb = p.p.v + at * PgBytes<HD, CODES>::V;
-    float *sb = CODES ? p.p.scales + at * 2 * PG_ROWS : nullptr;
-    constexpr int C = HD / 8;
-    auto fetch = [&](const void *x) {
-        for (int e = tid; e < n * C; e += PG_TPB) {
-            const int r = e / C, d = e % C * 8;
-            float v[8];
-            load8(x, p.dtype, ((long long)(run.in0 + r) * p.p.Hkv + kvh) * HD + d, v);
 #pragma unroll
-            for (int i = 0; i < 8; i++) s_x[r * XS + d + i] = v[i];
-        }
-        __syncthreads();
-    };
-    /* K: eight lanes a row, lane j the chunks j, j + 8, .. of 8 elements */
-    fetch(p.k_in);
-    const int j = tid & 7;
-    constexpr int NC = (C + 7) / 8;
-    for (int r0 = 0; r0 < n; r0 += PG_TPB / 8) {
-        const int r = r0 + tid / 8;
-        const bool live = r < n;
-        float *x = s_x + min(r, n - 1) * XS;
-        float y[NC][8];
-        float ri = 1.0f;
-        if (p.k_norm) {
-            float ss = 0.0f;
-            for (int d0 = 8 * j; d0 < HD; d0 += 64)
-#pragma unroll
-                for (int i = 0; i < 8; i++) ss = fmaf(x[d0 + i], x[d0 + i], ss);
-            ss += __shfl_xor(ss, 1);
-            ss += __shfl_xor(ss, 2);
-            ss += __shfl_xor(ss, 4);
-            ri = 1.0f / sqrtf(ss / (float)HD + p.norm_eps);
-        }
-        const long long pos = (long long)run.page * PG_ROWS + run.r0 + min(r, n - 1);
-        unsigned m = 0;
+    for (int e = 0; e < 4; e++) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[e]), __float_as_uint(v[e + 4]), false, false);
+        v[e] = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+        if (LR == 8) v[e] = f(v[e], ror8(v[e]));
+    }
+}
+
+constexpr int PA_TPB = 512, PA_WAVES = PA_TPB / 64; /* a k_pg_append workgroup */
+
+template <int HD>
+struct PgKGeom {
+    static constexpr int C = HD / 8, LR = HD > 128 ? 16 : 8, NC = (C + LR - 1) / LR;
+    static constexpr int RW = PA_TPB / LR, NP = PG_ROWS / RW; /* rows of a pass, passes of a page */
+    static constexpr bool SAME = HD == 128 || HD == 256;      /* a NeoX partner is in the same lane */
+};
+/* the rotation's table for a row of a K workgroup, the same for all heads: lane j of the row's LR holds its chunks j, j + LR, .. of eight
+ * elements (a wave's loads and stores are whole lines) */
+template <int HD>
+struct PgKTable {
+    static constexpr int NC = PgKGeom<HD>::NC;
+    float4 c[NC][2], s[NC][2];
+    __device__ __forceinline__ void load(const PgRunParams &p, long long pos, int j) {
+        const int kind = p.p.rope_kind;
+        if (kind == SMOL_ROPE_OFF) return;
 #pragma unroll
         for (int k = 0; k < NC; k++) {
-            const int d0 = 8 * j + 64 * k;
+            const int d0 = 8 * j + 8 * PgKGeom<HD>::LR * k;
+            if (HD % 64 != 0 && d0 >= HD) continue;
+            /* its rows repeat their first half (NeoX) */
+            if (!PgKGeom<HD>::SAME || kind == SMOL_ROPE_INTERLEAVED_K || k < NC / 2) {
+                const float4 *ct = reinterpret_cast<const float4 *>(p.p.rope_cos + pos * HD + d0);
+                const float4 *st = reinterpret_cast<const float4 *>(p.p.rope_sin + pos * HD + d0);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                y[k][i] = 0.0f;
-                const int d = d0 + i;
-                if (HD % 64 != 0 && d >= HD) continue;
-                float a = x[d];
-                if (p.k_norm) a = a * p.k_norm[d] * ri;
-                if (p.p.rope_kind != SMOL_ROPE_OFF) {
-                    const int pd = rope_partner(d, HD, p.p.rope_kind);
-                    float b = x[pd];
-                    if (p.k_norm) b = b * p.k_norm[pd] * ri;
-                    const bool low = p.p.rope_kind == SMOL_ROPE_NEOX_K ? d < HD / 2 : (d & 1) == 0;
-                    a = a * p.p.rope_cos[pos * HD + d] + (low ? -b : b) * p.p.rope_sin[pos * HD + d];
+                for (int i = 0; i < 2; i++) {
+                    c[k][i] = ct[i];
+                    s[k][i] = st[i];
                 }
-                y[k][i] = a;
-                m = max(m, __float_as_uint(a) & 0x7FFFFFFFu);
             }
         }
-        m = max(m, (unsigned)__shfl_xor((int)m, 1));
-        m = max(m, (unsigned)__shfl_xor((int)m, 2));
-        m = max(m, (unsigned)__shfl_xor((int)m, 4));
-        const PgScale sc = CODES ? pg_scale(m) : PgScale{1.0f, 1.0f};
-        wave_fence(); /* the row's lanes have read their partners: the stored values take its place */
-        if (live) {
-            const int row = run.r0 + r;
-            if (CODES && j == 0) sb[row] = sc.s;
+    }
+};
+/* a row of a head. load() only requests, so that the next one's data is under way while this one's is worked on */
+template <int HD, bool BF>
+struct PgKStep {
+    static constexpr int LR = PgKGeom<HD>::LR, NC = PgKGeom<HD>::NC;
+    static constexpr bool SAME = PgKGeom<HD>::SAME;
+    Raw8<BF> x[NC], pr[SAME ? 1 : NC];
+    uint32_t pe[SAME ? 1 : NC][8];
+
+    __device__ __forceinline__ void load(const PgRunParams &p, long long in, int j) {
+        const int kind = p.p.rope_kind;
+#pragma unroll
+        for (int k = 0; k < NC; k++) {
+            const int d0 = 8 * j + 8 * LR * k;
+            if (HD % 64 != 0 && d0 >= HD) continue;
+            raw_load<BF>(x[k], p.k_in, in + d0);
+            if (!SAME && kind == SMOL_ROPE_NEOX_K) {
+                if (HD % 16 == 0) { /* half a head is whole chunks */
+                    raw_load<BF>(pr[k], p.k_in, in + (d0 < HD / 2 ? d0 + HD / 2 : d0 - HD / 2));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        pe[k][i] = __float_as_uint(in_at(p.k_in, BF ? SMOL_IN_BF16 : SMOL_IN_F32, in + rope_partner(d0 + i, HD, SMOL_ROPE_NEOX_K)));
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ static float at(const float4 (&v)[2], int i) {
+        const float4 &q = v[i >> 2];
+        return (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
+    }
+    /* y: the normalised, rotated chunks (zeros behind the row) */
+    __device__ __forceinline__ void finish(const PgRunParams &p, const PgKTable<HD> &t, int j, float (&y)[NC][8]) const {
+        const int kind = p.p.rope_kind;
+        float v[NC][8], o[SAME ? 1 : NC][8];
+#pragma unroll
+        for (int k = 0; k < NC; k++) {
+            const int d0 = 8 * j + 8 * LR * k;
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[k][i] = 0.0f;
+            if (HD % 64 != 0 && d0 >= HD) continue;
+            raw_unpack<BF>(x[k], v[k]);
+            if (!SAME && kind == SMOL_ROPE_NEOX_K) {
+                if (HD % 16 == 0) raw_unpack<BF>(pr[k], o[k]);
+                else
+#pragma unroll
+                    for (int i = 0; i < 8; i++) o[k][i] = __uint_as_float(pe[k][i]);
+            }
+        }
+        if (p.k_norm) {
+            float ss[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) ss[i & 3] = fmaf(v[k][i], v[k][i], ss[i & 3]);
+            float sum = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+#pragma unroll
+            for (int sh = 1; sh < LR; sh <<= 1) sum += __shfl_xor(sum, sh);
+            /* 1 / sqrt in 64 bits: rounded once */
+            const float ri = (float)(1.0 / sqrt((double)sum / HD + (double)p.norm_eps));
 #pragma unroll
             for (int k = 0; k < NC; k++) {
-                const int d0 = 8 * j + 64 * k;
+                const int d0 = 8 * j + 8 * LR * k;
                 if (HD % 64 != 0 && d0 >= HD) continue;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    v[k][i] *= p.k_norm[d0 + i] * ri;
+                    if (!SAME && kind == SMOL_ROPE_NEOX_K) o[k][i] *= p.k_norm[rope_partner(d0 + i, HD, SMOL_ROPE_NEOX_K)] * ri;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < NC; k++) {
+            constexpr int H = NC / 2 ? NC / 2 : 1;
+            const int d0 = 8 * j + 8 * LR * k;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                float a = v[k][i];
+                if (kind == SMOL_ROPE_NEOX_K) {
+                    const float b = (SAME ? v[(k + H) % NC][i] : o[SAME ? 0 : k][i]) * at(SAME ? t.s[k % H] : t.s[k], i);
+                    a = fmaf(a, at(SAME ? t.c[k % H] : t.c[k], i), (SAME ? k < H : d0 + i < HD / 2) ? -b : b);
+                } else if (kind == SMOL_ROPE_INTERLEAVED_K) {
+                    const float b = v[k][i ^ 1] * at(t.s[k], i);
+                    a = fmaf(a, at(t.c[k], i), i & 1 ? b : -b);
+                }
+                y[k][i] = HD % 64 != 0 && d0 >= HD ? 0.0f : a;
+            }
+        }
+    }
+};
+
+/* K rows of heads [h0, h1) into a page, and its bounds */
+template <int HD, bool CODES, bool BF>
+__device__ __forceinline__ void pg_append_k(const PgRunParams &p, const PgRun &run, long long page, int h0, int h1) {
+    typedef PgKStep<HD, BF> Step;
+    typedef PgKGeom<HD> Geo;
+    constexpr int C = Geo::C, LR = Geo::LR, NC = Geo::NC, RW = Geo::RW, NP = Geo::NP;
+    __shared__ float s_lo[2][PA_WAVES][HD], s_hi[2][PA_WAVES][HD]; /* of the heads by turns: one barrier a head is enough */
+    __shared__ unsigned s_none[2][PA_WAVES][C];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, j = tid & (LR - 1), n = run.r1 - run.r0;
+    auto request = [&](Step &st, int h, int pass) {
+        st.load(p, ((long long)(run.in0 + min(RW * pass + tid / LR, n - 1)) * p.p.Hkv + h) * HD, j);
+    };
+    Step next;
+    request(next, h0, 0);
+    PgKTable<HD> table[NP];
+#pragma unroll
+    for (int pass = 0; pass < NP; pass++)
+        table[pass].load(p, (long long)run.page * PG_ROWS + run.r0 + min(RW * pass + tid / LR, n - 1), j);
+    for (int h = h0; h < h1; h++) {
+        const long long at = page * p.p.Hkv + h;
+        const int turn = (h - h0) & 1;
+        unsigned char *kb = p.p.k + at * PgBytes<HD, CODES>::K;
+        float lo[16], hi[16]; /* element 8 k + i */
+        unsigned none[NC];    /* elements that are no number in some row */
+#pragma unroll
+        for (int pass = 0; pass < NP; pass++) {
+            if (RW * pass >= n) break;
+            const Step cur = next;
+            if (pass + 1 < NP && RW * (pass + 1) < n) request(next, h, pass + 1);
+            else if (h + 1 < h1) request(next, h + 1, 0);
+            /* lanes past the last row work on it once more: it changes no bound */
+            const int r = RW * pass + tid / LR, row = run.r0 + r;
+            float y[NC][8];
+            cur.finish(p, table[pass], j, y);
+            PgScale sc = {1.0f, 1.0f};
+            if (CODES) {
+                unsigned m = 0;
+#pragma unroll
+                for (int k = 0; k < NC; k++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(y[k][i]) & 0x7FFFFFFFu);
+#pragma unroll
+                for (int sh = 1; sh < LR; sh <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, sh));
+                sc = pg_scale(m);
+            }
+            if (CODES && j == 0 && r < n) p.p.scales[at * 2 * PG_ROWS + row] = sc.s;
+#pragma unroll
+            for (int k = 0; k < NC; k++) {
+                const int d0 = 8 * j + 8 * LR * k;
+                const bool put = r < n && (HD % 64 == 0 || d0 < HD);
+                float kept[8];
+                unsigned bad = 0;
                 if (CODES) {
-                    unsigned w[2] = {0, 0};
+                    float q[8];
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const int c = pg_code(y[k][i], sc.inv);
-                        w[i >> 2] |= ((unsigned)c & 0xFFu) << 8 * (i & 3);
-                        x[d0 + i] = (float)c * sc.s;
+                        q[i] = pg_code(y[k][i], sc.inv);
+                        kept[i] = (q[i] - PG_MAGIC) * sc.s;
                     }
                     unsigned char *to = kb + ((d0 >> 4) * PG_ROWS + row) * 16 + (d0 & 8);
-                    *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
-                    if (HD % 16 != 0 && d0 + 8 == HD) *reinterpret_cast<uint2 *>(to + 8) = make_uint2(0, 0);
+                    if (put) *reinterpret_cast<uint2 *>(to) = make_uint2(pg_pack4(q[0], q[1], q[2], q[3]), pg_pack4(q[4], q[5], q[6], q[7]));
+                    if (HD % 16 != 0 && put && d0 + 8 == HD) *reinterpret_cast<uint2 *>(to + 8) = make_uint2(0, 0);
+                    bad = sc.s == sc.s ? 0u : 0xFFu;
                 } else {
-                    unsigned w[4];
+                    unsigned o[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const uint16_t a = bf16_of(y[k][2 * i]), b = bf16_of(y[k][2 * i + 1]);
-                        w[i] = a | (unsigned)b << 16;
-                        x[d0 + 2 * i] = bf16_to_f32(a);
-                        x[d0 + 2 * i + 1] = bf16_to_f32(b);
+                        o[i] = a | (unsigned)b << 16;
+                        kept[2 * i] = bf16_to_f32(a);
+                        kept[2 * i + 1] = bf16_to_f32(b);
                     }
-                    *reinterpret_cast<uint4 *>(kb + ((d0 >> 3) * PG_ROWS + row) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (put) *reinterpret_cast<uint4 *>(kb + ((d0 >> 3) * PG_ROWS + row) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) bad |= kept[i] == kept[i] ? 0u : 1u << i;
+                }
+                none[k] = pass ? none[k] | bad : bad;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    lo[8 * k + i] = pass ? min_num(lo[8 * k + i], kept[i]) : kept[i];
+                    hi[8 * k + i] = pass ? max_num(hi[8 * k + i], kept[i]) : kept[i];
                 }
             }
         }
-    }
-    __syncthreads();
-    for (int d = tid; d < HD; d += PG_TPB) {
-        uint16_t *lo = p.p.bounds + at * 2 * HD + d, *hi = lo + HD;
-        float a = INFINITY, b = -INFINITY;
-        if (run.r0 > 0) {
-            a = bf16_to_f32(*lo);
-            b = bf16_to_f32(*hi);
-        }
-        for (int r = 0; r < n; r++) {
-            a = min_nan(a, s_x[r * XS + d]);
-            b = max_nan(b, s_x[r * XS + d]);
-        }
-        *lo = bf16_down(a);
-        *hi = bf16_up(b);
-    }
-    __syncthreads();
-
-    /* V */
-    fetch(p.v_in);
-    if (CODES) {
-        for (int r0 = 0; r0 < n; r0 += PG_TPB / 8) {
-            const int r = r0 + tid / 8;
-            unsigned m = 0;
-            if (r < n)
-                for (int d0 = 8 * j; d0 < HD; d0 += 64)
+        if (NC == 1) /* the join takes sixteen */
 #pragma unroll
-                    for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(s_x[r * XS + d0 + i]) & 0x7FFFFFFFu);
-            m = max(m, (unsigned)__shfl_xor((int)m, 1));
-            m = max(m, (unsigned)__shfl_xor((int)m, 2));
-            m = max(m, (unsigned)__shfl_xor((int)m, 4));
-            if (r < n && j == 0) {
-                const PgScale sc = pg_scale(m);
-                sb[PG_ROWS + run.r0 + r] = sc.s;
-                s_inv[r] = sc.inv;
-            }
+            for (int e = 8; e < 16; e++) lo[e] = hi[e] = 0.0f;
+        /* over the rows of the wave, then over the waves and what the page had */
+#pragma unroll
+        for (int k = 0; k < NC; k++) {
+            unsigned b = none[k];
+            if (LR == 8) b |= __shfl_xor((int)b, 8);
+            b |= __shfl_xor((int)b, 16);
+            b |= __shfl_xor((int)b, 32);
+            const int d0 = 8 * j + 8 * LR * k;
+            if (lane < LR && (HD % 64 == 0 || d0 < HD)) s_none[turn][wave][d0 / 8] = b;
+        }
+        rows_join<LR>(lo, min_num);
+        rows_join<LR>(hi, max_num);
+        if (LR == 16 || !(lane & 8)) {
+            const int e0 = 4 * (lane >> 4 & 1) + 8 * (lane >> 5), d = 8 * j + 8 * LR * (e0 >> 3) + (e0 & 7);
+            if (NC == 2 || e0 < 8)
+                if (HD % 64 == 0 || d < HD)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        s_lo[turn][wave][d + e] = lo[e];
+                        s_hi[turn][wave][d + e] = hi[e];
+                    }
         }
         __syncthreads();
-    }
-    /* a line of V in 16-byte pieces; pieces that hold other rows too by element */
-    constexpr int E = CODES ? 16 : 8, P = PG_ROWS / E;
-    for (int e = tid; e < HD * P; e += PG_TPB) {
-        const int d = CODES ? e >> 2 : (e >> 2) % HD, half = CODES ? 0 : (e >> 2) / HD, g = e & 3;
-        unsigned w[4] = {0, 0, 0, 0};
-        unsigned char *to = CODES ? vb + d * PG_ROWS + 16 * g : vb + ((half * HD + d) * 32 + 8 * g) * 2;
-        int rows[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            const int row = 32 * half + 16 * (i >> 2) + 4 * g + (i & 3), r = row - run.r0;
-            const bool in = r >= 0 && r < n;
-            rows[0] += in;
-            const float v = in ? s_x[r * XS + d] : 0.0f;
-            if (CODES) w[i >> 2] |= ((unsigned)(in ? pg_code(v, s_inv[r]) : 0) & 0xFFu) << 8 * (i & 3);
-            else w[i >> 1] |= (unsigned)bf16_of(v) << 16 * (i & 1);
-        }
-        if (rows[0] == E) {
-            *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else if (rows[0]) {
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                const int row = 32 * half + 16 * (i >> 2) + 4 * g + (i & 3), r = row - run.r0;
-                if (r < 0 || r >= n) continue;
-                if (CODES) to[i] = (unsigned char)(w[i >> 2] >> 8 * (i & 3));
-                else ((uint16_t *)to)[i] = (uint16_t)(w[i >> 1] >> 16 * (i & 1));
+        for (int d = tid; d < HD; d += PA_TPB) {
+            uint16_t *to = p.p.bounds + at * 2 * HD + d;
+            float l = INFINITY, u = -INFINITY;
+            bool bad = false;
+            if (run.r0 > 0) {
+                l = bf16_to_f32(to[0]);
+                u = bf16_to_f32(to[HD]);
+                bad = l != l || u != u;
             }
+#pragma unroll
+            for (int w = 0; w < PA_WAVES; w++) {
+                l = min_num(l, s_lo[turn][w][d]);
+                u = max_num(u, s_hi[turn][w][d]);
+                bad |= s_none[turn][w][d / 8] >> (d & 7) & 1;
+            }
+            to[0] = bad ? 0x7FC0 : bf16_down(l);
+            to[HD] = bad ? 0x7FC0 : bf16_up(u);
         }
     }
 }
 
-template <int HD, bool CODES>
-__global__ __launch_bounds__(PG_TPB) void k_pg_read(const PgRunParams p) {
-    constexpr int XS = HD + 1;
-    __shared__ float s_x[PG_ROWS * XS];
-    const int tid = threadIdx.x, kvh = blockIdx.y;
+/* V rows of heads [h0, h1) into a page: a thread takes four dims of the eight rows 32 half + 16 t + 4 g + i, which lie side by side
+ * along V's lines, and turns them round in its registers. 16 lanes hold 64 dims of a row, a wave half a page of them; what waves
+ * are left take the next heads. */
+template <int HD, bool CODES, bool BF>
+__device__ __forceinline__ void pg_append_v(const PgRunParams &p, const PgRun &run, long long page, int h0, int h1) {
+    constexpr int DB = (HD + 63) / 64, SUB = PA_WAVES / (2 * DB); /* blocks of 64 dims, heads at a time */
+    static_assert(SUB >= 1, "a head's waves");
+    __shared__ unsigned s_max[2][SUB][DB][PG_ROWS];
+    __shared__ __align__(16) float s_inv[PA_WAVES][32];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane & 3, n = run.r1 - run.r0;
+    const int half = wave & 1, block = wave / 2 % DB, sub = wave / (2 * DB), d = 64 * block + 4 * (lane >> 2);
+    const bool mine = HD % 64 == 0 || d < HD;
+    typedef typename std::conditional<BF, uint2, float4>::type Four;
+    Four next[8];
+    auto request = [&](int kvh) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int r = 32 * half + 16 * (e >> 2) + 4 * g + (e & 3) - run.r0;
+            next[e] = Four{};
+            if (kvh >= h1 || r < 0 || r >= n || !mine) continue;
+            const long long in = ((long long)(run.in0 + r) * p.p.Hkv + kvh) * HD + d;
+            next[e] = BF ? *reinterpret_cast<const Four *>((const uint16_t *)p.v_in + in) : *reinterpret_cast<const Four *>((const float *)p.v_in + in);
+        }
+    };
+    request(h0 + sub);
+    for (int hb = h0; hb < h1; hb += SUB) {
+        const int kvh = hb + sub, turn = (hb - h0) / SUB & 1; /* by turns: one barrier a step is enough */
+        const bool live = kvh < h1;
+        const long long at = page * p.p.Hkv + kvh;
+        unsigned char *vb = p.p.v + at * PgBytes<HD, CODES>::V;
+        float x[8][4];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if constexpr (BF) {
+                x[e][0] = __uint_as_float(next[e].x << 16);
+                x[e][1] = __uint_as_float(next[e].x & 0xFFFF0000u);
+                x[e][2] = __uint_as_float(next[e].y << 16);
+                x[e][3] = __uint_as_float(next[e].y & 0xFFFF0000u);
+            } else {
+                x[e][0] = next[e].x;
+                x[e][1] = next[e].y;
+                x[e][2] = next[e].z;
+                x[e][3] = next[e].w;
+            }
+        }
+        if (hb + SUB < h1) request(kvh + SUB);
+        float inv[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) inv[e] = 0.0f;
+        if (CODES) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                unsigned m = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) m = max(m, __float_as_uint(x[e][i]) & 0x7FFFFFFFu);
+                /* lanes of the same g */
+                m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x124, 0xF, 0xF, true));
+                m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x128, 0xF, 0xF, true));
+                m = row_maxu4(m);
+                if (lane < 4) s_max[turn][sub][block][32 * half + 16 * (e >> 2) + 4 * g + (e & 3)] = m;
+            }
+            __syncthreads();
+            /* a row's scale by one lane; its factor to the others of the wave */
+            const int row = 32 * half + (lane & 31);
+            unsigned m = 0;
+#pragma unroll
+            for (int b = 0; b < DB; b++) m = max(m, s_max[turn][sub][b][row]);
+            const PgScale sc = pg_scale(m);
+            if (lane < 32) {
+                s_inv[wave][lane] = sc.inv;
+                if (live && block == 0 && row >= run.r0 && row < run.r1) p.p.scales[(at * 2 + 1) * PG_ROWS + row] = sc.s;
+            }
+            wave_fence();
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const f4 v = *reinterpret_cast<const f4 *>(&s_inv[wave][16 * t + 4 * g]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) inv[4 * t + i] = v[i];
+            }
+            wave_fence();
+        }
+        if (!live || !mine) continue;
+        const bool all = run.r0 <= 32 * half + 4 * g && run.r1 >= 32 * half + 4 * g + 20;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            unsigned o[4];
+            if constexpr (CODES) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+                    o[t] = pg_pack4(pg_code(x[4 * t][i], inv[4 * t]), pg_code(x[4 * t + 1][i], inv[4 * t + 1]),
+                                    pg_code(x[4 * t + 2][i], inv[4 * t + 2]), pg_code(x[4 * t + 3][i], inv[4 * t + 3]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] = bf16_of(x[2 * e][i]) | (unsigned)bf16_of(x[2 * e + 1][i]) << 16;
+            }
+            unsigned char *to = CODES ? vb + (d + i) * PG_ROWS + 16 * g + 8 * half : vb + ((half * HD + d + i) * 32 + 8 * g) * 2;
+            if (all) {
+                if constexpr (CODES) *reinterpret_cast<uint2 *>(to) = make_uint2(o[0], o[1]);
+                else *reinterpret_cast<uint4 *>(to) = make_uint4(o[0], o[1], o[2], o[3]);
+            } else {
+                /* the other rows' elements stay as they are */
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int row = 32 * half + 16 * (e >> 2) + 4 * g + (e & 3);
+                    if (row < run.r0 || row >= run.r1) continue;
+                    if (CODES) to[e] = (unsigned char)(o[e >> 2] >> 8 * (e & 3));
+                    else ((uint16_t *)to)[e] = (uint16_t)(o[e >> 1] >> 16 * (e & 1));
+                }
+            }
+        }
+    }
+}
+} // namespace
+
+/* A workgroup takes the K (z 0) or the V (z 1) rows of `heads` kv heads of one page. */
+template <int HD, bool CODES, bool BF>
+__global__ __launch_bounds__(PA_TPB, HD == 64 || HD == 128 ? 4 : 2) void k_pg_append(const PgRunParams p) {
     PgRun run;
     if (!pg_find_run(p, blockIdx.x, run)) return;
     const int page = p.p.table[(long long)run.seq * p.p.stride + run.page];
-    const int n = run.r1 - run.r0;
+    if (pg_bad_page(page, p.p.n_pages)) {
+        if (threadIdx.x == 0) *p.p.flag = 1;
+        return;
+    }
+    const int h0 = blockIdx.y * p.heads, h1 = min(p.p.Hkv, h0 + p.heads);
+    if (blockIdx.z == 0) pg_append_k<HD, CODES, BF>(p, run, page, h0, h1);
+    else pg_append_v<HD, CODES, BF>(p, run, page, h0, h1);
+}
+
+namespace {
+/* N values, times s, as the output's type */
+template <bool BF, int N>
+__device__ __forceinline__ void pg_put(void *out, long long i, const float (&v)[N], float s) {
+    if (BF) {
+        unsigned w[N / 2];
+#pragma unroll
+        for (int e = 0; e < N / 2; e++) w[e] = bf16_of(v[2 * e] * s) | (unsigned)bf16_of(v[2 * e + 1] * s) << 16;
+        uint16_t *to = (uint16_t *)out + i;
+        if constexpr (N == 4) {
+            *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N / 8; e++) *reinterpret_cast<uint4 *>(to + 8 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        }
+    } else {
+        float *to = (float *)out + i;
+#pragma unroll
+        for (int e = 0; e < N / 4; e++) *reinterpret_cast<f4 *>(to + 4 * e) = f4{v[4 * e] * s, v[4 * e + 1] * s, v[4 * e + 2] * s, v[4 * e + 3] * s};
+    }
+}
+__device__ __forceinline__ float pg_byte(unsigned w, int i) { return (float)(int)(signed char)(w >> 8 * i & 0xFFu); }
+} // namespace
+
+/* A workgroup takes one page and kv head: K piece by piece (eight pieces of eight rows a wave: whole lines both ways), V four dims
+ * of eight rows a thread, turned round in registers, as k_pg_append does. */
+template <int HD, bool CODES, bool BF>
+__global__ __launch_bounds__(PG_TPB) void k_pg_read(const PgRunParams p) {
+    constexpr int E = CODES ? 16 : 8, CH = CODES ? PgGeom<HD>::CH8 : PgGeom<HD>::CHB;
+    constexpr int CB = (CH + 7) / 8, NK = CB * 8 / PG_WAVES; /* (8 pieces, 8 rows) tasks of a wave */
+    constexpr int DB = (HD + 63) / 64, NV = (2 * DB + PG_WAVES - 1) / PG_WAVES;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kvh = blockIdx.y, g = lane & 3;
+    PgRun run;
+    if (!pg_find_run(p, blockIdx.x, run)) return;
+    const int page = p.p.table[(long long)run.seq * p.p.stride + run.page];
     const bool bad = pg_bad_page(page, p.p.n_pages);
     if (bad && tid == 0) *p.p.flag = 1;
     const long long at = (long long)(bad ? 0 : page) * p.p.Hkv + kvh;
     const unsigned char *kb = p.p.k + at * PgBytes<HD, CODES>::K, *vb = p.p.v + at * PgBytes<HD, CODES>::V;
     const float *sb = CODES ? p.p.scales + at * 2 * PG_ROWS : nullptr;
-    auto put = [&](void *out, int r, int d, float v) {
-        const long long i = ((long long)(run.in0 + r) * p.p.Hkv + kvh) * HD + d;
-        if (bad) v = __uint_as_float(0x7FC00000u);
-        if (p.dtype == SMOL_IN_BF16) ((uint16_t *)out)[i] = bf16_of(v);
-        else ((float *)out)[i] = v;
-    };
-    for (int e = tid; e < n * HD; e += PG_TPB) {
-        const int r = e / HD, d = e % HD, row = run.r0 + r;
-        if (CODES) put(p.k_out, r, d, (float)((const signed char *)kb)[((d >> 4) * PG_ROWS + row) * 16 + (d & 15)] * sb[row]);
-        else put(p.k_out, r, d, bf16_to_f32(((const uint16_t *)kb)[((d >> 3) * PG_ROWS + row) * 8 + (d & 7)]));
+    const float none = __uint_as_float(0x7FC00000u);
+    auto index = [&](int row, int d) { return ((long long)(run.in0 + row - run.r0) * p.p.Hkv + kvh) * HD + d; };
+    uint4 kw[NK];
+    float ks[NK];
+    unsigned vw[NV][4][CODES ? 2 : 4];
+    f4 vs[NV][2];
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        const int task = wave + PG_WAVES * k, ch = task / 8 * 8 + (lane & 7), row = task % 8 * 8 + lane / 8;
+        if (row < run.r0 || row >= run.r1 || (CH % 8 != 0 && ch >= CH)) continue;
+        kw[k] = *reinterpret_cast<const uint4 *>(kb + (ch * PG_ROWS + row) * 16);
+        ks[k] = CODES ? sb[row] : 1.0f;
     }
-    for (int e = tid; e < HD * PG_ROWS; e += PG_TPB) {
-        const int row = e % PG_ROWS, d = e / PG_ROWS, r = row - run.r0;
-        if (r < 0 || r >= n) continue;
-        if (CODES) s_x[r * XS + d] = (float)((const signed char *)vb)[d * PG_ROWS + pg_order(row, true)] * sb[PG_ROWS + row];
-        else s_x[r * XS + d] = bf16_to_f32(((const uint16_t *)vb)[((row >> 5) * HD + d) * 32 + (pg_order(row, false) & 31)]);
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int task = wave + PG_WAVES * k, h = task & 1, d = 64 * (task >> 1) + 4 * (lane >> 2), r0 = 32 * h + 4 * g;
+        if (task >= 2 * DB || (HD % 64 != 0 && d >= HD) || r0 + 20 <= run.r0 || r0 >= run.r1) continue;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (CODES) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(vb + (d + i) * PG_ROWS + 16 * g + 8 * h);
+                vw[k][i][0] = v.x;
+                vw[k][i][1] = v.y;
+            } else {
+                const uint4 v = *reinterpret_cast<const uint4 *>(vb + ((h * HD + d + i) * 32 + 8 * g) * 2);
+                vw[k][i][0] = v.x;
+                vw[k][i][1] = v.y;
+                vw[k][i][CODES ? 0 : 2] = v.z;
+                vw[k][i][CODES ? 0 : 3] = v.w;
+            }
+        }
+        if (CODES) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) vs[k][t] = *reinterpret_cast<const f4 *>(sb + PG_ROWS + r0 + 16 * t);
+        }
     }
-    __syncthreads();
-    for (int e = tid; e < n * HD; e += PG_TPB) put(p.v_out, e / HD, e % HD, s_x[e / HD * XS + e % HD]);
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        const int task = wave + PG_WAVES * k, ch = task / 8 * 8 + (lane & 7), row = task % 8 * 8 + lane / 8;
+        if (row < run.r0 || row >= run.r1 || (CH % 8 != 0 && ch >= CH)) continue;
+        const unsigned w[4] = {kw[k].x, kw[k].y, kw[k].z, kw[k].w};
+        const float s = bad ? none : ks[k];
+        if constexpr (CODES) {
+            float v[2][8];
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i >> 3][i & 7] = pg_byte(w[i >> 2], i & 3);
+            pg_put<BF>(p.k_out, index(row, ch * E), v[0], s);
+            if (HD % 16 == 0 || ch * E + 8 < HD) pg_put<BF>(p.k_out, index(row, ch * E + 8), v[1], s);
+        } else {
+            float v[8];
+            unpack_bf16x8(kw[k], v);
+            pg_put<BF>(p.k_out, index(row, ch * E), v, s);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int task = wave + PG_WAVES * k, h = task & 1, d = 64 * (task >> 1) + 4 * (lane >> 2);
+        if (task >= 2 * DB || (HD % 64 != 0 && d >= HD)) continue;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int row = 32 * h + 16 * (e >> 2) + 4 * g + (e & 3);
+            if (row < run.r0 || row >= run.r1) continue;
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                v[i] = CODES ? pg_byte(vw[k][i][e >> 2], e & 3)
+                             : __uint_as_float(e & 1 ? vw[k][i][CODES ? 0 : e >> 1] & 0xFFFF0000u : vw[k][i][CODES ? 0 : e >> 1] << 16);
+            pg_put<BF>(p.v_out, index(row, d), v, bad ? none : CODES ? vs[k][e >> 2][e & 3] : 1.0f);
+        }
+    }
 }
 
 /* ---------------------------------------------------------------- launches */
@@ -1294,19 +1623,30 @@ __global__ __launch_bounds__(PG_TPB) void k_pg_read(const PgRunParams p) {
     default: return -1; \
     }
 
+/* workgroups (of one head) from which one takes two heads, and so on */
+#ifndef PG_HEADS_FROM
+#define PG_HEADS_FROM 2048
+#endif
+
 /* workgroups of k_pg on a compute unit */
 extern "C" int smol_paged_occupancy(int hd, int codes) { return 2; }
 
-extern "C" int smol_launch_pages(const PgRunParams *p, int hd, int write, hipStream_t st, hipEvent_t e0, hipEvent_t e1) {
-    const dim3 grid((unsigned)pg_max_run_pages(p->p.n_seq, p->rows), p->p.Hkv), tpb(PG_TPB);
+extern "C" int smol_launch_pages(const PgRunParams *pp, int hd, int write, hipStream_t st, hipEvent_t e0, hipEvent_t e1) {
+    PgRunParams args = *pp, *p = &args;
+    const long long pages = pg_max_run_pages(p->p.n_seq, p->rows);
+    p->heads = 1;
+    if (write)
+        while (p->heads < 8 && 2 * p->heads <= p->p.Hkv && pages * p->p.Hkv / p->heads >= PG_HEADS_FROM) p->heads *= 2;
+    const dim3 grid((unsigned)pages, (p->p.Hkv + p->heads - 1) / p->heads, write ? 2 : 1), tpb(write ? PA_TPB : PG_TPB);
+    const bool bf = p->dtype == SMOL_IN_BF16;
+#define PG_GO(HD, C, B) \
+    if (write) hipExtLaunchKernelGGL((k_pg_append<HD, C, B>), grid, tpb, 0, st, e0, e1, 0, *p); \
+    else hipExtLaunchKernelGGL((k_pg_read<HD, C, B>), grid, tpb, 0, st, e0, e1, 0, *p)
 #define PG_RUN(HD) \
-    if (write) { \
-        if (p->p.codes) hipExtLaunchKernelGGL((k_pg_append<HD, true>), grid, tpb, 0, st, e0, e1, 0, *p); \
-        else hipExtLaunchKernelGGL((k_pg_append<HD, false>), grid, tpb, 0, st, e0, e1, 0, *p); \
-    } else { \
-        if (p->p.codes) hipExtLaunchKernelGGL((k_pg_read<HD, true>), grid, tpb, 0, st, e0, e1, 0, *p); \
-        else hipExtLaunchKernelGGL((k_pg_read<HD, false>), grid, tpb, 0, st, e0, e1, 0, *p); \
-    }
+    if (p->p.codes && bf) { PG_GO(HD, true, true); } \
+    else if (p->p.codes) { PG_GO(HD, true, false); } \
+    else if (bf) { PG_GO(HD, false, true); } \
+    else { PG_GO(HD, false, false); }
     PG_BY_HD(hd, PG_RUN)
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }
