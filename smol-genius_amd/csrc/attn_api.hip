@@ -56,7 +56,7 @@ extern "C" int smol_shared_mass_chunks(long long pairs, int max_len);
 extern "C" int smol_launch_shared(const ShParams *p, int hd, int tile_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
 extern "C" int smol_evict_fused(int max_moves);
 extern "C" int smol_launch_evict(const EvictParams *p, int max_rows, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
-extern "C" int smol_paged_occupancy(int hd, int codes);
+extern "C" int smol_paged_occupancy(int hd);
 extern "C" int smol_launch_paged(const PgParams *p, int hd, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
 extern "C" int smol_launch_pages(const PgRunParams *p, int hd, int write, hipStream_t st, hipEvent_t e0, hipEvent_t e1);
 extern "C" int smol_launch_to_bf16_trunc(const float *x, uint16_t *y, long long n, hipStream_t st);
@@ -230,6 +230,7 @@ struct smol_attn_ctx {
     DevBuf work;   /* a call's own arrays: Q scratch, staged K and V, partials (WorkPlan) */
     DevBuf out32; /* fp32 result of a call whose output is bf16 */
     DevBuf dec_part; /* k_dec partial slots and flags */
+    DevBuf pg_count; /* k_pg: chunks that have ended, zero between calls */
     /* flags, 384 bytes of pinned host memory that kernels write to (only when
      * there is something to report) and the host reads without a copy: word 0
      * is set when fp16 staging overflows, word 32 (its own 128-byte line) by
@@ -429,7 +430,7 @@ extern "C" int smol_attn_ctx_destroy(smol_attn_ctx *ctx) {
     if (!ctx) return SMOL_ATTN_OK;
     hipSetDevice(ctx->device);
     hipStreamSynchronize(ctx->stream);
-    DevBuf *bufs[] = {&ctx->desc, &ctx->work, &ctx->out32, &ctx->dec_part};
+    DevBuf *bufs[] = {&ctx->desc, &ctx->work, &ctx->out32, &ctx->dec_part, &ctx->pg_count};
     for (DevBuf *b : bufs) dev_free(*b);
     if (ctx->range_flag) hipHostFree(ctx->range_flag);
     if (ctx->mark) hipEventDestroy(ctx->mark);
@@ -2419,15 +2420,20 @@ static int decode_paged(smol_attn_ctx *ctx, smol_kv_pages *kp, int layer, const 
     if (top > 0 && (long long)n_seq * ((stride + 63) / 64) > PG_MAX_BLOCKS)
         return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d sequences, page table rows of %d", n_seq, stride);
     if (pg.tiles > 65535) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d heads a kv head", G);
-    pg.slots = std::max(1, ctx->cu_count * smol_paged_occupancy(hd, pg.p.codes) / (Hkv * pg.tiles));
-    const long long items = pg_max_chunks(n_seq, pg.slots);
-    pg.max_items = (int)items;
+    pg.slots = std::max(1, ctx->cu_count * smol_paged_occupancy(hd) / (Hkv * pg.tiles));
+    if ((long long)n_seq * (2LL * stride + PG_EXTRA) > 1 << 30)
+        return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d sequences, page table rows of %d", n_seq, stride);
+    const long long items = 2LL * pg.slots;
     WorkPlan wk;
-    const size_t o_o = wk.take((size_t)items * n_heads * hd * 4), o_ml = wk.take((size_t)items * n_heads * 8);
+    const size_t o_o = wk.take((size_t)items * n_heads * hd * 4), o_ml = wk.take((size_t)items * n_heads * 16);
     const size_t o_list = wk.take(top > 0 && !chosen ? (size_t)n_seq * Hkv * top * 4 : 0);
     const size_t o_score = wk.take(top > 0 ? (size_t)n_seq * Hkv * stride * 8 : 0);
     if ((rc = check_capture(ctx, "workspace growth", wk.bytes > ctx->work.cap))) return rc;
     if ((rc = dev_reserve(ctx->work, wk.bytes, ctx->stream))) return rc;
+    const size_t counts = (size_t)n_seq * Hkv * pg.tiles * sizeof(unsigned);
+    if ((rc = check_capture(ctx, "workspace growth", counts > ctx->pg_count.cap))) return rc;
+    if ((rc = dev_reserve(ctx->pg_count, counts, ctx->stream, true))) return rc;
+    pg.count = (unsigned *)ctx->pg_count.p;
     unsigned char *w = (unsigned char *)ctx->work.p;
     pg.part_o = (float *)(w + o_o);
     pg.part_ml = (float *)(w + o_ml);

@@ -354,7 +354,7 @@ typedef struct {
     int heads;                        /* kv heads of a workgroup */
 } PgRunParams;
 
-/* k_pg, k_pg_merge, k_pg_score, k_pg_select: a decode step */
+/* k_pg, k_pg_score, k_pg_select: a decode step */
 typedef struct {
     PgPool p;
     const int *len;                   /* [n_seq] cached rows; the new token becomes row len */
@@ -364,10 +364,10 @@ typedef struct {
     double scale;
     float *out; int Hq, G;
     int window; float cap2;           /* window > 0: positions > len - window; cap2 > 0: softcap in log2 units */
-    int slots;                        /* whole chunks at most (pg_chunk) */
-    int max_items;                    /* workgroups a kv head and tile of heads */
+    int slots;                        /* workgroups a kv head and tile of heads: pieces of the line at most (pg_piece) */
     int tiles;                        /* tiles of 16 heads of a kv head */
-    float *part_o; float *part_ml;    /* [kv][max_items][G]: outputs [hd], (m, l) */
+    float *part_o; float *part_ml;    /* [kv][2 slots][G]: outputs [hd], (m, l, 0, 0) */
+    unsigned *count;                  /* [n_seq][kv][tiles] chunks that have ended; zero between calls */
     /* top > 0: at most that many pages of each (sequence, kv head), which `list` names in ascending order */
     int top, first, recent;
     int *list;                        /* [n_seq][kv][top], -1 behind the last */

@@ -1,12 +1,14 @@
 /*
  * paged.hip - a KV cache in pages of 64 rows, bf16 or codes of 8 bits: rows
  * into their pages (k_pg_append) and back (k_pg_read), a decode step over them
- * (k_pg, k_pg_merge), and the choice of the pages that such a step reads
+ * (k_pg), and the choice of the pages that such a step reads
  * (k_pg_score, k_pg_select). Layouts: attn_internal.h; who takes what:
  * paged_plan.h.
  */
 #include "attn_device.h"
 #include "paged_plan.h"
+
+#include <algorithm>
 
 namespace {
 
@@ -223,66 +225,50 @@ __device__ void pg_store_row(const PgPool &p, int page, int g, int r, const floa
         ((signed char *)base)[((HD >> 4) * PG_ROWS + r) * 16 + HD % 16 + lane] = 0;
 }
 
-/* ---- the plan, by one wave: which chunk of which sequence workgroup u takes ---- */
-struct PgItem {
-    int seq, len;
-    PgUnits units;
-    int item0, chunks; /* its chunks are items item0 .. */
-};
-__device__ __forceinline__ int wave_scan(int v) { /* inclusive sums over the lanes */
-#pragma unroll
-    for (int sh = 1; sh < 64; sh <<= 1) {
-        const int x = __shfl_up(v, sh);
-        if ((int)(threadIdx.x & 63) >= sh) v += x;
-    }
+/* inclusive sums over the lanes of a wave, without LDS */
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true); /* from 1, 2, 4, 8 lanes below, within 16 */
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false); /* the 16 lanes' sums to the next 16, then to the upper half */
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
     return v;
 }
-__device__ __forceinline__ PgUnits pg_units_of(const PgParams &p, int len) {
-    return pg_units(len, p.p.stride, p.p.positions, p.window, p.top, pg_unit(p.p.codes));
-}
-/* units of a chunk of this call */
-__device__ __forceinline__ int pg_chunk_of(const PgParams &p) {
-    const int lane = threadIdx.x & 63;
-    long long sum = 0;
-    for (int b = 0; b < p.p.n_seq; b += 64) {
-        const int i = b + lane;
-        const int n = i < p.p.n_seq ? pg_units_of(p, p.len[i]).n : 0;
-        sum += __shfl(wave_scan(n), 63);
+
+/* ---- the plan, by each wave: a lane's sequence of the 64 from b on ---- */
+struct PgLane {
+    int len, off; /* its first place on the line */
+    PgUnits un;
+    int end;      /* places of all sequences up to these 64's last */
+    __device__ __forceinline__ void load(const PgParams &p, int b, int before) {
+        const int i = b + (threadIdx.x & 63);
+        len = i < p.p.n_seq ? p.len[i] : -1;
+        place(p, before);
     }
-    return __builtin_amdgcn_readfirstlane(pg_chunk(sum, p.slots));
-}
-/* by item: the one whose items hold u; otherwise sequence u itself. false: none */
-template <bool BY_ITEM>
-__device__ __forceinline__ bool pg_find(const PgParams &p, int u, int chunk, PgItem &it) {
-    const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int b = 0; b < p.p.n_seq; b += 64) {
-        const int i = b + lane;
-        const int len = i < p.p.n_seq ? p.len[i] : -1;
-        const PgUnits un = pg_units_of(p, len);
-        const int n = pg_chunks(len, un.n, chunk);
-        const int end = before + wave_scan(n);
-        const unsigned long long hit = BY_ITEM ? __ballot(end - n <= u && u < end) : __ballot(i == u && n > 0);
-        if (hit) {
-            const int from = __ffsll(hit) - 1;
-            it.seq = b + from;
-            it.len = __builtin_amdgcn_readlane(len, from);
-            it.units.first = __builtin_amdgcn_readlane(un.first, from);
-            it.units.n = __builtin_amdgcn_readlane(un.n, from);
-            it.item0 = __builtin_amdgcn_readlane(end - n, from);
-            it.chunks = __builtin_amdgcn_readlane(n, from);
-            return true;
-        }
-        if (!BY_ITEM && u < b + 64) return false;
-        before = __builtin_amdgcn_readlane(end, 63);
+    __device__ __forceinline__ void place(const PgParams &p, int before) {
+        un = pg_units(len, p.p.stride, p.p.positions, p.window, p.top, pg_unit(p.p.codes));
+        const int n = pg_places(len, un.n), upto = before + wave_scan(n);
+        off = upto - n;
+        end = __builtin_amdgcn_readlane(upto, 63);
     }
-    return false;
+};
+/* places of all sequences; s: the first 64 */
+__device__ __forceinline__ int pg_line(const PgParams &p, PgLane &s) {
+    s.load(p, 0, 0);
+    int end = s.end;
+    for (int b = 64; b < p.p.n_seq; b += 64) {
+        PgLane t;
+        t.load(p, b, end);
+        end = t.end;
+    }
+    return end;
 }
 
 /* ---- one wave's softmax state over the units it takes ---- */
 template <int HD>
 struct PgState {
-    float m, l;
+    float m, l, bad; /* bad: no number once a row was none (codes) */
     f4 o[PgGeom<HD>::DT]; /* rows: dims 4 g + i of tile dt, column: head */
 };
 
@@ -303,90 +289,122 @@ __device__ __forceinline__ void pg_raise(PgState<HD> &st, float m) {
 
 /* ------------------------------------------------------------------ decode */
 
-/* Q of a tile as the matrix operand */
+namespace {
+/* the bytes 2, 1 and 0 of four words, four of a kind in a word */
+__device__ __forceinline__ void pg_split4(const unsigned (&x)[4], int &a, int &b, int &c) {
+    const unsigned l01 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), l23 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+    const unsigned h01 = __builtin_amdgcn_perm(x[1], x[0], 0x0c0c0602u), h23 = __builtin_amdgcn_perm(x[3], x[2], 0x0c0c0602u);
+    a = (int)__builtin_amdgcn_perm(h23, h01, 0x05040100u);
+    b = (int)__builtin_amdgcn_perm(l23, l01, 0x07060302u);
+    c = (int)__builtin_amdgcn_perm(l23, l01, 0x05040100u);
+}
+} // namespace
+
+/* Q of a tile as the matrix operand, three parts: in registers, or, at head_dim 256, where they would leave room for one wave a SIMD
+ * alone, in LDS (a workgroup's waves read the same) */
 template <int HD, bool CODES>
-struct PgQ;
-template <int HD>
-struct PgQ<HD, true> {
-    i4 part[3][PgGeom<HD>::KS8]; /* digits of 65536, 256, 1 */
-    float unit;                  /* what the last digit stands for */
-    __device__ __forceinline__ void make(const float *row, bool live, int g) {
-        constexpr int KS = PgGeom<HD>::KS8;
-        float x[KS][16];
-        unsigned m = 0;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int d = 64 * ks + 16 * g + e;
-                f4 v = {0.f, 0.f, 0.f, 0.f};
-                if (live && (HD % 64 == 0 || d < HD)) v = *reinterpret_cast<const f4 *>(row + d);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[ks][e + i] = v[i];
-                    m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-                }
-            }
-        m = row_maxu4(m);
-        const float a = __uint_as_float(m);
-        /* 24-bit whole numbers against the row's largest element; a row with no number or an infinity: no numbers; one that is
-         * all but zero: zeros */
-        const float inv = m >= 0x7F800000u || a < PG_TINY ? 0.0f : PG_FIX / a;
-        unit = m >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : a < PG_TINY ? 0.0f : a / PG_FIX;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                unsigned w[3] = {0, 0, 0};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float y = rintf(x[ks][e + i] * inv);
-                    const unsigned n = pg_digits(y == y ? (int)y : 0);
-                    w[0] |= ((n >> 16) & 0xFFu) << 8 * i;
-                    w[1] |= ((n >> 8) & 0xFFu) << 8 * i;
-                    w[2] |= (n & 0xFFu) << 8 * i;
-                }
-#pragma unroll
-                for (int q = 0; q < 3; q++) part[q][ks][e / 4] = (int)w[q];
-            }
+struct PgQ {
+    static constexpr int KS = CODES ? PgGeom<HD>::KS8 : PgGeom<HD>::KSB;
+    static constexpr bool FAR = HD > 128;
+    static constexpr int LDS = FAR ? 3 * KS * 64 * 16 : 0; /* bytes */
+    typedef typename std::conditional<CODES, i4, b8>::type Part;
+    Part reg[FAR ? 1 : 3][FAR ? 1 : KS];
+    const uint4 *lds;
+    float unit; /* codes: what the last digit stands for */
+
+    __device__ __forceinline__ Part part(int q, int ks) const {
+        if constexpr (FAR) {
+            const uint4 v = lds[(q * KS + ks) * 64 + (threadIdx.x & 63)];
+            return *reinterpret_cast<const Part *>(&v);
+        } else {
+            return reg[q][ks];
+        }
     }
-};
-template <int HD>
-struct PgQ<HD, false> {
-    b8 part[3][PgGeom<HD>::KSB];
-    __device__ __forceinline__ void make(const float *row, bool live, int g) {
+    __device__ __forceinline__ void put(uint4 *to, int q, int ks, Part v) {
+        if constexpr (FAR) {
+            if (ks % PG_WAVES == (int)(threadIdx.x >> 6)) to[(q * KS + ks) * 64 + (threadIdx.x & 63)] = *reinterpret_cast<const uint4 *>(&v);
+        } else {
+            reg[q][ks] = v;
+        }
+    }
+    /* of this lane's column's row; with FAR a barrier is needed before part() */
+    __device__ __forceinline__ void make(const float *row, bool live, int g, uint4 *to) {
+        lds = to;
+        if constexpr (CODES) {
+            unsigned m = 0;
 #pragma unroll
-        for (int ks = 0; ks < PgGeom<HD>::KSB; ks++) {
-            const int d = 32 * ks + 8 * g;
-            float x[8];
+            for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = live && (HD % 32 == 0 || d < HD) ? row[d + e] : 0.0f;
+                for (int e = 0; e < 16; e += 4) {
+                    const int d = 64 * ks + 16 * g + e;
+                    f4 v = {0.f, 0.f, 0.f, 0.f};
+                    if (live && (HD % 64 == 0 || d < HD)) v = *reinterpret_cast<const f4 *>(row + d);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const __bf16 a = (__bf16)x[e];
-                const float r = x[e] - (float)a;
-                const __bf16 b = (__bf16)r;
-                part[0][ks][e] = a;
-                part[1][ks][e] = b;
-                part[2][ks][e] = (__bf16)(r - (float)b);
+                    for (int i = 0; i < 4; i++) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+                }
+            m = row_maxu4(m);
+            const float a = __uint_as_float(m);
+            /* 24-bit whole numbers against the row's largest element; a row with no number or an infinity: no numbers; one that is
+             * all but zero: zeros */
+            const float inv = m >= 0x7F800000u || a < PG_TINY ? 0.0f : PG_FIX / a;
+            unit = m >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : a < PG_TINY ? 0.0f : a / PG_FIX;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                i4 w[3];
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const int d = 64 * ks + 16 * g + e;
+                    f4 v = {0.f, 0.f, 0.f, 0.f};
+                    if (live && (HD % 64 == 0 || d < HD)) v = *reinterpret_cast<const f4 *>(row + d);
+                    unsigned n[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float y = rintf(v[i] * inv);
+                        n[i] = pg_digits(y == y ? (int)y : 0);
+                    }
+                    int a, b, c;
+                    pg_split4(n, a, b, c);
+                    w[0][e / 4] = a;
+                    w[1][e / 4] = b;
+                    w[2][e / 4] = c;
+                }
+#pragma unroll
+                for (int q = 0; q < 3; q++) put(to, q, ks, w[q]);
+            }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const int d = 32 * ks + 8 * g;
+                b8 w[3];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float x = live && (HD % 32 == 0 || d < HD) ? row[d + e] : 0.0f;
+                    const __bf16 a = (__bf16)x;
+                    const float r = x - (float)a;
+                    const __bf16 b = (__bf16)r;
+                    w[0][e] = a;
+                    w[1][e] = b;
+                    w[2][e] = (__bf16)(r - (float)b);
+                }
+#pragma unroll
+                for (int q = 0; q < 3; q++) put(to, q, ks, w[q]);
             }
         }
     }
 };
 
-/* one unit's rows in registers */
+/* One unit's rows in registers, K and V apart: K of the next unit is requested when this one's scores are formed, V when this one's is
+ * used, so something is always under way. Scales: one of K's and one of V's a lane (row = lane), laid out through LDS when needed. */
 template <int HD, bool CODES>
 struct PgUnitRegs;
 template <int HD>
 struct PgUnitRegs<HD, true> {
     i4 k[4][PgGeom<HD>::KS8], v[PgGeom<HD>::DT];
-    f4 ks[4], vs[4];
-    __device__ __forceinline__ void load(const PgPool &p, int page, int kvh, int half, int c, int g) {
+    float ks, vs;
+    __device__ __forceinline__ void load_k(const PgPool &p, int page, int kvh, int half, int c, int g) {
         const long long at = (long long)page * p.Hkv + kvh;
-        const unsigned char *kb = p.k + at * PgBytes<HD, true>::K, *vb = p.v + at * PgBytes<HD, true>::V;
-        const float *sb = p.scales + at * 2 * PG_ROWS;
-#pragma unroll
-        for (int t = 0; t < 4; t++) ks[t] = *reinterpret_cast<const f4 *>(sb + 16 * t + 4 * g);
+        const unsigned char *kb = p.k + at * PgBytes<HD, true>::K;
+        ks = p.scales[at * 2 * PG_ROWS + (threadIdx.x & 63)];
 #pragma unroll
         for (int s = 0; s < PgGeom<HD>::KS8; s++)
 #pragma unroll
@@ -395,8 +413,11 @@ struct PgUnitRegs<HD, true> {
                 k[t][s] = i4{0, 0, 0, 0};
                 if (HD % 64 == 0 || ch < PgGeom<HD>::CH8) k[t][s] = *reinterpret_cast<const i4 *>(kb + (ch * PG_ROWS + 16 * t + c) * 16);
             }
-#pragma unroll
-        for (int t = 0; t < 4; t++) vs[t] = *reinterpret_cast<const f4 *>(sb + PG_ROWS + 16 * t + 4 * g);
+    }
+    __device__ __forceinline__ void load_v(const PgPool &p, int page, int kvh, int half, int c, int g) {
+        const long long at = (long long)page * p.Hkv + kvh;
+        const unsigned char *vb = p.v + at * PgBytes<HD, true>::V;
+        vs = p.scales[(at * 2 + 1) * PG_ROWS + (threadIdx.x & 63)];
 #pragma unroll
         for (int dt = 0; dt < PgGeom<HD>::DT; dt++) {
             const int d = 16 * dt + c;
@@ -408,10 +429,8 @@ struct PgUnitRegs<HD, true> {
 template <int HD>
 struct PgUnitRegs<HD, false> {
     uint4 k[2][PgGeom<HD>::KSB], v[PgGeom<HD>::DT];
-    __device__ __forceinline__ void load(const PgPool &p, int page, int kvh, int half, int c, int g) {
-        const long long at = (long long)page * p.Hkv + kvh;
-        const unsigned char *kb = p.k + at * PgBytes<HD, false>::K + half * 512;
-        const unsigned char *vb = p.v + at * PgBytes<HD, false>::V + half * HD * 64;
+    __device__ __forceinline__ void load_k(const PgPool &p, int page, int kvh, int half, int c, int g) {
+        const unsigned char *kb = p.k + ((long long)page * p.Hkv + kvh) * PgBytes<HD, false>::K + half * 512;
 #pragma unroll
         for (int s = 0; s < PgGeom<HD>::KSB; s++)
 #pragma unroll
@@ -420,6 +439,9 @@ struct PgUnitRegs<HD, false> {
                 k[t][s] = make_uint4(0, 0, 0, 0);
                 if (HD % 32 == 0 || ch < PgGeom<HD>::CHB) k[t][s] = *reinterpret_cast<const uint4 *>(kb + (ch * PG_ROWS + 16 * t + c) * 16);
             }
+    }
+    __device__ __forceinline__ void load_v(const PgPool &p, int page, int kvh, int half, int c, int g) {
+        const unsigned char *vb = p.v + ((long long)page * p.Hkv + kvh) * PgBytes<HD, false>::V + half * HD * 64;
 #pragma unroll
         for (int dt = 0; dt < PgGeom<HD>::DT; dt++) {
             const int d = 16 * dt + c;
@@ -433,38 +455,55 @@ struct PgUnitRegs<HD, false> {
  * A score is exact up to its last sum: K's codes and the digits of Q are whole numbers, and so are their dot products. The
  * weights p vs (vs: V's scales) are taken against the unit's largest as 24-bit whole numbers, digit by digit on the matrix
  * cores again, so V needs no conversion either. */
-template <int HD>
-__device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, true> &q, PgUnitRegs<HD, true> &u, float cap2, int g, int lo, int hi) {
+template <int HD, class F>
+__device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, true> &q, PgUnitRegs<HD, true> &u, float cap2, int g, int lo, int hi,
+                                        float *lds, F next_k) {
     constexpr int DT = PgGeom<HD>::DT;
     const i4 zero = {0, 0, 0, 0};
     const bool part = lo > 0 || hi < 64;
+    const int lane = threadIdx.x & 63;
     float s[4][4];
-    if (part) { /* the scales of rows that are not seen could be anything */
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int r = 16 * t + 4 * g + i;
-                if (r < lo || r >= hi) u.ks[t][i] = u.vs[t][i] = 0.0f;
-            }
-    }
-    unsigned kbits = 0, vbits = 0;
+    /* the scales of rows that are not seen could be anything */
+    float ksc[4][4], vsc[4][4];
+    if (part && (lane < lo || lane >= hi)) u.ks = u.vs = 0.0f;
+    lds[lane] = u.ks;
+    lds[64 + lane] = u.vs;
+    wave_fence();
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-        i4 d0 = zero, d1 = zero, d2 = zero;
+        const f4 a = *reinterpret_cast<const f4 *>(lds + 16 * t + 4 * g);
 #pragma unroll
-        for (int ks = 0; ks < PgGeom<HD>::KS8; ks++) {
-            d0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(u.k[t][ks], q.part[0][ks], d0, 0, 0, 0);
-            d1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(u.k[t][ks], q.part[1][ks], d1, 0, 0, 0);
-            d2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(u.k[t][ks], q.part[2][ks], d2, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            s[t][i] = fmaf((float)d0[i], 65536.0f, fmaf((float)d1[i], 256.0f, (float)d2[i])) * (q.unit * u.ks[t][i]);
-            kbits = max(kbits, __float_as_uint(u.ks[t][i]));
-            vbits = max(vbits, __float_as_uint(u.vs[t][i]));
-        }
+        for (int i = 0; i < 4; i++) ksc[t][i] = a[i];
     }
+    const unsigned kbits = __float_as_uint(u.ks);
+    const float top = __uint_as_float(wave_max(__float_as_uint(u.vs))); /* as bits: a NaN is the largest */
+    i4 d[4][3];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        d[t][0] = d[t][1] = d[t][2] = zero;
+    }
+#pragma unroll
+    for (int ks = 0; ks < PgGeom<HD>::KS8; ks++)
+#pragma unroll
+        for (int pt = 0; pt < 3; pt++) {
+            const i4 x = q.part(pt, ks);
+#pragma unroll
+            for (int t = 0; t < 4; t++) d[t][pt] = __builtin_amdgcn_mfma_i32_16x16x64_i8(u.k[t][ks], x, d[t][pt], 0, 0, 0);
+            if (q.FAR && pt == 2) __builtin_amdgcn_sched_barrier(0); /* parts of Q are not read ahead: registers */
+        }
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            s[t][i] = fmaf((float)d[t][0][i], 65536.0f, fmaf((float)d[t][1][i], 256.0f, (float)d[t][2][i])) * (q.unit * ksc[t][i]);
+    next_k();
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const f4 a = *reinterpret_cast<const f4 *>(lds + 64 + 16 * t + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; i++) vsc[t][i] = a[i];
+    }
+    wave_fence(); /* read before the next unit's are written */
     if (cap2 > 0.0f) {
 #pragma unroll
         for (int t = 0; t < 4; t++)
@@ -484,8 +523,7 @@ __device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, true> &q,
 #pragma unroll
     for (int e = 1; e < 16; e++) mu = fmaxf(mu, s[e >> 2][e & 3]);
     mu = row_max4(mu);
-    vbits = row_maxu4(vbits);
-    const float top = __uint_as_float(vbits), f = top > 0.0f ? 1.0f / top : 0.0f;
+    const float f = top > 0.0f ? 1.0f / top : 0.0f;
     float sum = 0.0f;
     i4 w0, w1, w2;
 #pragma unroll
@@ -496,19 +534,20 @@ __device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, true> &q,
             const float pr = __builtin_amdgcn_exp2f(s[t][i] - mu);
             sum += pr;
             /* 2^23 + n: the low bits of the sum are the whole number n, rounded to nearest */
-            const float y = fmaf(pr * (u.vs[t][i] * f), PG_FIX, 8388608.0f);
+            const float y = fmaf(pr * (vsc[t][i] * f), PG_FIX, 8388608.0f);
             x[i] = (__float_as_uint(y) + 0x8080u) ^ 0x8080u;
         }
-        const unsigned l01 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), l23 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
-        const unsigned h01 = __builtin_amdgcn_perm(x[1], x[0], 0x0c0c0602u), h23 = __builtin_amdgcn_perm(x[3], x[2], 0x0c0c0602u);
-        w0[t] = (int)__builtin_amdgcn_perm(h23, h01, 0x05040100u);
-        w1[t] = (int)__builtin_amdgcn_perm(l23, l01, 0x07060302u);
-        w2[t] = (int)__builtin_amdgcn_perm(l23, l01, 0x05040100u);
+        int a, b, c;
+        pg_split4(x, a, b, c);
+        w0[t] = a;
+        w1[t] = b;
+        w2[t] = c;
     }
     pg_raise(st, mu);
     const float b = __builtin_amdgcn_exp2f(mu - st.m);
-    /* a scale that is no number, or infinite, spoils the sum */
-    st.l = fmaf(b, sum, st.l) + (0.0f * __uint_as_float(kbits) + 0.0f * top);
+    /* a scale that is no number, or infinite, spoils the sum: V's here, K's (this lane's row) when the lanes' sums are joined */
+    st.l = fmaf(b, sum, st.l) + 0.0f * top;
+    st.bad += 0.0f * __uint_as_float(kbits);
     const float bo = b * (top * (1.0f / PG_FIX));
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) {
@@ -522,20 +561,22 @@ __device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, true> &q,
 }
 
 /* A unit of 32 bf16 rows joins the state. Q and the weights are split into three bf16 parts each (24 bits). */
-template <int HD>
-__device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, false> &q, PgUnitRegs<HD, false> &u, float cap2, int g, int lo, int hi) {
+template <int HD, class F>
+__device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, false> &q, PgUnitRegs<HD, false> &u, float cap2, int g, int lo, int hi,
+                                        float *, F next_k) {
     constexpr int DT = PgGeom<HD>::DT;
     const bool part = lo > 0 || hi < 32;
-    f4 s[2];
+    f4 s[2] = {};
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-        s[t] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int pt = 2; pt >= 0; pt--)
 #pragma unroll
-        for (int pt = 2; pt >= 0; pt--)
+        for (int ks = 0; ks < PgGeom<HD>::KSB; ks++) {
+            const b8 x = q.part(pt, ks);
 #pragma unroll
-            for (int ks = 0; ks < PgGeom<HD>::KSB; ks++)
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(u.k[t][ks]), q.part[pt][ks], s[t], 0, 0, 0);
-    }
+            for (int t = 0; t < 2; t++) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(u.k[t][ks]), x, s[t], 0, 0, 0);
+            if (q.FAR && ks % 4 == 3) __builtin_amdgcn_sched_barrier(0); /* parts of Q are not read ahead: registers */
+        }
+    next_k();
     float odd = 0.0f; /* no number if a visible score is none, or infinite */
     if (part) {
         /* rows that are not seen: no score, and zeros for values (0 times an infinity is no number) */
@@ -600,22 +641,68 @@ __device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, false> &q
         for (int dt = 0; dt < DT; dt++) st.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(u.v[dt]), w[pt], st.o[dt], 0, 0, 0);
 }
 
-/* A chunk of a sequence's units against a tile of 16 heads of a kv head; the last chunk also takes the new token and stores
- * its row. */
+namespace {
+/* O and (m, l) of a chunk go to the workgroup that joins them past the caches of the XCDs */
+__device__ __forceinline__ void put_far(rsrc_t r, f4 v, unsigned off) {
+    __builtin_amdgcn_raw_buffer_store_b128(u4v{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}, r,
+                                           off, 0, CPOL_SC1);
+}
+__device__ __forceinline__ f4 get_far(rsrc_t r, unsigned off) {
+    const u4v v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, CPOL_SC1);
+    return f4{__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3])};
+}
+} // namespace
+
+/* A piece of the sequences' units against a tile of 16 heads of a kv head, sequence by sequence; a sequence's last chunk also takes the
+ * new token and stores its row. Of a sequence with several chunks the workgroup that ends last joins them, in their order. */
 template <int HD, bool CODES>
-__global__ __launch_bounds__(PG_TPB) void k_pg(const PgParams p) {
-    constexpr int XS = PgGeom<HD>::XSTR, DT = PgGeom<HD>::DT, U = CODES ? 64 : 32;
-    /* the rows of Q (scaled), the new key; then the waves' outputs */
-    __shared__ __align__(16) float s_mem[PG_WAVES * PG_HEADS * XS];
+__global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams p) {
+    constexpr bool DEEP = HD > 128; /* one wave a SIMD, whose registers hold two units */
+    constexpr int XS = PgGeom<HD>::XSTR, DT = PgGeom<HD>::DT, U = CODES ? 64 : 32, QD = HD / 4;
+    /* Q's parts (head_dim 256); then the rows of Q (scaled) and the new key, and when they are done with, the waves' outputs */
+    extern __shared__ __align__(16) unsigned char s_dyn[];
+    uint4 *s_q = reinterpret_cast<uint4 *>(s_dyn);
+    float *s_mem = reinterpret_cast<float *>(s_dyn + PgQ<HD, CODES>::LDS);
+    __shared__ __align__(16) float s_scale[PG_WAVES][CODES ? 128 : 4];
     __shared__ float s_v[HD], s_m[PG_WAVES + 1][PG_HEADS], s_l[PG_WAVES][PG_HEADS];
-    __shared__ int s_bad[PG_HEADS];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    __shared__ int s_bad[PG_HEADS], s_turn;
     const int kvh = blockIdx.y, tile = blockIdx.z, h0 = tile * PG_HEADS, R = min(PG_HEADS, p.G - h0);
-    const int chunk = pg_chunk_of(p);
-    PgItem it;
-    if (!pg_find<true>(p, blockIdx.x, chunk, it)) return;
-    const int nth = blockIdx.x - it.item0, u0 = nth * chunk, u1 = min(it.units.n, u0 + chunk);
-    const bool ok = pg_len_ok(it.len, p.p.stride, p.p.positions), last = nth == it.chunks - 1;
+    PgLane sl;
+    const int piece = pg_piece(pg_line(p, sl), p.slots), w = blockIdx.x;
+    int b0 = 0; /* the first of the 64 sequences in sl */
+    unsigned long long todo = 0;
+    bool fresh = true;
+    for (;;) {
+    /* hidden from the compiler, which else forms every address before the loop and has no registers left in it */
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    /* the next sequence that this piece holds something of: the same for all waves */
+    if (fresh) todo = __ballot(sl.len >= 0 && pg_cut(sl.off, sl.un.n, piece, w).mine);
+    fresh = false;
+    if (todo == 0) {
+        b0 += 64;
+        if (b0 >= p.p.n_seq || sl.end >= (w + 1) * piece) return;
+        sl.load(p, b0, sl.end);
+        fresh = true;
+        continue;
+    }
+    struct {
+        int seq, len, off;
+        PgUnits units;
+    } it;
+    {
+        const int from = __ffsll(todo) - 1;
+        todo &= todo - 1;
+        it.seq = b0 + from;
+        it.len = __builtin_amdgcn_readlane(sl.len, from);
+        it.off = __builtin_amdgcn_readlane(sl.off, from);
+        it.units.first = __builtin_amdgcn_readlane(sl.un.first, from);
+        it.units.n = __builtin_amdgcn_readlane(sl.un.n, from);
+    }
+    const PgCut cut = pg_cut(it.off, it.units.n, piece, w);
+    const int u0 = cut.u0, u1 = cut.u1;
+    const bool ok = pg_len_ok(it.len, p.p.stride, p.p.positions), last = cut.nth == cut.chunks - 1;
     const int *row_table = p.p.table + (long long)it.seq * p.p.stride;
     const int *list = p.top > 0 ? p.list + ((long long)it.seq * p.p.Hkv + kvh) * p.top : nullptr;
     bool bad = !ok;
@@ -629,26 +716,31 @@ __global__ __launch_bounds__(PG_TPB) void k_pg(const PgParams p) {
             const int row = list ? list[un / (PG_ROWS / U)] * PG_ROWS + un % (PG_ROWS / U) * U : (it.units.first + un) * U;
             at = row;
             page = row_table[row / PG_ROWS];
-            if (pg_bad_page(page, p.p.n_pages)) {
-                bad = true;
-                page = 0;
-            }
+        }
+    };
+    auto checked = [&](int from) { /* once the numbers are here */
+        if (from + PG_WAVES * lane < u1 && pg_bad_page(page, p.p.n_pages)) {
+            bad = true;
+            page = 0;
         }
     };
     pages(u0 + wave);
     int new_page = 0;
-    if (last && ok) {
-        new_page = row_table[it.len / PG_ROWS];
-        if (pg_bad_page(new_page, p.p.n_pages)) {
-            bad = true;
-            new_page = -1;
-        }
-    }
+    if (last && ok) new_page = row_table[it.len / PG_ROWS];
+    PgUnitRegs<HD, CODES> u[DEEP ? 2 : 1] = {}; /* (what is not set here would be carried from sequence to sequence) */
+    auto load_k = [&](PgUnitRegs<HD, CODES> &to, int n) {
+        const int row = __builtin_amdgcn_readlane(at, n), pg = __builtin_amdgcn_readlane(page, n);
+        to.load_k(p.p, pg, kvh, CODES ? 0 : row % PG_ROWS / 32, c, g);
+    };
+    auto load_v = [&](PgUnitRegs<HD, CODES> &to, int n) {
+        const int row = __builtin_amdgcn_readlane(at, n), pg = __builtin_amdgcn_readlane(page, n);
+        to.load_v(p.p, pg, kvh, CODES ? 0 : row % PG_ROWS / 32, c, g);
+    };
     {
         /* rows of Q and the new key, normalised and rotated */
         constexpr int NR = (PG_HEADS + 1 + PG_WAVES - 1) / PG_WAVES;
-        PgRow<HD> r[NR];
-        PgTurn<HD> turn;
+        PgRow<HD> r[NR] = {};
+        PgTurn<HD> turn = {};
         const int n = R + (last ? 1 : 0), pos = ok ? it.len : 0;
 #pragma unroll
         for (int k = 0; k < NR; k++) {
@@ -663,6 +755,14 @@ __global__ __launch_bounds__(PG_TPB) void k_pg(const PgParams p) {
         turn.load(p.p, pos);
         if (last)
             for (int d = tid; d < HD; d += PG_TPB) s_v[d] = in_at(p.v_in, p.in_dtype, ((long long)it.seq * p.p.Hkv + kvh) * HD + d);
+        /* the first unit is requested behind them: a compute unit returns data in the order of its requests */
+        __builtin_amdgcn_sched_barrier(0);
+        checked(u0 + wave);
+        if (u0 + wave < u1) {
+            load_k(u[0], 0);
+            load_v(u[0], 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < NR; k++) {
             const int i = wave + PG_WAVES * k;
@@ -673,32 +773,55 @@ __global__ __launch_bounds__(PG_TPB) void k_pg(const PgParams p) {
             }
         }
     }
+    if (last && ok && pg_bad_page(new_page, p.p.n_pages)) {
+        bad = true;
+        new_page = -1;
+    }
     if (tid < PG_HEADS) s_bad[tid] = 0;
     __syncthreads();
     PgQ<HD, CODES> q;
-    q.make(s_mem + c * XS, c < R, g);
+    q.make(s_mem + c * XS, c < R, g, s_q);
+    if (PgQ<HD, CODES>::FAR) __syncthreads();
 
     PgState<HD> st;
     st.m = -INFINITY;
-    st.l = 0.0f;
+    st.l = st.bad = 0.0f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) st.o[dt] = f4{0.f, 0.f, 0.f, 0.f};
     const int lo = p.top > 0 ? 0 : pg_first_row(it.len, p.window);
-    for (int un = u0 + wave, n = 0; un < u1; un += PG_WAVES, n++) {
-        if (n == 64) {
+    int un = u0 + wave, n = 0;
+    /* one unit, and the requests for the next: K when this one's scores are formed and V when this one's is used, into the same
+     * registers, or (DEEP) both beforehand into others */
+    auto step = [&](PgUnitRegs<HD, CODES> &cur, PgUnitRegs<HD, CODES> &next) {
+        const int row = __builtin_amdgcn_readlane(at, n);
+        n = (n + 1) & 63;
+        un += PG_WAVES;
+        const bool more = un < u1;
+        if (more && n == 0) {
             pages(un);
-            n = 0;
+            checked(un);
         }
-        const int row = __builtin_amdgcn_readlane(at, n), pg = __builtin_amdgcn_readlane(page, n);
-        if (row >= it.len) continue; /* the second half of a listed page that ends before it */
-        PgUnitRegs<HD, CODES> u;
-        u.load(p.p, pg, kvh, CODES ? 0 : row % PG_ROWS / 32, c, g);
-        pg_take<HD>(st, q, u, p.cap2, g, max(0, lo - row), min(U, it.len - row));
+        if (DEEP && more) {
+            load_k(next, n);
+            load_v(next, n);
+        }
+        if (DEEP) __builtin_amdgcn_sched_barrier(0);
+        auto next_k = [&]() {
+            if (!DEEP && more) load_k(next, n);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if (row < it.len) pg_take<HD>(st, q, cur, p.cap2, g, max(0, lo - row), min(U, it.len - row), s_scale[wave], next_k);
+        else next_k(); /* the second half of a listed page that ends before it */
+        if (!DEEP && more) load_v(next, n);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    while (un < u1) {
+        step(u[0], u[DEEP ? 1 : 0]);
+        if (DEEP && un < u1) step(u[DEEP ? 1 : 0], u[0]);
     }
-    if (__any(bad)) {
-        if (lane == 0) *p.p.flag = 1;
-        st.l = __uint_as_float(0x7FC00000u);
-    }
+    st.l += st.bad;
+    if (__any(bad || st.bad != st.bad)) st.l = __uint_as_float(0x7FC00000u);
+    if (__any(bad) && lane == 0) *p.p.flag = 1;
     st.l = row_sum4(st.l);
 
     if (last) {
@@ -721,99 +844,96 @@ __global__ __launch_bounds__(PG_TPB) void k_pg(const PgParams p) {
     if (c < R) {
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
-            if (HD % 16 == 0 || 16 * dt + 4 * g < HD) *reinterpret_cast<f4 *>(s_mem + (wave * PG_HEADS + c) * XS + 16 * dt + 4 * g) = st.o[dt];
+            if (HD % 16 == 0 || 16 * dt + 4 * g < HD) *reinterpret_cast<f4 *>(s_mem + (wave * R + c) * XS + 16 * dt + 4 * g) = st.o[dt];
         if (g == 0) {
             s_m[wave][c] = st.m;
             s_l[wave][c] = st.l;
         }
     }
     __syncthreads();
-    /* the waves' states and the new token's as one */
-    const bool whole = it.chunks == 1;
-    const long long prow = ((long long)kvh * p.max_items + blockIdx.x) * p.G + h0;
-    float *out = whole ? p.out + ((long long)it.seq * p.Hq + kvh * p.G + h0) * HD : p.part_o + prow * HD;
-    constexpr int QD = HD / 4;
-    auto join = [&](int e, f4 &o) {
-        const int r = e / QD, d = e % QD * 4;
-        float m = last ? s_m[PG_WAVES][r] : -INFINITY;
-        const float mn = m;
+    /* the waves' states and the new token's as one; a whole sequence's is the answer, others wait in memory */
+    const bool whole = cut.chunks == 1;
+    const int slot0 = it.units.n ? 2 * ((it.off + PG_EXTRA) / piece) : 0; /* the places of this sequence's chunks begin here */
+    const long long first = ((long long)kvh * 2 * p.slots + slot0) * p.G + h0;
+    const rsrc_t ro = make_rsrc(p.part_o + first * HD, 1LL << 31), rm = make_rsrc(p.part_ml + first * 4, 1LL << 31);
+    auto place = [&](int n, int r) { return (pg_slot(it.off, piece, n) - slot0) * p.G + r; };
+    float *out = p.out + ((long long)it.seq * p.Hq + kvh * p.G + h0) * HD;
+    constexpr int NJ = (PG_HEADS * QD + PG_TPB - 1) / PG_TPB;
+    f4 o[NJ] = {};
+#pragma unroll
+    for (int k = 0; k < NJ; k++) {
+        const int e = tid + k * PG_TPB, r = e / QD, d = e % QD * 4;
+        if (e >= R * QD) continue;
+        const float mn = last ? s_m[PG_WAVES][r] : -INFINITY;
+        float m = mn;
 #pragma unroll
         for (int w = 0; w < PG_WAVES; w++) m = fmaxf(m, s_m[w][r]);
         float l = 0.0f;
-        o = f4{0.f, 0.f, 0.f, 0.f};
+        f4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < PG_WAVES; w++) {
             const float lw = s_l[w][r], f = s_m[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[w][r] - m);
             l = fmaf(f, lw, l);
             if (lw != lw) l = lw; /* a wave that saw nothing but rows that are no numbers */
-            o += *reinterpret_cast<const f4 *>(s_mem + (w * PG_HEADS + r) * XS + d) * f;
+            a += *reinterpret_cast<const f4 *>(s_mem + (w * R + r) * XS + d) * f;
         }
         if (last) {
             const float f = mn != mn ? mn : __builtin_amdgcn_exp2f(mn - m);
             l += f;
-            o += *reinterpret_cast<const f4 *>(s_v + d) * f;
+            a += *reinterpret_cast<const f4 *>(s_v + d) * f;
         }
-        if (!whole) {
-            if (d == 0) {
-                p.part_ml[(prow + r) * 2] = m;
-                p.part_ml[(prow + r) * 2 + 1] = l;
-            }
-            return;
+        if (whole) {
+            a *= 1.0f / l;
+            /* what is not finite in one dim spoils the row */
+            if (!(fabsf(a[0]) + fabsf(a[1]) + fabsf(a[2]) + fabsf(a[3]) < INFINITY)) s_bad[r] = 1;
+        } else {
+            put_far(ro, a, (place(cut.nth, r) * HD + d) * 4);
+            if (d == 0) put_far(rm, f4{m, l, 0.f, 0.f}, place(cut.nth, r) * 16);
         }
-        o *= 1.0f / l;
-        /* what is not finite in one dim spoils the row */
-        if (!(fabsf(o[0]) + fabsf(o[1]) + fabsf(o[2]) + fabsf(o[3]) < INFINITY)) s_bad[r] = 1;
-    };
-    constexpr int NJ = (PG_HEADS * QD + PG_TPB - 1) / PG_TPB;
-    f4 o[NJ];
-#pragma unroll
-    for (int k = 0; k < NJ; k++)
-        if (tid + k * PG_TPB < R * QD) join(tid + k * PG_TPB, o[k]);
-    if (whole) __syncthreads();
-#pragma unroll
-    for (int k = 0; k < NJ; k++) {
-        const int e = tid + k * PG_TPB;
-        if (e >= R * QD) continue;
-        if (whole && s_bad[e / QD]) o[k] = f4{NAN, NAN, NAN, NAN};
-        *reinterpret_cast<f4 *>(out + (long long)e * 4) = o[k];
-    }
-}
-
-/* Joins the chunks of a sequence that has more than one: a workgroup a (sequence, kv head) */
-template <int HD>
-__global__ __launch_bounds__(PG_TPB) void k_pg_merge(const PgParams p) {
-    constexpr int QD = HD / 4;
-    __shared__ int s_bad[PG_HEADS];
-    const int tid = threadIdx.x, kvh = blockIdx.y, h0 = blockIdx.z * PG_HEADS, R = min(PG_HEADS, p.G - h0);
-    const int chunk = pg_chunk_of(p);
-    PgItem it;
-    if (!pg_find<false>(p, blockIdx.x, chunk, it) || it.chunks == 1) return;
-    if (tid < PG_HEADS) s_bad[tid] = 0;
-    __syncthreads();
-    const long long base = ((long long)kvh * p.max_items + it.item0) * p.G + h0;
-    float *out = p.out + ((long long)it.seq * p.Hq + kvh * p.G + h0) * HD;
-    constexpr int NJ = (PG_HEADS * QD + PG_TPB - 1) / PG_TPB;
-    f4 o[NJ];
-#pragma unroll
-    for (int k = 0; k < NJ; k++) {
-        const int e = tid + k * PG_TPB, r = e / QD, d = e % QD * 4;
-        if (e >= R * QD) continue;
-        float m = -INFINITY, l = 0.0f;
-        f4 a = {0.f, 0.f, 0.f, 0.f};
-        for (int n = 0; n < it.chunks; n++) {
-            const long long row = base + (long long)n * p.G + r;
-            const float mc = p.part_ml[row * 2], lc = p.part_ml[row * 2 + 1];
-            const f4 oc = *reinterpret_cast<const f4 *>(p.part_o + row * HD + d);
-            const float mn = fmaxf(m, mc), fa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-            const float fb = mc == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mc - mn);
-            l = l * fa + lc * fb;
-            if (lc != lc) l = lc;
-            a = a * fa + oc * fb;
-            m = mn;
-        }
-        a *= 1.0f / l;
-        if (!(fabsf(a[0]) + fabsf(a[1]) + fabsf(a[2]) + fabsf(a[3]) < INFINITY)) s_bad[r] = 1;
         o[k] = a;
+    }
+    if (!whole) {
+        /* what this workgroup wrote has arrived where others read before it counts itself in; the count starts anew by itself */
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) s_turn = (int)atomicInc(p.count + ((long long)it.seq * p.p.Hkv + kvh) * p.tiles + tile, cut.chunks - 1);
+        __syncthreads();
+        if (s_turn != cut.chunks - 1) continue;
+#pragma unroll
+        for (int k = 0; k < NJ; k++) {
+            const int e = tid + k * PG_TPB, r = e / QD, d = e % QD * 4;
+            if (e >= R * QD) continue;
+            float m = -INFINITY, l = 0.0f;
+            f4 a = {0.f, 0.f, 0.f, 0.f};
+            constexpr int B = 8; /* chunks in flight */
+            for (int n0 = 0; n0 < cut.chunks; n0 += B) {
+                f4 ml[B], oc[B];
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    const int n = min(n0 + b, cut.chunks - 1);
+                    ml[b] = get_far(rm, place(n, r) * 16);
+                    oc[b] = get_far(ro, (place(n, r) * HD + d) * 4);
+                }
+                float mn = m;
+#pragma unroll
+                for (int b = 0; b < B; b++) mn = fmaxf(mn, ml[b][0]);
+                const float fa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+                l *= fa;
+                a *= fa;
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    if (n0 + b >= cut.chunks) break;
+                    const float f = ml[b][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[b][0] - mn);
+                    l = fmaf(ml[b][1], f, l);
+                    if (ml[b][1] != ml[b][1]) l = ml[b][1];
+                    a += oc[b] * f;
+                }
+                m = mn;
+            }
+            a *= 1.0f / l;
+            if (!(fabsf(a[0]) + fabsf(a[1]) + fabsf(a[2]) + fabsf(a[3]) < INFINITY)) s_bad[r] = 1;
+            o[k] = a;
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -822,6 +942,8 @@ __global__ __launch_bounds__(PG_TPB) void k_pg_merge(const PgParams p) {
         if (e >= R * QD) continue;
         if (s_bad[e / QD]) o[k] = f4{NAN, NAN, NAN, NAN};
         *reinterpret_cast<f4 *>(out + (long long)e * 4) = o[k];
+    }
+    __syncthreads();
     }
 }
 
@@ -1628,8 +1750,8 @@ __global__ __launch_bounds__(PG_TPB) void k_pg_read(const PgRunParams p) {
 #define PG_HEADS_FROM 2048
 #endif
 
-/* workgroups of k_pg on a compute unit */
-extern "C" int smol_paged_occupancy(int hd, int codes) { return 2; }
+/* workgroups of k_pg on a compute unit (registers) */
+extern "C" int smol_paged_occupancy(int hd) { return hd > 128 ? 1 : 2; }
 
 extern "C" int smol_launch_pages(const PgRunParams *pp, int hd, int write, hipStream_t st, hipEvent_t e0, hipEvent_t e1) {
     PgRunParams args = *pp, *p = &args;
@@ -1662,11 +1784,11 @@ extern "C" int smol_launch_paged(const PgParams *p, int hd, hipStream_t st, hipE
         if (p->p.stride <= PS_LDS) hipExtLaunchKernelGGL(k_pg_select<true>, gl, tpb, 0, st, nullptr, nullptr, 0, *p);
         else hipExtLaunchKernelGGL(k_pg_select<false>, gl, tpb, 0, st, nullptr, nullptr, 0, *p);
     }
-    const dim3 grid(p->max_items, p->p.Hkv, p->tiles), gm(p->p.n_seq, p->p.Hkv, p->tiles);
+    const dim3 grid(p->slots, p->p.Hkv, p->tiles);
+    const int rows = std::max(2, PG_WAVES * std::min(p->G, PG_HEADS)); /* of s_mem: the waves' outputs, never fewer than Q and the key */
 #define PG_STEP(HD) \
-    if (p->p.codes) hipExtLaunchKernelGGL((k_pg<HD, true>), grid, tpb, 0, st, first, nullptr, 0, *p); \
-    else hipExtLaunchKernelGGL((k_pg<HD, false>), grid, tpb, 0, st, first, nullptr, 0, *p); \
-    hipExtLaunchKernelGGL(k_pg_merge<HD>, gm, tpb, 0, st, nullptr, e1, 0, *p)
+    if (p->p.codes) hipExtLaunchKernelGGL((k_pg<HD, true>), grid, tpb, PgQ<HD, true>::LDS + rows * PgGeom<HD>::XSTR * 4, st, first, e1, 0, *p); \
+    else hipExtLaunchKernelGGL((k_pg<HD, false>), grid, tpb, PgQ<HD, false>::LDS + rows * PgGeom<HD>::XSTR * 4, st, first, e1, 0, *p)
     PG_BY_HD(hd, PG_STEP)
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }

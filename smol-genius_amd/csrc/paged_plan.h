@@ -4,12 +4,12 @@
  * and device, so that a CPU test covers it with every length and page number.
  *
  * A sequence of `len` cached rows and a table of `stride` pages: rows
- * [lo, len) are visible, cut into units of PG_UNIT rows (64 codes rows, or 32
- * bf16 rows, what one round of matrix products takes), and the units into
- * chunks, one workgroup each. The lengths are on the device, so every
- * workgroup forms the cut for itself from the sum of all sequences' units:
- * chunks of equal length, as short as leaves at most `slots` whole chunks and
- * one short one a sequence.
+ * [lo, len) are visible, cut into units (64 rows of codes, or 32 bf16 rows: what
+ * one round of matrix products takes). The sequences' units lie on one line,
+ * each sequence behind PG_EXTRA places that stand for its start-up, and every
+ * workgroup takes a piece of that line of the same length: all of them end
+ * together, whatever the lengths, and their number is fixed by the machine.
+ * The lengths are on the device, so each workgroup forms the line for itself.
  */
 #ifndef SMOL_PAGED_PLAN_H
 #define SMOL_PAGED_PLAN_H
@@ -52,18 +52,45 @@ PG_FN PgUnits pg_units(int len, int stride, int positions, int window, int top, 
     return u;
 }
 
-/* units of a chunk */
-PG_FN int pg_chunk(long long sum, int slots) {
+/* What the start of a sequence costs a workgroup, in units: its rows of Q, and no unit under way before them. */
+#define PG_EXTRA 12
+
+/* places of a sequence on the line */
+PG_FN int pg_places(int len, int units) { return len < 0 ? 0 : PG_EXTRA + units; }
+
+/* places of a piece, for `sum` of them in all: at most `slots` pieces */
+PG_FN int pg_piece(long long sum, int slots) {
     long long c = (sum + slots - 1) / slots;
     c = (c + PG_WAVES - 1) / PG_WAVES * PG_WAVES;
     return c < PG_WAVES ? PG_WAVES : (int)c;
 }
 
-/* chunks of a sequence: one at least, which takes the new token; none for what is no sequence */
-PG_FN int pg_chunks(int len, int units, int chunk) { return len < 0 ? 0 : units == 0 ? 1 : (units + chunk - 1) / chunk; }
-
-/* workgroups that the chunks of n sequences need at most */
-PG_FN long long pg_max_chunks(int n, int slots) { return (long long)slots + n; }
+/* What piece w holds of a sequence whose places begin at `off`: units [u0, u1), of which it is number `nth` of `chunks` pieces; a sequence
+ * without units belongs to the piece with its first place. A chunk of several leaves its state in place `slot`: 2 w when it is the
+ * first of its piece, 2 w + 1 when it begins behind others; no piece has two of either. */
+struct PgCut {
+    bool mine;
+    int u0, u1, nth, chunks;
+};
+PG_FN PgCut pg_cut(int off, int units, int piece, int w) {
+    PgCut c = {false, 0, 0, 0, 1};
+    const int at = off + PG_EXTRA, lo = w * piece, hi = lo + piece;
+    if (units == 0) {
+        c.mine = off >= lo && off < hi;
+        return c;
+    }
+    c.u0 = lo > at ? lo - at : 0;
+    c.u1 = hi < at + units ? hi - at : units;
+    c.mine = c.u0 < c.u1;
+    const int first = at / piece;
+    c.nth = w - first;
+    c.chunks = (at + units - 1) / piece - first + 1;
+    return c;
+}
+PG_FN int pg_slot(int off, int piece, int nth) {
+    const int at = off + PG_EXTRA, first = at / piece;
+    return nth == 0 && at % piece ? 2 * first + 1 : 2 * (first + nth);
+}
 
 /* a page number that is none of the pool's */
 PG_FN bool pg_bad_page(int page, int n_pages) { return page < 0 || page >= n_pages; }

@@ -400,6 +400,8 @@ DECODE = [
     # more heads a kv head than a tile has
     dict(hq=17, hkv=1, hd=64, lens=[70, 0, 200]),
     dict(hq=40, hkv=1, hd=128, lens=[130], cap=50.0),
+    dict(hq=16, hkv=1, hd=256, lens=[130, 2000]),
+    dict(hq=33, hkv=1, hd=256, lens=[90, 1], inter=True),
     # more sequences than a wave has lanes, some of them none
     dict(hq=2, hkv=1, hd=64, lens=[(7 * i) % 150 if i % 9 else -1 for i in range(150)]),
     # windows: one row, within a page, over pages, longer than all

@@ -21,9 +21,13 @@ int units(int len, int stride, int positions, int window, int top, int unit, int
 }
 int len_ok(int len, int stride, int positions) { return pg_len_ok(len, stride, positions); }
 int first_row(int len, int window) { return pg_first_row(len, window); }
-int chunk(long long sum, int slots) { return pg_chunk(sum, slots); }
-int chunks(int len, int units, int c) { return pg_chunks(len, units, c); }
-long long max_chunks(int n, int slots) { return pg_max_chunks(n, slots); }
+int piece(long long sum, int slots) { return pg_piece(sum, slots); }
+int places(int len, int units) { return pg_places(len, units); }
+void cut(int off, int units, int piece, int w, int *out) {
+    PgCut c = pg_cut(off, units, piece, w);
+    out[0] = c.mine, out[1] = c.u0, out[2] = c.u1, out[3] = c.nth, out[4] = c.chunks;
+}
+int slot(int off, int piece, int nth) { return pg_slot(off, piece, nth); }
 int bad_page(int page, int n) { return pg_bad_page(page, n); }
 int order(int r, int codes) { return pg_order(r, codes != 0); }
 int run_ok(int a, int b, int rows, int pos, int stride, int positions) { return pg_run_ok(a, b, rows, pos, stride, positions); }
@@ -45,14 +49,14 @@ def plan(tmp_path_factory):
     subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-shared",
                     "-fPIC", "-I" + inc, str(src), "-o", str(so)], check=True)
     lib = ctypes.CDLL(str(so))
-    for f in ("max_chunks", "max_run_pages"):
-        getattr(lib, f).restype = ctypes.c_longlong
-    lib.chunk.argtypes = [ctypes.c_longlong, ctypes.c_int]
+    lib.max_run_pages.restype = ctypes.c_longlong
+    lib.piece.argtypes = [ctypes.c_longlong, ctypes.c_int]
     lib.digits.restype = ctypes.c_uint
     return lib
 
 
 INT_MAX = 2 ** 31 - 1
+EXTRA = 12  # PG_EXTRA
 WILD = [-2 ** 31, -1, 0, 1, 31, 32, 33, 63, 64, 65, 127, 128, 1000, 4095, 4096, 4097, INT_MAX - 64, INT_MAX - 1, INT_MAX]
 
 
@@ -85,27 +89,45 @@ def test_lengths(plan):
 
 
 @pytest.mark.parametrize("seed", range(6))
-def test_chunks_cover_every_unit_once(plan, seed):
-    """the workgroups that the host starts are enough, and their chunks share every sequence's units out"""
+def test_pieces_cover_every_unit_once(plan, seed):
+    """the workgroups that the host starts share every sequence's units out, each live sequence has one last chunk, no sequence none,
+    and no two chunks leave their state in one place"""
     r = random.Random(seed)
-    first = ctypes.c_int()
-    for _ in range(300):
-        n, stride = r.choice([1, 2, 5, 64, 65, 200]), r.choice([1, 4, 64, 300])
-        unit, window, slots = r.choice([32, 64]), r.choice([0, 0, 1, 100]), r.choice([1, 2, 7, 64, 512])
+    first, out = ctypes.c_int(), (ctypes.c_int * 5)()
+    for _ in range(120):
+        n, stride = r.choice([1, 2, 5, 64, 65, 130]), r.choice([1, 4, 64, 300])
+        unit, window, slots = r.choice([32, 64]), r.choice([0, 0, 1, 100]), r.choice([1, 2, 7, 64, 256])
         top = r.choice([0, 0, 3, 40]) if not window else 0
         lens = [r.choice(WILD + [r.randrange(stride * 64) for _ in range(20)]) for _ in range(n)]
         counts = [plan.units(l, stride, INT_MAX, window, top, unit, ctypes.byref(first)) for l in lens]
-        c = plan.chunk(sum(counts), slots)
-        assert c >= 4 and c % 4 == 0
-        each = [plan.chunks(l, k, c) for l, k in zip(lens, counts)]
-        assert sum(each) <= plan.max_chunks(n, slots)
-        for l, k, e in zip(lens, counts, each):
+        places = [plan.places(l, k) for l, k in zip(lens, counts)]
+        assert all(p == (0 if l < 0 else EXTRA + k) for p, l, k in zip(places, lens, counts))
+        c = plan.piece(sum(places), slots)
+        assert c >= 4 and c % 4 == 0 and c * slots >= sum(places)
+        used, off = set(), 0
+        for l, k, p in zip(lens, counts, places):
             if l < 0:
-                assert e == 0  # no sequence: no workgroup, nothing read, nothing written
-                continue
-            got = [u for w in range(e) for u in range(w * c, min(k, (w + 1) * c))]
-            assert e >= 1 and got == list(range(k))
-            assert e == 1 or all(w * c < k for w in range(e))
+                continue  # the kernel asks no piece about it
+            got, chunks = [], None
+            for w in range(max(0, off // c - 1), min(slots, (off + p) // c + 2)):
+                plan.cut(off, k, c, w, out)
+                mine, u0, u1, nth, chunks = out[:]
+                if not mine:
+                    continue
+                assert nth == len(got) and off // c <= w <= (off + p) // c
+                got.append((u0, u1))
+                if chunks > 1:
+                    s = plan.slot(off, c, nth)
+                    assert s // 2 == w and s < 2 * slots and s not in used
+                    assert s >= 2 * ((off + EXTRA) // c)  # where the sequence's places begin
+                    used.add(s)
+            assert len(got) == chunks
+            if k == 0:
+                assert got == [(0, 0)]
+            else:
+                assert got[0][0] == 0 and got[-1][1] == k and all(a < b for a, b in got)
+                assert all(a[1] == b[0] for a, b in zip(got, got[1:]))
+            off += p
 
 
 def test_page_numbers(plan):
