@@ -189,40 +189,55 @@ __device__ __forceinline__ float max_nan(float a, float b) { return a != a ? a :
 /* One row (HD values in LDS) into row r of page `page`, by one wave: K pieces or V's column, scale, and for K the page's bounds */
 template <int HD, bool CODES, bool KEY>
 __device__ void pg_store_row(const PgPool &p, int page, int g, int r, const float *x) {
+    constexpr int NE = PgGeom<HD>::NE;
     const int lane = threadIdx.x & 63;
     const long long at = (long long)page * p.Hkv + g;
+    uint16_t *bounds = p.bounds + at * 2 * HD;
+    float lo[NE], hi[NE], v[NE];
     PgScale sc = {0.0f, 0.0f};
+    unsigned m = 0;
+#pragma unroll
+    for (int e = 0; e < NE; e++) {
+        const int d = lane + 64 * e;
+        lo[e] = INFINITY;
+        hi[e] = -INFINITY;
+        v[e] = 0.0f;
+        if (HD % 64 != 0 && d >= HD) continue;
+        v[e] = x[d];
+        if (KEY && r > 0) {
+            lo[e] = bf16_to_f32(bounds[d]);
+            hi[e] = bf16_to_f32(bounds[HD + d]);
+        }
+        m = max(m, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    }
     if (CODES) {
-        unsigned m = 0;
-        for (int d = lane; d < HD; d += 64) m = max(m, __float_as_uint(x[d]) & 0x7FFFFFFFu);
         sc = pg_scale(wave_max(m));
         if (lane == 0) p.scales[(at * 2 + (KEY ? 0 : 1)) * PG_ROWS + r] = sc.s;
     }
     unsigned char *base = KEY ? p.k + at * PgBytes<HD, CODES>::K : p.v + at * PgBytes<HD, CODES>::V;
-    for (int d = lane; d < HD; d += 64) {
-        float kept;
+#pragma unroll
+    for (int e = 0; e < NE; e++) {
+        const int d = lane + 64 * e;
+        if (HD % 64 != 0 && d >= HD) continue;
         if (CODES) {
-            const float y = pg_code(x[d], sc.inv);
+            const float y = pg_code(v[e], sc.inv);
             const unsigned char c = (unsigned char)__float_as_uint(y);
-            kept = (y - PG_MAGIC) * sc.s;
+            v[e] = (y - PG_MAGIC) * sc.s;
             if (KEY) base[((d >> 4) * PG_ROWS + r) * 16 + (d & 15)] = c;
             else base[d * PG_ROWS + pg_order(r, true)] = c;
         } else {
-            const uint16_t b = bf16_of(x[d]);
-            kept = bf16_to_f32(b);
+            const uint16_t b = bf16_of(v[e]);
+            v[e] = bf16_to_f32(b);
             if (KEY) ((uint16_t *)base)[((d >> 3) * PG_ROWS + r) * 8 + (d & 7)] = b;
             else ((uint16_t *)base)[((r >> 5) * HD + d) * 32 + (pg_order(r, false) & 31)] = b;
         }
         if (KEY) {
-            uint16_t *lo = p.bounds + at * 2 * HD + d, *hi = lo + HD;
-            const float a = r == 0 ? kept : min_nan(kept, bf16_to_f32(*lo)), b = r == 0 ? kept : max_nan(kept, bf16_to_f32(*hi));
-            *lo = bf16_down(a);
-            *hi = bf16_up(b);
+            bounds[d] = bf16_down(min_nan(lo[e], v[e]));
+            bounds[HD + d] = bf16_up(max_nan(hi[e], v[e]));
         }
     }
     /* the padding of a row's last piece */
-    if (KEY && CODES && HD % 16 != 0 && lane < 16 - HD % 16)
-        ((signed char *)base)[((HD >> 4) * PG_ROWS + r) * 16 + HD % 16 + lane] = 0;
+    if (KEY && CODES && HD % 16 != 0 && lane < 16 - HD % 16) base[((HD >> 4) * PG_ROWS + r) * 16 + HD % 16 + lane] = 0;
 }
 
 /* inclusive sums over the lanes of a wave, without LDS */
