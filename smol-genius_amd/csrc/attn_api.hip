@@ -2439,6 +2439,10 @@ static int decode_paged(smol_attn_ctx *ctx, smol_kv_pages *kp, int layer, const 
     pg.part_ml = (float *)(w + o_ml);
     pg.list = chosen ? chosen : (int *)(w + o_list);
     pg.score = (double *)(w + o_score);
+    /* A workgroup spends 5 us on Q's sums before its first score: 64 pages each while that fills no more than the machine, more where
+     * the workgroups would wait for each other */
+    pg.per = 64;
+    while (pg.per < 1024 && (long long)n_seq * Hkv * ((stride + pg.per - 1) / pg.per) > 8LL * ctx->cu_count) pg.per *= 2;
     const int mk = timing_begin(ctx, 1);
     rc = smol_launch_paged(&pg, hd, ctx->stream, mark_a(ctx, mk), mark_b(ctx, mk));
     if (rc) return fail(SMOL_ATTN_ERR_DEVICE, "paged decode (hd %d): %s", hd, hipGetErrorString(hipGetLastError()));

@@ -354,7 +354,7 @@ typedef struct {
     int heads;                        /* kv heads of a workgroup */
 } PgRunParams;
 
-/* k_pg, k_pg_score, k_pg_select: a decode step */
+/* k_pg, k_pg_choose: a decode step */
 typedef struct {
     PgPool p;
     const int *len;                   /* [n_seq] cached rows; the new token becomes row len */
@@ -371,7 +371,8 @@ typedef struct {
     /* top > 0: at most that many pages of each (sequence, kv head), which `list` names in ascending order */
     int top, first, recent;
     int *list;                        /* [n_seq][kv][top], -1 behind the last */
-    double *score;                    /* [n_seq][kv][stride] */
+    double *score;                    /* [n_seq][kv][stride], as keys of the same order */
+    int per;                          /* pages of a k_pg_choose workgroup, a multiple of 64 */
 } PgParams;
 
 /* ---- k_gemm (gemm.hip), k_gemm_rs (gemm_rs.hip) and k_gemm_sw (gemm_sw.hip): the projections on bf16 MFMA ---- */

@@ -2,7 +2,7 @@
  * paged.hip - a KV cache in pages of 64 rows, bf16 or codes of 8 bits: rows
  * into their pages (k_pg_append) and back (k_pg_read), a decode step over them
  * (k_pg), and the choice of the pages that such a step reads
- * (k_pg_score, k_pg_select). Layouts: attn_internal.h; who takes what:
+ * (k_pg_choose). Layouts: attn_internal.h; who takes what:
  * paged_plan.h.
  */
 #include "attn_device.h"
@@ -965,86 +965,95 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
 /* ------------------------------------------------------- which pages to read */
 
 namespace {
-constexpr int PS_PAGES = 64;   /* pages of a k_pg_score workgroup */
 constexpr int PS_BINS = 2048;
-constexpr int PS_LDS = 4096;   /* pages whose keys k_pg_select keeps in LDS */
+constexpr int PS_LDS = 4096; /* pages whose keys a choosing workgroup keeps in LDS */
+typedef unsigned u2w __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ int pg_pages(int len) { return (len + PG_ROWS - 1) / PG_ROWS; }
-} // namespace
 
 /* score = sum over the heads of a kv head and the dims of max(q lo, q hi): an upper bound of the sum of a page's scores,
  * q+ . hi + q- . lo with q+ (q-) the sums of the heads' positive (negative) elements, so a page costs two products whatever the
  * number of heads. In 64 bits, and a page's terms in one order whatever the page: pages with equal bounds tie. */
 template <int HD>
-__global__ __launch_bounds__(PG_TPB) void k_pg_score(const PgParams p) {
-    constexpr int LPP = HD <= 64 ? 8 : HD <= 128 ? 16 : 32, NE = PgGeom<HD>::NE;
-    __shared__ double s_row[PG_WAVES][HD], s_sum[PG_WAVES][2][HD];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kvh = blockIdx.y;
-    const int blocks = (p.p.stride + PS_PAGES - 1) / PS_PAGES, seq = blockIdx.x / blocks, j0 = blockIdx.x % blocks * PS_PAGES;
-    const int len = p.len[seq];
-    if (!pg_len_ok(len, p.p.stride, p.p.positions)) return;
-    const int pages = pg_pages(len);
-    if (pages <= p.top || j0 >= pages) return;
-    PgTurn<HD> turn;
-    turn.load(p.p, len);
-    double up[NE], dn[NE];
+struct PgScore {
+    static constexpr int LPP = HD <= 64 ? 8 : HD <= 128 ? 16 : 32; /* lanes of a page, eight dims each */
+    double up[8], dn[8];
+
+    /* q+ and q- of a sequence and kv head, the heads by the waves in turn, through LDS; then this lane's dims of them. All threads of
+     * the workgroup call; next(): what is requested behind the first head's row */
+    template <class F>
+    __device__ __forceinline__ void make(const PgParams &p, int seq, int kvh, int len, double (*s_row)[HD], double (*s_sum)[2][HD], F next) {
+        constexpr int NE = PgGeom<HD>::NE;
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        PgTurn<HD> turn;
+        turn.load(p.p, len);
+        double u[NE], d[NE];
 #pragma unroll
-    for (int e = 0; e < NE; e++) up[e] = dn[e] = 0.0;
-    for (int h = wave; h < p.G; h += PG_WAVES) {
+        for (int e = 0; e < NE; e++) u[e] = d[e] = 0.0;
         PgRow<HD> r;
-        r.load(p.q_in, p.in_dtype, ((long long)seq * p.Hq + kvh * p.G + h) * HD, p.q_norm);
-        pg_finish<HD, double>(r, p.q_norm != nullptr, p.norm_eps, turn, p.p.rope_kind, p.scale, s_row[wave]);
+        auto request = [&](int h) { r.load(p.q_in, p.in_dtype, ((long long)seq * p.Hq + kvh * p.G + h) * HD, p.q_norm); };
+        request(min(wave, p.G - 1));
+        __builtin_amdgcn_sched_barrier(0);
+        next();
+        __builtin_amdgcn_sched_barrier(0);
+        for (int h = wave; h < p.G; h += PG_WAVES) {
+            const PgRow<HD> now = r;
+            if (h + PG_WAVES < p.G) request(h + PG_WAVES);
+            pg_finish<HD, double>(now, p.q_norm != nullptr, p.norm_eps, turn, p.p.rope_kind, p.scale, s_row[wave]);
 #pragma unroll
-        for (int e = 0; e < NE; e++) {
-            if (HD % 64 != 0 && lane + 64 * e >= HD) continue;
-            const double x = s_row[wave][lane + 64 * e];
-            up[e] += x > 0.0 ? x : 0.0; /* a NaN makes none of both */
-            dn[e] += x > 0.0 ? 0.0 : x;
+            for (int e = 0; e < NE; e++) {
+                if (HD % 64 != 0 && lane + 64 * e >= HD) continue;
+                const double x = s_row[wave][lane + 64 * e];
+                u[e] += x > 0.0 ? x : 0.0;
+                d[e] += x > 0.0 ? 0.0 : x; /* takes a NaN */
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < NE; e++)
+            if (HD % 64 == 0 || lane + 64 * e < HD) {
+                s_sum[wave][0][lane + 64 * e] = u[e];
+                s_sum[wave][1][lane + 64 * e] = d[e];
+            }
+        __syncthreads();
+        const int waves = min(p.G, PG_WAVES);
+        for (int e = tid; e < 2 * HD; e += PG_TPB) {
+            double x = s_sum[0][0][e];
+            for (int w = 1; w < waves; w++) x += s_sum[w][0][e];
+            s_sum[0][0][e] = x;
+        }
+        __syncthreads();
+        const int ch = lane % LPP;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            up[i] = 8 * ch < HD ? s_sum[0][0][8 * ch + i] : 0.0;
+            dn[i] = 8 * ch < HD ? s_sum[0][1][8 * ch + i] : 0.0;
         }
     }
-#pragma unroll
-    for (int e = 0; e < NE; e++)
-        if (HD % 64 == 0 || lane + 64 * e < HD) {
-            s_sum[wave][0][lane + 64 * e] = up[e];
-            s_sum[wave][1][lane + 64 * e] = dn[e];
-        }
-    __syncthreads();
-    const int ch = lane % LPP;
-    const bool live = 8 * ch < HD;
-    double u[8], d[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        u[i] = d[i] = 0.0;
-        if (!live) continue;
-#pragma unroll
-        for (int w = 0; w < PG_WAVES; w++) {
-            u[i] += s_sum[w][0][8 * ch + i];
-            d[i] += s_sum[w][1][8 * ch + i];
-        }
+    struct Bounds {
+        uint4 lo, hi;
+    };
+    __device__ __forceinline__ void load(const PgPool &p, int page, int kvh, Bounds &b) const {
+        const int ch = threadIdx.x % LPP;
+        b.lo = b.hi = make_uint4(0, 0, 0, 0);
+        if (8 * ch >= HD) return;
+        const uint16_t *at = p.bounds + ((long long)page * p.Hkv + kvh) * 2 * HD + 8 * ch;
+        b.lo = *reinterpret_cast<const uint4 *>(at);
+        b.hi = *reinterpret_cast<const uint4 *>(at + HD);
     }
-    const int *row_table = p.p.table + (long long)seq * p.p.stride;
-    double *score = p.score + ((long long)seq * p.p.Hkv + kvh) * p.p.stride;
-    for (int j = j0 + tid / LPP; j < min(j0 + PS_PAGES, (pages + 63) & ~63); j += PG_TPB / LPP) {
+    /* the score, in all lanes of the page */
+    __device__ __forceinline__ double of(const Bounds &b) const {
+        float lo[8], hi[8];
+        unpack_bf16x8(b.lo, lo);
+        unpack_bf16x8(b.hi, hi);
         double s = 0.0;
-        bool bad = false;
-        if (j < pages && live) {
-            int page = row_table[j];
-            if ((bad = pg_bad_page(page, p.p.n_pages))) page = 0;
-            const uint16_t *b = p.p.bounds + ((long long)page * p.p.Hkv + kvh) * 2 * HD + 8 * ch;
-            float lo[8], hi[8];
-            unpack_bf16x8(*reinterpret_cast<const uint4 *>(b), lo);
-            unpack_bf16x8(*reinterpret_cast<const uint4 *>(b + HD), hi);
 #pragma unroll
-            for (int i = 0; i < 8; i++) s = fma(u[i], (double)hi[i], fma(d[i], (double)lo[i], s));
-        }
+        for (int i = 0; i < 8; i++) s = fma(up[i], (double)hi[i], fma(dn[i], (double)lo[i], s));
 #pragma unroll
         for (int sh = LPP / 2; sh; sh >>= 1) s += __shfl_xor(s, sh);
-        if (bad) s = __longlong_as_double(0x7FF8000000000000LL);
-        if (j < pages && ch == 0) score[j] = s;
+        return s;
     }
-}
+};
 
-namespace {
 /* a score as a whole number of the same order: what stays by its place above all, then NaN, then the numbers (-0 as 0) */
 __device__ __forceinline__ unsigned long long pg_key(double s, int j, int pages, int first, int recent) {
     if (j < first || j >= pages - recent) return ~0ULL;
@@ -1052,35 +1061,37 @@ __device__ __forceinline__ unsigned long long pg_key(double s, int j, int pages,
     const unsigned long long u = s == 0.0 ? 0ULL : (unsigned long long)__double_as_longlong(s);
     return u >> 63 ? ~u : u | 0x8000000000000000ULL;
 }
-} // namespace
 
-/* The `top` pages of the largest keys of one (sequence, kv head), in ascending order. The top-th largest key is found by the
- * highest eleven bits in which the keys still in question differ, again and again: a histogram of them in LDS says which bin
- * holds it. Mostly two rounds: the first leaves a few keys. */
-template <bool LDS>
-__global__ __launch_bounds__(PG_TPB) void k_pg_select(const PgParams p) {
-    __shared__ unsigned long long s_key[LDS ? PS_LDS : 1], s_or[PG_WAVES], s_and[PG_WAVES];
-    __shared__ int s_hist[PS_BINS], s_part[PG_WAVES], s_found[2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.x, kvh = blockIdx.y;
-    const int len = p.len[seq];
-    if (!pg_len_ok(len, p.p.stride, p.p.positions)) return;
-    const int pages = pg_pages(len);
-    int *list = p.list + ((long long)seq * p.p.Hkv + kvh) * p.top;
-    if (pages <= p.top) {
-        for (int j = tid; j < p.top; j += PG_TPB) list[j] = j < pages ? j : -1;
-        return;
-    }
-    const double *score = p.score + ((long long)seq * p.p.Hkv + kvh) * p.p.stride;
-    if (LDS) {
-        for (int j = tid; j < pages; j += PG_TPB) s_key[j] = pg_key(score[j], j, pages, p.first, p.recent);
-        __syncthreads();
-    }
-    auto key = [&](int j) { return LDS ? s_key[j] : pg_key(score[j], j, pages, p.first, p.recent); };
+/* exclusive sums over the TPB threads, through s_part [TPB / 64]; the threads meet twice */
+template <int TPB>
+__device__ __forceinline__ int block_before(int v, int *s_part) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, incl = wave_scan(v);
+    if (lane == 63) s_part[wave] = incl;
+    __syncthreads();
+    int at = incl - v;
+#pragma unroll
+    for (int w = 0; w < TPB / 64; w++)
+        if (w < wave) at += s_part[w];
+    __syncthreads();
+    return at;
+}
+
+struct PgChoose {
+    unsigned long long any[PG_WAVES], all[PG_WAVES];
+    int hist[PS_BINS], part[PG_WAVES], found[2];
+};
+
+/* The `top` pages of the largest keys, in ascending order. The top-th largest key is found by the highest eleven bits in which the
+ * keys still in question differ, again and again: a histogram of them in LDS says which bin holds it. Mostly two rounds: the first
+ * leaves a few keys. */
+template <int TPB, class F>
+__device__ __forceinline__ void pg_choose(F key, int pages, int top, int *list, PgChoose &s) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     unsigned long long prefix = 0, mask = 0; /* in question: keys with (key & mask) == prefix; larger ones are taken */
-    int need = p.top, held = pages;          /* to take of those in question, and how many there are */
+    int need = top, held = pages;            /* to take of those in question, and how many there are */
     while (held > need) {
         unsigned long long any = 0, all = ~0ULL;
-        for (int j = tid; j < pages; j += PG_TPB) {
+        for (int j = tid; j < pages; j += TPB) {
             const unsigned long long k = key(j);
             if ((k & mask) == prefix) {
                 any |= k;
@@ -1093,84 +1104,185 @@ __global__ __launch_bounds__(PG_TPB) void k_pg_select(const PgParams p) {
             all &= __shfl_xor(all, sh);
         }
         if (lane == 0) {
-            s_or[wave] = any;
-            s_and[wave] = all;
+            s.any[wave] = any;
+            s.all[wave] = all;
         }
-        for (int b = tid; b < PS_BINS; b += PG_TPB) s_hist[b] = 0;
+        for (int b = tid; b < PS_BINS; b += TPB) s.hist[b] = 0;
         __syncthreads();
         any = 0;
         all = ~0ULL;
 #pragma unroll
-        for (int w = 0; w < PG_WAVES; w++) {
-            any |= s_or[w];
-            all &= s_and[w];
+        for (int w = 0; w < TPB / 64; w++) {
+            any |= s.any[w];
+            all &= s.all[w];
         }
         const unsigned long long differ = any & ~all;
         if (differ == 0) break; /* all equal: the lowest pages of them */
         const int shift = max(0, 63 - __clzll(differ) - 10);
-        for (int j = tid; j < pages; j += PG_TPB) {
+        for (int j = tid; j < pages; j += TPB) {
             const unsigned long long k = key(j);
-            if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & (PS_BINS - 1)], 1);
+            if ((k & mask) == prefix) atomicAdd(&s.hist[(k >> shift) & (PS_BINS - 1)], 1);
         }
         __syncthreads();
-        constexpr int NB = PS_BINS / PG_TPB;
+        constexpr int NB = PS_BINS / TPB;
         int cnt[NB], sum = 0;
 #pragma unroll
-        for (int b = 0; b < NB; b++) sum += cnt[b] = s_hist[PS_BINS - 1 - NB * tid - b];
-        const int incl = wave_scan(sum);
-        if (lane == 63) s_part[wave] = incl;
-        __syncthreads();
-        int above = incl - sum;
-#pragma unroll
-        for (int w = 0; w < PG_WAVES; w++)
-            if (w < wave) above += s_part[w];
+        for (int b = 0; b < NB; b++) sum += cnt[b] = s.hist[PS_BINS - 1 - NB * tid - b];
+        int above = block_before<TPB>(sum, s.part);
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             if (above < need && above + cnt[b] >= need) {
-                s_found[0] = PS_BINS - 1 - NB * tid - b;
-                s_found[1] = need - above;
+                s.found[0] = PS_BINS - 1 - NB * tid - b;
+                s.found[1] = need - above;
             }
             above += cnt[b];
         }
         __syncthreads();
-        const int bin = s_found[0];
-        held = s_hist[bin];
-        need = s_found[1];
+        const int bin = s.found[0];
+        held = s.hist[bin];
+        need = s.found[1];
         /* the bits at and above the bin's are known now: those above it are the same in all keys in question */
         mask = ~((1ULL << shift) - 1);
         prefix = (shift + 11 < 64 ? all >> (shift + 11) << (shift + 11) : 0ULL) | (unsigned long long)bin << shift;
         __syncthreads();
     }
     /* keys above the prefix, and the lowest `need` pages at it, by threads that take consecutive pages */
-    const int per = (pages + PG_TPB - 1) / PG_TPB, b0 = min(pages, tid * per), b1 = min(pages, b0 + per);
+    const int per = (pages + TPB - 1) / TPB, b0 = min(pages, tid * per), b1 = min(pages, b0 + per);
     int eq = 0, more = 0;
     for (int j = b0; j < b1; j++) {
         const unsigned long long k = key(j) & mask;
         eq += k == prefix;
         more += k > prefix;
     }
-    const int ie = wave_scan(eq);
-    __syncthreads();
-    if (lane == 63) s_part[wave] = ie;
-    __syncthreads();
-    int e = ie - eq;
-#pragma unroll
-    for (int w = 0; w < PG_WAVES; w++)
-        if (w < wave) e += s_part[w];
-    const int mine = more + max(0, min(need, e + eq) - min(need, e));
-    const int im = wave_scan(mine);
-    __syncthreads();
-    if (lane == 63) s_part[wave] = im;
-    __syncthreads();
-    int at = im - mine;
-#pragma unroll
-    for (int w = 0; w < PG_WAVES; w++)
-        if (w < wave) at += s_part[w];
+    int e = block_before<TPB>(eq, s.part);
+    int at = block_before<TPB>(more + max(0, min(need, e + eq) - min(need, e)), s.part);
     for (int j = b0; j < b1; j++) {
         const unsigned long long k = key(j) & mask;
         if (k > prefix || (k == prefix && e < need)) list[at++] = j;
         e += k == prefix;
     }
+}
+
+/* The same for up to TPB pages, one key a thread: a page stays if fewer than `top` come before it. One pass over the keys where the
+ * digits take a dozen barriers (256 pages: 1.5 us, and 4). */
+template <int TPB>
+__device__ __forceinline__ void pg_choose_few(const unsigned long long *key, int pages, int top, int *list, PgChoose &s) {
+    const int j = threadIdx.x;
+    const unsigned long long mine = key[min(j, pages - 1)];
+    int before = 0;
+    const int own = threadIdx.x & ~63; /* pages below this wave's come before one of an equal key, those above do not */
+    constexpr int U = 16;
+    typedef unsigned long long k2 __attribute__((ext_vector_type(2)));
+    unsigned long long k[U];
+    auto read = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < U; u += 2) {
+            const k2 v = *reinterpret_cast<const k2 *>(key + i0 + u);
+            k[u] = v[0];
+            k[u + 1] = v[1];
+        }
+    };
+    for (int i0 = 0; i0 < pages; i0 += U) { /* key[] is padded with zeros, which no key is */
+        read(i0);
+        if (i0 < own) {
+#pragma unroll
+            for (int u = 0; u < U; u++) before += k[u] >= mine;
+        } else if (i0 >= own + 64) {
+#pragma unroll
+            for (int u = 0; u < U; u++) before += k[u] > mine;
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++) before += k[u] > mine || (k[u] == mine && i0 + u < j);
+        }
+    }
+    const bool in = j < pages && before < top;
+    const int at = block_before<TPB>(in, s.part);
+    if (in) list[at] = j;
+}
+} // namespace
+
+/* Scores of the pages, `per` of them a workgroup, and the choice by the workgroup of a (sequence, kv head) that ends last. */
+template <int HD>
+__global__ __launch_bounds__(PG_TPB) void k_pg_choose(const PgParams p) {
+    typedef PgScore<HD> Score;
+    constexpr int LPP = Score::LPP, PP = PG_TPB / LPP, U = 64 / PP; /* pages of a step, such steps in flight */
+    __shared__ union {
+        struct {
+            double row[PG_WAVES][HD];
+            __align__(16) double sum[PG_WAVES][2][HD];
+        } q;
+        PgChoose c;
+    } s;
+    extern __shared__ __align__(16) unsigned char s_dyn[];
+    unsigned long long *s_key = reinterpret_cast<unsigned long long *>(s_dyn); /* [min(stride + 16, PS_LDS)] */
+    __shared__ int s_turn;
+    const int tid = threadIdx.x, kvh = blockIdx.y;
+    const int blocks = (p.p.stride + p.per - 1) / p.per, seq = blockIdx.x / blocks, j0 = blockIdx.x % blocks * p.per;
+    const int len = p.len[seq];
+    if (!pg_len_ok(len, p.p.stride, p.p.positions)) return;
+    const int pages = pg_pages(len), j1 = min(pages, j0 + p.per);
+    if (j0 >= pages && j0 > 0) return;
+    const long long pair = (long long)seq * p.p.Hkv + kvh;
+    int *list = p.list + pair * p.top;
+    if (pages <= p.top) {
+        if (j0 == 0)
+            for (int j = tid; j < p.top; j += PG_TPB) list[j] = j < pages ? j : -1;
+        return;
+    }
+    const int *row_table = p.p.table + (long long)seq * p.p.stride;
+    Score sc;
+    typename Score::Bounds b[U];
+    bool bad[U];
+    auto load = [&](int j) { /* the pages of a step whose first is j */
+        int page[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) page[u] = row_table[min(j + u * PP + tid / LPP, pages - 1)];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            bad[u] = pg_bad_page(page[u], p.p.n_pages);
+            sc.load(p.p, bad[u] ? 0 : page[u], kvh, b[u]);
+        }
+    };
+    sc.make(p, seq, kvh, len, s.q.row, s.q.sum, [&]() { load(j0); });
+    const bool one = pages <= p.per;
+    const rsrc_t far = make_rsrc(p.score + pair * p.p.stride, (long long)p.p.stride * 8);
+    for (int j = j0; j < j1; j += 64) {
+        double x[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            x[u] = sc.of(b[u]);
+            if (bad[u]) x[u] = __longlong_as_double(0x7FF8000000000000LL); /* chosen, so that the step meets it */
+        }
+        if (j + 64 < j1) load(j + 64);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int at = j + u * PP + tid / LPP;
+            if (at >= j1 || tid % LPP) continue;
+            const unsigned long long k = pg_key(x[u], at, pages, p.first, p.recent);
+            if (one) s_key[at] = k;
+            else __builtin_amdgcn_raw_buffer_store_b64(u2w{(unsigned)k, (unsigned)(k >> 32)}, far, at * 8, 0, CPOL_SC1);
+        }
+    }
+    auto there = [&](int j) {
+        const u2w v = __builtin_amdgcn_raw_buffer_load_b64(far, j * 8, 0, CPOL_SC1);
+        return (unsigned long long)v[1] << 32 | v[0];
+    };
+    if (!one) {
+        /* as in k_pg: what is written has arrived before the workgroup counts itself in */
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const unsigned n = (pages + p.per - 1) / p.per;
+        if (tid == 0) s_turn = (int)atomicInc(p.count + pair * p.tiles, n - 1);
+        __syncthreads();
+        if (s_turn != (int)n - 1) return;
+        if (pages <= PS_LDS)
+            for (int j = tid; j < pages; j += PG_TPB) s_key[j] = there(j);
+    }
+    if (tid < 16 && pages <= PG_TPB) s_key[pages + tid] = 0;
+    __syncthreads();
+    if (pages <= PG_TPB) pg_choose_few<PG_TPB>(s_key, pages, p.top, list, s.c);
+    else if (pages <= PS_LDS) pg_choose<PG_TPB>([&](int j) { return s_key[j]; }, pages, p.top, list, s.c);
+    else pg_choose<PG_TPB>(there, pages, p.top, list, s.c);
 }
 
 /* ------------------------------------------------------ rows in and out */
@@ -1792,12 +1904,10 @@ extern "C" int smol_launch_paged(const PgParams *p, int hd, hipStream_t st, hipE
     const dim3 tpb(PG_TPB);
     hipEvent_t first = e0;
     if (p->top > 0) {
-        const dim3 gs((unsigned)(p->p.n_seq * ((p->p.stride + PS_PAGES - 1) / PS_PAGES)), p->p.Hkv), gl(p->p.n_seq, p->p.Hkv);
-#define PG_SCORE(HD) hipExtLaunchKernelGGL(k_pg_score<HD>, gs, tpb, 0, st, first, nullptr, 0, *p)
-        PG_BY_HD(hd, PG_SCORE)
+        const dim3 gc((unsigned)(p->p.n_seq * ((p->p.stride + p->per - 1) / p->per)), p->p.Hkv);
+#define PG_CHOOSE(HD) hipExtLaunchKernelGGL(k_pg_choose<HD>, gc, tpb, std::min(p->p.stride + 16, PS_LDS) * 8, st, e0, nullptr, 0, *p)
+        PG_BY_HD(hd, PG_CHOOSE)
         first = nullptr;
-        if (p->p.stride <= PS_LDS) hipExtLaunchKernelGGL(k_pg_select<true>, gl, tpb, 0, st, nullptr, nullptr, 0, *p);
-        else hipExtLaunchKernelGGL(k_pg_select<false>, gl, tpb, 0, st, nullptr, nullptr, 0, *p);
     }
     const dim3 grid(p->slots, p->p.Hkv, p->tiles);
     const int rows = std::max(2, PG_WAVES * std::min(p->G, PG_HEADS)); /* of s_mem: the waves' outputs, never fewer than Q and the key */

@@ -443,6 +443,8 @@ TOP = [
     # a table longer than what the choice keeps on the chip
     dict(hq=2, hkv=1, hd=64, lens=[900, 5], top=3, stride=5000, rope=False),
     dict(hq=2, hkv=1, hd=64, lens=[8000, 8001, 12], top=20, std=4.0),
+    dict(hq=6, hkv=2, hd=128, lens=[70000, 65000], top=30, stride=2000),
+    dict(hq=2, hkv=1, hd=72, lens=[5000, 300], top=30, stride=1100, rope=False),
 ]
 
 
