@@ -76,14 +76,20 @@ __device__ __forceinline__ double sqrt_of(double x) { return sqrt(x); }
  * dst[d] = f * rope(x w / sqrt(mean x^2 + eps)). T double where pages are chosen by what comes of it. */
 template <int HD>
 struct PgRow {
-    float x[PgGeom<HD>::NE], w[PgGeom<HD>::NE];
+    uint32_t x[PgGeom<HD>::NE]; /* as loaded: a conversion here would wait for each element */
+    float w[PgGeom<HD>::NE];
     __device__ __forceinline__ void load(const void *base, int dtype, long long row, const float *norm) {
         const int lane = threadIdx.x & 63;
+        if (dtype == SMOL_IN_BF16) {
 #pragma unroll
-        for (int e = 0; e < PgGeom<HD>::NE; e++) {
-            const int d = lane + 64 * e;
-            x[e] = HD % 64 == 0 || d < HD ? in_at(base, dtype, row + d) : 0.0f;
-            if (norm) w[e] = HD % 64 == 0 || d < HD ? norm[d] : 0.0f;
+            for (int e = 0; e < PgGeom<HD>::NE; e++) x[e] = HD % 64 == 0 || lane + 64 * e < HD ? ((const uint16_t *)base)[row + lane + 64 * e] : 0;
+        } else {
+#pragma unroll
+            for (int e = 0; e < PgGeom<HD>::NE; e++) x[e] = HD % 64 == 0 || lane + 64 * e < HD ? ((const uint32_t *)base)[row + lane + 64 * e] : 0;
+        }
+        if (norm) {
+#pragma unroll
+            for (int e = 0; e < PgGeom<HD>::NE; e++) w[e] = HD % 64 == 0 || lane + 64 * e < HD ? norm[lane + 64 * e] : 0.0f;
         }
     }
 };
@@ -102,12 +108,12 @@ struct PgTurn {
     }
 };
 template <int HD, class T>
-__device__ __forceinline__ void pg_finish(const PgRow<HD> &r, bool norm, float eps, const PgTurn<HD> &turn, int kind, T f, T *dst) {
+__device__ __forceinline__ void pg_finish(const PgRow<HD> &r, int dtype, bool norm, float eps, const PgTurn<HD> &turn, int kind, T f, T *dst) {
     constexpr int NE = PgGeom<HD>::NE;
     const int lane = threadIdx.x & 63;
     T x[NE];
 #pragma unroll
-    for (int e = 0; e < NE; e++) x[e] = (T)r.x[e];
+    for (int e = 0; e < NE; e++) x[e] = (T)__uint_as_float(dtype == SMOL_IN_BF16 ? r.x[e] << 16 : r.x[e]);
     if (norm) {
         T ss = 0;
 #pragma unroll
@@ -674,12 +680,13 @@ template <int HD, bool CODES>
 __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams p) {
     constexpr bool DEEP = HD > 128; /* one wave a SIMD, whose registers hold two units */
     constexpr int XS = PgGeom<HD>::XSTR, DT = PgGeom<HD>::DT, U = CODES ? 64 : 32, QD = HD / 4;
-    /* Q's parts (head_dim 256); then the rows of Q (scaled) and the new key, and when they are done with, the waves' outputs */
+    /* Q's parts (head_dim 256); then the rows of Q (scaled), and when they are done with, the waves' outputs */
     extern __shared__ __align__(16) unsigned char s_dyn[];
     uint4 *s_q = reinterpret_cast<uint4 *>(s_dyn);
     float *s_mem = reinterpret_cast<float *>(s_dyn + PgQ<HD, CODES>::LDS);
     __shared__ __align__(16) float s_scale[PG_WAVES][CODES ? 128 : 4];
-    __shared__ float s_v[HD], s_m[PG_WAVES + 1][PG_HEADS], s_l[PG_WAVES][PG_HEADS];
+    __shared__ __align__(16) float s_k[HD], s_v[HD]; /* the new token */
+    __shared__ float s_m[PG_WAVES + 1][PG_HEADS], s_l[PG_WAVES][PG_HEADS];
     __shared__ int s_bad[PG_HEADS], s_turn;
     const int kvh = blockIdx.y, tile = blockIdx.z, h0 = tile * PG_HEADS, R = min(PG_HEADS, p.G - h0);
     PgLane sl;
@@ -768,8 +775,11 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
             }
         }
         turn.load(p.p, pos);
-        if (last)
-            for (int d = tid; d < HD; d += PG_TPB) s_v[d] = in_at(p.v_in, p.in_dtype, ((long long)it.seq * p.p.Hkv + kvh) * HD + d);
+        uint32_t v_new = 0; /* HD <= PG_TPB: an element a thread */
+        if (last && tid < HD) {
+            const long long i = ((long long)it.seq * p.p.Hkv + kvh) * HD + tid;
+            v_new = p.in_dtype == SMOL_IN_BF16 ? ((const uint16_t *)p.v_in)[i] : ((const uint32_t *)p.v_in)[i];
+        }
         /* the first unit is requested behind them: a compute unit returns data in the order of its requests */
         __builtin_amdgcn_sched_barrier(0);
         checked(u0 + wave);
@@ -783,10 +793,11 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
             const int i = wave + PG_WAVES * k;
             if (i < n) {
                 const bool key = i == R;
-                pg_finish<HD, float>(r[k], (key ? p.k_norm : p.q_norm) != nullptr, p.norm_eps, turn, p.p.rope_kind, key ? 1.0f : p.qscale,
-                                     s_mem + i * XS);
+                pg_finish<HD, float>(r[k], p.in_dtype, (key ? p.k_norm : p.q_norm) != nullptr, p.norm_eps, turn, p.p.rope_kind, key ? 1.0f : p.qscale,
+                                     key ? s_k : s_mem + i * XS);
             }
         }
+        if (last && tid < HD) s_v[tid] = __uint_as_float(p.in_dtype == SMOL_IN_BF16 ? v_new << 16 : v_new);
     }
     if (last && ok && pg_bad_page(new_page, p.p.n_pages)) {
         bad = true;
@@ -840,19 +851,15 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
     st.l = row_sum4(st.l);
 
     if (last) {
-        /* the new token's scores, and its row into its page */
+        /* the new token's scores */
         for (int r = wave; r < R; r += PG_WAVES) {
             float d = 0.0f;
 #pragma unroll
             for (int e = 0; e < PgGeom<HD>::NE; e++)
-                if (HD % 64 == 0 || lane + 64 * e < HD) d = fmaf(s_mem[r * XS + lane + 64 * e], s_mem[R * XS + lane + 64 * e], d);
+                if (HD % 64 == 0 || lane + 64 * e < HD) d = fmaf(s_mem[r * XS + lane + 64 * e], s_k[lane + 64 * e], d);
             d = wave_sum(d);
             /* an infinite score is no number, also behind a cap */
             if (lane == 0) s_m[PG_WAVES][r] = pg_capped(d, p.cap2) + 0.0f * d;
-        }
-        if (tile == 0 && ok && new_page >= 0) {
-            if (wave == 2) pg_store_row<HD, CODES, true>(p.p, new_page, kvh, it.len % PG_ROWS, s_mem + R * XS);
-            if (wave == 3) pg_store_row<HD, CODES, false>(p.p, new_page, kvh, it.len % PG_ROWS, s_v);
         }
     }
     __syncthreads();
@@ -913,50 +920,71 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
         __syncthreads();
         if (tid == 0) s_turn = (int)atomicInc(p.count + ((long long)it.seq * p.p.Hkv + kvh) * p.tiles + tile, cut.chunks - 1);
         __syncthreads();
-        if (s_turn != cut.chunks - 1) continue;
+    }
+    const bool answer = whole || s_turn == cut.chunks - 1;
+    if (!whole && answer) {
+        float m[NJ], l[NJ];
 #pragma unroll
         for (int k = 0; k < NJ; k++) {
-            const int e = tid + k * PG_TPB, r = e / QD, d = e % QD * 4;
-            if (e >= R * QD) continue;
-            float m = -INFINITY, l = 0.0f;
-            f4 a = {0.f, 0.f, 0.f, 0.f};
-            constexpr int B = 8; /* chunks in flight */
-            for (int n0 = 0; n0 < cut.chunks; n0 += B) {
-                f4 ml[B], oc[B];
+            m[k] = -INFINITY;
+            l[k] = 0.0f;
+            o[k] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+        constexpr int B = 8; /* chunks in flight */
+        for (int n0 = 0; n0 < cut.chunks; n0 += B) {
+            f4 ml[NJ][B] = {}, oc[NJ][B] = {};
+#pragma unroll
+            for (int k = 0; k < NJ; k++) {
+                const int e = min(tid + k * PG_TPB, R * QD - 1), r = e / QD, d = e % QD * 4;
+                if (k * PG_TPB >= R * QD) break;
 #pragma unroll
                 for (int b = 0; b < B; b++) {
                     const int n = min(n0 + b, cut.chunks - 1);
-                    ml[b] = get_far(rm, place(n, r) * 16);
-                    oc[b] = get_far(ro, (place(n, r) * HD + d) * 4);
+                    ml[k][b] = get_far(rm, place(n, r) * 16);
+                    oc[k][b] = get_far(ro, (place(n, r) * HD + d) * 4);
                 }
-                float mn = m;
+            }
 #pragma unroll
-                for (int b = 0; b < B; b++) mn = fmaxf(mn, ml[b][0]);
-                const float fa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-                l *= fa;
-                a *= fa;
+            for (int k = 0; k < NJ; k++) {
+                if (k * PG_TPB >= R * QD) break;
+                float mn = m[k];
+#pragma unroll
+                for (int b = 0; b < B; b++) mn = fmaxf(mn, ml[k][b][0]);
+                const float fa = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k] - mn);
+                l[k] *= fa;
+                o[k] *= fa;
 #pragma unroll
                 for (int b = 0; b < B; b++) {
                     if (n0 + b >= cut.chunks) break;
-                    const float f = ml[b][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[b][0] - mn);
-                    l = fmaf(ml[b][1], f, l);
-                    if (ml[b][1] != ml[b][1]) l = ml[b][1];
-                    a += oc[b] * f;
+                    const float f = ml[k][b][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k][b][0] - mn);
+                    l[k] = fmaf(ml[k][b][1], f, l[k]);
+                    if (ml[k][b][1] != ml[k][b][1]) l[k] = ml[k][b][1];
+                    o[k] += oc[k][b] * f;
                 }
-                m = mn;
+                m[k] = mn;
             }
-            a *= 1.0f / l;
-            if (!(fabsf(a[0]) + fabsf(a[1]) + fabsf(a[2]) + fabsf(a[3]) < INFINITY)) s_bad[r] = 1;
-            o[k] = a;
+        }
+#pragma unroll
+        for (int k = 0; k < NJ; k++) {
+            if (tid + k * PG_TPB >= R * QD) continue;
+            o[k] *= 1.0f / l[k];
+            if (!(fabsf(o[k][0]) + fabsf(o[k][1]) + fabsf(o[k][2]) + fabsf(o[k][3]) < INFINITY)) s_bad[(tid + k * PG_TPB) / QD] = 1;
         }
     }
-    __syncthreads();
+    if (answer) {
+        __syncthreads();
 #pragma unroll
-    for (int k = 0; k < NJ; k++) {
-        const int e = tid + k * PG_TPB;
-        if (e >= R * QD) continue;
-        if (s_bad[e / QD]) o[k] = f4{NAN, NAN, NAN, NAN};
-        *reinterpret_cast<f4 *>(out + (long long)e * 4) = o[k];
+        for (int k = 0; k < NJ; k++) {
+            const int e = tid + k * PG_TPB;
+            if (e >= R * QD) continue;
+            if (s_bad[e / QD]) o[k] = f4{NAN, NAN, NAN, NAN};
+            *reinterpret_cast<f4 *>(out + (long long)e * 4) = o[k];
+        }
+    }
+    /* the new row into its page, when nobody waits for it any more */
+    if (last && tile == 0 && ok && new_page >= 0) {
+        if (wave == 2) pg_store_row<HD, CODES, true>(p.p, new_page, kvh, it.len % PG_ROWS, s_k);
+        if (wave == 3) pg_store_row<HD, CODES, false>(p.p, new_page, kvh, it.len % PG_ROWS, s_v);
     }
     __syncthreads();
     }
@@ -999,7 +1027,7 @@ struct PgScore {
         for (int h = wave; h < p.G; h += PG_WAVES) {
             const PgRow<HD> now = r;
             if (h + PG_WAVES < p.G) request(h + PG_WAVES);
-            pg_finish<HD, double>(now, p.q_norm != nullptr, p.norm_eps, turn, p.p.rope_kind, p.scale, s_row[wave]);
+            pg_finish<HD, double>(now, p.in_dtype, p.q_norm != nullptr, p.norm_eps, turn, p.p.rope_kind, p.scale, s_row[wave]);
 #pragma unroll
             for (int e = 0; e < NE; e++) {
                 if (HD % 64 != 0 && lane + 64 * e >= HD) continue;
@@ -1427,43 +1455,43 @@ struct PgKStep {
         const float4 &q = v[i >> 2];
         return (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
     }
-    /* y: the normalised, rotated chunks (zeros behind the row) */
+    /* y: the normalised, rotated chunks (zeros behind the row), in T. Codes take fp32, whose roundings are 2^-16 of a code's step;
+     * bf16 rows 64 bits, so that they are the formula's own rounding (in fp32 one element of 16000 is a step beside it). */
+    template <class T>
     __device__ __forceinline__ void finish(const PgRunParams &p, const PgKTable<HD> &t, int j, float (&y)[NC][8]) const {
         const int kind = p.p.rope_kind;
-        float v[NC][8], o[SAME ? 1 : NC][8];
+        T v[NC][8], o[SAME ? 1 : NC][8];
 #pragma unroll
         for (int k = 0; k < NC; k++) {
             const int d0 = 8 * j + 8 * LR * k;
+            float f[8] = {};
+            if (HD % 64 == 0 || d0 < HD) raw_unpack<BF>(x[k], f);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[k][i] = 0.0f;
-            if (HD % 64 != 0 && d0 >= HD) continue;
-            raw_unpack<BF>(x[k], v[k]);
-            if (!SAME && kind == SMOL_ROPE_NEOX_K) {
-                if (HD % 16 == 0) raw_unpack<BF>(pr[k], o[k]);
-                else
+            for (int i = 0; i < 8; i++) v[k][i] = (T)f[i];
+            if (!SAME && kind == SMOL_ROPE_NEOX_K && (HD % 64 == 0 || d0 < HD)) {
+                if (HD % 16 == 0) raw_unpack<BF>(pr[k], f);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) o[k][i] = __uint_as_float(pe[k][i]);
+                for (int i = 0; i < 8; i++) o[SAME ? 0 : k][i] = (T)(HD % 16 == 0 ? f[i] : __uint_as_float(pe[SAME ? 0 : k][i]));
             }
         }
         if (p.k_norm) {
-            float ss[4] = {0.f, 0.f, 0.f, 0.f};
+            T ss[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int k = 0; k < NC; k++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) ss[i & 3] = fmaf(v[k][i], v[k][i], ss[i & 3]);
-            float sum = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+                for (int i = 0; i < 8; i++) ss[i & 3] += v[k][i] * v[k][i];
+            T sum = (ss[0] + ss[1]) + (ss[2] + ss[3]);
 #pragma unroll
             for (int sh = 1; sh < LR; sh <<= 1) sum += __shfl_xor(sum, sh);
-            /* 1 / sqrt in 64 bits: rounded once */
-            const float ri = (float)(1.0 / sqrt((double)sum / HD + (double)p.norm_eps));
+            const T ri = (T)(1.0 / sqrt((double)sum / HD + (double)p.norm_eps)); /* in 64 bits: rounded once */
 #pragma unroll
             for (int k = 0; k < NC; k++) {
                 const int d0 = 8 * j + 8 * LR * k;
                 if (HD % 64 != 0 && d0 >= HD) continue;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    v[k][i] *= p.k_norm[d0 + i] * ri;
-                    if (!SAME && kind == SMOL_ROPE_NEOX_K) o[k][i] *= p.k_norm[rope_partner(d0 + i, HD, SMOL_ROPE_NEOX_K)] * ri;
+                    v[k][i] *= (T)p.k_norm[d0 + i] * ri;
+                    if (!SAME && kind == SMOL_ROPE_NEOX_K) o[SAME ? 0 : k][i] *= (T)p.k_norm[rope_partner(d0 + i, HD, SMOL_ROPE_NEOX_K)] * ri;
                 }
             }
         }
@@ -1473,15 +1501,15 @@ struct PgKStep {
             const int d0 = 8 * j + 8 * LR * k;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                float a = v[k][i];
+                T a = v[k][i];
                 if (kind == SMOL_ROPE_NEOX_K) {
-                    const float b = (SAME ? v[(k + H) % NC][i] : o[SAME ? 0 : k][i]) * at(SAME ? t.s[k % H] : t.s[k], i);
-                    a = fmaf(a, at(SAME ? t.c[k % H] : t.c[k], i), (SAME ? k < H : d0 + i < HD / 2) ? -b : b);
+                    const T b = (SAME ? v[(k + H) % NC][i] : o[SAME ? 0 : k][i]) * (T)at(SAME ? t.s[k % H] : t.s[k], i);
+                    a = a * (T)at(SAME ? t.c[k % H] : t.c[k], i) + ((SAME ? k < H : d0 + i < HD / 2) ? -b : b);
                 } else if (kind == SMOL_ROPE_INTERLEAVED_K) {
-                    const float b = v[k][i ^ 1] * at(t.s[k], i);
-                    a = fmaf(a, at(t.c[k], i), i & 1 ? b : -b);
+                    const T b = v[k][i ^ 1] * (T)at(t.s[k], i);
+                    a = a * (T)at(t.c[k], i) + (i & 1 ? b : -b);
                 }
-                y[k][i] = HD % 64 != 0 && d0 >= HD ? 0.0f : a;
+                y[k][i] = HD % 64 != 0 && d0 >= HD ? 0.0f : (float)a;
             }
         }
     }
@@ -1520,7 +1548,7 @@ __device__ __forceinline__ void pg_append_k(const PgRunParams &p, const PgRun &r
             /* lanes past the last row work on it once more: it changes no bound */
             const int r = RW * pass + tid / LR, row = run.r0 + r;
             float y[NC][8];
-            cur.finish(p, table[pass], j, y);
+            cur.template finish<typename std::conditional<CODES, float, double>::type>(p, table[pass], j, y);
             PgScale sc = {1.0f, 1.0f};
             if (CODES) {
                 unsigned m = 0;
@@ -1734,7 +1762,7 @@ __device__ __forceinline__ void pg_append_v(const PgRunParams &p, const PgRun &r
 
 /* A workgroup takes the K (z 0) or the V (z 1) rows of `heads` kv heads of one page. */
 template <int HD, bool CODES, bool BF>
-__global__ __launch_bounds__(PA_TPB, HD == 64 || HD == 128 ? 4 : 2) void k_pg_append(const PgRunParams p) {
+__global__ __launch_bounds__(PA_TPB, HD == 64 || (HD == 128 && CODES) ? 4 : 2) void k_pg_append(const PgRunParams p) {
     PgRun run;
     if (!pg_find_run(p, blockIdx.x, run)) return;
     const int page = p.p.table[(long long)run.seq * p.p.stride + run.page];
@@ -1910,7 +1938,7 @@ extern "C" int smol_launch_paged(const PgParams *p, int hd, hipStream_t st, hipE
         first = nullptr;
     }
     const dim3 grid(p->slots, p->p.Hkv, p->tiles);
-    const int rows = std::max(2, PG_WAVES * std::min(p->G, PG_HEADS)); /* of s_mem: the waves' outputs, never fewer than Q and the key */
+    const int rows = PG_WAVES * std::min(p->G, PG_HEADS); /* of s_mem: the waves' outputs */
 #define PG_STEP(HD) \
     if (p->p.codes) hipExtLaunchKernelGGL((k_pg<HD, true>), grid, tpb, PgQ<HD, true>::LDS + rows * PgGeom<HD>::XSTR * 4, st, first, e1, 0, *p); \
     else hipExtLaunchKernelGGL((k_pg<HD, false>), grid, tpb, PgQ<HD, false>::LDS + rows * PgGeom<HD>::XSTR * 4, st, first, e1, 0, *p)

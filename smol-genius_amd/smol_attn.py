@@ -662,16 +662,19 @@ def pages_read(pages, layer, table, starts, pos, rows, dtype=None, k_out=None, v
     ctx = pages.ctx
     n, stride, tp = _page_table(ctx, table)
     if dtype is None:
-        dtype = torch.bfloat16 if k_out is None else k_out.dtype
+        dtype = k_out.dtype if k_out is not None else v_out.dtype if v_out is not None else torch.bfloat16
     shape = (rows, pages.n_kv_heads * pages.head_dim)
-    if k_out is None:
+    if k_out is None and v_out is None:
         k_out = torch.empty(shape, dtype=dtype, device=table.device)
-    if v_out is None:
-        v_out = torch.empty(shape, dtype=dtype, device=table.device)
+        v_out = torch.empty_like(k_out)
+        kp, vp = k_out.data_ptr(), v_out.data_ptr()
+    else:
+        k_out = torch.empty_like(v_out) if k_out is None else k_out
+        v_out = torch.empty_like(k_out) if v_out is None else v_out
+        kp, vp = _on(ctx, k_out, dtype, shape, "k_out"), _on(ctx, v_out, dtype, shape, "v_out")
     dt = F32 if dtype is torch.float32 else BF16 if dtype is torch.bfloat16 else _dtype_code(k_out)
     rc = load().smol_kv_pages_read(pages.h, layer, n, tp, stride, _on(ctx, starts, torch.int32, (n + 1,), "starts"),
-                                   _on(ctx, pos, torch.int32, (n,), "pos"), rows, _on(ctx, k_out, dtype, shape, "k_out"),
-                                   _on(ctx, v_out, dtype, shape, "v_out"), dt)
+                                   _on(ctx, pos, torch.int32, (n,), "pos"), rows, kp, vp, dt)
     if rc:
         _check(rc, "smol_kv_pages_read")
     return k_out, v_out
