@@ -735,9 +735,14 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
         const int un = from + PG_WAVES * lane;
         at = page = 0;
         if (un < u1) {
-            const int row = list ? list[un / (PG_ROWS / U)] * PG_ROWS + un % (PG_ROWS / U) * U : (it.units.first + un) * U;
+            int row = (it.units.first + un) * U;
+            if (list) {
+                /* (a list that was written over meanwhile leads nowhere) */
+                const int j = list[un / (PG_ROWS / U)];
+                row = j >= 0 && j <= it.len / PG_ROWS ? j * PG_ROWS + un % (PG_ROWS / U) * U : it.len;
+            }
             at = row;
-            page = row_table[row / PG_ROWS];
+            page = row_table[min(row, it.len) / PG_ROWS];
         }
     };
     auto checked = [&](int from) { /* once the numbers are here */

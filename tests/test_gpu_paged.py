@@ -635,6 +635,64 @@ def test_captured_and_replayed(sa, codes, top):
     ctx.close()
 
 
+@pytest.mark.parametrize("codes", [False, True], ids=["bf16", "int8"])
+def test_a_batch_of_nobody(sa, ctx, codes):
+    """a captured size without a request: nothing is read or written"""
+    for top in (0, 2):
+        s = Step(sa, ctx, hq=4, hkv=2, hd=64, lens=[-1] * 70, codes=codes, top=top)
+        out = torch.full((70, 4 * 64), 3.0, device="cuda")
+        s.call(out=out)
+        ctx.synchronize()
+        assert (out == 3.0).all()
+        for a, b in zip(s.before, s.pool.bits()):
+            assert a is None or torch.equal(a, b)
+
+
+@pytest.mark.parametrize("codes", [False, True], ids=["bf16", "int8"])
+def test_two_streams(sa, codes):
+    """two contexts on two streams, neither of them the current one, calls of both under way at once; the same step again gives the
+    same bits"""
+    runs = []
+    for i in range(2):
+        side = torch.cuda.Stream()
+        c = sa.Context(0, stream=side.cuda_stream)
+        runs.append((side, c, Step(sa, c, hq=8, hkv=2, hd=128, lens=[4000 + 100 * i, 9, 2000], codes=codes, top=8 * i, seed=30 + i)))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for i, (side, c, s) in enumerate(runs):
+            with torch.cuda.stream(side):
+                outs[i].append(s.call())
+    for i, (side, c, s) in enumerate(runs):
+        c.synchronize()
+        s.check(outs[i][0])
+        for o in outs[i][1:]:
+            assert torch.equal(o, outs[i][0])
+        c.close()
+
+
+@pytest.mark.parametrize("codes", [False, True], ids=["bf16", "int8"])
+def test_what_the_products_carry(sa, ctx, codes):
+    """The error of a row of out against its own norm. Scores: Q whole or at 2^-24 of its largest element, fp32 sums: their errors are random,
+    about sqrt(hd) 2^-24 of |q| |k| scale (here at most 3), so 2^-20 on a weight; weights at 2^-24; the sum over 1000 rows in fp32
+    2^-20. With a root of two for numerator and denominator and twice that to spare: 2^-18. Two parts of 8 bits for Q or
+    the weights would leave 2^-16 of each."""
+    s = Step(sa, ctx, hq=4, hkv=2, hd=128, lens=[1000, 1001, 64], codes=codes, norm=False)
+    out = s.call().cpu().double().view(3, 2, 2, 128)
+    ctx.synchronize()
+    q, k, v = s.turned()
+    kk, vv = s.rows
+    for i, l in enumerate(s.lens):
+        for h in range(2):
+            at = torch.arange(l)
+            page = s.t[i, at // P].long()
+            o, _ = attend(q[i].view(2, 2, 128)[h], torch.cat([kk[page, h, at % P], k[i, h:h + 1]]),
+                          torch.cat([vv[page, h, at % P], v[i, h:h + 1]]), s.scale, 0.0, codes, 128, torch.zeros(l + 1))
+            err = (out[i, h] - o).norm(dim=-1) / o.norm(dim=-1)
+            print("codes %d: %.2g" % (codes, float(err.max())), flush=True)
+            assert (err <= 2.0 ** -18).all()
+
+
 def test_growth_under_capture_is_refused(sa):
     side = torch.cuda.Stream()
     ctx = sa.Context(0, stream=side.cuda_stream)
