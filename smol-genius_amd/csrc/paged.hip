@@ -13,7 +13,6 @@
 namespace {
 
 typedef int i4 __attribute__((ext_vector_type(4)));
-typedef unsigned short u2v __attribute__((ext_vector_type(2)));
 
 constexpr int PG_TPB = 64 * PG_WAVES;
 constexpr int PG_HEADS = 16; /* query heads of a tile: the columns of a matrix product */
@@ -1195,43 +1194,6 @@ __device__ __forceinline__ void pg_choose(F key, int pages, int top, int *list, 
         e += k == prefix;
     }
 }
-
-/* The same for up to TPB pages, one key a thread: a page stays if fewer than `top` come before it. One pass over the keys where the
- * digits take a dozen barriers (256 pages: 1.5 us, and 4). */
-template <int TPB>
-__device__ __forceinline__ void pg_choose_few(const unsigned long long *key, int pages, int top, int *list, PgChoose &s) {
-    const int j = threadIdx.x;
-    const unsigned long long mine = key[min(j, pages - 1)];
-    int before = 0;
-    const int own = threadIdx.x & ~63; /* pages below this wave's come before one of an equal key, those above do not */
-    constexpr int U = 16;
-    typedef unsigned long long k2 __attribute__((ext_vector_type(2)));
-    unsigned long long k[U];
-    auto read = [&](int i0) {
-#pragma unroll
-        for (int u = 0; u < U; u += 2) {
-            const k2 v = *reinterpret_cast<const k2 *>(key + i0 + u);
-            k[u] = v[0];
-            k[u + 1] = v[1];
-        }
-    };
-    for (int i0 = 0; i0 < pages; i0 += U) { /* key[] is padded with zeros, which no key is */
-        read(i0);
-        if (i0 < own) {
-#pragma unroll
-            for (int u = 0; u < U; u++) before += k[u] >= mine;
-        } else if (i0 >= own + 64) {
-#pragma unroll
-            for (int u = 0; u < U; u++) before += k[u] > mine;
-        } else {
-#pragma unroll
-            for (int u = 0; u < U; u++) before += k[u] > mine || (k[u] == mine && i0 + u < j);
-        }
-    }
-    const bool in = j < pages && before < top;
-    const int at = block_before<TPB>(in, s.part);
-    if (in) list[at] = j;
-}
 } // namespace
 
 /* Scores of the pages, `per` of them a workgroup, and the choice by the workgroup of a (sequence, kv head) that ends last. */
@@ -1247,7 +1209,7 @@ __global__ __launch_bounds__(PG_TPB) void k_pg_choose(const PgParams p) {
         PgChoose c;
     } s;
     extern __shared__ __align__(16) unsigned char s_dyn[];
-    unsigned long long *s_key = reinterpret_cast<unsigned long long *>(s_dyn); /* [min(stride + 16, PS_LDS)] */
+    unsigned long long *s_key = reinterpret_cast<unsigned long long *>(s_dyn); /* [min(stride, PS_LDS)] */
     __shared__ int s_turn;
     const int tid = threadIdx.x, kvh = blockIdx.y;
     const int blocks = (p.p.stride + p.per - 1) / p.per, seq = blockIdx.x / blocks, j0 = blockIdx.x % blocks * p.per;
@@ -1311,10 +1273,8 @@ __global__ __launch_bounds__(PG_TPB) void k_pg_choose(const PgParams p) {
         if (pages <= PS_LDS)
             for (int j = tid; j < pages; j += PG_TPB) s_key[j] = there(j);
     }
-    if (tid < 16 && pages <= PG_TPB) s_key[pages + tid] = 0;
     __syncthreads();
-    if (pages <= PG_TPB) pg_choose_few<PG_TPB>(s_key, pages, p.top, list, s.c);
-    else if (pages <= PS_LDS) pg_choose<PG_TPB>([&](int j) { return s_key[j]; }, pages, p.top, list, s.c);
+    if (pages <= PS_LDS) pg_choose<PG_TPB>([&](int j) { return s_key[j]; }, pages, p.top, list, s.c);
     else pg_choose<PG_TPB>(there, pages, p.top, list, s.c);
 }
 
@@ -1906,9 +1866,7 @@ __global__ __launch_bounds__(PG_TPB) void k_pg_read(const PgRunParams p) {
     }
 
 /* workgroups (of one head) from which one takes two heads, and so on */
-#ifndef PG_HEADS_FROM
 #define PG_HEADS_FROM 2048
-#endif
 
 /* workgroups of k_pg on a compute unit (registers) */
 extern "C" int smol_paged_occupancy(int hd) { return hd > 128 ? 1 : 2; }
@@ -1938,7 +1896,7 @@ extern "C" int smol_launch_paged(const PgParams *p, int hd, hipStream_t st, hipE
     hipEvent_t first = e0;
     if (p->top > 0) {
         const dim3 gc((unsigned)(p->p.n_seq * ((p->p.stride + p->per - 1) / p->per)), p->p.Hkv);
-#define PG_CHOOSE(HD) hipExtLaunchKernelGGL(k_pg_choose<HD>, gc, tpb, std::min(p->p.stride + 16, PS_LDS) * 8, st, e0, nullptr, 0, *p)
+#define PG_CHOOSE(HD) hipExtLaunchKernelGGL(k_pg_choose<HD>, gc, tpb, std::min(p->p.stride, PS_LDS) * 8, st, e0, nullptr, 0, *p)
         PG_BY_HD(hd, PG_CHOOSE)
         first = nullptr;
     }
