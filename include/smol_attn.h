@@ -403,14 +403,14 @@ SMOL_ATTN_API int smol_kv_pages_pointers(const smol_kv_pages *pages, int layer, 
 
 /* Writes rows of a ragged batch: rows starts[i] .. starts[i + 1] - 1 of k_new, v_new [rows][n_kv_heads * head_dim] (dtype
  * SMOL_ATTN_F32 or _BF16) are positions pos[i], pos[i] + 1, .. of sequence i, K normalised (k_norm [head_dim], NULL: not) and
- * rotated (rope NULL: not) in fp32 as smol_attn_decode_qknorm's. starts [n_seq + 1], pos [n_seq]: device ints, starts not
- * falling; a sequence may have no rows. */
+ * rotated (rope NULL: not) as smol_attn_decode_qknorm's, for codes in fp32, for bf16 rows in 64 bits. starts [n_seq + 1],
+ * pos [n_seq]: device ints, starts not falling; a sequence may have no rows. */
 SMOL_ATTN_API int smol_kv_pages_append(smol_kv_pages *pages, int layer, const smol_rope_table *rope, int n_seq, const int *table,
                                        int stride, const int *starts, const int *pos, int rows, const void *k_new,
                                        const void *v_new, int dtype, const float *k_norm, float eps);
 /* The values that rows stand for, into k_out, v_out [rows][n_kv_heads * head_dim] of dtype (bf16: nearest even); starts and pos
  * as above. What a chunk of a prompt attends to with smol_attn_causal, for one use. Rows between the sequences' ranges are left
- * as they were. */
+ * as they were, and so are those of a range that is none. The outputs overlap neither each other nor the pool. */
 SMOL_ATTN_API int smol_kv_pages_read(smol_kv_pages *pages, int layer, int n_seq, const int *table, int stride, const int *starts,
                                      const int *pos, int rows, void *k_out, void *v_out, int dtype);
 
@@ -418,7 +418,7 @@ SMOL_ATTN_API int smol_kv_pages_read(smol_kv_pages *pages, int layer, int n_seq,
  * has a page. out[i] is the attention of q[i] over its rows and the new token; norm, RoPE, window, cap and layouts as for
  * smol_attn_decode_qknorm (NULL norm weights skip a norm). A negative len[i] is no sequence: nothing of it is read or written,
  * out[i] stays (a batch padded to a captured size).
- * The new token is used in fp32. bf16 pools: products as of smol_attn_decode_shared. int8 pools: Q and the weights as 24-bit
+ * The new token is used in fp32, and its row is rounded from that. out overlaps no input. bf16 pools: products as of smol_attn_decode_shared. int8 pools: Q and the weights as 24-bit
  * whole numbers against their row's (their page's) largest, products with the codes exact, sums fp32; the 8 bits of the cache
  * are all that is lost. A visible row that is not finite, be it in one element, makes NaN of all outputs of the heads that
  * read it, and of no other; rows at or past a sequence's length are never used. A sequence's result does not depend on the

@@ -2251,6 +2251,8 @@ extern "C" int smol_kv_pages_create(smol_attn_ctx *ctx, int n_layers, int n_page
     if (n_kv > 65535) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d kv heads", n_kv);
     if (!hd_supported(hd)) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "head_dim %d", hd);
     if (type != SMOL_PAGES_BF16 && type != SMOL_PAGES_INT8) return fail(SMOL_ATTN_ERR_ARG, "page type %d", type);
+    int rc = check_capture(ctx, "a pool of pages", true);
+    if (rc) return rc;
     const bool codes = type == SMOL_PAGES_INT8;
     auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     const size_t at = (size_t)n_pages * n_kv;
@@ -2261,8 +2263,7 @@ extern "C" int smol_kv_pages_create(smol_attn_ctx *ctx, int n_layers, int n_page
     proto.b_bytes = up(at * 2 * hd * 2);
     if (proto.layer_bytes() > ((size_t)1 << 46) / n_layers)
         return fail(SMOL_ATTN_ERR_NOMEM, "pool of %d layers of %zu bytes", n_layers, proto.layer_bytes());
-    const int rc = set_device(ctx);
-    if (rc) return rc;
+    if ((rc = set_device(ctx))) return rc;
     const size_t bytes = proto.layer_bytes() * n_layers;
     void *mem = nullptr;
     hipError_t e = hipMalloc(&mem, bytes);
@@ -2416,7 +2417,8 @@ static int decode_paged(smol_attn_ctx *ctx, smol_kv_pages *kp, int layer, const 
     pg.window = window;
     pg.cap2 = cap > 0.0f ? (float)(cap * LOG2E_D) : 0.0f;
     pg.tiles = (G + 15) / 16;
-    pg.top = top; pg.first = first; pg.recent = recent;
+    pg.top = chosen ? top : std::min(top, stride); /* more pages than a table can have are all of them */
+    pg.first = first; pg.recent = recent;
     if (top > 0 && (long long)n_seq * ((stride + 63) / 64) > PG_MAX_BLOCKS)
         return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d sequences, page table rows of %d", n_seq, stride);
     if (pg.tiles > 65535) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d heads a kv head", G);
@@ -2426,7 +2428,7 @@ static int decode_paged(smol_attn_ctx *ctx, smol_kv_pages *kp, int layer, const 
     const long long items = 2LL * pg.slots;
     WorkPlan wk;
     const size_t o_o = wk.take((size_t)items * n_heads * hd * 4), o_ml = wk.take((size_t)items * n_heads * 16);
-    const size_t o_list = wk.take(top > 0 && !chosen ? (size_t)n_seq * Hkv * top * 4 : 0);
+    const size_t o_list = wk.take(top > 0 && !chosen ? (size_t)n_seq * Hkv * pg.top * 4 : 0);
     const size_t o_score = wk.take(top > 0 ? (size_t)n_seq * Hkv * stride * 8 : 0);
     if ((rc = check_capture(ctx, "workspace growth", wk.bytes > ctx->work.cap))) return rc;
     if ((rc = dev_reserve(ctx->work, wk.bytes, ctx->stream))) return rc;

@@ -630,11 +630,12 @@ class KVPages:
             pass
 
 
-def _page_table(ctx, table):
+def _page_table(ctx, table, n=None):
     import torch
     if table.dim() != 2:
         raise SmolAttnError("table must be [sequences, pages]")
-    n, stride = table.shape
+    stride = table.shape[1]
+    n = table.shape[0] if n is None else n
     return n, stride, _on(ctx, table, torch.int32, (n, stride), "table")
 
 
@@ -686,9 +687,8 @@ def decode_paged(ctx, pages, layer, rope, table, lens, q, k_new, v_new, n_heads,
     smol_attn_decode_paged. Returns out [n, n_heads*hd]."""
     import torch
     n, qp, kp, vp, dt, qw, kw, out, op = _step_args(ctx, pages, q, k_new, v_new, n_heads, q_norm, k_norm, out)
-    stride = table.shape[1]
-    rc = load().smol_attn_decode_paged(ctx.h, pages.h, layer, rope.h if rope else None, n,
-                                       _on(ctx, table, torch.int32, (n, stride), "table"), stride,
+    n, stride, tp = _page_table(ctx, table, n)
+    rc = load().smol_attn_decode_paged(ctx.h, pages.h, layer, rope.h if rope else None, n, tp, stride,
                                        _on(ctx, lens, torch.int32, (n,), "lens"), qp, kp, vp, dt, n_heads, scale, window, cap, qw,
                                        kw, eps, op)
     if rc:
@@ -702,11 +702,11 @@ def decode_paged_top(ctx, pages, layer, rope, table, lens, q, k_new, v_new, n_he
     recent ones among them; see smol_attn_decode_paged_top. Returns out and chosen (int32 [n, kv_heads, top])."""
     import torch
     n, qp, kp, vp, dt, qw, kw, out, op = _step_args(ctx, pages, q, k_new, v_new, n_heads, q_norm, k_norm, out)
-    stride, shape = table.shape[1], (n, pages.n_kv_heads, top)
+    n, stride, tp = _page_table(ctx, table, n)
+    shape = (n, pages.n_kv_heads, top)
     if chosen is None:
         chosen = torch.empty(shape, dtype=torch.int32, device=q.device)
-    rc = load().smol_attn_decode_paged_top(ctx.h, pages.h, layer, rope.h if rope else None, n,
-                                           _on(ctx, table, torch.int32, (n, stride), "table"), stride,
+    rc = load().smol_attn_decode_paged_top(ctx.h, pages.h, layer, rope.h if rope else None, n, tp, stride,
                                            _on(ctx, lens, torch.int32, (n,), "lens"), top, first, recent, qp, kp, vp, dt, n_heads,
                                            scale, cap, qw, kw, eps, _on(ctx, chosen, torch.int32, shape, "chosen"), op)
     if rc:

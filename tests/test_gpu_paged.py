@@ -60,14 +60,12 @@ def i32(a):
 def outward(x, up):
     """fp32 as the next bf16 at or above (below)"""
     b = x.to(torch.bfloat16).float()
-    step = torch.nextafter(x, torch.full_like(x, math.inf if up else -math.inf))
     wrong = b < x if up else b > x
     # the other neighbour: bf16 numbers are those with the low 16 bits zero
     bits = x.view(torch.int32) & -65536
     cut = bits.view(torch.float32)
     away = (bits + 65536).view(torch.float32)
     other = torch.where((x > 0) == up, away, cut)
-    assert step is not None
     return torch.where(wrong, other, b)
 
 
@@ -710,6 +708,40 @@ def test_growth_under_capture_is_refused(sa):
     ctx.close()
 
 
+def test_a_pool_under_capture_is_refused(sa):
+    """its clearing would be part of the graph"""
+    side = torch.cuda.Stream()
+    ctx = sa.Context(0, stream=side.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            with pytest.raises(sa.SmolAttnError, match="under stream capture"):
+                sa.KVPages(ctx, 1, 4, 2, 64)
+            torch.zeros(4, device="cuda").add_(1)
+    ctx.close()
+
+
+@pytest.mark.parametrize("codes", [False, True], ids=["bf16", "int8"])
+def test_choices_not_wanted(sa, ctx, codes):
+    """without an array for them the step is the same; more pages than the table can have are all of them"""
+    s = Step(sa, ctx, hq=4, hkv=2, hd=64, lens=[700, 64, 0, 390], codes=codes, top=4)
+    a = s.call()
+    ctx.synchronize()
+    s.check(a, what=" top")
+    d, w = s.dev
+    p = lambda x: x.data_ptr()  # noqa: E731
+    for top in (4, 2 ** 24 - 1):
+        out = torch.empty_like(a)
+        assert sa.load().smol_attn_decode_paged_top(
+            ctx.h, s.pool.pool.h, s.pool.layer, s.rope.h, s.n, p(s.td), s.td.shape[1], p(s.ld), top, 1, 1, p(d["q"]), p(d["k_new"]),
+            p(d["v_new"]), 0, s.hq, s.scale, 0.0, p(w["q_norm"]), p(w["k_norm"]), EPS, None, p(out)) == 0
+        ctx.synchronize()
+        if top == 4:
+            assert torch.equal(out, a)
+    s.top = 0
+    s.check(out, stored=False)
+
+
 def test_pool_past_four_gigabytes(sa, ctx):
     """pages whose addresses pass 32 bits"""
     hkv, hd = 8, 256
@@ -808,6 +840,8 @@ def test_refusals(sa, ctx):
     step("not a multiple", n_heads=3, q=normal(g, 1, 3 * 64).cuda())
     step("lens must be", lens=ld.long())
     step("table must be", table=t.long())
+    step("table must be", table=t[0])
+    step("table must be", fn=sa.decode_paged_top, top=2, table=t[0])
     step("must be float32 or bfloat16", q=q.double())
     step("rope table head_dim", rope=sa.RopeTable(ctx, 128, 1e4))
     step("first", fn=sa.decode_paged_top, top=2, first=2)
