@@ -2427,7 +2427,7 @@ static int decode_paged(smol_attn_ctx *ctx, smol_kv_pages *kp, int layer, const 
         return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d sequences, page table rows of %d", n_seq, stride);
     const long long items = 2LL * pg.slots;
     WorkPlan wk;
-    const size_t o_o = wk.take((size_t)items * n_heads * hd * 4), o_ml = wk.take((size_t)items * n_heads * 16);
+    const size_t o_part = wk.take((size_t)items * n_heads * PG_PART(hd) * 4);
     const size_t o_list = wk.take(top > 0 && !chosen ? (size_t)n_seq * Hkv * pg.top * 4 : 0);
     const size_t o_score = wk.take(top > 0 ? (size_t)n_seq * Hkv * stride * 8 : 0);
     if ((rc = check_capture(ctx, "workspace growth", wk.bytes > ctx->work.cap))) return rc;
@@ -2437,8 +2437,7 @@ static int decode_paged(smol_attn_ctx *ctx, smol_kv_pages *kp, int layer, const 
     if ((rc = dev_reserve(ctx->pg_count, counts, ctx->stream, true))) return rc;
     pg.count = (unsigned *)ctx->pg_count.p;
     unsigned char *w = (unsigned char *)ctx->work.p;
-    pg.part_o = (float *)(w + o_o);
-    pg.part_ml = (float *)(w + o_ml);
+    pg.part = (float *)(w + o_part);
     pg.list = chosen ? chosen : (int *)(w + o_list);
     pg.score = (double *)(w + o_score);
     /* A workgroup spends 5 us on Q's sums before its first score: 64 pages each while that fills no more than the machine, more where

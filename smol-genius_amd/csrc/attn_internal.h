@@ -354,6 +354,9 @@ typedef struct {
     int heads;                        /* kv heads of a workgroup */
 } PgRunParams;
 
+/* floats of a chunk's output for one head, with m and l (and two unused) behind it */
+#define PG_PART(hd) ((hd) + 4)
+
 /* k_pg, k_pg_choose: a decode step */
 typedef struct {
     PgPool p;
@@ -366,7 +369,7 @@ typedef struct {
     int window; float cap2;           /* window > 0: positions > len - window; cap2 > 0: softcap in log2 units */
     int slots;                        /* workgroups a kv head and tile of heads: pieces of the line at most (pg_piece) */
     int tiles;                        /* tiles of 16 heads of a kv head */
-    float *part_o; float *part_ml;    /* [kv][2 slots][G]: outputs [hd], (m, l, 0, 0) */
+    float *part;                      /* [kv][2 slots][G][PG_PART(hd)]: an output, then m and l */
     unsigned *count;                  /* [n_seq][kv][tiles] chunks that have ended; zero between calls */
     /* top > 0: at most that many pages of each (sequence, kv head), which `list` names in ascending order */
     int top, first, recent;

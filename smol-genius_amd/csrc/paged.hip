@@ -13,6 +13,7 @@
 namespace {
 
 typedef int i4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2w __attribute__((ext_vector_type(2)));
 
 constexpr int PG_TPB = 64 * PG_WAVES;
 constexpr int PG_HEADS = 16; /* query heads of a tile: the columns of a matrix product */
@@ -671,6 +672,16 @@ __device__ __forceinline__ f4 get_far(rsrc_t r, unsigned off) {
     const u4v v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, CPOL_SC1);
     return f4{__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3])};
 }
+__device__ __forceinline__ void put_far(rsrc_t r, float m, float l, unsigned off) {
+    __builtin_amdgcn_raw_buffer_store_b64(u2w{__float_as_uint(m), __float_as_uint(l)}, r, off, 0, CPOL_SC1);
+}
+__device__ __forceinline__ void get_far(rsrc_t r, unsigned off, float &m, float &l) {
+    const u2w v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, CPOL_SC1);
+    m = __uint_as_float(v[0]);
+    l = __uint_as_float(v[1]);
+}
+template <int N>
+using PgInt = std::integral_constant<int, N>;
 } // namespace
 
 /* A piece of the sequences' units against a tile of 16 heads of a kv head, sequence by sequence; a sequence's last chunk also takes the
@@ -881,8 +892,8 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
     const bool whole = cut.chunks == 1;
     const int slot0 = it.units.n ? 2 * ((it.off + PG_EXTRA) / piece) : 0; /* the places of this sequence's chunks begin here */
     const long long first = ((long long)kvh * 2 * p.slots + slot0) * p.G + h0;
-    const rsrc_t ro = make_rsrc(p.part_o + first * HD, 1LL << 31), rm = make_rsrc(p.part_ml + first * 4, 1LL << 31);
-    auto place = [&](int n, int r) { return (pg_slot(it.off, piece, n) - slot0) * p.G + r; };
+    const rsrc_t far = make_rsrc(p.part + first * PG_PART(HD), 1LL << 31);
+    auto place = [&](int n, int r) { return ((pg_slot(it.off, piece, n) - slot0) * p.G + r) * PG_PART(HD) * 4; };
     float *out = p.out + ((long long)it.seq * p.Hq + kvh * p.G + h0) * HD;
     constexpr int NJ = (PG_HEADS * QD + PG_TPB - 1) / PG_TPB;
     f4 o[NJ] = {};
@@ -913,8 +924,8 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
             /* what is not finite in one dim spoils the row */
             if (!(fabsf(a[0]) + fabsf(a[1]) + fabsf(a[2]) + fabsf(a[3]) < INFINITY)) s_bad[r] = 1;
         } else {
-            put_far(ro, a, (place(cut.nth, r) * HD + d) * 4);
-            if (d == 0) put_far(rm, f4{m, l, 0.f, 0.f}, place(cut.nth, r) * 16);
+            put_far(far, a, place(cut.nth, r) + d * 4);
+            if (d == 0) put_far(far, m, l, place(cut.nth, r) + HD * 4);
         }
         o[k] = a;
     }
@@ -927,52 +938,64 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
     }
     const bool answer = whole || s_turn == cut.chunks - 1;
     if (!whole && answer) {
-        float m[NJ], l[NJ];
+        /* N places of the outputs a thread, B chunks in flight for each: what the chunks' round trips past the caches allow. At
+         * head_dim 256 few heads leave registers for more of them (one sequence of 8191 rows, 67 chunks: 27.5 us, 8 in flight
+         * 32.6); below, a second form of the loop costs what it saves */
+        auto join = [&](auto n_of, auto b_of) {
+            constexpr int N = decltype(n_of)::value, B = decltype(b_of)::value;
+            float m[N], l[N];
 #pragma unroll
-        for (int k = 0; k < NJ; k++) {
-            m[k] = -INFINITY;
-            l[k] = 0.0f;
-            o[k] = f4{0.f, 0.f, 0.f, 0.f};
-        }
-        constexpr int B = 8; /* chunks in flight */
-        for (int n0 = 0; n0 < cut.chunks; n0 += B) {
-            f4 ml[NJ][B] = {}, oc[NJ][B] = {};
+            for (int k = 0; k < N; k++) {
+                m[k] = -INFINITY;
+                l[k] = 0.0f;
+                o[k] = f4{0.f, 0.f, 0.f, 0.f};
+            }
+            for (int n0 = 0; n0 < cut.chunks; n0 += B) {
+                float mc[N][B] = {}, lc[N][B] = {};
+                f4 oc[N][B] = {};
 #pragma unroll
-            for (int k = 0; k < NJ; k++) {
-                const int e = min(tid + k * PG_TPB, R * QD - 1), r = e / QD, d = e % QD * 4;
-                if (k * PG_TPB >= R * QD) break;
+                for (int k = 0; k < N; k++) {
+                    const int e = min(tid + k * PG_TPB, R * QD - 1), r = e / QD, d = e % QD * 4;
+                    if (k * PG_TPB >= R * QD) break;
 #pragma unroll
-                for (int b = 0; b < B; b++) {
-                    const int n = min(n0 + b, cut.chunks - 1);
-                    ml[k][b] = get_far(rm, place(n, r) * 16);
-                    oc[k][b] = get_far(ro, (place(n, r) * HD + d) * 4);
+                    for (int b = 0; b < B; b++) {
+                        const int n = min(n0 + b, cut.chunks - 1);
+                        get_far(far, place(n, r) + HD * 4, mc[k][b], lc[k][b]);
+                        oc[k][b] = get_far(far, place(n, r) + d * 4);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < N; k++) {
+                    if (k * PG_TPB >= R * QD) break;
+                    float mn = m[k];
+#pragma unroll
+                    for (int b = 0; b < B; b++) mn = fmaxf(mn, mc[k][b]);
+                    const float fa = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k] - mn);
+                    l[k] *= fa;
+                    o[k] *= fa;
+#pragma unroll
+                    for (int b = 0; b < B; b++) {
+                        /* (places behind the last are the last once more; a branch here would send its loads one by one) */
+                        const float f = n0 + b >= cut.chunks || mc[k][b] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mc[k][b] - mn);
+                        l[k] = lc[k][b] != lc[k][b] ? lc[k][b] : fmaf(lc[k][b], f, l[k]);
+                        o[k] += oc[k][b] * f;
+                    }
+                    m[k] = mn;
                 }
             }
 #pragma unroll
-            for (int k = 0; k < NJ; k++) {
-                if (k * PG_TPB >= R * QD) break;
-                float mn = m[k];
-#pragma unroll
-                for (int b = 0; b < B; b++) mn = fmaxf(mn, ml[k][b][0]);
-                const float fa = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k] - mn);
-                l[k] *= fa;
-                o[k] *= fa;
-#pragma unroll
-                for (int b = 0; b < B; b++) {
-                    if (n0 + b >= cut.chunks) break;
-                    const float f = ml[k][b][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k][b][0] - mn);
-                    l[k] = fmaf(ml[k][b][1], f, l[k]);
-                    if (ml[k][b][1] != ml[k][b][1]) l[k] = ml[k][b][1];
-                    o[k] += oc[k][b] * f;
-                }
-                m[k] = mn;
+            for (int k = 0; k < N; k++) {
+                if (tid + k * PG_TPB >= R * QD) continue;
+                o[k] *= 1.0f / l[k];
+                if (!(fabsf(o[k][0]) + fabsf(o[k][1]) + fabsf(o[k][2]) + fabsf(o[k][3]) < INFINITY)) s_bad[(tid + k * PG_TPB) / QD] = 1;
             }
-        }
-#pragma unroll
-        for (int k = 0; k < NJ; k++) {
-            if (tid + k * PG_TPB >= R * QD) continue;
-            o[k] *= 1.0f / l[k];
-            if (!(fabsf(o[k][0]) + fabsf(o[k][1]) + fabsf(o[k][2]) + fabsf(o[k][3]) < INFINITY)) s_bad[(tid + k * PG_TPB) / QD] = 1;
+        };
+        if constexpr (DEEP) {
+            if (R * QD <= PG_TPB) join(PgInt<1>(), PgInt<16>());
+            else if (R * QD <= 2 * PG_TPB) join(PgInt<2>(), PgInt<16>());
+            else join(PgInt<NJ>(), PgInt<8>());
+        } else {
+            join(PgInt<NJ>(), PgInt<8>());
         }
     }
     if (answer) {
@@ -999,7 +1022,6 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
 namespace {
 constexpr int PS_BINS = 2048;
 constexpr int PS_LDS = 4096; /* pages whose keys a choosing workgroup keeps in LDS */
-typedef unsigned u2w __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ int pg_pages(int len) { return (len + PG_ROWS - 1) / PG_ROWS; }
 
