@@ -2441,7 +2441,9 @@ static int decode_paged(smol_attn_ctx *ctx, smol_kv_pages *kp, int layer, const 
     pg.list = chosen ? chosen : (int *)(w + o_list);
     pg.score = (double *)(w + o_score);
     /* A workgroup spends 5 us on Q's sums before its first score: 64 pages each while that fills no more than the machine, more where
-     * the workgroups would wait for each other */
+     * the workgroups would wait for each other. The whole call with 64, 128, 256 pages: one sequence of 16384 rows, 8 kv heads, 27.4,
+     * 29.1, 31.6 us; 16 of 16000 to 32768, 60.3, 61.1, 64.2; with 64 of these (4096 workgroups of 64 pages) 165 with 64 and 155
+     * with 128 as the rule has it, with 128 of them 327 and (256) 313 */
     pg.per = 64;
     while (pg.per < 1024 && (long long)n_seq * Hkv * ((stride + pg.per - 1) / pg.per) > 8LL * ctx->cu_count) pg.per *= 2;
     const int mk = timing_begin(ctx, 1);

@@ -685,7 +685,20 @@ using PgInt = std::integral_constant<int, N>;
 } // namespace
 
 /* A piece of the sequences' units against a tile of 16 heads of a kv head, sequence by sequence; a sequence's last chunk also takes the
- * new token and stores its row. Of a sequence with several chunks the workgroup that ends last joins them, in their order. */
+ * new token and stores its row. Of a sequence with several chunks the workgroup that ends last joins them, in their order.
+ *
+ * One pass over the rows with the running maximum m and sum l of the softmax, O scaled down when m grows. Heads are the columns of the
+ * matrix products (16, of which few may be live), so K and V come from memory straight into the operand's registers and each row is
+ * read once for all heads that share it; the pages' layout is that operand's. The matrix cores are idle most of the time: what bounds
+ * a batch is memory. 16 heads over 8 of 128, 64 sequences of 4000 to 16384 rows of codes (1.38 GB): 253 us, 5.5 TB/s, where a plain
+ * read reaches 5.96; 16 sequences of 3000 to 4160 (121 MB): 37 us, of which 6 to 11 pass before the first unit is there
+ * (plan 1.5, rows of Q 1 to 4) and 4 in the join. One sequence of 1024 rows: 12.3 us, all of it latency.
+ *
+ * Equal pieces of one line, as many as the machine holds at once: with pieces a sequence (the first form) a second round of workgroups
+ * cost 16 sequences 51 us instead of 37. A piece has at least PG_WAVES units: of 8, one sequence of 1024 rows takes 14.0 us instead
+ * of 12.3, though one of 4096 bf16 rows gains (16.2 and 17.1). Two workgroups a compute unit up to head_dim 128 (256 registers
+ * a lane); at 256 the state and two units in flight take all 512 (one unit and Q's parts in LDS for a second workgroup: 78 us
+ * where this takes 38, 24 sequences of 500 to 8191 rows). */
 template <int HD, bool CODES>
 __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams p) {
     constexpr bool DEEP = HD > 128; /* one wave a SIMD, whose registers hold two units */
@@ -1218,7 +1231,11 @@ __device__ __forceinline__ void pg_choose(F key, int pages, int top, int *list, 
 }
 } // namespace
 
-/* Scores of the pages, `per` of them a workgroup, and the choice by the workgroup of a (sequence, kv head) that ends last. */
+/* Scores of the pages, `per` of them a workgroup, and the choice by the workgroup of a (sequence, kv head) that ends last: one launch,
+ * whose last part no other workgroup waits for. Few bytes (a page's bounds are 512 of head_dim 128), so what it takes is its chain of
+ * round trips: Q's rows and their sums over the heads 5 us, the bounds 2, the scores past the caches 2, then the choice's rounds of LDS
+ * and barriers 3: 11.5 us for 256 pages of one sequence, 18.5 for 250 to 512 of each of 16. Scores and choice by one workgroup of
+ * 1024 threads were slower (one compute unit's 64-bit arithmetic). */
 template <int HD>
 __global__ __launch_bounds__(PG_TPB) void k_pg_choose(const PgParams p) {
     typedef PgScore<HD> Score;
@@ -1747,7 +1764,11 @@ __device__ __forceinline__ void pg_append_v(const PgRunParams &p, const PgRun &r
 }
 } // namespace
 
-/* A workgroup takes the K (z 0) or the V (z 1) rows of `heads` kv heads of one page. */
+/* A workgroup takes the K (z 0) or the V (z 1) rows of `heads` kv heads of one page: a page is the unit whose bounds and whose lines of V
+ * belong to one sequence, so nothing is shared and every store but those at a run's ends is a whole line. K: a row by 8 (16) lanes, its
+ * rotation table read once for all heads; V: turned round in registers. Memory, and behind it the vector instructions (60 of the 97 us):
+ * 16 sequences of 2000 to 4096 bf16 rows of 8 heads of 128 into codes (310 MB) take 97 us, 3.2 TB/s, where a copy of as much takes
+ * 66; a chunk of 26 rows 5.8. */
 template <int HD, bool CODES, bool BF>
 __global__ __launch_bounds__(PA_TPB, HD == 64 || (HD == 128 && CODES) ? 4 : 2) void k_pg_append(const PgRunParams p) {
     PgRun run;
@@ -1787,7 +1808,9 @@ __device__ __forceinline__ float pg_byte(unsigned w, int i) { return (float)(int
 } // namespace
 
 /* A workgroup takes one page and kv head: K piece by piece (eight pieces of eight rows a wave: whole lines both ways), V four dims
- * of eight rows a thread, turned round in registers, as k_pg_append does. */
+ * of eight rows a thread, turned round in registers, as k_pg_append does. All of a thread's loads are requested before the first is
+ * used. Memory: 8 sequences of 4000 to 8192 rows of codes, 8 heads of 128, to bf16 (303 MB): 60 us, 5.0 TB/s (a copy 4.7); 1500 rows of
+ * 4 heads of 64: 5.4 us, latency. */
 template <int HD, bool CODES, bool BF>
 __global__ __launch_bounds__(PG_TPB) void k_pg_read(const PgRunParams p) {
     constexpr int E = CODES ? 16 : 8, CH = CODES ? PgGeom<HD>::CH8 : PgGeom<HD>::CHB;
@@ -1887,7 +1910,9 @@ __global__ __launch_bounds__(PG_TPB) void k_pg_read(const PgRunParams p) {
     default: return -1; \
     }
 
-/* workgroups (of one head) from which one takes two heads, and so on */
+/* Workgroups (of one head) from which one takes two heads, and so on to eight: the rotation table and the run's search are then read
+ * once, and the next head's rows are under way while one is worked on, as long as enough workgroups are left. 800 pages of 8 heads: one
+ * head each 140 us, two 109, four (the rule) 97, eight 97. */
 #define PG_HEADS_FROM 2048
 
 /* workgroups of k_pg on a compute unit (registers) */

@@ -52,7 +52,9 @@ PG_FN PgUnits pg_units(int len, int stride, int positions, int window, int top, 
     return u;
 }
 
-/* What the start of a sequence costs a workgroup, in units: its rows of Q, and no unit under way before them. */
+/* What the start of a sequence costs a workgroup, in units: its rows of Q, and no unit under way before them. Measured with 0, 4, 12 and 24,
+ * us: 16 sequences of 3000 to 4160 rows of codes 42.5, 40.2, 36.4 and 39.2; 24 of 500 to 8191 bf16 rows of head_dim 256 46.7, 44.0, 38.0
+ * and 37.8; 64 of 4000 to 16384 rows of codes 256, 252, 251 and 255. */
 #define PG_EXTRA 12
 
 /* places of a sequence on the line */
