@@ -123,7 +123,7 @@ PG_FN long long pg_max_run_pages(int n, int rows) { return (long long)rows / PG_
 /* ---- 24-bit fixed point in three balanced base-256 digits ----
  * n in [-127 * 65536, 127 * 65536 + 1]: n = 65536 a + 256 b + c with a, b, c in [-128, 127]. Adding 128 to the two lower digits makes
  * them the bytes of a plain number, and taking it off each byte again is an exclusive or. */
-#define PG_FIX 8323072.0f /* 127 * 65536 */
+#define PG_FIX (127.0f * 65536.0f)
 PG_FN unsigned pg_digits(int n) { return ((unsigned)n + 0x8080u) ^ 0x8080u; }
 
 #endif
