@@ -418,9 +418,10 @@ SMOL_ATTN_API int smol_kv_pages_read(smol_kv_pages *pages, int layer, int n_seq,
  * has a page. out[i] is the attention of q[i] over its rows and the new token; norm, RoPE, window, cap and layouts as for
  * smol_attn_decode_qknorm (NULL norm weights skip a norm). A negative len[i] is no sequence: nothing of it is read or written,
  * out[i] stays (a batch padded to a captured size).
- * The new token is used in fp32, and its row is rounded from that. out overlaps no input. bf16 pools: products as of smol_attn_decode_shared. int8 pools: Q and the weights as 24-bit
- * whole numbers against their row's (their page's) largest, products with the codes exact, sums fp32; the 8 bits of the cache
- * are all that is lost. A visible row that is not finite, be it in one element, makes NaN of all outputs of the heads that
+ * The new token is used in fp32, and its row is rounded from that. out overlaps no input. bf16 pools: products as of
+ * smol_attn_decode_shared. int8 pools: Q as 24-bit whole numbers against its row's largest, the weights times V's scales as
+ * 24-bit whole numbers against the largest such product of their page (2^-100 at least, beside a largest weight of one), products
+ * with the codes exact, sums fp32; the 8 bits of the cache are all that is lost. A visible row that is not finite, be it in one element, makes NaN of all outputs of the heads that
  * read it, and of no other; rows at or past a sequence's length are never used. A sequence's result does not depend on the
  * pages that hold its rows; the order of its sums follows the batch's lengths. */
 SMOL_ATTN_API int smol_attn_decode_paged(smol_attn_ctx *ctx, smol_kv_pages *pages, int layer, const smol_rope_table *rope,

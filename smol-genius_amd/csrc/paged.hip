@@ -472,10 +472,14 @@ struct PgUnitRegs<HD, false> {
     }
 };
 
+/* The weights' unit is of 2^-100 at least, so that it and its inverse stay normal numbers: V's smallest scale is near 2^-97 (PG_TINY) */
+#define PG_LEAST 7.888609052210118e-31f
+
 /* A unit of codes joins the state; visible rows of it [lo, hi).
  * A score is exact up to its last sum: K's codes and the digits of Q are whole numbers, and so are their dot products. The
- * weights p vs (vs: V's scales) are taken against the unit's largest as 24-bit whole numbers, digit by digit on the matrix
- * cores again, so V needs no conversion either. */
+ * weights p vs (vs: V's scales) are taken against the largest product of the unit and head as 24-bit whole numbers, digit by digit on
+ * the matrix cores again, so V needs no conversion either. The product, not the largest vs alone: the row that has the weight
+ * may be one of small values (against the largest vs it would keep 14 of its bits where they are 1000 times smaller). */
 template <int HD, class F>
 __device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, true> &q, PgUnitRegs<HD, true> &u, float cap2, int g, int lo, int hi,
                                         float *lds, F next_k) {
@@ -496,8 +500,8 @@ __device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, true> &q,
 #pragma unroll
         for (int i = 0; i < 4; i++) ksc[t][i] = a[i];
     }
-    const unsigned kbits = __float_as_uint(u.ks);
-    const float top = __uint_as_float(wave_max(__float_as_uint(u.vs))); /* as bits: a NaN is the largest */
+    /* a visible scale that is no number, or infinite, spoils the sum when the lanes' are joined */
+    const float odd = 0.0f * u.ks + 0.0f * u.vs;
     i4 d[4][3];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
@@ -544,18 +548,26 @@ __device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, true> &q,
 #pragma unroll
     for (int e = 1; e < 16; e++) mu = fmaxf(mu, s[e >> 2][e & 3]);
     mu = row_max4(mu);
-    const float f = top > 0.0f ? 1.0f / top : 0.0f;
-    float sum = 0.0f;
+    float sum = 0.0f, top = PG_LEAST;
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float pr = __builtin_amdgcn_exp2f(s[t][i] - mu);
+            sum += pr;
+            s[t][i] = pr * vsc[t][i];
+            top = fmaxf(top, s[t][i]);
+        }
+    top = row_max4(top);
+    const float f = 1.0f / top;
     i4 w0, w1, w2;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         unsigned x[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float pr = __builtin_amdgcn_exp2f(s[t][i] - mu);
-            sum += pr;
             /* 2^23 + n: the low bits of the sum are the whole number n, rounded to nearest */
-            const float y = fmaf(pr * (vsc[t][i] * f), PG_FIX, 8388608.0f);
+            const float y = fmaf(s[t][i] * f, PG_FIX, 8388608.0f);
             x[i] = (__float_as_uint(y) + 0x8080u) ^ 0x8080u;
         }
         int a, b, c;
@@ -566,9 +578,8 @@ __device__ __forceinline__ void pg_take(PgState<HD> &st, const PgQ<HD, true> &q,
     }
     pg_raise(st, mu);
     const float b = __builtin_amdgcn_exp2f(mu - st.m);
-    /* a scale that is no number, or infinite, spoils the sum: V's here, K's (this lane's row) when the lanes' sums are joined */
-    st.l = fmaf(b, sum, st.l) + 0.0f * top;
-    st.bad += 0.0f * __uint_as_float(kbits);
+    st.l = fmaf(b, sum, st.l);
+    st.bad += odd;
     const float bo = b * (top * (1.0f / PG_FIX));
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) {

@@ -1,0 +1,123 @@
+"""Rows of a paged cache whose sizes lie far apart, against 64-bit forms: one cached row has nearly all of the softmax weight.
+
+Bound, derived before any run. Scores are off by at most d_j = (hd + 16) 2^-24 a_j, a_j = scale max|q| sum_d |k_jd| (Q at 2^-24 of its
+row's largest element or whole, its norm, rotation and scaling, the fp32 sum of the products). To first order an output moves by
+sum_j p_j d_j |v_j - out|, so the row that has all of the weight moves nothing; doubled for the second order. exp, the sums, the joins and
+the parts of the weights: 2^-20 sum_j p_j |v_j|. Weights of codes are 24-bit whole numbers against the largest p s of their 64 rows, each
+off by half of 2^-23 / 127 of that at most, times codes of up to 127: sum over the pages of 64 127 2^-24 max(p s). s is amax / 127, and the
+row's own largest code may be as low as 64: twice.
+"""
+import pytest
+
+from conftest import pkg  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_paged import P, Step, ctx, order, outward, sa  # noqa: E402,F401
+
+
+def set_row(s, page, h, r, k=None, v=None):
+    """k and v [hd] as row r of a page of kv head h"""
+    kk, vv, sc, b = s.pool.views
+    o = int(order(s.codes)[r])
+    for which, x in ((0, k), (1, v)):
+        if x is None:
+            continue
+        if s.codes:
+            step = x.abs().max() / 127
+            sc[page, h, which, r] = step.item()
+            x = (x / step).round()
+        x = x.to(torch.int8 if s.codes else torch.bfloat16)
+        if which:
+            if s.codes:
+                vv[page, h, :, o] = x.cuda()
+            else:
+                vv[page, h, o // 32, :, o % 32] = x.cuda()
+        else:
+            e = kk.shape[-1]
+            kk[page, h, :, r] = torch.nn.functional.pad(x, (0, -len(x) % e)).view(-1, e).cuda()
+    rows = s.pool.rows()[0][page, h].float()
+    b[page, h] = torch.stack([outward(rows.amin(0), False), outward(rows.amax(0), True)]).to(torch.bfloat16).cuda()
+    s.before, s.rows = s.pool.bits(), s.pool.rows()
+
+
+def with_the_weight(s, at, gap, v_of):
+    """row `at` of each sequence scores about `gap` with every head; v_of(i, h): its value"""
+    q = s.turned()[0]
+    G = s.hq // s.hkv
+    for i in range(s.n):
+        for h in range(s.hkv):
+            u = q[i].view(s.hkv, G, s.hd)[h]
+            k = (u / u.pow(2).sum(-1, keepdim=True)).sum(0) * gap / s.scale
+            set_row(s, int(s.t[i, at // P]), h, at % P, k.float(), v_of(i, h))
+
+
+def check(s, out, what):
+    """out against 64 bits under the bound above"""
+    q, k, v = s.turned()
+    G, hd = s.hq // s.hkv, s.hd
+    out = out.cpu().double().view(s.n, s.hkv, G, hd)
+    assert torch.isfinite(out).all(), what
+    worst = 0.0
+    for i, l in enumerate(s.lens):
+        for h in range(s.hkv):
+            x, at = q[i].view(s.hkv, G, hd)[h], torch.arange(l)
+            if s.top:
+                pages = s.choose(i, h, x)
+                assert s.chosen[i, h].tolist() == pages + [-1] * (s.top - len(pages))
+                at = at[torch.isin(at // P, torch.tensor(pages))]
+            page = s.t[i, at // P].long()
+            keys, vals = (torch.cat([c[page, h, at % P], new[i, h:h + 1]]) for c, new in zip(s.rows, (k, v)))
+            p = torch.softmax(x @ keys.T * s.scale, -1)
+            o = p @ vals
+            d = (hd + 16) * 2.0 ** -24 * s.scale * x.abs().amax(-1, keepdim=True) * keys.abs().sum(-1)
+            tol = torch.stack([(p[g] * d[g]) @ (vals - o[g]).abs() for g in range(G)]) * 2 + 2.0 ** -20 * (p @ vals.abs())
+            if s.codes:
+                ps = p * vals.abs().amax(-1) / 127
+                of = torch.cat([at // P, torch.tensor([-1])])
+                for u in of.unique():
+                    tol = tol + 2 * 64 * 127 * 2.0 ** -24 * ps[:, of == u].amax(-1, keepdim=True)
+            worst = max(worst, float(((out[i, h] - o).abs() / tol).max()))
+    print("%s: %.3f of the bound" % (what, worst), flush=True)
+    assert worst <= 1.0
+
+
+@pytest.mark.parametrize("codes", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("small,gap", [(1e-1, 25.0), (1e-3, 12.0), (1e-3, 25.0), (1e-6, 25.0), (1e-6, 40.0)])
+@pytest.mark.parametrize("hq,hkv,hd", [(4, 2, 128), (3, 3, 80), (8, 1, 256), (2, 1, 64)])
+def test_a_small_value_with_the_weight(sa, ctx, hq, hkv, hd, small, gap, top, codes):
+    """the row that everything attends to has values far below the other rows' of its page"""
+    s = Step(sa, ctx, hq=hq, hkv=hkv, hd=hd, lens=[700, 130, 64], codes=codes, norm=False, top=top, seed=hd + 1)
+    g = torch.Generator().manual_seed(3)
+    with_the_weight(s, 5, gap, lambda i, h: torch.randn(hd, generator=g) * small)
+    out = s.call()
+    ctx.synchronize()
+    check(s, out, "small %g gap %g hd %d codes %d top %d" % (small, gap, hd, codes, top))
+
+
+@pytest.mark.parametrize("codes", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("what", ["spread", "zeros", "tiny"])
+def test_values_of_all_sizes(sa, ctx, what, codes):
+    """every seventh row with values of 1e-9 to 1e9, or zero; or all values near 1e-25"""
+    s = Step(sa, ctx, hq=4, hkv=2, hd=128, lens=[500, 65, 3], codes=codes, norm=False, seed=8)
+    g = torch.Generator().manual_seed(4)
+    for i, l in enumerate(s.lens):
+        for r in range(0, l if what == "spread" else 0, 7):
+            for h in range(2):
+                set_row(s, int(s.t[i, r // P]), h, r % P, v=torch.randn(128, generator=g) * 10.0 ** float(18 * torch.rand(1, generator=g) - 9))
+    if what == "zeros":
+        if codes:
+            s.pool.views[2][:, :, 1, ::7] = 0
+        else:
+            s.pool.views[1][..., ::7] = 0
+    if what == "tiny":
+        (s.pool.views[2][:, :, 1] if codes else s.pool.views[1]).mul_(1e-25)
+        s.v *= 1e-25
+        s.dev[0]["v_new"].mul_(1e-25)
+    s.before, s.rows = s.pool.bits(), s.pool.rows()
+    out = s.call()
+    ctx.synchronize()
+    check(s, out, "sizes %s codes %d" % (what, codes))
