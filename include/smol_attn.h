@@ -421,8 +421,9 @@ SMOL_ATTN_API int smol_kv_pages_read(smol_kv_pages *pages, int layer, int n_seq,
  * The new token is used in fp32, and its row is rounded from that. out overlaps no input. bf16 pools: products as of
  * smol_attn_decode_shared. int8 pools: Q as 24-bit whole numbers against its row's largest, the weights times V's scales as
  * 24-bit whole numbers against the largest such product of their page (2^-100 at least, beside a largest weight of one), products
- * with the codes exact, sums fp32; the 8 bits of the cache are all that is lost. A visible row that is not finite, be it in one element, makes NaN of all outputs of the heads that
- * read it, and of no other; rows at or past a sequence's length are never used. A sequence's result does not depend on the
+ * with the codes exact, sums fp32; the 8 bits of the cache are all that is lost. A visible row that is not finite, be it in one
+ * element, makes NaN of all outputs of the heads that read it, and of no other (sums are fp32: so does a score, or a sum of p |v|
+ * with the largest p as 1, past 3.4e38); rows at or past a sequence's length are never used. A sequence's result does not depend on the
  * pages that hold its rows; the order of its sums follows the batch's lengths. */
 SMOL_ATTN_API int smol_attn_decode_paged(smol_attn_ctx *ctx, smol_kv_pages *pages, int layer, const smol_rope_table *rope,
                                          int n_seq, const int *table, int stride, const int *len, const void *q,

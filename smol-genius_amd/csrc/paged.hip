@@ -691,6 +691,8 @@ __device__ __forceinline__ void get_far(rsrc_t r, unsigned off, float &m, float 
     m = __uint_as_float(v[0]);
     l = __uint_as_float(v[1]);
 }
+/* What is not finite in one dim spoils its row. Each by itself: a sum of finite numbers may pass the largest */
+__device__ __forceinline__ bool pg_odd(f4 a) { return 0.0f * a[0] + 0.0f * a[1] + 0.0f * a[2] + 0.0f * a[3] != 0.0f; }
 template <int N>
 using PgInt = std::integral_constant<int, N>;
 } // namespace
@@ -945,8 +947,7 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
         }
         if (whole) {
             a *= 1.0f / l;
-            /* what is not finite in one dim spoils the row */
-            if (!(fabsf(a[0]) + fabsf(a[1]) + fabsf(a[2]) + fabsf(a[3]) < INFINITY)) s_bad[r] = 1;
+            if (pg_odd(a)) s_bad[r] = 1;
         } else {
             put_far(far, a, place(cut.nth, r) + d * 4);
             if (d == 0) put_far(far, m, l, place(cut.nth, r) + HD * 4);
@@ -1011,7 +1012,7 @@ __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams 
             for (int k = 0; k < N; k++) {
                 if (tid + k * PG_TPB >= R * QD) continue;
                 o[k] *= 1.0f / l[k];
-                if (!(fabsf(o[k][0]) + fabsf(o[k][1]) + fabsf(o[k][2]) + fabsf(o[k][3]) < INFINITY)) s_bad[(tid + k * PG_TPB) / QD] = 1;
+                if (pg_odd(o[k])) s_bad[(tid + k * PG_TPB) / QD] = 1;
             }
         };
         if constexpr (DEEP) {

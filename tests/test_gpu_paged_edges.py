@@ -121,3 +121,25 @@ def test_values_of_all_sizes(sa, ctx, what, codes):
     out = s.call()
     ctx.synchronize()
     check(s, out, "sizes %s codes %d" % (what, codes))
+
+
+@pytest.mark.parametrize("codes", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("hq,hkv,hd,lens", [(4, 2, 128, [40, 64, 130]), (4, 2, 128, [6000, 70]), (2, 2, 72, [33, 900]), (8, 1, 256, [2500, 65]),
+                                            (16, 1, 256, [3000, 6]), (17, 1, 64, [1500, 9])])
+def test_large_finite_values(sa, ctx, hq, hkv, hd, lens, codes):
+    """values whose sum over a few dims passes the largest fp32 number, though none of them does: of a cached row, of the new one"""
+    for new in (False, True):
+        s = Step(sa, ctx, hq=hq, hkv=hkv, hd=hd, lens=lens, codes=codes, norm=False, seed=hd + 2, rope=False)
+        g = torch.Generator().manual_seed(6)
+        huge = lambda *shape: (torch.randint(0, 2, shape, generator=g) * 2 - 1) * 1.2e38  # noqa: E731
+        if new:  # the new row has the weight: its key is along its heads' queries
+            q = s.turned()[0].view(s.n, hkv, hq // hkv, hd)
+            s.k = ((q / q.pow(2).sum(-1, keepdim=True)).sum(2) * 40 / s.scale).float().view(s.n, -1)
+            s.v = huge(s.n, hkv * hd)
+            s.dev[0]["k_new"].copy_(s.k)
+            s.dev[0]["v_new"].copy_(s.v)
+        else:
+            with_the_weight(s, 5, 40.0, lambda i, h: huge(hd))
+        out = s.call()
+        ctx.synchronize()
+        check(s, out, "large, %s, hd %d codes %d" % ("new" if new else "cached", hd, codes))
