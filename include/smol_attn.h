@@ -435,7 +435,7 @@ SMOL_ATTN_API int smol_attn_decode_paged(smol_attn_ctx *ctx, smol_kv_pages *page
  * q normalised and rotated, lo and hi the page's bounds, all in 64 bits: no page whose rows all score lower than another's can
  * be chosen before it on a single head. NaN counts above infinity, ties go to the lower page; first + recent <= top. chosen:
  * device ints [n_seq][n_kv_heads][top], the chosen pages' places in the sequence (0 the first), ascending, -1 behind the
- * last; NULL: not wanted. */
+ * last; all -1 where len[i] is out of range, left as they were where it is negative; NULL: not wanted. */
 SMOL_ATTN_API int smol_attn_decode_paged_top(smol_attn_ctx *ctx, smol_kv_pages *pages, int layer, const smol_rope_table *rope,
                                              int n_seq, const int *table, int stride, const int *len, int top, int first,
                                              int recent, const void *q, const void *k_new, const void *v_new, int dtype,

@@ -1265,8 +1265,9 @@ __global__ __launch_bounds__(PG_TPB) void k_pg_choose(const PgParams p) {
     const int tid = threadIdx.x, kvh = blockIdx.y;
     const int blocks = (p.p.stride + p.per - 1) / p.per, seq = blockIdx.x / blocks, j0 = blockIdx.x % blocks * p.per;
     const int len = p.len[seq];
-    if (!pg_len_ok(len, p.p.stride, p.p.positions)) return;
-    const int pages = pg_pages(len), j1 = min(pages, j0 + p.per);
+    if (len < 0) return;
+    /* a length that is none: no page is chosen, and k_pg reports it */
+    const int pages = pg_len_ok(len, p.p.stride, p.p.positions) ? pg_pages(len) : 0, j1 = min(pages, j0 + p.per);
     if (j0 >= pages && j0 > 0) return;
     const long long pair = (long long)seq * p.p.Hkv + kvh;
     int *list = p.list + pair * p.top;

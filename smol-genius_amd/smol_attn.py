@@ -684,7 +684,7 @@ def pages_read(pages, layer, table, starts, pos, rows, dtype=None, k_out=None, v
 def decode_paged(ctx, pages, layer, rope, table, lens, q, k_new, v_new, n_heads, scale, window=0, cap=0.0, out=None, q_norm=None,
                  k_norm=None, eps=1e-6):
     """One decode step over a paged cache: lens (device int32 [n]) rows of each sequence before the step, -1 for no sequence; see
-    smol_attn_decode_paged. Returns out [n, n_heads*hd]."""
+    smol_attn_decode_paged. Returns out [n, n_heads*hd], whose rows of no sequence are not written: a padded batch gives its own."""
     import torch
     n, qp, kp, vp, dt, qw, kw, out, op = _step_args(ctx, pages, q, k_new, v_new, n_heads, q_norm, k_norm, out)
     n, stride, tp = _page_table(ctx, table, n)
@@ -699,7 +699,8 @@ def decode_paged(ctx, pages, layer, rope, table, lens, q, k_new, v_new, n_heads,
 def decode_paged_top(ctx, pages, layer, rope, table, lens, q, k_new, v_new, n_heads, scale, top, first=1, recent=1, cap=0.0,
                      out=None, chosen=None, q_norm=None, k_norm=None, eps=1e-6):
     """decode_paged over the `top` pages of each sequence and kv head whose bounds promise the largest scores, the first and the
-    recent ones among them; see smol_attn_decode_paged_top. Returns out and chosen (int32 [n, kv_heads, top])."""
+    recent ones among them; see smol_attn_decode_paged_top. Returns out and chosen (int32 [n, kv_heads, top]); where lens is
+    negative nothing is written to either, so a padded batch gives arrays of its own."""
     import torch
     n, qp, kp, vp, dt, qw, kw, out, op = _step_args(ctx, pages, q, k_new, v_new, n_heads, q_norm, k_norm, out)
     n, stride, tp = _page_table(ctx, table, n)

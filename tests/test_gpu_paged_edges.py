@@ -143,3 +143,21 @@ def test_large_finite_values(sa, ctx, hq, hkv, hd, lens, codes):
         out = s.call()
         ctx.synchronize()
         check(s, out, "large, %s, hd %d codes %d" % ("new" if new else "cached", hd, codes))
+
+
+@pytest.mark.parametrize("top", [1, 3, 40])
+def test_choices_of_a_length_that_is_none(sa, ctx, top):
+    """no page is chosen where a length is past the table's end, and nothing is written where it is negative"""
+    s = Step(sa, ctx, hq=4, hkv=2, hd=64, lens=[1500, 130, -1, 64], codes=True, top=top, first=0, seed=12)
+    for none in (s.td.shape[1] * P, 2 ** 31 - 1):
+        s.ld[1] = none
+        chosen = torch.full((s.n, s.hkv, top), 777, dtype=torch.int32, device="cuda")
+        out = torch.full((s.n, s.hq * s.hd), 777.0, device="cuda")
+        s.call(out=out, chosen=chosen)
+        with pytest.raises(sa.SmolAttnPageError):
+            ctx.synchronize()
+        assert (chosen[1] == -1).all() and out[1].isnan().all()
+        assert (chosen[2] == 777).all() and (out[2] == 777.0).all()
+        for i in (0, 3):
+            pages = -(-s.lens[i] // P)
+            assert ((chosen[i] >= 0).sum(-1) == min(top, pages)).all() and (chosen[i] < pages).all()
