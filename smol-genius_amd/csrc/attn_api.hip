@@ -2304,8 +2304,6 @@ extern "C" int smol_kv_pages_pointers(const smol_kv_pages *kp, int layer, void *
     return SMOL_ATTN_OK;
 }
 
-constexpr long long PG_MAX_BLOCKS = (1 << 24) - 1; /* a grid's threads along one axis: below 2^32 */
-
 /* what all calls on a pool check and hand to the kernels; the table of positions grows to what the page table can hold */
 static int paged_pool(smol_kv_pages *kp, int layer, const smol_rope_table *rope, int n_seq, const int *table, int stride, PgPool &pp) {
     if (!kp) return fail(SMOL_ATTN_ERR_ARG, "pool is NULL");
@@ -2351,7 +2349,7 @@ static int paged_run(smol_kv_pages *kp, int layer, const smol_rope_table *rope, 
     if (!starts || !pos || rows < 0) return fail(SMOL_ATTN_ERR_ARG, "bad batch of %d rows", rows);
     if (((uintptr_t)starts | (uintptr_t)pos) & 3) return fail(SMOL_ATTN_ERR_ARG, "starts and pos must be 4-byte aligned");
     if (rows > 0 && (!a || !b)) return fail(SMOL_ATTN_ERR_ARG, "NULL tensor");
-    if (pg_max_run_pages(n_seq, rows) > PG_MAX_BLOCKS) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d rows", rows);
+    if (pg_max_run_pages(n_seq, rows) > pg_max_blocks(write ? PG_APPEND_TPB : PG_TPB)) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d rows", rows);
     int rc;
     if ((rc = check_aligned(a, b))) return rc;
     if ((rc = paged_pool(kp, layer, rope, n_seq, table, stride, rp.p))) return rc;
@@ -2419,7 +2417,7 @@ static int decode_paged(smol_attn_ctx *ctx, smol_kv_pages *kp, int layer, const 
     pg.tiles = (G + 15) / 16;
     pg.top = chosen ? top : std::min(top, stride); /* more pages than a table can have are all of them */
     pg.first = first; pg.recent = recent;
-    if (top > 0 && (long long)n_seq * ((stride + 63) / 64) > PG_MAX_BLOCKS)
+    if (top > 0 && (long long)n_seq * ((stride + 63) / 64) > pg_max_blocks(PG_TPB))
         return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d sequences, page table rows of %d", n_seq, stride);
     if (pg.tiles > 65535) return fail(SMOL_ATTN_ERR_UNSUPPORTED, "%d heads a kv head", G);
     pg.slots = std::max(1, ctx->cu_count * smol_paged_occupancy(hd) / (Hkv * pg.tiles));

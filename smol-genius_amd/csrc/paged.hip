@@ -15,7 +15,6 @@ namespace {
 typedef int i4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2w __attribute__((ext_vector_type(2)));
 
-constexpr int PG_TPB = 64 * PG_WAVES;
 constexpr int PG_HEADS = 16; /* query heads of a tile: the columns of a matrix product */
 
 template <int HD>
@@ -1408,7 +1407,7 @@ __device__ __forceinline__ void rows_join(float (&v)[16], F f) {
     }
 }
 
-constexpr int PA_TPB = 512, PA_WAVES = PA_TPB / 64; /* a k_pg_append workgroup */
+constexpr int PA_TPB = PG_APPEND_TPB, PA_WAVES = PA_TPB / 64; /* a k_pg_append workgroup */
 
 template <int HD>
 struct PgKGeom {

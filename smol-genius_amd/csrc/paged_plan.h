@@ -117,6 +117,10 @@ PG_FN int pg_run_pages(int start, int end, int rows, int pos, int stride, int po
     if (!pg_run_ok(start, end, rows, pos, stride, positions) || end == start) return 0;
     return (pos + (end - start) - 1) / PG_ROWS - pos / PG_ROWS + 1;
 }
+/* workgroups along one axis of a grid: its threads are counted in 32 bits */
+#define PG_TPB (64 * PG_WAVES) /* threads of a workgroup */
+#define PG_APPEND_TPB 512      /* of one that writes rows */
+PG_FN long long pg_max_blocks(int threads) { return 0xFFFFFFFFLL / threads; }
 /* pages of all runs at most: each row opens one, and a run's first and last may be parts */
 PG_FN long long pg_max_run_pages(int n, int rows) { return (long long)rows / PG_ROWS + 2LL * n; }
 
