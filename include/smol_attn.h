@@ -432,7 +432,7 @@ SMOL_ATTN_API int smol_attn_decode_paged(smol_attn_ctx *ctx, smol_kv_pages *page
 /* The same over at most `top` pages of each sequence and kv head. Of the ceil(len / 64) pages that hold rows, the first `first`
  * and the last `recent` (at least 1) stay; the others by the larger
  *   sum over the heads h of the kv head and over d of max(scale q_h[d] lo[d], scale q_h[d] hi[d]),
- * q normalised and rotated, lo and hi the page's bounds, all in 64 bits: no page whose rows all score lower than another's can
+ * q normalised and rotated, lo and hi the page's bounds (an infinite one adds nothing where q is zero), all in 64 bits: no page whose rows all score lower than another's can
  * be chosen before it on a single head. NaN counts above infinity, ties go to the lower page; first + recent <= top. chosen:
  * device ints [n_seq][n_kv_heads][top], the chosen pages' places in the sequence (0 the first), ascending, -1 behind the
  * last; all -1 where len[i] is out of range, left as they were where it is negative; NULL: not wanted. */

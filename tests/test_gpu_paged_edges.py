@@ -161,3 +161,34 @@ def test_choices_of_a_length_that_is_none(sa, ctx, top):
         for i in (0, 3):
             pages = -(-s.lens[i] // P)
             assert ((chosen[i] >= 0).sum(-1) == min(top, pages)).all() and (chosen[i] < pages).all()
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(2, 2, 128), (4, 2, 64), (8, 1, 256), (3, 3, 72)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_infinite_bounds(sa, ctx, hq, hkv, hd, sign):
+    """A row with an infinite element leaves an infinite bound, which counts for the heads that pick it and not for others: a page stays
+    unchosen whose infinity the heads' queries all turn away from, and is chosen (and spoils the head) where one turns towards it."""
+    s = Step(sa, ctx, hq=hq, hkv=hkv, hd=hd, lens=[64 * 40, 64 * 21 + 9], codes=False, norm=False, top=6, seed=hd + 3)
+    q = s.turned()[0].view(s.n, hkv, hq // hkv, hd)
+    b = s.before[3].view(torch.bfloat16)
+    away, towards = [], []
+    for i in range(s.n):
+        for h in range(hkv):
+            pages = -(-s.lens[i] // P)
+            bb = b[s.t[i, :pages].long(), h].double()
+            score = sum(torch.maximum(bb[:, 0] * x, bb[:, 1] * x).sum(-1) for x in q[i, h])
+            low = int(score[1:pages - 1].argmin()) + 1     # neither fixed nor among the best
+            all_away = (sign * q[i, h] < 0).all(0).nonzero()[:, 0].tolist()
+            d = all_away[0] if all_away and (i + h) % 3 else int((sign * q[i, h] > 0).any(0).nonzero()[0])
+            (away if d in all_away else towards).append((i, h))
+            k = s.pool.views[0]
+            k[int(s.t[i, low]), h, d // 8, 11, d % 8] = sign * float("inf")
+            s.pool.views[3][int(s.t[i, low]), h, 1 if sign > 0 else 0, d] = sign * float("inf")
+    s.before, s.rows = s.pool.bits(), s.pool.rows()
+    out = s.call().cpu().view(s.n, hkv, -1)
+    ctx.synchronize()
+    assert towards
+    for i in range(s.n):
+        for h in range(hkv):
+            assert s.chosen[i, h].tolist() == s.choose(i, h, q[i, h]), (i, h)
+            assert out[i, h].isfinite().all() == ((i, h) in away) and out[i, h].isnan().all() == ((i, h) in towards), (i, h)
