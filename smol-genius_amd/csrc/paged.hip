@@ -1327,7 +1327,11 @@ __global__ __launch_bounds__(PG_TPB) void k_pg_choose(const PgParams p) {
         }
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (bad[u]) x[u] = __longlong_as_double(0x7FF8000000000000LL); /* chosen, so that the step meets it */
+            if (bad[u]) {
+                /* chosen before numbers, so that the step meets it; reported here, since others without a number may leave no place */
+                x[u] = __longlong_as_double(0x7FF8000000000000LL);
+                *p.p.flag = 1;
+            }
         if (j + 64 < j1) load(j + 64);
 #pragma unroll
         for (int u = 0; u < U; u++) {

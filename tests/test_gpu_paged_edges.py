@@ -192,3 +192,21 @@ def test_infinite_bounds(sa, ctx, hq, hkv, hd, sign):
         for h in range(hkv):
             assert s.chosen[i, h].tolist() == s.choose(i, h, q[i, h]), (i, h)
             assert out[i, h].isfinite().all() == ((i, h) in away) and out[i, h].isnan().all() == ((i, h) in towards), (i, h)
+
+
+@pytest.mark.parametrize("codes", [False, True], ids=["bf16", "int8"])
+def test_a_bad_page_that_is_scored_only(sa, ctx, codes):
+    """a page number that is none is reported also where pages without numbers for bounds take all places before it"""
+    s = Step(sa, ctx, hq=4, hkv=2, hd=128, lens=[64 * 40, 64 * 3], codes=codes, top=4, first=1, recent=1, seed=15)
+    for j in (1, 2):
+        s.pool.views[3][int(s.t[0, j])] = float("nan")
+    s.before = s.pool.bits()
+    s.call()
+    ctx.synchronize()
+    assert s.chosen[0].tolist() == [[0, 1, 2, 39]] * 2
+    for page in (-1, s.pool.n, 2 ** 31 - 1):
+        s.td[0, 17] = page
+        out = s.call()
+        with pytest.raises(sa.SmolAttnPageError):
+            ctx.synchronize()
+        assert s.chosen[0].tolist() == [[0, 1, 2, 39]] * 2 and out.isfinite().all()
