@@ -432,8 +432,9 @@ SMOL_ATTN_API int smol_attn_decode_paged(smol_attn_ctx *ctx, smol_kv_pages *page
 /* The same over at most `top` pages of each sequence and kv head. Of the ceil(len / 64) pages that hold rows, the first `first`
  * and the last `recent` (at least 1) stay; the others by the larger
  *   sum over the heads h of the kv head and over d of max(scale q_h[d] lo[d], scale q_h[d] hi[d]),
- * q normalised and rotated, lo and hi the page's bounds (an infinite one adds nothing where q is zero), all in 64 bits: no page whose rows all score lower than another's can
- * be chosen before it on a single head. NaN counts above infinity, ties go to the lower page; first + recent <= top. chosen:
+ * q normalised and rotated, lo and hi the page's bounds (an infinite one adds nothing where q is zero), all in 64 bits. That is no
+ * less than the score, summed over those heads before any cap, of any row within the page's bounds: no row of a page left out
+ * scores higher than the value of a page chosen by it. (It may choose a page of lower scores whose bounds are wide.) NaN counts above infinity, ties go to the lower page; first + recent <= top. chosen:
  * device ints [n_seq][n_kv_heads][top], the chosen pages' places in the sequence (0 the first), ascending, -1 behind the
  * last; all -1 where len[i] is out of range, left as they were where it is negative; NULL: not wanted. */
 SMOL_ATTN_API int smol_attn_decode_paged_top(smol_attn_ctx *ctx, smol_kv_pages *pages, int layer, const smol_rope_table *rope,

@@ -1049,7 +1049,7 @@ constexpr int PS_LDS = 4096; /* pages whose keys a choosing workgroup keeps in L
 
 __device__ __forceinline__ int pg_pages(int len) { return (len + PG_ROWS - 1) / PG_ROWS; }
 
-/* score = sum over the heads of a kv head and the dims of max(q lo, q hi): an upper bound of the sum of a page's scores,
+/* score = sum over the heads of a kv head and the dims of max(q lo, q hi): an upper bound of any row's score, summed over the heads,
  * q+ . hi + q- . lo with q+ (q-) the sums of the heads' positive (negative) elements, so a page costs two products whatever the
  * number of heads. In 64 bits, and a page's terms in one order whatever the page: pages with equal bounds tie. */
 template <int HD>

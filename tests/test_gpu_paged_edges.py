@@ -210,3 +210,48 @@ def test_a_bad_page_that_is_scored_only(sa, ctx, codes):
         with pytest.raises(sa.SmolAttnPageError):
             ctx.synchronize()
         assert s.chosen[0].tolist() == [[0, 1, 2, 39]] * 2 and out.isfinite().all()
+
+
+def append_pages(sa, ctx, pages_of_rows, hd, codes):
+    """a sequence whose pages hold the rows [64, hd] given, written by the append, and its table"""
+    n = len(pages_of_rows)
+    pool = sa.KVPages(ctx, 1, n + 1, 1, hd, sa.INT8 if codes else sa.BF16)
+    t = torch.arange(n + 1, dtype=torch.int32).flip(0)[None].contiguous().cuda()
+    rows = torch.cat(pages_of_rows).cuda()
+    at = torch.tensor([0, n * P], dtype=torch.int32).cuda()
+    sa.pages_append(pool, 0, None, t, at, at[:1].clone(), rows, rows.clone())
+    return pool, t, at
+
+
+@pytest.mark.parametrize("codes", [False, True], ids=["bf16", "int8"])
+def test_what_the_choice_promises(sa, ctx, codes):
+    """no row of a page left out scores above the value of a page chosen by it; a page of lower scores and wider bounds may be chosen"""
+    hd = 64
+    g = torch.Generator().manual_seed(17)
+    narrow, wide = torch.zeros(P, hd), torch.zeros(P, hd)
+    narrow[:, :2] = 1.0                    # scores 2, value 2
+    wide[::2, 0], wide[::2, 1] = 10.0, -10.0
+    wide[1::2, 0], wide[1::2, 1] = -10.0, 10.0  # scores 0, value 20
+    pool, t, at = append_pages(sa, ctx, [narrow, wide, torch.zeros(P, hd)], hd, codes)
+    q, new = torch.zeros(1, hd), torch.zeros(1, hd).cuda()
+    q[0, :2] = 1.0
+    _, chosen = sa.decode_paged_top(ctx, pool, 0, None, t, at[1:].clone(), q.cuda(), new, new.clone(), 1, 1.0, 2, first=0, recent=1)
+    assert chosen.tolist() == [[[1, 2]]]
+    pool.close()
+    n, top, G = 40, 9, 3
+    pages = [torch.randn(P, hd, generator=g) * float(torch.rand(1, generator=g) + 0.1) + 0.5 * torch.randn(hd, generator=g) for _ in range(n)]
+    pool, t, at = append_pages(sa, ctx, pages, hd, codes)
+    k, _ = sa.pages_read(pool, 0, t, at, at[:1].clone(), n * P, dtype=torch.float32)
+    q = torch.randn(1, G * hd, generator=g)
+    _, chosen = sa.decode_paged_top(ctx, pool, 0, None, t, at[1:].clone(), q.cuda(), new, new.clone(), G, 0.125, top, first=1, recent=2)
+    ctx.synchronize()
+    by_value = [j for j in chosen[0, 0].tolist() if 1 <= j < n - 2]
+    assert len(by_value) == top - 3
+    x = 0.125 * q.double().view(G, hd)
+    b = pool.views(0)[3].cpu()[t[0, :n].cpu().long(), 0].double()
+    value = sum(torch.maximum(b[:, 0] * h, b[:, 1] * h).sum(-1) for h in x)
+    score = (k.cpu().double() @ x.T).sum(-1).view(n, P).amax(-1)
+    left = [j for j in range(1, n - 2) if j not in by_value]
+    assert (score <= value + 1e-12).all()
+    assert max(float(score[j]) for j in left) <= min(float(value[j]) for j in by_value)
+    pool.close()
