@@ -385,7 +385,8 @@ SMOL_ATTN_API int smol_kv_cache_evict(smol_kv_cache *kv, int layer, int n_seq, c
 #define SMOL_PAGES_INT8 2
 typedef struct smol_kv_pages smol_kv_pages;
 
-/* a pool of n_pages pages for each of n_layers layers, zero-filled; it does not grow */
+/* a pool of n_pages pages for each of n_layers layers, zero-filled (waits for the context's stream, so that the pages may be
+ * filled on any other); it does not grow */
 SMOL_ATTN_API int smol_kv_pages_create(smol_attn_ctx *ctx, int n_layers, int n_pages, int n_kv_heads, int head_dim, int type,
                                        smol_kv_pages **out);
 /* waits for the context's stream, then frees the pool (before its context) */

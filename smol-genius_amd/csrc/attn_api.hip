@@ -2267,7 +2267,9 @@ extern "C" int smol_kv_pages_create(smol_attn_ctx *ctx, int n_layers, int n_page
     const size_t bytes = proto.layer_bytes() * n_layers;
     void *mem = nullptr;
     hipError_t e = hipMalloc(&mem, bytes);
+    /* cleared on the context's stream and waited for: a caller may fill its pages on any other */
     if (e == hipSuccess) e = hipMemsetAsync(mem, 0, bytes, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) {
         if (mem) hipFree(mem);
         hipGetLastError();

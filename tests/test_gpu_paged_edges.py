@@ -255,3 +255,23 @@ def test_what_the_choice_promises(sa, ctx, codes):
     assert (score <= value + 1e-12).all()
     assert max(float(score[j]) for j in left) <= min(float(value[j]) for j in by_value)
     pool.close()
+
+
+def test_a_new_pool_is_cleared_before_it_is_filled(sa):
+    """its clearing, behind other work of the context's stream, does not undo what another stream writes to the new pages"""
+    side = torch.cuda.Stream()
+    c = sa.Context(0, stream=side.cuda_stream)
+    with torch.cuda.stream(side):
+        x = torch.randn(4096, 4096, device="cuda")
+        for _ in range(50):
+            x = torch.nn.functional.normalize(x @ x)
+    pool = sa.KVPages(c, 1, 8, 2, 64, sa.INT8)
+    views = pool.views(0)
+    for v in views:
+        v.fill_(3)
+    torch.cuda.current_stream().synchronize()
+    c.synchronize()
+    for v in views:
+        assert (v == 3).all()
+    pool.close()
+    c.close()
