@@ -367,8 +367,9 @@ SMOL_ATTN_API int smol_kv_cache_evict(smol_kv_cache *kv, int layer, int n_seq, c
  * a row range that is none are not followed; what they would give is NaN, what
  * they would write is not written, and the next smol_attn_ctx_synchronize
  * returns SMOL_ATTN_ERR_PAGE. Work is enqueued on the context's stream. A call
- * grows the RoPE table to stride * SMOL_PAGE_ROWS positions (4194304 at most)
- * and the context's workspace; under stream capture it may not
+ * grows the RoPE table to stride * SMOL_PAGE_ROWS positions (4194304 at most;
+ * 8 * head_dim bytes each, also where the sequences are short: a table as wide
+ * as they may become, not as wide as it could be) and the context's workspace; under stream capture it may not
  * (SMOL_ATTN_ERR_UNSUPPORTED: run the call once before), its replays are
  * ordered with the context's other calls by the caller, and growth after the
  * capture leaves the graph with freed memory. n_seq at most 65535, alignment 16

@@ -24,6 +24,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <memory>
 #include <mutex>
 #include <new>
 #include <numeric>
@@ -561,16 +562,33 @@ extern "C" void smol_rope_fill_host(float *cos_out, float *sin_out, int pos0, in
     }
 }
 
+/* The table's rows are built and uploaded piece by piece behind the ones it
+ * has: a page table's width asks for gigabytes of them, which the host need
+ * not hold and might not have. */
 static int rope_upload(smol_rope_table *rt, int new_cap) {
     smol_attn_ctx *ctx = rt->ctx;
-    std::vector<float> c((size_t)new_cap * rt->hd), s((size_t)new_cap * rt->hd);
-    smol_rope_fill_host(c.data(), s.data(), 0, new_cap, rt->hd, rt->theta, rt->type);
+    const size_t hd = rt->hd, piece = std::min(new_cap - rt->cap, 16384), old = (size_t)rt->cap * hd * sizeof(float);
+    std::unique_ptr<float[]> c(new (std::nothrow) float[piece * hd]), s(new (std::nothrow) float[piece * hd]);
+    if (!c || !s) return fail(SMOL_ATTN_ERR_NOMEM, "RoPE table: no host memory");
     float *cd = nullptr, *sd = nullptr;
     HIP_TRY(hipStreamSynchronize(ctx->stream));
-    HIP_TRY(hipMalloc(&cd, c.size() * sizeof(float)));
-    HIP_TRY(hipMalloc(&sd, s.size() * sizeof(float)));
-    HIP_TRY(hipMemcpy(cd, c.data(), c.size() * sizeof(float), hipMemcpyHostToDevice));
-    HIP_TRY(hipMemcpy(sd, s.data(), s.size() * sizeof(float), hipMemcpyHostToDevice));
+    hipError_t e = hipMalloc(&cd, new_cap * hd * sizeof(float));
+    if (e == hipSuccess) e = hipMalloc(&sd, new_cap * hd * sizeof(float));
+    if (e == hipSuccess && old) e = hipMemcpy(cd, rt->cos_d, old, hipMemcpyDeviceToDevice);
+    if (e == hipSuccess && old) e = hipMemcpy(sd, rt->sin_d, old, hipMemcpyDeviceToDevice);
+    for (int at = rt->cap; e == hipSuccess && at < new_cap; at += (int)piece) {
+        const int n = std::min((int)piece, new_cap - at);
+        smol_rope_fill_host(c.get(), s.get(), at, n, rt->hd, rt->theta, rt->type);
+        e = hipMemcpy(cd + at * hd, c.get(), n * hd * sizeof(float), hipMemcpyHostToDevice);
+        if (e == hipSuccess) e = hipMemcpy(sd + at * hd, s.get(), n * hd * sizeof(float), hipMemcpyHostToDevice);
+    }
+    if (e != hipSuccess) {
+        if (cd) hipFree(cd);
+        if (sd) hipFree(sd);
+        hipGetLastError();
+        return fail(e == hipErrorOutOfMemory ? SMOL_ATTN_ERR_NOMEM : SMOL_ATTN_ERR_DEVICE, "RoPE table of %d positions: %s", new_cap,
+                    hipGetErrorString(e));
+    }
     if (rt->cos_d) hipFree(rt->cos_d);
     if (rt->sin_d) hipFree(rt->sin_d);
     rt->cos_d = cd;
