@@ -369,11 +369,16 @@ SMOL_ATTN_API int smol_kv_cache_evict(smol_kv_cache *kv, int layer, int n_seq, c
  * returns SMOL_ATTN_ERR_PAGE. Work is enqueued on the context's stream. A call
  * grows the RoPE table to stride * SMOL_PAGE_ROWS positions (4194304 at most;
  * 8 * head_dim bytes each, also where the sequences are short: a table as wide
- * as they may become, not as wide as it could be) and the context's workspace; under stream capture it may not
- * (SMOL_ATTN_ERR_UNSUPPORTED: run the call once before), its replays are
- * ordered with the context's other calls by the caller, and growth after the
- * capture leaves the graph with freed memory. n_seq at most 65535, alignment 16
- * bytes for rows, 4 for numbers.
+ * as they may become, not as wide as it could be) and the context's workspace;
+ * under stream capture it may not (SMOL_ATTN_ERR_UNSUPPORTED: run the call once
+ * before). Growth after the capture leaves the graph the arrays that it has
+ * (a workspace for which the device has no room beside the larger one is freed:
+ * capture anew). Replays are ordered with the context's other calls by the
+ * caller. The kernels read the arrays more than once: what they hold stays as it
+ * is until the call's (the replay's) kernels have ended. Lengths that change
+ * meanwhile leave that call's outputs undefined, and those of later steps on the
+ * context: make it anew. n_seq at most 65535, alignment 16 bytes for rows, 4 for
+ * numbers.
  *
  * Types. SMOL_PAGES_BF16: rows rounded to nearest even. SMOL_PAGES_INT8: a row of
  * a kv head, K's and V's each, is 8-bit codes times a scale of its own:

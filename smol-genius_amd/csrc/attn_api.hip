@@ -311,6 +311,7 @@ struct smol_rope_table {
     int hd, type, cap;
     float theta;
     float *cos_d = nullptr, *sin_d = nullptr;
+    std::vector<float *> old; /* smaller tables that a captured graph may still read */
 };
 
 struct smol_kv_cache {
@@ -589,8 +590,9 @@ static int rope_upload(smol_rope_table *rt, int new_cap) {
         return fail(e == hipErrorOutOfMemory ? SMOL_ATTN_ERR_NOMEM : SMOL_ATTN_ERR_DEVICE, "RoPE table of %d positions: %s", new_cap,
                     hipGetErrorString(e));
     }
-    if (rt->cos_d) hipFree(rt->cos_d);
-    if (rt->sin_d) hipFree(rt->sin_d);
+    /* as with a context's buffers, the tables before it stay: capacities double, so they are less than this one */
+    if (rt->cos_d) rt->old.push_back(rt->cos_d);
+    if (rt->sin_d) rt->old.push_back(rt->sin_d);
     rt->cos_d = cd;
     rt->sin_d = sd;
     rt->cap = new_cap;
@@ -640,6 +642,7 @@ extern "C" int smol_rope_table_destroy(smol_rope_table *rt) {
     hipStreamSynchronize(rt->stream);
     if (rt->cos_d) hipFree(rt->cos_d);
     if (rt->sin_d) hipFree(rt->sin_d);
+    for (float *p : rt->old) hipFree(p);
     delete rt;
     return SMOL_ATTN_OK;
 }
@@ -1720,8 +1723,8 @@ static int check_aligned(const void *a, const void *b) {
 
 static int check_rope(smol_attn_ctx *ctx, const smol_rope_table *rope, int hd, int need) {
     if (!rope) return 0;
-    /* a table grows on its own context's stream and frees the old arrays once
-     * that stream is idle: kernels of another context could still read them */
+    /* a table belongs to its context and goes with it: kernels of another
+     * could still read it */
     if (rope->ctx != ctx) return fail(SMOL_ATTN_ERR_ARG, "rope table belongs to another context");
     if (rope->hd != hd) return fail(SMOL_ATTN_ERR_ARG, "rope table head_dim %d != %d", rope->hd, hd);
     return smol_rope_table_ensure(const_cast<smol_rope_table *>(rope), need);

@@ -275,3 +275,37 @@ def test_a_new_pool_is_cleared_before_it_is_filled(sa):
         assert (v == 3).all()
     pool.close()
     c.close()
+
+
+@pytest.mark.parametrize("top", [0, 4])
+def test_a_graph_outlives_growth(sa, top):
+    """a captured step replays after calls with a wider page table and more sequences grew the RoPE table and the workspace"""
+    side = torch.cuda.Stream()
+    c = sa.Context(0, stream=side.cuda_stream)
+    s = Step(sa, c, hq=4, hkv=2, hd=128, lens=[900, 700, 12], codes=True, top=top, seed=41)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        out = torch.zeros((3, 4 * 128), device="cuda")
+        s.call(out=out)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            s.call(out=out)
+        cap = s.rope.capacity
+        big = Step(sa, c, hq=4, hkv=2, hd=128, lens=[50 * i for i in range(90)], codes=True, top=top, seed=42, stride=1500)
+        big.rope = s.rope
+        torch.cuda.synchronize()
+        for turn in range(3):
+            big.call()
+            c.synchronize()
+            assert s.rope.capacity > cap
+            # memory that was freed would hold these by now
+            junk = [torch.full((n,), float("nan"), device="cuda") for n in (1 << 17, 1 << 18, 1 << 20, 1 << 22)]
+            s.pool.views[3].copy_(s.before[3].view(torch.bfloat16))
+            out.fill_(777.0)
+            side.synchronize()
+            graph.replay()
+            c.synchronize()
+            s.check(out, stored=False, what=" replay %d" % turn)
+            del junk
+    c.close()
