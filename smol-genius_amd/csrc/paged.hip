@@ -1321,7 +1321,8 @@ __global__ __launch_bounds__(PG_TPB) void k_pg_choose(const PgParams p) {
         if (__any(none)) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const double y = sc.again(p.p, bad[u] ? 0 : row_table[min(j + u * PP + tid / LPP, pages - 1)], kvh, s.q.sum[0]);
+                const int page = row_table[min(j + u * PP + tid / LPP, pages - 1)]; /* looked at like the first time */
+                const double y = sc.again(p.p, pg_bad_page(page, p.p.n_pages) ? 0 : page, kvh, s.q.sum[0]);
                 if (!(x[u] == x[u])) x[u] = y;
             }
         }
