@@ -391,64 +391,86 @@ SMOL_ATTN_API int smol_kv_cache_evict(smol_kv_cache *kv, int layer, int n_seq, c
 #define SMOL_PAGES_INT8 2
 typedef struct smol_kv_pages smol_kv_pages;
 
-/* a pool of n_pages pages for each of n_layers layers, zero-filled (waits for the context's stream, so that the pages may be
- * filled on any other); it does not grow */
-SMOL_ATTN_API int smol_kv_pages_create(smol_attn_ctx *ctx, int n_layers, int n_pages, int n_kv_heads, int head_dim, int type,
+/* a pool of n_pages pages for each of n_layers layers, zero-filled (waits for the context's
+ * stream, so that the pages may be filled on any other); it does not grow */
+SMOL_ATTN_API int smol_kv_pages_create(smol_attn_ctx *ctx, int n_layers, int n_pages,
+                                       int n_kv_heads, int head_dim, int type,
                                        smol_kv_pages **out);
 /* waits for the context's stream, then frees the pool (before its context) */
 SMOL_ATTN_API int smol_kv_pages_destroy(smol_kv_pages *pages);
-/* device addresses of one layer, for callers that copy, move or fill pages. With e = 16 (int8) or 8 (bf16) elements in 16 bytes:
+/* device addresses of one layer, for callers that copy, move or fill pages. With e = 16 (int8) or
+ * 8 (bf16) elements in 16 bytes:
  *   *k       [n_pages][n_kv_heads][ceil(head_dim / e)][64][e], a row's last e padded with zeros
- *   *v       int8 [n_pages][n_kv_heads][head_dim][64]: row 16 t + 4 g + i of the page at 16 g + 4 t + i;
- *            bf16 [n_pages][n_kv_heads][2][head_dim][32]: row 32 h + 16 t + 4 g + i in half h at 8 g + 4 t + i
+ *   *v       int8 [n_pages][n_kv_heads][head_dim][64]: row 16 t + 4 g + i of the page at
+ *            16 g + 4 t + i; bf16 [n_pages][n_kv_heads][2][head_dim][32]: row
+ *            32 h + 16 t + 4 g + i in half h at 8 g + 4 t + i
  *   *scales  fp32 [n_pages][n_kv_heads][2][64], K's rows and V's (never negative); NULL for bf16
- *   *bounds  bf16 [n_pages][n_kv_heads][2][head_dim]: the lowest and the highest stored value of K's rows, rounded outward;
- *            smol_attn_decode_paged_top chooses by them. A call that writes a page's row 0 starts its bounds anew, any other
- *            widens them, so rows that were written over may still count. */
-SMOL_ATTN_API int smol_kv_pages_pointers(const smol_kv_pages *pages, int layer, void **k, void **v, float **scales,
-                                         uint16_t **bounds);
+ *   *bounds  bf16 [n_pages][n_kv_heads][2][head_dim]: the lowest and the highest stored value of
+ *            K's rows, rounded outward; smol_attn_decode_paged_top chooses by them. A call that
+ *            writes a page's row 0 starts its bounds anew, any other widens them, so rows that
+ *            were written over may still count. */
+SMOL_ATTN_API int smol_kv_pages_pointers(const smol_kv_pages *pages, int layer, void **k,
+                                         void **v, float **scales, uint16_t **bounds);
 
-/* Writes rows of a ragged batch: rows starts[i] .. starts[i + 1] - 1 of k_new, v_new [rows][n_kv_heads * head_dim] (dtype
- * SMOL_ATTN_F32 or _BF16) are positions pos[i], pos[i] + 1, .. of sequence i, K normalised (k_norm [head_dim], NULL: not) and
- * rotated (rope NULL: not) as smol_attn_decode_qknorm's, for codes in fp32, for bf16 rows in 64 bits. starts [n_seq + 1],
- * pos [n_seq]: device ints, starts not falling; a sequence may have no rows. */
-SMOL_ATTN_API int smol_kv_pages_append(smol_kv_pages *pages, int layer, const smol_rope_table *rope, int n_seq, const int *table,
-                                       int stride, const int *starts, const int *pos, int rows, const void *k_new,
-                                       const void *v_new, int dtype, const float *k_norm, float eps);
-/* The values that rows stand for, into k_out, v_out [rows][n_kv_heads * head_dim] of dtype (bf16: nearest even); starts and pos
- * as above. What a chunk of a prompt attends to with smol_attn_causal, for one use. Rows between the sequences' ranges are left
- * as they were, and so are those of a range that is none. The outputs overlap neither each other nor the pool. */
-SMOL_ATTN_API int smol_kv_pages_read(smol_kv_pages *pages, int layer, int n_seq, const int *table, int stride, const int *starts,
-                                     const int *pos, int rows, void *k_out, void *v_out, int dtype);
+/* Writes rows of a ragged batch: rows starts[i] .. starts[i + 1] - 1 of k_new, v_new
+ * [rows][n_kv_heads * head_dim] (dtype SMOL_ATTN_F32 or _BF16) are positions pos[i], pos[i] + 1,
+ * .. of sequence i, K normalised (k_norm [head_dim], NULL: not) and rotated (rope NULL: not) as
+ * smol_attn_decode_qknorm's, for codes in fp32, for bf16 rows in 64 bits. starts [n_seq + 1], pos
+ * [n_seq]: device ints, starts not falling; a sequence may have no rows. */
+SMOL_ATTN_API int smol_kv_pages_append(smol_kv_pages *pages, int layer,
+                                       const smol_rope_table *rope, int n_seq, const int *table,
+                                       int stride, const int *starts, const int *pos, int rows,
+                                       const void *k_new, const void *v_new, int dtype,
+                                       const float *k_norm, float eps);
+/* The values that rows stand for, into k_out, v_out [rows][n_kv_heads * head_dim] of dtype (bf16:
+ * nearest even); starts and pos as above. What a chunk of a prompt attends to with
+ * smol_attn_causal, for one use. Rows between the sequences' ranges are left as they were, and so
+ * are those of a range that is none. The outputs overlap neither each other nor the pool. */
+SMOL_ATTN_API int smol_kv_pages_read(smol_kv_pages *pages, int layer, int n_seq, const int *table,
+                                     int stride, const int *starts, const int *pos, int rows,
+                                     void *k_out, void *v_out, int dtype);
 
-/* One decode step: sequence i has len[i] rows (device ints); its new token gets row and position len[i], for which its table
- * has a page. out[i] is the attention of q[i] over its rows and the new token; norm, RoPE, window, cap and layouts as for
- * smol_attn_decode_qknorm (NULL norm weights skip a norm). A negative len[i] is no sequence: nothing of it is read or written,
+/* One decode step: sequence i has len[i] rows (device ints); its new token gets row and position
+ * len[i], for which its table has a page. out[i] is the attention of q[i] over its rows and the
+ * new token; norm, RoPE, window, cap and layouts as for smol_attn_decode_qknorm (NULL norm
+ * weights skip a norm). A negative len[i] is no sequence: nothing of it is read or written,
  * out[i] stays (a batch padded to a captured size).
- * The new token is used in fp32, and its row is rounded from that. out overlaps no input. bf16 pools: products as of
- * smol_attn_decode_shared. int8 pools: Q as 24-bit whole numbers against its row's largest, the weights times V's scales as
- * 24-bit whole numbers against the largest such product of their page (2^-100 at least, beside a largest weight of one), products
- * with the codes exact, sums fp32; the 8 bits of the cache are all that is lost. A visible row that is not finite, be it in one
- * element, makes NaN of all outputs of the heads that read it, and of no other (sums are fp32: so does a score, or a sum of p |v|
- * with the largest p as 1, past 3.4e38); rows at or past a sequence's length are never used. A sequence's result does not depend on the
+ * The new token is used in fp32, and its row is rounded from that. out overlaps no input. bf16
+ * pools: products as of smol_attn_decode_shared. int8 pools: Q as 24-bit whole numbers against
+ * its row's largest, the weights times V's scales as 24-bit whole numbers against the largest
+ * such product of their page (2^-100 at least, beside a largest weight of one), products with the
+ * codes exact, sums fp32; the 8 bits of the cache are all that is lost. A visible row that is not
+ * finite, be it in one element, makes NaN of all outputs of the heads that read it, and of no
+ * other (sums are fp32: so does a score, or a sum of p |v| with the largest p as 1, past 3.4e38);
+ * rows at or past a sequence's length are never used. A sequence's result does not depend on the
  * pages that hold its rows; the order of its sums follows the batch's lengths. */
-SMOL_ATTN_API int smol_attn_decode_paged(smol_attn_ctx *ctx, smol_kv_pages *pages, int layer, const smol_rope_table *rope,
-                                         int n_seq, const int *table, int stride, const int *len, const void *q,
-                                         const void *k_new, const void *v_new, int dtype, int n_heads, float scale, int window,
-                                         float cap, const float *q_norm, const float *k_norm, float eps, float *out);
-/* The same over at most `top` pages of each sequence and kv head. Of the ceil(len / 64) pages that hold rows, the first `first`
- * and the last `recent` (at least 1) stay; the others by the larger
+SMOL_ATTN_API int smol_attn_decode_paged(smol_attn_ctx *ctx, smol_kv_pages *pages, int layer,
+                                         const smol_rope_table *rope, int n_seq, const int *table,
+                                         int stride, const int *len, const void *q,
+                                         const void *k_new, const void *v_new, int dtype,
+                                         int n_heads, float scale, int window, float cap,
+                                         const float *q_norm, const float *k_norm, float eps,
+                                         float *out);
+/* The same over at most `top` pages of each sequence and kv head. Of the ceil(len / 64) pages
+ * that hold rows, the first `first` and the last `recent` (at least 1) stay; the others by the
+ * larger
  *   sum over the heads h of the kv head and over d of max(scale q_h[d] lo[d], scale q_h[d] hi[d]),
- * q normalised and rotated, lo and hi the page's bounds (an infinite one adds nothing where q is zero), all in 64 bits. That is no
- * less than the score, summed over those heads before any cap, of any row within the page's bounds: no row of a page left out
- * scores higher than the value of a page chosen by it. (It may choose a page of lower scores whose bounds are wide.) NaN counts above infinity, ties go to the lower page; first + recent <= top. chosen:
- * device ints [n_seq][n_kv_heads][top], the chosen pages' places in the sequence (0 the first), ascending, -1 behind the
- * last; all -1 where len[i] is out of range, left as they were where it is negative; NULL: not wanted. */
-SMOL_ATTN_API int smol_attn_decode_paged_top(smol_attn_ctx *ctx, smol_kv_pages *pages, int layer, const smol_rope_table *rope,
-                                             int n_seq, const int *table, int stride, const int *len, int top, int first,
-                                             int recent, const void *q, const void *k_new, const void *v_new, int dtype,
-                                             int n_heads, float scale, float cap, const float *q_norm, const float *k_norm,
-                                             float eps, int *chosen, float *out);
+ * q normalised and rotated, lo and hi the page's bounds (an infinite one adds nothing where q is
+ * zero), all in 64 bits. That is no less than the score, summed over those heads before any cap,
+ * of any row within the page's bounds: no row of a page left out scores higher than the value of
+ * a page chosen by it. (It may choose a page of lower scores whose bounds are wide.) NaN counts
+ * above infinity, ties go to the lower page; first + recent <= top. chosen: device ints
+ * [n_seq][n_kv_heads][top], the chosen pages' places in the sequence (0 the first), ascending, -1
+ * behind the last; all -1 where len[i] is out of range, left as they were where it is negative;
+ * NULL: not wanted. */
+SMOL_ATTN_API int smol_attn_decode_paged_top(smol_attn_ctx *ctx, smol_kv_pages *pages, int layer,
+                                             const smol_rope_table *rope, int n_seq,
+                                             const int *table, int stride, const int *len,
+                                             int top, int first, int recent, const void *q,
+                                             const void *k_new, const void *v_new, int dtype,
+                                             int n_heads, float scale, float cap,
+                                             const float *q_norm, const float *k_norm, float eps,
+                                             int *chosen, float *out);
 
 /* Causal attention on flat device arrays, no cache and no RoPE: the device
  * form of smol_causal_attention (attention.c:153-170). K, V: [seq_k][n_kv*hd]. */

@@ -702,14 +702,15 @@ using PgInt = std::integral_constant<int, N>;
  * One pass over the rows with the running maximum m and sum l of the softmax, O scaled down when m grows. Heads are the columns of the
  * matrix products (16, of which few may be live), so K and V come from memory straight into the operand's registers and each row is
  * read once for all heads that share it; the pages' layout is that operand's. The matrix cores are idle most of the time: what bounds
- * a batch is memory. 16 heads over 8 of 128, 64 sequences of 4000 to 16384 rows of codes (1.38 GB): 253 us, 5.5 TB/s, where a plain
- * read reaches 5.96; 16 sequences of 3000 to 4160 (121 MB): 37 us, of which 6 to 11 pass before the first unit is there
- * (plan 1.5, rows of Q 1 to 4) and 4 in the join. One sequence of 1024 rows: 12.3 us, all of it latency.
+ * a batch is memory. 16 heads over 8 of 128, 64 sequences of 4000 to 16384 rows of codes (1.38 GB): 250 us, 5.5 TB/s of what has to be
+ * read (the counters see 1.32 GB), where a plain read reaches 5.96; 16 sequences of 3000 to 4160 (121 MB): 36 us, of which 6 to 11 pass
+ * before the first unit is there (plan 1.5, rows of Q 1 to 4) and 4 in the join. One sequence of 1024 bf16 rows: 12.8 us, all of it
+ * latency; of codes 15: units of 64 rows share them out to half as many waves, and each weight has its digits to be formed.
  *
  * Equal pieces of one line, as many as the machine holds at once: with pieces a sequence (the first form) a second round of workgroups
  * cost 16 sequences 51 us instead of 37. A piece has at least PG_WAVES units: of 8, one sequence of 1024 rows takes 14.0 us instead
  * of 12.3, though one of 4096 bf16 rows gains (16.2 and 17.1). Two workgroups a compute unit up to head_dim 128 (256 registers
- * a lane); at 256 the state and two units in flight take all 512 (one unit and Q's parts in LDS for a second workgroup: 78 us
+ * a lane, of which codes spill 5 at 96 and 8 at 128); at 256 the state and two units in flight take all 512 (one unit and Q's parts in LDS for a second workgroup: 78 us
  * where this takes 38, 24 sequences of 500 to 8191 rows). */
 template <int HD, bool CODES>
 __global__ __launch_bounds__(PG_TPB, HD > 128 ? 1 : 2) void k_pg(const PgParams p) {
