@@ -377,8 +377,8 @@ SMOL_ATTN_API int smol_kv_cache_evict(smol_kv_cache *kv, int layer, int n_seq, c
  * caller. The kernels read the arrays more than once: what they hold stays as it
  * is until the call's (the replay's) kernels have ended. Lengths that change
  * meanwhile leave that call's outputs undefined, and those of later steps on the
- * context: make it anew. n_seq at most 65535, alignment 16 bytes for rows, 4 for
- * numbers.
+ * context: make it anew. n_seq at most 65535 (a decode step: n_seq * (2 stride +
+ * 12) at most 2^30), alignment 16 bytes for rows, 4 for numbers.
  *
  * Types. SMOL_PAGES_BF16: rows rounded to nearest even. SMOL_PAGES_INT8: a row of
  * a kv head, K's and V's each, is 8-bit codes times a scale of its own:
